@@ -16,6 +16,7 @@ F32, F16, BF16 = 0, 1, 2
 ROUND_NEAREST, ROUND_STOCH_NOISE, ROUND_STOCH_PHILOX = 0, 1, 2
 FLAG_CLAMP, FLAG_SQUASH = 1, 2
 ACT_RELU, ACT_RELU6, ACT_GELU, ACT_SILU = 0, 1, 2, 3
+LIN_ACTS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 BN_NORM, BN_QUANT, BN_RELU_QUANT, BN_RELU6_QUANT = 0, 1, 2, 3
 
 OK, EBITS, EINVAL, EUNSUPPORTED, EHIP = 0, -1, -2, -3, -4
@@ -62,6 +63,15 @@ EXPORTS = (
     "dopt_graph_replace_memsets",
     "dopt_alam_quant_pack",
     "dopt_alam_dequant_unpack",
+    "dopt_layer_norm_forward",
+    "dopt_layer_norm_workspace_floats",
+    "dopt_layer_norm_backward",
+    "dopt_dropout",
+    "dopt_linear_forward",
+    "dopt_linear_input_grad",
+    "dopt_linear_act_grad",
+    "dopt_linear_weight_grad_workspace_floats",
+    "dopt_linear_weight_grad",
 )
 
 _lib = None
@@ -185,6 +195,26 @@ def lib() -> ctypes.CDLL:
         L.dopt_alam_quant_pack.restype = i32
         L.dopt_alam_dequant_unpack.argtypes = [vp, vp, vp, i64, i32, i32, i32, ctypes.c_uint64, vp, vp]
         L.dopt_alam_dequant_unpack.restype = i32
+        L.dopt_layer_norm_forward.argtypes = [vp, i32, i64, i64, vp, vp, i32, f32, vp, i32, vp, vp, vp]
+        L.dopt_layer_norm_forward.restype = i32
+        L.dopt_layer_norm_workspace_floats.argtypes = [i64, i64]
+        L.dopt_layer_norm_workspace_floats.restype = i64
+        # dy, dy_dt, x, x_dt, rows, dim, mean, rstd, weight, param_dt, dresidual, dx, workspace, dweight, dbias, stream
+        L.dopt_layer_norm_backward.argtypes = [vp, i32, vp, i32, i64, i64, vp, vp, vp, i32, vp, vp, vp, vp, vp, vp]
+        L.dopt_layer_norm_backward.restype = i32
+        L.dopt_dropout.argtypes = [vp, i32, vp, i64, ctypes.c_double, u64, u64, vp, vp, i32, vp]
+        L.dopt_dropout.restype = i32
+        # x, ldx, weight, ldw, dt, M, N, K, bias, bias_dt, residual, act, y, y_dt, pre, stream
+        L.dopt_linear_forward.argtypes = [vp, i64, vp, i64, i32, i64, i64, i64, vp, i32, vp, i32, vp, i32, vp, vp]
+        L.dopt_linear_forward.restype = i32
+        L.dopt_linear_input_grad.argtypes = [vp, i64, vp, i64, i32, i64, i64, i64, vp, i32, vp, vp]
+        L.dopt_linear_input_grad.restype = i32
+        L.dopt_linear_act_grad.argtypes = [vp, i64, vp, i32, i32, i64, i64, vp, i64, vp]
+        L.dopt_linear_act_grad.restype = i32
+        L.dopt_linear_weight_grad_workspace_floats.argtypes = [i64, i64, i64]
+        L.dopt_linear_weight_grad_workspace_floats.restype = i64
+        L.dopt_linear_weight_grad.argtypes = [vp, i64, vp, i64, i32, i64, i64, i64, vp, vp, vp, vp, vp]
+        L.dopt_linear_weight_grad.restype = i32
         _lib = L
     return _lib
 

@@ -30,6 +30,10 @@ SOURCES = [
     "dw_gemm.hip",
     "graph_tools.hip",
     "alam.hip",
+    "layer_norm_fwd.hip",
+    "layer_norm_bwd.hip",
+    "dropout.hip",
+    "linear_gemm.hip",
 ]
 
 ARCH = "gfx950"

@@ -10,6 +10,8 @@
 #include "bn_fused.h"
 #include "dequant_unpack.h"
 #include "dw_gemm.h"
+#include "layer_norm.h"
+#include "linear_epilogue.h"
 #include "quant_pack.h"
 
 namespace dopt {
@@ -35,6 +37,12 @@ int launch_alam_quant_pack(const void* x, int dt, int64_t n_groups, int g, int b
 int launch_alam_dequant(const uint32_t* packed, const uint16_t* scale, const uint16_t* minv, int64_t n_groups,
                         int g, int bits, int alam, uint64_t seed, uint16_t* y, hipStream_t s);
 int launch_alam_act_dequant_mul(const DequantArgs& d, int g, int bits, int dy_f32, uint64_t seed, hipStream_t s);
+int launch_dropout(const void* x, int x_dt, const void* residual, uint64_t n, uint32_t threshold, uint64_t seed,
+                   uint64_t offset, const int64_t* step, void* y, int y_dt, hipStream_t s);
+bool lin_shape_fits(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb);
+int launch_linear(const LinArgs& p, bool kn, bool f16, hipStream_t s);
+int launch_linear_act_grad(const uint16_t* src, int64_t src_ld, const uint16_t* pre, int act, bool f16, int64_t rows,
+                           int64_t cols, uint16_t* dst, int64_t ld_dst, hipStream_t s);
 }  // namespace dopt
 
 namespace {
@@ -1082,6 +1090,184 @@ int dopt_dw_gemm_any(const void* dy, int64_t ldd, const void* x_hat, int64_t ldx
     if (dopt::launch_dw_gemm(a, dopt::DW_B_BF16, db != nullptr, dw_f32, (uint16_t*)dw_bf16, db, (hipStream_t)stream))
         return fail(DOPT_EUNSUPPORTED, "no dw_gemm_any kernel for this shape");
     return hip_status("dw_gemm_any launch");
+}
+
+// ---------------------------------------------------------------- transformer blocks
+static int check_float(int dt, const char* what) {
+    if (dt != DOPT_F32 && dt != DOPT_F16 && dt != DOPT_BF16)
+        return fail(DOPT_EINVAL, "%s must be DOPT_F32, DOPT_F16 or DOPT_BF16, got %d", what, dt);
+    return DOPT_OK;
+}
+
+static int check_layer_norm(int64_t rows, int64_t dim, int x_dt, int y_dt, const void* params, int param_dt) {
+    if (rows < 0 || dim < 1 || dim >= ((int64_t)1 << 30) || rows >= ((int64_t)1 << 62) / dim)
+        return fail(DOPT_EINVAL, "layer norm needs rows >= 0 and 1 <= dim < 2^30, got rows=%lld dim=%lld", (long long)rows, (long long)dim);
+    if (int rc = check_float(x_dt, "layer norm: the input's type")) return rc;
+    if (int rc = check_float(y_dt, "layer norm: the output's type")) return rc;
+    return params ? check_float(param_dt, "layer norm: the parameters' type") : DOPT_OK;
+}
+
+int dopt_layer_norm_forward(const void* x, int x_dtype, int64_t rows, int64_t dim, const void* weight, const void* bias,
+                            int param_dtype, float eps, void* y, int y_dtype, float* mean, float* rstd, void* stream) {
+    if (int rc = check_layer_norm(rows, dim, x_dtype, y_dtype, weight ? weight : bias, param_dtype)) return rc;
+    if (!(eps >= 0.0f)) return fail(DOPT_EINVAL, "layer norm: eps must be >= 0, got %g", (double)eps);
+    if (rows == 0) return ok();
+    if (!x || !y || !mean || !rstd) return fail(DOPT_EINVAL, "null x/y/mean/rstd pointer");
+    const dopt::LnFwdArgs a{x, y, weight, bias, mean, rstd, rows, (int)dim, y_dtype, param_dtype, eps};
+    (void)hipGetLastError();
+    dopt::launch_layer_norm_fwd(a, x_dtype, (hipStream_t)stream);
+    return hip_status("layer_norm_forward launch");
+}
+
+int64_t dopt_layer_norm_workspace_floats(int64_t rows, int64_t dim) {
+    if (rows < 0 || dim < 1 || dim >= ((int64_t)1 << 30)) return 0;
+    return dopt::layer_norm_groups(rows, (int)dim) * 2 * dim;
+}
+
+int dopt_layer_norm_backward(const void* dy, int dy_dtype, const void* x, int x_dtype, int64_t rows, int64_t dim,
+                             const float* mean, const float* rstd, const void* weight, int param_dtype,
+                             const void* dresidual, void* dx, float* workspace, float* dweight, float* dbias, void* stream) {
+    if (int rc = check_layer_norm(rows, dim, x_dtype, dy_dtype, weight, param_dtype)) return rc;
+    if (rows > 0 && (!dy || !x || !mean || !rstd || !dx)) return fail(DOPT_EINVAL, "null dy/x/mean/rstd/dx pointer");
+    if ((dweight || dbias) && rows > 0 && !workspace) return fail(DOPT_EINVAL, "the parameter gradients need a workspace");
+    const dopt::LnBwdArgs a{dy, x, mean, rstd, weight, dresidual, dx, dweight || dbias ? workspace : nullptr, rows, (int)dim, param_dtype};
+    (void)hipGetLastError();
+    dopt::launch_layer_norm_bwd(a, x_dtype, dy_dtype, dweight, dbias, (hipStream_t)stream);
+    return hip_status("layer_norm_backward launch");
+}
+
+int dopt_dropout(const void* x, int x_dtype, const void* residual, int64_t n, double p, uint64_t seed, uint64_t offset,
+                 const int64_t* step, void* y, int y_dtype, void* stream) {
+    if (!(p >= 0.0 && p <= 1.0)) return fail(DOPT_EINVAL, "dropout: p must lie in [0, 1], got %g", p);
+    if (n < 0) return fail(DOPT_EINVAL, "dropout: n must be >= 0, got %lld", (long long)n);
+    if (int rc = check_float(x_dtype, "dropout: the input's type")) return rc;
+    if (int rc = check_float(y_dtype, "dropout: the output's type")) return rc;
+    if (n == 0) return ok();
+    if (!x || !y) return fail(DOPT_EINVAL, "null x/y pointer");
+    (void)hipGetLastError();
+    dopt::launch_dropout(x, x_dtype, residual, (uint64_t)n, (uint32_t)(p * 65536.0 + 0.5), seed, offset, step, y, y_dtype,
+                         (hipStream_t)stream);
+    return hip_status("dropout launch");
+}
+
+static bool lin_rows(const void* p, int64_t ld, int64_t cols) { return ld >= (cols + 7) / 8 * 8 && ld % 8 == 0 && aligned16(p); }
+
+static int check_linear(int dtype, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int act) {
+    if (dtype != DOPT_F16 && dtype != DOPT_BF16)
+        return fail(DOPT_EINVAL, "linear: the operands must be DOPT_F16 or DOPT_BF16, got %d", dtype);
+    if (M < 0 || N < 0 || K < 0)
+        return fail(DOPT_EINVAL, "linear: sizes must be >= 0 (got %lld, %lld, %lld)", (long long)M, (long long)N, (long long)K);
+    if (act < DOPT_LIN_NONE || act > DOPT_LIN_SILU) return fail(DOPT_EINVAL, "linear: unknown activation %d", act);
+    if (!dopt::lin_shape_fits(M, N, K, lda, ldb))
+        return fail(DOPT_EUNSUPPORTED, "linear: row strides must be below 2^21 and the sum below 2^28 long (got strides %lld, %lld, "
+                    "rows %lld, columns %lld, sum %lld)", (long long)lda, (long long)ldb, (long long)M, (long long)N, (long long)K);
+    return DOPT_OK;
+}
+
+int dopt_linear_forward(const void* x, int64_t ldx, const void* weight, int64_t ldw, int dtype, int64_t M, int64_t N,
+                        int64_t K, const void* bias, int bias_dtype, const void* residual, int act, void* y, int y_dtype,
+                        void* pre, void* stream) {
+    if (int rc = check_linear(dtype, M, N, K, ldx, ldw, act)) return rc;
+    if (y_dtype != dtype && y_dtype != DOPT_F32)
+        return fail(DOPT_EINVAL, "linear: the result has the operands' type or DOPT_F32, got %d", y_dtype);
+    if (bias)
+        if (int rc = check_float(bias_dtype, "linear: the bias's type")) return rc;
+    if (M == 0 || N == 0) return ok();
+    if (!y || (K > 0 && (!x || !weight))) return fail(DOPT_EINVAL, "null x/weight/y pointer");
+    if (K > 0 && (!lin_rows(x, ldx, K) || !lin_rows(weight, ldw, K)))
+        return fail(DOPT_EINVAL, "linear: x and weight must be 16-byte aligned, their row strides multiples of 8 and at least K rounded up to one");
+    dopt::LinArgs p{};
+    p.A = (const uint16_t*)x;
+    p.B = (const uint16_t*)weight;
+    p.M = M;
+    p.N = N;
+    p.K = K;
+    p.lda = ldx;
+    p.ldb = ldw;
+    p.bias = bias;
+    p.bias_dt = bias_dtype;
+    p.res = residual;
+    p.act = act;
+    p.y = y;
+    p.y_f32 = y_dtype == DOPT_F32;
+    p.pre = (uint16_t*)pre;
+    (void)hipGetLastError();
+    dopt::launch_linear(p, false, dtype == DOPT_F16, (hipStream_t)stream);
+    return hip_status("linear_forward launch");
+}
+
+int dopt_linear_input_grad(const void* dz, int64_t ldz, const void* weight, int64_t ldw, int dtype, int64_t M, int64_t N,
+                           int64_t K, const void* in_pre, int in_act, void* dx, void* stream) {
+    if (int rc = check_linear(dtype, M, K, N, ldz, ldw, in_act)) return rc;
+    if (M == 0 || K == 0) return ok();
+    if (!dx || (N > 0 && (!dz || !weight))) return fail(DOPT_EINVAL, "null dz/weight/dx pointer");
+    if (in_act != DOPT_LIN_NONE && !in_pre) return fail(DOPT_EINVAL, "linear: in_act needs in_pre");
+    if (N > 0 && (!lin_rows(dz, ldz, N) || !lin_rows(weight, ldw, K)))
+        return fail(DOPT_EINVAL, "linear: dz and weight must be 16-byte aligned, their row strides multiples of 8 and at least N and K rounded up to one");
+    dopt::LinArgs p{};
+    p.A = (const uint16_t*)dz;
+    p.B = (const uint16_t*)weight;
+    p.M = M;
+    p.N = K;
+    p.K = N;
+    p.lda = ldz;
+    p.ldb = ldw;
+    p.aux = (const uint16_t*)in_pre;
+    p.act = in_act;
+    p.y = dx;
+    (void)hipGetLastError();
+    dopt::launch_linear(p, true, dtype == DOPT_F16, (hipStream_t)stream);
+    return hip_status("linear_input_grad launch");
+}
+
+int dopt_linear_act_grad(const void* dy, int64_t ld_dy, const void* pre, int act, int dtype, int64_t rows, int64_t cols,
+                         void* dz, int64_t ld_dz, void* stream) {
+    if (int rc = check_linear(dtype, rows, cols, 0, 0, 0, act)) return rc;
+    if (rows == 0 || cols == 0) return ok();
+    if (!dy || !dz || (act != DOPT_LIN_NONE && !pre)) return fail(DOPT_EINVAL, "null dy/pre/dz pointer");
+    if (ld_dy < cols || !lin_rows(dz, ld_dz, cols))
+        return fail(DOPT_EINVAL, "linear: dz must be 16-byte aligned, its row stride a multiple of 8 and at least cols; dy's at least cols");
+    (void)hipGetLastError();
+    dopt::launch_linear_act_grad((const uint16_t*)dy, ld_dy, (const uint16_t*)pre, act, dtype == DOPT_F16, rows, cols,
+                                 (uint16_t*)dz, ld_dz, (hipStream_t)stream);
+    return hip_status("linear_act_grad launch");
+}
+
+static bool linear_dw_shape(int64_t M, int64_t N, int64_t K) {
+    return M >= 0 && N > 0 && K > 0 && K % 8 == 0 && N < ((int64_t)1 << 20) && K < ((int64_t)1 << 20);
+}
+
+int64_t dopt_linear_weight_grad_workspace_floats(int64_t M, int64_t N, int64_t K) {
+    return linear_dw_shape(M, N, K) ? dopt::dw_any_workspace_floats(N, K, M) : 0;
+}
+
+int dopt_linear_weight_grad(const void* dz, int64_t ldz, const void* x, int64_t ldx, int dtype, int64_t M, int64_t N,
+                            int64_t K, float* workspace, float* dw_f32, void* dw_16, float* db, void* stream) {
+    if (dtype != DOPT_F16 && dtype != DOPT_BF16)
+        return fail(DOPT_EINVAL, "linear: the operands must be DOPT_F16 or DOPT_BF16, got %d", dtype);
+    if (!linear_dw_shape(M, N, K))
+        return fail(DOPT_EUNSUPPORTED, "linear weight gradient needs N >= 1 and K a positive multiple of 8, both below 2^20 (got M=%lld N=%lld K=%lld)",
+                    (long long)M, (long long)N, (long long)K);
+    if ((M > 0 && (!dz || !x)) || !workspace || (!dw_f32 && !dw_16))
+        return fail(DOPT_EINVAL, "null dz/x/workspace/output pointer");
+    if (M > 0 && (!lin_rows(dz, ldz, N) || !lin_rows(x, ldx, K) || ldz >= ((int64_t)1 << 24) || ldx >= ((int64_t)1 << 24)))
+        return fail(DOPT_EINVAL, "linear: dz and x must be 16-byte aligned, their row strides multiples of 8, at least N and K rounded up to one and below 2^24");
+    if (((uintptr_t)workspace & 15u) || (dw_f32 && ((uintptr_t)dw_f32 & 15u)) || (dw_16 && ((uintptr_t)dw_16 & 7u)))
+        return fail(DOPT_EINVAL, "workspace / dw_f32 must be 16-byte and dw_16 8-byte aligned");
+    dopt::DwArgs a{};
+    a.dy = (const uint16_t*)dz;
+    a.ldd = ldz;
+    a.xh = (const uint16_t*)x;
+    a.ldx = ldx;
+    a.M = N;
+    a.N = K;
+    a.K = M;
+    a.partial = workspace;
+    a.f16 = dtype == DOPT_F16;
+    (void)hipGetLastError();
+    if (dopt::launch_dw_gemm(a, dopt::DW_B_BF16, db != nullptr, dw_f32, (uint16_t*)dw_16, db, (hipStream_t)stream))
+        return fail(DOPT_EUNSUPPORTED, "no weight-gradient kernel for this shape");
+    return hip_status("linear_weight_grad launch");
 }
 
 int dopt_graph_node_counts(void* graph, int64_t* counts, int n_counts) {

@@ -25,6 +25,7 @@ struct DwArgs {
     float* partial;           // workspace: [splits][M][N] fp32, then [splits][M] for db; one split: the fp32 result
     uint16_t* out16;          // the bf16 result, of the kernels that write it in place of partial
     float* db_partial;        // set by the launcher
+    bool f16 = false;         // dy, xh and out16 are fp16 (DW_B_BF16 only; M may then be any number below ldd)
 };
 
 int dw_splits(int64_t M, int64_t N, int64_t K);

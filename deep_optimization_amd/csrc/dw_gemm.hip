@@ -49,6 +49,18 @@ __device__ __forceinline__ f32x16_t mfma_bf16(const uint4& a, const uint4& b, co
                                                    c, 0, 0, 0);
 }
 
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+
+template <bool F16>
+__device__ __forceinline__ f32x16_t mfma_16bit(const uint4& a, const uint4& b, const f32x16_t& c) {
+    if constexpr (F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+    else
+        return mfma_bf16(a, b, c);
+}
+__device__ __forceinline__ uint16_t to_f16(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
+
 // byte offset of 16-byte chunk `ch` of LDS row `r`
 __device__ __forceinline__ int lds_off(int r, int ch) { return r * ROWB + ((ch ^ ((r >> 1) & 7)) << 4); }
 
@@ -360,13 +372,15 @@ struct V2Codes {
 // O16 (bf16 x_hat, one split): the result goes out in bf16, not as an fp32 partial matrix that a second kernel
 // rounds, 10 bytes an element for 2 (4096 x 4096 over 333 tokens 41.8 -> 22.5 us, 10000 x 512 over 64 with db
 // 21.1 -> 10.3; torch's product and sum take 12.9 there).
-template <int BITS, bool DB, int NW, int BMT, int BNT = 256, bool RAG = false, bool O16 = false>
+// F16 (ragged instances, which take every shape): fp16 operands and, with O16, an fp16 result.
+template <int BITS, bool DB, int NW, int BMT, int BNT = 256, bool RAG = false, bool O16 = false, bool F16 = false>
 __global__ __launch_bounds__(64 * NW, 1) void dw_gemm_v2_kernel(DwArgs a) {
     static_assert(BITS == 0 || BITS == 1 || BITS == 2 || BITS == 4, "bf16, or 1/2/4-bit codes");
     static_assert(NW == 4 || (NW == 8 && BITS == 0), "8 waves for bf16 x_hat only");
     static_assert(BNT == 256 || (BNT == 128 && RAG), "narrow x_hat tiles for the ragged kernel only");
     static_assert(!RAG || BITS == 0, "ragged shapes: bf16 x_hat only");
     static_assert(!O16 || BITS == 0, "bf16 results: bf16 x_hat only");
+    static_assert(!F16 || RAG, "fp16 operands: the ragged instances");
     using CS = V2Codes<BITS>;
     constexpr int WN = NW / 2;            // waves along n
     constexpr int CW = BNT / WN;          // columns per wave
@@ -561,8 +575,15 @@ __global__ __launch_bounds__(64 * NW, 1) void dw_gemm_v2_kernel(DwArgs a) {
     // bias-gradient pairs of fragment row ii
     auto db_row = [&](const uint4* fa, int ii) {
         if (db_wave) {
-            const bf16x2_t one = __builtin_bit_cast(bf16x2_t, 0x3f803f80u);
             const uint32_t w[4] = {fa[ii].x, fa[ii].y, fa[ii].z, fa[ii].w};
+            if constexpr (F16) {
+                const f16x2_t one = __builtin_bit_cast(f16x2_t, 0x3c003c00u);
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    dbacc[ii] = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, w[q]), one, dbacc[ii], false);
+                return;
+            }
+            const bf16x2_t one = __builtin_bit_cast(bf16x2_t, 0x3f803f80u);
 #pragma unroll
             for (int q = 0; q < 4; ++q)
                 dbacc[ii] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w[q]), one, dbacc[ii], false);
@@ -571,7 +592,7 @@ __global__ __launch_bounds__(64 * NW, 1) void dw_gemm_v2_kernel(DwArgs a) {
     // the MFMAs of fragment row ii
     auto mma_row = [&](const uint4* fa, const uint4* fb, int ii) {
 #pragma unroll
-        for (int jj = 0; jj < TNW; ++jj) acc[ii][jj] = mfma_bf16(fa[ii], fb[jj], acc[ii][jj]);
+        for (int jj = 0; jj < TNW; ++jj) acc[ii][jj] = mfma_16bit<F16>(fa[ii], fb[jj], acc[ii][jj]);
     };
     auto mma = [&](const uint4* fa, const uint4* fb) {
 #pragma unroll
@@ -674,7 +695,7 @@ __global__ __launch_bounds__(64 * NW, 1) void dw_gemm_v2_kernel(DwArgs a) {
 #pragma unroll
                 for (int v = 0; v < 16; ++v) {
                     const uint32_t o = off + (uint32_t)(i * 32 + 8 * (v >> 2) + (v & 3)) * rowb;
-                    __builtin_amdgcn_raw_buffer_store_b16(to_bf16(acc[i][j][v]), rp, o, 0, 0);
+                    __builtin_amdgcn_raw_buffer_store_b16(F16 ? to_f16(acc[i][j][v]) : to_bf16(acc[i][j][v]), rp, o, 0, 0);
                 }
         }
     } else if constexpr (RAG) {
@@ -735,7 +756,7 @@ __device__ __forceinline__ void add4(float4& s, const float4& p) {
     s.w += p.w;
 }
 
-template <int SUB>
+template <int SUB, bool F16>
 __global__ __launch_bounds__(256) void dw_reduce_kernel(const float* __restrict__ partial, int splits, int64_t MN,
                                                         float* __restrict__ out32, uint16_t* __restrict__ out16,
                                                         const float* __restrict__ dbp, int64_t M,
@@ -770,7 +791,13 @@ __global__ __launch_bounds__(256) void dw_reduce_kernel(const float* __restrict_
     }
     if (i < MN && j == 0) {
         if (out32) *(float4*)(out32 + i) = s;
-        if (out16) *(uint2*)(out16 + i) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
+        if (out16) {
+            if constexpr (F16)
+                *(uint2*)(out16 + i) = make_uint2((uint32_t)to_f16(s.x) | ((uint32_t)to_f16(s.y) << 16),
+                                                  (uint32_t)to_f16(s.z) | ((uint32_t)to_f16(s.w) << 16));
+            else
+                *(uint2*)(out16 + i) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
+        }
     }
     if (db && t < M) {
         float d = splits > 0 ? dbp[t] : 0.0f;
@@ -790,11 +817,15 @@ __global__ __launch_bounds__(256) void dw_reduce_kernel(const float* __restrict_
 
 // one launch of the reduce: SUB lanes per output for a wide split count (more loads in flight)
 void launch_dw_reduce(const float* partial, int used, int64_t MN, float* out32, uint16_t* out16, const float* dbp,
-                      int64_t M, float* db, hipStream_t st) {
+                      int64_t M, float* db, bool f16, hipStream_t st) {
     const int sub = used > 16 ? 8 : used > 8 ? 4 : used > 4 ? 2 : 1;
     const int64_t threads = std::max<int64_t>(MN / 4 * sub, M);
     const dim3 grid((unsigned)((threads + 255) / 256));
-#define DOPT_RED(S_) hipLaunchKernelGGL(dw_reduce_kernel<S_>, grid, dim3(256), 0, st, partial, used, MN, out32, out16, dbp, M, db)
+#define DOPT_RED(S_)                                                                                                          \
+    do {                                                                                                                      \
+        if (f16) hipLaunchKernelGGL((dw_reduce_kernel<S_, true>), grid, dim3(256), 0, st, partial, used, MN, out32, out16, dbp, M, db); \
+        else hipLaunchKernelGGL((dw_reduce_kernel<S_, false>), grid, dim3(256), 0, st, partial, used, MN, out32, out16, dbp, M, db);   \
+    } while (0)
     if (sub == 8) DOPT_RED(8);
     else if (sub == 4) DOPT_RED(4);
     else if (sub == 2) DOPT_RED(2);
@@ -860,7 +891,7 @@ int launch_dw_gemm(DwArgs a, int mode, bool with_db, float* out32, uint16_t* out
     // (the pipelined kernel keeps a slab's lane offsets in 32 bits: 32 rows of either operand
     // must span less than 4 GiB)
     const bool v2_offsets = a.ldd < ((int64_t)1 << 26) && a.ldx < ((int64_t)1 << 26) && a.N < ((int64_t)1 << 26);
-    const bool ragged = a.K % V2_BK != 0 || a.M % BM != 0 || a.N % BN != 0;
+    const bool ragged = a.f16 || a.K % V2_BK != 0 || a.M % BM != 0 || a.N % BN != 0;
     // (the ragged instances keep 32 rows of either operand and 256 rows of the partial matrix in a buffer
     // resource's 31-bit range)
     const bool v2_ragged = mode == DW_B_BF16 && a.ldd < ((int64_t)1 << 24) && a.ldx < ((int64_t)1 << 24) &&
@@ -875,9 +906,9 @@ int launch_dw_gemm(DwArgs a, int mode, bool with_db, float* out32, uint16_t* out
     a.out16 = out16;
     const auto reduce = [&](int used) {
         if (!direct)
-            launch_dw_reduce(a.partial, used, a.M * a.N, out32, out16, a.db_partial, a.M, with_db ? db : nullptr, st);
+            launch_dw_reduce(a.partial, used, a.M * a.N, out32, out16, a.db_partial, a.M, with_db ? db : nullptr, a.f16, st);
         else if (out32 && out16)
-            launch_dw_reduce(out32, used, a.M * a.N, nullptr, out16, nullptr, a.M, nullptr, st);
+            launch_dw_reduce(out32, used, a.M * a.N, nullptr, out16, nullptr, a.M, nullptr, a.f16, st);
     };
     if (v2) {
         // the transpose-free kernel: 32-token tiles, split at the same token boundaries as the
@@ -915,20 +946,39 @@ int launch_dw_gemm(DwArgs a, int mode, bool with_db, float* out32, uint16_t* out
         else if (bmt == 128) DOPT_DW2T(0, 128, 256, false, O16_);        \
         else DOPT_DW2T(0, 256, 256, false, O16_);                        \
     } while (0)
-        if (mode == DW_B_BF16 && o16) DOPT_DW2B(true);
+// fp16 operands: the ragged instances
+#define DOPT_DW2H(BMT_, BNT_, O16_)                                                                                        \
+    do {                                                                                                                   \
+        if (with_db)                                                                                                       \
+            hipLaunchKernelGGL((dw_gemm_v2_kernel<0, true, 4, BMT_, BNT_, true, O16_, true>), grid, dim3(256), 0, st, a);   \
+        else                                                                                                               \
+            hipLaunchKernelGGL((dw_gemm_v2_kernel<0, false, 4, BMT_, BNT_, true, O16_, true>), grid, dim3(256), 0, st, a);  \
+    } while (0)
+        if (a.f16) {
+            if (o16) {
+                if (bmt == 256) DOPT_DW2H(256, 256, true);
+                else if (bnt == 256) DOPT_DW2H(128, 256, true);
+                else DOPT_DW2H(128, 128, true);
+            } else {
+                if (bmt == 256) DOPT_DW2H(256, 256, false);
+                else if (bnt == 256) DOPT_DW2H(128, 256, false);
+                else DOPT_DW2H(128, 128, false);
+            }
+        } else if (mode == DW_B_BF16 && o16) DOPT_DW2B(true);
         else if (mode == DW_B_BF16) DOPT_DW2B(false);
         else if (a.bits == 1) DOPT_DW2(1);
         else if (a.bits == 2) DOPT_DW2(2);
         else DOPT_DW2(4);
 #undef DOPT_DW2B
+#undef DOPT_DW2H
 #undef DOPT_DW2
 #undef DOPT_DW2T
         reduce(used);
         return 0;
     }
-    if (a.M % BM != 0 || a.N % BN != 0) {
+    if (a.f16 || a.M % BM != 0 || a.N % BN != 0) {
         if (a.K > 0) return -1;  // outside the ragged instances' offsets
-        launch_dw_reduce(a.partial, 0, a.M * a.N, out32, out16, a.partial, a.M, with_db ? db : nullptr, st);
+        launch_dw_reduce(a.partial, 0, a.M * a.N, out32, out16, a.partial, a.M, with_db ? db : nullptr, a.f16, st);
         return 0;
     }
     const int64_t kts = (a.K + BK - 1) / BK;

@@ -1,0 +1,220 @@
+// Layer norm backward. With xh = (x - mean) rstd and g = dy w, a row's input gradient is
+//   dx = rstd (g - avg(g) - xh avg(g xh)) [+ dresidual]
+// and the parameters' are sums over the rows, dweight = sum dy xh, dbias = sum dy.
+//
+// One read of dy, x (and dresidual) and one write of dx: a row lies in registers as in the forward kernel, both
+// averages come out of one exchange, and each lane adds its columns of dy xh and dy over the rows it takes, in fp32.
+// A workgroup's lanes of equal columns then meet in LDS, each workgroup writes one partial row of both sums, and
+// ln_param_kernel adds those rows: everything in an order that the sizes alone fix (no atomics). The grid is one
+// workgroup of 16 waves per CU, so that the partial rows are few (256 of 2 dim floats).
+#include <algorithm>
+
+#include "layer_norm.h"
+
+namespace dopt {
+namespace {
+
+constexpr int LNB_THREADS = 1024, LNB_GROUPS = 256;
+
+template <int DTX, int DTY, int TPR, int ACC>
+__global__ __launch_bounds__(LNB_THREADS) void ln_bwd_kernel(LnBwdArgs p) {
+    constexpr int RPW = LNB_THREADS / TPR;  // rows at a time
+    __shared__ float red[TPR > 64 ? 2 * LNB_THREADS / 64 : 1];
+    __shared__ __attribute__((aligned(16))) float meet[RPW > 1 ? RPW / 2 * TPR * ACC * 4 : 4];
+    const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, dim = p.dim;
+    const float inv = 1.0f / (float)dim;
+    LnCol col[ACC];
+    float w[ACC][4], dw[ACC][4] = {}, db[ACC][4] = {};
+#pragma unroll
+    for (int a = 0; a < ACC; ++a) {
+        col[a] = ln_col<TPR>(a, t, dim);
+        load_param4(p.weight, p.param_dt, col[a].at, 1.0f, w[a]);
+    }
+    const int64_t last = p.rows - 1;
+    // (the same trip count for every lane of the workgroup; a row past the end is computed as the last one, neither
+    // stored nor added)
+    for (int64_t base = (int64_t)blockIdx.x * RPW; base < p.rows; base += (int64_t)gridDim.x * RPW) {
+        const bool live = base + sub <= last;
+        const int64_t row = live ? base + sub : last;
+        Raw4<DTX> rx[ACC], rr[ACC];
+        Raw4<DTY> ry[ACC];
+#pragma unroll
+        for (int a = 0; a < ACC; ++a) {
+            ry[a] = load4<DTY>(p.dy, row * dim + col[a].at);
+            rx[a] = load4<DTX>(p.x, row * dim + col[a].at);
+        }
+        if (p.dres) {
+#pragma unroll
+            for (int a = 0; a < ACC; ++a) rr[a] = load4<DTX>(p.dres, row * dim + col[a].at);
+        }
+        const float mean = p.mean[row], rstd = p.rstd[row];
+        float xh[ACC][4], g[ACC][4], s[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int a = 0; a < ACC; ++a) {
+            widen4<DTX>(rx[a], xh[a]);
+            widen4<DTY>(ry[a], g[a]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                xh[a][e] = (xh[a][e] - mean) * rstd;
+                if (live) {
+                    dw[a][e] = __builtin_fmaf(g[a][e], xh[a][e], dw[a][e]);
+                    db[a][e] += g[a][e];
+                }
+                g[a][e] *= w[a][e];
+                const float q = e >= col[a].first ? g[a][e] : 0.0f;
+                s[0] += q;
+                s[1] = __builtin_fmaf(q, e >= col[a].first ? xh[a][e] : 0.0f, s[1]);
+            }
+        }
+        row_sums<TPR, 2>(s, red);
+        if (!live) continue;
+        const float c0 = s[0] * inv, c1 = s[1] * inv;
+#pragma unroll
+        for (int a = 0; a < ACC; ++a) {
+            if (col[a].first == 4) continue;
+            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (p.dres) widen4<DTX>(rr[a], d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[e] = __builtin_fmaf(rstd, g[a][e] - c0 - xh[a][e] * c1, d[e]);
+            store4<DTX>(p.dx, row * dim + col[a].at, d);
+        }
+    }
+    if (!p.partial) return;
+    // the RPW lanes of equal columns, by halves
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+        float(*v)[4] = part ? db : dw;
+#pragma unroll
+        for (int h = RPW / 2; h > 0; h >>= 1) {
+            __syncthreads();
+            if (sub >= h && sub < 2 * h) {
+#pragma unroll
+                for (int a = 0; a < ACC; ++a)
+                    *(float4*)(meet + (((sub - h) * ACC + a) * TPR + t) * 4) = make_float4(v[a][0], v[a][1], v[a][2], v[a][3]);
+            }
+            __syncthreads();
+            if (sub < h) {
+#pragma unroll
+                for (int a = 0; a < ACC; ++a) {
+                    const float4 o = *(const float4*)(meet + ((sub * ACC + a) * TPR + t) * 4);
+                    v[a][0] += o.x;
+                    v[a][1] += o.y;
+                    v[a][2] += o.z;
+                    v[a][3] += o.w;
+                }
+            }
+        }
+        if (sub == 0) {
+            float* out = p.partial + ((int64_t)blockIdx.x * 2 + part) * dim;
+#pragma unroll
+            for (int a = 0; a < ACC; ++a)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (e >= col[a].first) out[col[a].at + e] = v[a][e];
+        }
+    }
+}
+
+// any width: a workgroup for each row at a time; its partial sums lie in its own row of `partial`, each element
+// read and written by one lane only
+__global__ __launch_bounds__(LNB_THREADS) void ln_bwd_any_kernel(LnBwdArgs p, int x_dt, int dy_dt) {
+    __shared__ float red[2 * LNB_THREADS / 64];
+    const float inv = 1.0f / (float)p.dim;
+    float* pw = p.partial ? p.partial + (int64_t)blockIdx.x * 2 * p.dim : nullptr;
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const int64_t at = row * p.dim;
+        const float mean = p.mean[row], rstd = p.rstd[row];
+        float s[2] = {0.0f, 0.0f};
+        for (int i = threadIdx.x; i < p.dim; i += LNB_THREADS) {
+            const float d = load1(p.dy, dy_dt, at + i), xh = (load1(p.x, x_dt, at + i) - mean) * rstd;
+            const float g = p.weight ? d * load1(p.weight, p.param_dt, i) : d;
+            s[0] += g;
+            s[1] = __builtin_fmaf(g, xh, s[1]);
+            if (pw) {
+                const bool first = row == blockIdx.x;
+                pw[i] = __builtin_fmaf(d, xh, first ? 0.0f : pw[i]);
+                pw[p.dim + i] = d + (first ? 0.0f : pw[p.dim + i]);
+            }
+        }
+        row_sums<LNB_THREADS, 2>(s, red);
+        const float c0 = s[0] * inv, c1 = s[1] * inv;
+        for (int i = threadIdx.x; i < p.dim; i += LNB_THREADS) {
+            const float d = load1(p.dy, dy_dt, at + i), xh = (load1(p.x, x_dt, at + i) - mean) * rstd;
+            const float g = p.weight ? d * load1(p.weight, p.param_dt, i) : d;
+            const float r = p.dres ? load1(p.dres, x_dt, at + i) : 0.0f;
+            store1(p.dx, x_dt, at + i, __builtin_fmaf(rstd, g - c0 - xh * c1, r));
+        }
+    }
+}
+
+// dweight and dbias: the sums of the partial rows. A workgroup takes 64 columns of [2][dim]; its 16 waves take
+// every 16th row, and the wave sums are added in order.
+__global__ __launch_bounds__(1024) void ln_param_kernel(const float* partial, int groups, int dim, float* dweight, float* dbias) {
+    __shared__ float part[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t c = (int64_t)blockIdx.x * 64 + lane, n = 2 * (int64_t)dim;
+    float s = 0.0f;
+    if (c < n) {
+#pragma unroll 8
+        for (int g = wave; g < groups; g += 16) s += partial[g * n + c];
+    }
+    part[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && c < n) {
+#pragma unroll
+        for (int k = 1; k < 16; ++k) s += part[k][lane];
+        float* out = c < dim ? dweight : dbias;
+        if (out) out[c < dim ? c : c - dim] = s;
+    }
+}
+
+// widths past this (and under 4) go through ln_bwd_any_kernel: with 3 accesses a lane over 1024 lanes the row, its
+// columns' sums and the weight no longer fit the 128 registers that 16 waves a CU leave (26 spilled)
+constexpr int LNB_MAX_DIM = 8192;
+
+int rows_at_a_time(int dim) { return dim < 4 ? 1 : dim <= 768 ? 16 : dim <= 3072 ? 4 : 1; }
+
+template <int DTX, int DTY>
+void pick(const LnBwdArgs& a, int64_t groups, hipStream_t s) {
+    const int d = a.dim;
+    const dim3 g((uint32_t)groups), b(LNB_THREADS);
+    if (d <= 256) hipLaunchKernelGGL((ln_bwd_kernel<DTX, DTY, 64, 1>), g, b, 0, s, a);
+    else if (d <= 512) hipLaunchKernelGGL((ln_bwd_kernel<DTX, DTY, 64, 2>), g, b, 0, s, a);
+    else if (d <= 768) hipLaunchKernelGGL((ln_bwd_kernel<DTX, DTY, 64, 3>), g, b, 0, s, a);
+    else if (d <= 1024) hipLaunchKernelGGL((ln_bwd_kernel<DTX, DTY, 256, 1>), g, b, 0, s, a);
+    else if (d <= 2048) hipLaunchKernelGGL((ln_bwd_kernel<DTX, DTY, 256, 2>), g, b, 0, s, a);
+    else if (d <= 3072) hipLaunchKernelGGL((ln_bwd_kernel<DTX, DTY, 256, 3>), g, b, 0, s, a);
+    else if (d <= 4096) hipLaunchKernelGGL((ln_bwd_kernel<DTX, DTY, 1024, 1>), g, b, 0, s, a);
+    else hipLaunchKernelGGL((ln_bwd_kernel<DTX, DTY, 1024, 2>), g, b, 0, s, a);
+}
+
+template <int DTX>
+void pick_dy(const LnBwdArgs& a, int dy_dt, int64_t groups, hipStream_t s) {
+    if (dy_dt == DT_F32) pick<DTX, DT_F32>(a, groups, s);
+    else if (dy_dt == DT_F16) pick<DTX, DT_F16>(a, groups, s);
+    else pick<DTX, DT_BF16>(a, groups, s);
+}
+
+}  // namespace
+
+int64_t layer_norm_groups(int64_t rows, int dim) {
+    const int64_t r = rows_at_a_time(dim);
+    return std::min<int64_t>((rows + r - 1) / r, LNB_GROUPS);
+}
+
+int launch_layer_norm_bwd(const LnBwdArgs& a, int x_dt, int dy_dt, float* dweight, float* dbias, hipStream_t s) {
+    const int64_t groups = layer_norm_groups(a.rows, a.dim);
+    if (groups > 0) {
+        if (a.dim < 4 || a.dim > LNB_MAX_DIM)
+            hipLaunchKernelGGL(ln_bwd_any_kernel, dim3((uint32_t)groups), dim3(LNB_THREADS), 0, s, a, x_dt, dy_dt);
+        else if (x_dt == DT_F32) pick_dy<DT_F32>(a, dy_dt, groups, s);
+        else if (x_dt == DT_F16) pick_dy<DT_F16>(a, dy_dt, groups, s);
+        else pick_dy<DT_BF16>(a, dy_dt, groups, s);
+    }
+    if (dweight || dbias)  // (no rows: zeros)
+        hipLaunchKernelGGL(ln_param_kernel, dim3((uint32_t)((2 * (int64_t)a.dim + 63) / 64)), dim3(1024), 0, s, a.partial,
+                           (int)groups, a.dim, dweight, dbias);
+    return 0;
+}
+
+}  // namespace dopt

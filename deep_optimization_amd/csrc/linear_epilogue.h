@@ -1,0 +1,167 @@
+// What is fused into a Linear layer's products: bias, activation and residual of the forward product, the derivative of
+// the activation that feeds the layer in the input gradient's. All in fp32, each result rounded once.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "layer_norm.h"
+
+namespace dopt {
+
+enum { LIN_NONE = 0, LIN_RELU = 1, LIN_GELU = 2, LIN_GELU_TANH = 3, LIN_SILU = 4 };
+
+struct LinArgs {
+    const uint16_t *A, *B;     // A [M][lda]; B [N][ldb] (NT) or [K][ldb] (KN)
+    int64_t M, N, K, lda, ldb;  // K: of the sum
+    uint32_t tiles_m, tiles_n;  // set by the launcher
+    // the rest: [M][N] rows without padding, or null
+    const void* bias;     // [N], of dtype bias_dt
+    const void* res;      // of y's type
+    const uint16_t* aux;  // KN: the argument of the activation whose derivative multiplies the result
+    void* y;
+    uint16_t* pre;        // the activation's argument
+    int bias_dt, act, y_f32;
+};
+
+// GELU through the normal distribution's upper tail: with a = |z| and Q(a) = 1 - Phi(a),
+//   gelu(z) = max(z, 0) - a Q(a),  Q(a) = t P(t) e^{-a^2 / 2} / 2,  t = 1 / (1 + c a)
+// (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26, whose erf is within 1.5e-7: nothing cancels
+// on either side). a stops at 30, where Q is 0 in fp32, so that a Q is 0 and not inf * 0 for an infinite z; the
+// z * 0 of the other side keeps NaN.
+struct GeluParts {
+    float a, q, e;  // |z|, Q(a), e^{-a^2 / 2}
+};
+__device__ __forceinline__ GeluParts gelu_parts(float z) {
+    const float a = fminf(fabsf(z), 30.0f);
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(a, 0.3275911f * 0.70710678118654752f, 1.0f));
+    float s = __builtin_fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
+    s = __builtin_fmaf(s, t, 0.5f * 1.421413741f);
+    s = __builtin_fmaf(s, t, 0.5f * -0.284496736f);
+    s = __builtin_fmaf(s, t, 0.5f * 0.254829592f);
+    const float e = __builtin_amdgcn_exp2f(a * a * -0.72134752044448170f);  // -log2(e) / 2
+    return GeluParts{a, s * t * e, e};
+}
+__device__ __forceinline__ float gelu_erf(float z) {
+    const GeluParts g = gelu_parts(z);
+    const float pos = z > 0.0f ? z : z * 0.0f;
+    return __builtin_fmaf(-g.a, g.q, pos);
+}
+// Phi(z) + z phi(z)
+__device__ __forceinline__ float gelu_erf_grad(float z) {
+    const GeluParts g = gelu_parts(z);
+    const float phi = z > 0.0f ? 1.0f - g.q : g.q + z * 0.0f;
+    return __builtin_fmaf(__builtin_copysignf(g.a, z), 0.39894228040143268f * g.e, phi);
+}
+
+__device__ __forceinline__ void lin_act8(int act, float* v) {
+    if (act == LIN_NONE) return;
+    if (act == LIN_GELU) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = gelu_erf(v[e]);
+    } else if (act == LIN_RELU) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = v[e] < 0.0f ? 0.0f : v[e];  // (NaN stays)
+    } else if (act == LIN_SILU) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= fast_sigmoid(v[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float d;
+            gelu_and_grad(v[e], v[e], d);
+        }
+    }
+}
+// v[e] *= act'(z[e])
+__device__ __forceinline__ void lin_act_grad8(int act, const float* z, float* v) {
+    if (act == LIN_NONE) return;
+    if (act == LIN_GELU) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= gelu_erf_grad(z[e]);
+    } else if (act == LIN_RELU) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = z[e] > 0.0f ? v[e] : 0.0f;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float y, d;
+            if (act == LIN_SILU) silu_and_grad(z[e], y, d);
+            else gelu_and_grad(z[e], y, d);
+            v[e] *= d;
+        }
+    }
+}
+
+// 8 elements of a row from element i on, of which the first `have` (1..8) exist
+template <int DT>
+__device__ __forceinline__ void lin_load8(const void* p, int64_t i, int have, float* f) {
+    if (have == 8) {
+        widen4<DT>(load4<DT>(p, i), f);
+        widen4<DT>(load4<DT>(p, i + 4), f + 4);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = e < have ? load1(p, DT, i + e) : 0.0f;
+    }
+}
+template <int DT>
+__device__ __forceinline__ void lin_store8(void* p, int64_t i, int have, const float* f) {
+    if (have == 8) {
+        if constexpr (DT == DT_F32) {
+            store4<DT>(p, i, f);
+            store4<DT>(p, i + 4, f + 4);
+        } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                w[k] = DT == DT_BF16 ? pack_bf16x2(f[2 * k], f[2 * k + 1]) : pack_f16x2(f[2 * k], f[2 * k + 1]);
+            __builtin_memcpy((uint16_t*)p + i, w, 16);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < have) store1(p, DT, i + e, f[e]);
+    }
+}
+
+__device__ __forceinline__ void lin_bias8(const LinArgs& p, int64_t n, float* b) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) b[e] = 0.0f;
+    if (!p.bias || n >= p.N) return;
+    const int have = (int)min((int64_t)8, p.N - n);
+    if (p.bias_dt == DT_F32) lin_load8<DT_F32>(p.bias, n, have, b);
+    else if (p.bias_dt == DT_BF16) lin_load8<DT_BF16>(p.bias, n, have, b);
+    else lin_load8<DT_F16>(p.bias, n, have, b);
+}
+
+// row m, columns n .. n + 7 (those below N) of the result from the sums v
+template <bool KN, bool F16>
+__device__ __forceinline__ void lin_finish8(const LinArgs& p, int64_t m, int64_t n, const float* bias, float* v) {
+    constexpr int DT = F16 ? DT_F16 : DT_BF16;
+    const int64_t i = m * p.N + n;
+    const int have = (int)min((int64_t)8, p.N - n);
+    if constexpr (KN) {
+        if (p.act != LIN_NONE) {
+            float z[8];
+            lin_load8<DT>(p.aux, i, have, z);
+            lin_act_grad8(p.act, z, v);
+        }
+        lin_store8<DT>(p.y, i, have, v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += bias[e];
+        if (p.pre) lin_store8<DT>(p.pre, i, have, v);
+        lin_act8(p.act, v);
+        if (p.res) {
+            float r[8];
+            if (p.y_f32) lin_load8<DT_F32>(p.res, i, have, r);
+            else lin_load8<DT>(p.res, i, have, r);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += r[e];
+        }
+        if (p.y_f32) lin_store8<DT_F32>(p.y, i, have, v);
+        else lin_store8<DT>(p.y, i, have, v);
+    }
+}
+
+}  // namespace dopt

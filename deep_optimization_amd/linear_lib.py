@@ -1,0 +1,183 @@
+"""The Linear layer's products with bias, activation and residual in their epilogue: ``torch.ops.act_lib.linear_act_fwd`` /
+``linear_act_bwd`` on the gfx950 MFMA kernels behind dopt_linear_forward, dopt_linear_input_grad and
+dopt_linear_weight_grad. No counterparts in the reference, whose Linear layers call F.linear
+(Activation_Compression/modules/ops.py:481) and whose activations are separate modules.
+
+    linear_act_fwd(x, weight, bias, residual, act, save_pre) -> (y, pre)
+        z = x weight^T + bias;  y = act(z) + residual;  pre = z (None unless save_pre)
+    linear_act_bwd(dy, x, weight, pre, act, in_pre, in_act, input_grad, weight_grad, bias_grad, grad_dtype)
+            -> (dx, dweight, dbias)
+        dz = dy act'(pre);  dx = (dz weight) in_act'(in_pre);  dweight = dz^T x;  dbias = sum of dz over the rows
+
+x [..., K] and weight [N, K] in bf16 or fp16 (fp32 sums, fp32 epilogue, each result rounded once), ``act`` one of "none",
+"relu", "gelu" (the exact one), "gelu_tanh", "silu". bias [N] in bf16, fp16 or fp32; residual [..., N] in x's type or fp32,
+y in residual's type (x's without one). pre [..., N] in x's type.
+
+Backward: dy and pre [..., N] in x's type. With ``in_act`` other than "none", x is in_act(in_pre), the output of the
+activation that feeds the layer, and dx is the gradient of in_pre [..., K]: an MLP's second layer hands its first one the
+gradient of the pre-activation in one pass. dz is rounded to x's type for the products (both read it on matrix
+instructions of that type). dweight and dbias come in ``grad_dtype`` (float32 or x's type; both are summed in fp32);
+what is not asked for is None, and bias_grad alone still runs the weight gradient's product, which sums dz on its way.
+
+Rows of x may be strided (x[:, 0] of a [B, T, K] tensor) where the stride is a multiple of 8 elements and the rows start
+at 16 bytes; other layouts, and operands whose K (N) is no multiple of 8, are copied into aligned rows first.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch import Tensor
+
+from . import _lib
+from .act_lib import _DTYPE_CODE, _op, _require_cuda, _stream
+
+_TYPES = (torch.bfloat16, torch.float16)
+
+
+def _act_code(act: str) -> int:
+    try:
+        return _lib.LIN_ACTS[act]
+    except KeyError:
+        raise ValueError(f"act must be one of {', '.join(_lib.LIN_ACTS)}, got {act!r}") from None
+
+
+def _pad8(n: int) -> int:
+    return (n + 7) // 8 * 8
+
+
+def _rows(t: Tensor, cols: int):
+    """t [..., cols] as (tensor, row stride): rows at 16-byte aligned addresses that hold whole 8-element chunks, zero
+    past ``cols``."""
+    t2 = t.reshape(-1, cols) if t.dim() != 2 else t
+    if cols % 8 == 0 and t2.stride(1) == 1 and cols <= t2.stride(0) < 1 << 21 and t2.stride(0) % 8 == 0 and t2.data_ptr() % 16 == 0:
+        return t2, int(t2.stride(0))
+    t2 = t2.contiguous()
+    if cols % 8 == 0 and t2.data_ptr() % 16 == 0:
+        return t2, cols
+    return _act_grad_rows(t2, None, "none"), _pad8(cols)
+
+
+def _act_grad_rows(dy: Tensor, pre: Optional[Tensor], act: str) -> Tensor:
+    """dy act'(pre) [rows, cols] in rows padded with zeros to a multiple of 8."""
+    rows, cols = dy.shape
+    out = torch.empty((rows, _pad8(cols)), dtype=dy.dtype, device=dy.device)
+    rc = _lib.lib().dopt_linear_act_grad(dy.data_ptr(), cols, None if pre is None else pre.data_ptr(), _act_code(act),
+                                         _DTYPE_CODE[dy.dtype], rows, cols, out.data_ptr(), out.shape[1], _stream(dy))
+    _lib.check(rc, "linear_act")
+    return out
+
+
+def _check_operands(what: str, x: Tensor, weight: Tensor):
+    """(rows, N, K)"""
+    if x.dtype not in _TYPES or weight.dtype != x.dtype or x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
+        raise RuntimeError(f"{what}: x [..., K] and weight [N, K] must both be bfloat16 or float16, got {tuple(x.shape)} {x.dtype} and "
+                           f"{tuple(weight.shape)} {weight.dtype}")
+    rows = 1
+    for n in x.shape[:-1]:
+        rows *= int(n)
+    return rows, int(weight.shape[0]), int(weight.shape[1])
+
+
+def _check_like(what: str, name: str, t: Tensor, shape, dtypes) -> None:
+    if tuple(t.shape) != tuple(shape) or t.dtype not in dtypes:
+        raise RuntimeError(f"{what}: {name} must be {tuple(shape)} in {' or '.join(str(d) for d in dtypes)}, got {tuple(t.shape)} {t.dtype}")
+
+
+def _linear_act_fwd(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Optional[Tensor], act: str, save_pre: bool):
+    what = "linear_act_fwd"
+    code = _act_code(act)
+    M, N, K = _check_operands(what, x, weight)
+    shape = (*x.shape[:-1], N)
+    if bias is not None:
+        _check_like(what, "bias", bias, (N,), tuple(_DTYPE_CODE))
+    if residual is not None:
+        _check_like(what, "residual", residual, shape, (x.dtype, torch.float32))
+    _require_cuda(x, weight, bias, residual)
+    a, lda = _rows(x, K) if M and K else (x, _pad8(K))
+    b, ldb = _rows(weight, K) if N and K else (weight, _pad8(K))
+    bias = None if bias is None else bias.contiguous()
+    residual = None if residual is None else residual.contiguous()
+    y = torch.empty(shape, dtype=x.dtype if residual is None else residual.dtype, device=x.device)
+    pre = torch.empty(shape, dtype=x.dtype, device=x.device) if save_pre else None
+    rc = _lib.lib().dopt_linear_forward(
+        a.data_ptr(), lda, b.data_ptr(), ldb, _DTYPE_CODE[x.dtype], M, N, K, None if bias is None else bias.data_ptr(),
+        _lib.F32 if bias is None else _DTYPE_CODE[bias.dtype], None if residual is None else residual.data_ptr(), code,
+        y.data_ptr(), _DTYPE_CODE[y.dtype], None if pre is None else pre.data_ptr(), _stream(x))
+    _lib.check(rc, what)
+    return y, pre
+
+
+def _linear_act_fwd_fake(x, weight, bias, residual, act, save_pre):
+    shape = (*x.shape[:-1], weight.shape[0])
+    return x.new_empty(shape, dtype=x.dtype if residual is None else residual.dtype), (x.new_empty(shape) if save_pre else None)
+
+
+linear_act_fwd = _op(
+    "linear_act_fwd(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, str act, bool save_pre) -> (Tensor, Tensor?)",
+    _linear_act_fwd, _linear_act_fwd_fake)
+
+
+def _linear_act_bwd(dy: Tensor, x: Tensor, weight: Tensor, pre: Optional[Tensor], act: str, in_pre: Optional[Tensor], in_act: str,
+                    input_grad: bool, weight_grad: bool, bias_grad: bool, grad_dtype: torch.dtype):
+    what = "linear_act_bwd"
+    code, in_code = _act_code(act), _act_code(in_act)
+    M, N, K = _check_operands(what, x, weight)
+    _check_like(what, "dy", dy, (*x.shape[:-1], N), (x.dtype,))
+    if grad_dtype not in (torch.float32, x.dtype):
+        raise RuntimeError(f"{what}: grad_dtype must be float32 or x's type, got {grad_dtype}")
+    if (code != 0) != (pre is not None):
+        raise RuntimeError(f"{what}: pre goes with an activation (act {act!r}, pre {'given' if pre is not None else 'missing'})")
+    if (in_code != 0) != (in_pre is not None):
+        raise RuntimeError(f"{what}: in_pre goes with in_act (in_act {in_act!r}, in_pre {'given' if in_pre is not None else 'missing'})")
+    if pre is not None:
+        _check_like(what, "pre", pre, dy.shape, (x.dtype,))
+    if in_pre is not None:
+        _check_like(what, "in_pre", in_pre, x.shape, (x.dtype,))
+    _require_cuda(dy, x, weight, pre, in_pre)
+    L, dt, stream = _lib.lib(), _DTYPE_CODE[x.dtype], _stream(x)
+    if M and N:
+        if code:
+            dz = _act_grad_rows(dy.contiguous().view(M, N), pre.contiguous(), act)
+            ldz = _pad8(N)
+        else:
+            dz, ldz = _rows(dy, N)
+    else:
+        dz, ldz = dy, _pad8(N)
+    dx = dw = db = None
+    if input_grad:
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        in_pre = None if in_pre is None else in_pre.contiguous()
+        w, ldw = _rows(weight, K) if N and K else (weight, _pad8(K))
+        rc = L.dopt_linear_input_grad(dz.data_ptr(), ldz, w.data_ptr(), ldw, dt, M, N, K, None if in_pre is None else in_pre.data_ptr(),
+                                      in_code, dx.data_ptr(), stream)
+        _lib.check(rc, what)
+    if weight_grad or bias_grad:
+        if N == 0 or K == 0:
+            dw = torch.empty((N, K), dtype=grad_dtype, device=x.device)
+            db = dz.reshape(M, dz.shape[-1])[:, :N].float().sum(0)
+        else:
+            xr, ldx = _rows(x, K) if M else (x, _pad8(K))
+            K8 = _pad8(K)
+            ws = torch.empty(max(int(L.dopt_linear_weight_grad_workspace_floats(M, N, K8)), 4), dtype=torch.float32, device=x.device)
+            dw = torch.empty((N, K8), dtype=grad_dtype, device=x.device)
+            db = torch.empty(N, dtype=torch.float32, device=x.device) if bias_grad else None
+            f32 = grad_dtype == torch.float32
+            rc = L.dopt_linear_weight_grad(dz.data_ptr(), ldz, xr.data_ptr(), ldx, dt, M, N, K8, ws.data_ptr(), dw.data_ptr() if f32 else None,
+                                           None if f32 else dw.data_ptr(), None if db is None else db.data_ptr(), stream)
+            _lib.check(rc, what)
+            if K8 != K:
+                dw = dw[:, :K].contiguous()
+    return dx, dw if weight_grad else None, db.to(grad_dtype) if bias_grad else None
+
+
+def _linear_act_bwd_fake(dy, x, weight, pre, act, in_pre, in_act, input_grad, weight_grad, bias_grad, grad_dtype):
+    return (x.new_empty(x.shape) if input_grad else None, weight.new_empty(weight.shape, dtype=grad_dtype) if weight_grad else None,
+            weight.new_empty((weight.shape[0],), dtype=grad_dtype) if bias_grad else None)
+
+
+linear_act_bwd = _op(
+    "linear_act_bwd(Tensor dy, Tensor x, Tensor weight, Tensor? pre, str act, Tensor? in_pre, str in_act, bool input_grad, "
+    "bool weight_grad, bool bias_grad, ScalarType grad_dtype) -> (Tensor?, Tensor?, Tensor?)", _linear_act_bwd, _linear_act_bwd_fake)
+
+__all__ = ["linear_act_fwd", "linear_act_bwd"]

@@ -436,6 +436,63 @@ int64_t dopt_dw_gemm_any_workspace_floats(int64_t M, int64_t N, int64_t K);
 int dopt_dw_gemm_any(const void* dy, int64_t ldd, const void* x_hat, int64_t ldx, int64_t M, int64_t N, int64_t K,
                      float* workspace, float* dw_f32, void* dw_bf16, float* db, void* stream);
 
+/* ---------------------------------------------------------------- transformer blocks
+ * Layer norm, dropout and the products of a Linear layer with what is around them. No counterparts in the reference,
+ * whose Transformer models leave all of these to torch. Rows are contiguous unless a stride is given; any base address
+ * that holds whole elements unless an alignment is asked for.
+ *
+ * Layer norm over the last axis of x [rows, dim] (fp32, fp16 or bf16; dim >= 1):
+ *   y = (x - mean) * rstd * weight + bias,  rstd = 1 / sqrt(biased variance + eps), in fp32, one rounding.
+ * weight, bias [dim] of param_dtype, either may be NULL (ones, zeros). mean, rstd: fp32 [rows].
+ * Backward, with xh = (x - mean) * rstd and g = dy * weight:
+ *   dx = rstd * (g - avg(g) - xh * avg(g * xh)) + dresidual,  dweight = sum dy * xh,  dbias = sum dy (over rows)
+ * dx and dresidual (NULL: none) are of x's type, dweight and dbias (fp32 [dim], either may be NULL) come from partial
+ * sums in `workspace` (dopt_layer_norm_workspace_floats floats; may be NULL without them) in a fixed order. */
+int dopt_layer_norm_forward(const void* x, int x_dtype, int64_t rows, int64_t dim, const void* weight, const void* bias,
+                            int param_dtype, float eps, void* y, int y_dtype, float* mean, float* rstd, void* stream);
+int64_t dopt_layer_norm_workspace_floats(int64_t rows, int64_t dim);
+int dopt_layer_norm_backward(const void* dy, int dy_dtype, const void* x, int x_dtype, int64_t rows, int64_t dim,
+                             const float* mean, const float* rstd, const void* weight, int param_dtype,
+                             const void* dresidual, void* dx, float* workspace, float* dweight, float* dbias, void* stream);
+
+/* y[i] = residual[i] + (kept(i) ? x[i] * scale : 0) for n elements; residual (NULL: none) is of y's type. kept(i):
+ * half-word i % 8 (little endian in the four output words) of Philox4x32-10 with counter {i / 8 (64 bit),
+ * offset + *step (64 bit)} and key seed is at least T = round(65536 p); scale = 65536 / (65536 - T). step: a device
+ * pointer or NULL (0), read by the kernel, so a captured graph can draw a new mask on each replay. The gradient of x is
+ * the same call on dy without a residual. 0 <= p <= 1, rounded to a multiple of 2^-16. */
+int dopt_dropout(const void* x, int x_dtype, const void* residual, int64_t n, double p, uint64_t seed, uint64_t offset,
+                 const int64_t* step, void* y, int y_dtype, void* stream);
+
+/* activations of the Linear layer's products */
+#define DOPT_LIN_NONE 0
+#define DOPT_LIN_RELU 1
+#define DOPT_LIN_GELU 2      /* z Phi(z) */
+#define DOPT_LIN_GELU_TANH 3 /* the tanh form */
+#define DOPT_LIN_SILU 4
+
+/* z = x weight^T + bias, y = act(z) + residual, pre = z: x [M, ldx], weight [N, ldw], both fp16 or bf16 (dtype), sums and
+ * epilogue in fp32, each result rounded once. bias [N] of bias_dtype, residual [M, N] of y's type, pre [M, N] of
+ * the operands' type; each may be NULL. y [M, N]: the operands' type or fp32. x and weight: 16-byte aligned, strides
+ * multiples of 8 (below 2^21) that are at least K rounded up to one; where K is not a multiple of 8 the elements up to
+ * that are read and must be zero. */
+int dopt_linear_forward(const void* x, int64_t ldx, const void* weight, int64_t ldw, int dtype, int64_t M, int64_t N,
+                        int64_t K, const void* bias, int bias_dtype, const void* residual, int act, void* y, int y_dtype,
+                        void* pre, void* stream);
+/* dx = (dz weight) * in_act'(in_pre): dz [M, ldz] (N columns, zeros up to a multiple of 8), weight [N, ldw] as in the
+ * forward call (K columns), dx and in_pre [M, K]. in_act DOPT_LIN_NONE: dx = dz weight, in_pre is not read. */
+int dopt_linear_input_grad(const void* dz, int64_t ldz, const void* weight, int64_t ldw, int dtype, int64_t M, int64_t N,
+                           int64_t K, const void* in_pre, int in_act, void* dx, void* stream);
+/* dz[r][c] = dy[r][c] * act'(pre[r][c]) for c < cols, 0 for the columns up to ld_dz (a multiple of 8, dz 16-byte
+ * aligned); pre [rows, cols]. With DOPT_LIN_NONE a copy into padded rows. */
+int dopt_linear_act_grad(const void* dy, int64_t ld_dy, const void* pre, int act, int dtype, int64_t rows, int64_t cols,
+                         void* dz, int64_t ld_dz, void* stream);
+/* dw = dz^T x (fp32 dw_f32 and / or dw_16 of the operands' type, [N, K]) and db = sum over rows of dz (fp32 [N], may be
+ * NULL): dopt_dw_gemm_any for fp16 or bf16 and any N; K a multiple of 8; the same alignment rules. workspace:
+ * dopt_linear_weight_grad_workspace_floats floats (not NULL). */
+int64_t dopt_linear_weight_grad_workspace_floats(int64_t M, int64_t N, int64_t K);
+int dopt_linear_weight_grad(const void* dz, int64_t ldz, const void* x, int64_t ldx, int dtype, int64_t M, int64_t N,
+                            int64_t K, float* workspace, float* dw_f32, void* dw_16, float* db, void* stream);
+
 /*
  * HIP graph tools for capturing a whole training step (forward, backward, optimizer step) as
  * Activation_Compression/cuda_graph_utils.py:82-120 (`Graph.capture_cuda_graph_qdrop`) does.

@@ -1,0 +1,192 @@
+"""act_lib::layer_norm_fwd / layer_norm_bwd against the formulas in 64 bits (tests/block_reference.py), within bounds from the
+sums' lengths and one rounding; the backward also against differences of the forward."""
+import pytest
+import torch
+
+import deep_optimization_amd  # noqa: F401
+from tests import block_reference as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+ops = torch.ops.act_lib
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+# every instance's widths (its largest, one past the smaller one's, odd ones), and those that go element by element
+WIDTHS = (1, 2, 3, 4, 5, 63, 64, 191, 256, 257, 511, 512, 591, 768, 769, 1000, 1024, 1025, 2048, 2305, 3071, 3072, 3073, 4096,
+          4097, 8192, 8193, 16383, 16384, 16385)
+
+
+def _rand(gen, shape, dtype, scale=1.0, shift=0.0):
+    return (torch.randn(shape, generator=gen, device=DEV) * scale + shift).to(dtype)
+
+
+def _check(shape, x_dt, y_dt, p_dt, seed, affine=True, dres=True, shift=0.5, eps=1e-6):
+    print(f"[layer norm] {shape} x {x_dt} y {y_dt} parameters {p_dt} affine {affine} dresidual {dres}", flush=True)
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    D = shape[-1]
+    x = _rand(gen, shape, x_dt, 1.5, shift)
+    w = _rand(gen, (D,), p_dt, 0.3, 1.0) if affine else None
+    b = _rand(gen, (D,), p_dt, 0.3) if affine else None
+    y, mean, rstd = ops.layer_norm_fwd(x, w, b, eps, y_dt)
+    wy, wmean, wrstd, tol, tmean, trstd = ref.layer_norm(x, w, b, eps)
+    assert y.dtype == y_dt and mean.dtype == rstd.dtype == F32 and mean.shape == x.shape[:-1]
+    ref.close(mean, wmean, tmean, "mean")
+    ref.close(rstd, wrstd, trstd, "rstd")
+    ref.close(y, wy, tol, "y")
+    dy = _rand(gen, shape, y_dt)
+    dr = _rand(gen, shape, x_dt) if dres else None
+    dx, dw, db = ops.layer_norm_bwd(dy, x, mean, rstd, w, dr, affine, affine)
+    wx, ww, wb, tx, tw, tb = ref.layer_norm_grads(dy, x, mean, rstd, w, dr)
+    assert dx.dtype == x_dt and dx.shape == x.shape
+    ref.close(dx, wx, tx, "dx")
+    if affine:
+        assert dw.dtype == db.dtype == F32
+        ref.close(dw, ww, tw, "dweight")
+        ref.close(db, wb, tb, "dbias")
+    else:
+        assert dw is None and db is None
+
+
+@pytest.mark.parametrize("dim", WIDTHS)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+def test_widths(dim, dtype):
+    _check((37, dim), dtype, dtype, F32, dim)
+
+
+@pytest.mark.parametrize("x_dt", [F32, F16, BF16], ids=["xf32", "xf16", "xbf16"])
+@pytest.mark.parametrize("y_dt", [F32, F16, BF16], ids=["yf32", "yf16", "ybf16"])
+@pytest.mark.parametrize("dim", [250, 500, 700, 900, 2000, 3000, 4000, 8000, 12000])
+def test_every_pair_of_types(x_dt, y_dt, dim):
+    """Every instance of both passes: the largest width but a few elements."""
+    for p_dt in (F32, F16, BF16) if dim == 700 else (BF16,):
+        _check((19, dim), x_dt, y_dt, p_dt, dim + 1)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 15, 16, 17, 4095, 4096, 4097, 20001])
+@pytest.mark.parametrize("dim", [64, 768, 1100])
+def test_rows(rows, dim):
+    _check((rows, dim), BF16, BF16, F32, rows, dres=rows % 2 == 0)
+
+
+@pytest.mark.parametrize("shape", [(768,), (3, 5, 197), (2, 1, 3, 64)])
+def test_shapes_of_any_rank(shape):
+    _check(shape, BF16, F32, F32, 3)
+
+
+def test_without_parameters_and_with_one():
+    _check((33, 300), F32, F32, F32, 4, affine=False)
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    x, w, b = _rand(gen, (9, 300), F32), _rand(gen, (300,), F32), _rand(gen, (300,), F32)
+    ref.close(ops.layer_norm_fwd(x, w, None, 1e-5, F32)[0], ref.layer_norm(x, w, None, 1e-5)[0], ref.layer_norm(x, w, None, 1e-5)[3])
+    y, mean, rstd = ops.layer_norm_fwd(x, None, b, 1e-5, F32)
+    ref.close(y, ref.layer_norm(x, None, b, 1e-5)[0], ref.layer_norm(x, None, b, 1e-5)[3])
+    dx, dw, db = ops.layer_norm_bwd(x, x, mean, rstd, None, None, False, True)
+    assert dw is None
+    ref.close(db, x.double().sum(0), 64 * ref.E * x.double().abs().sum(0))
+    dx2, dw2, db2 = ops.layer_norm_bwd(x, x, mean, rstd, None, None, True, False)
+    assert db2 is None and torch.equal(dx, dx2)
+
+
+def test_a_mean_far_from_zero_keeps_the_variance():
+    """mean 1000, deviation 1: sums of squares would lose it."""
+    _check((40, 768), F32, F32, F32, 6, shift=1000.0)
+
+
+def test_constant_rows():
+    x = torch.full((5, 768), 3.0, device=DEV)
+    y, mean, rstd = ops.layer_norm_fwd(x, None, None, 1e-6, F32)
+    assert torch.equal(y, torch.zeros_like(y)) and torch.equal(mean, torch.full((5,), 3.0, device=DEV))
+    assert torch.allclose(rstd, torch.full((5,), 1e3, device=DEV), rtol=1e-6, atol=0)
+
+
+def test_no_rows():
+    x = torch.empty((0, 768), device=DEV, dtype=BF16)
+    w = torch.ones(768, device=DEV)
+    y, mean, rstd = ops.layer_norm_fwd(x, w, w, 1e-6, BF16)
+    assert y.shape == (0, 768) and mean.shape == (0,)
+    dx, dw, db = ops.layer_norm_bwd(x, x, mean, rstd, w, None, True, True)
+    assert dx.shape == (0, 768) and not dw.any() and not db.any()
+
+
+@pytest.mark.parametrize("dim", [768, 20000])
+def test_nan_and_infinity_stay_in_their_row(dim):
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    x = _rand(gen, (21, dim), F32)
+    clean = ops.layer_norm_fwd(x, None, None, 1e-6, F32)[0]
+    bad = x.clone()
+    bad[3, 5], bad[7, dim - 1] = float("nan"), float("inf")
+    y = ops.layer_norm_fwd(bad, None, None, 1e-6, F32)[0]
+    rows = [r for r in range(21) if r not in (3, 7)]
+    assert torch.equal(y[rows], clean[rows]) and torch.isnan(y[3]).all() and torch.isnan(y[7]).any()
+
+
+def test_views_strides_and_odd_addresses():
+    gen = torch.Generator(device=DEV).manual_seed(9)
+    big = _rand(gen, (50, 800), BF16)
+    for x in (big[:, 7:775], big.t()[:300], big[::3, :640], big.reshape(-1)[1:1 + 40 * 591].view(40, 591)):
+        y, mean, rstd = ops.layer_norm_fwd(x, None, None, 1e-6, BF16)
+        y2, mean2, rstd2 = ops.layer_norm_fwd(x.contiguous().clone(), None, None, 1e-6, BF16)
+        assert torch.equal(y, y2) and torch.equal(mean, mean2) and torch.equal(rstd, rstd2)
+        dx, _, _ = ops.layer_norm_bwd(x, x, mean, rstd, None, x, False, False)
+        dx2, _, _ = ops.layer_norm_bwd(x.contiguous().clone(), x.contiguous().clone(), mean, rstd, None, x.contiguous().clone(), False, False)
+        assert torch.equal(dx, dx2)
+
+
+def test_parameter_gradients_are_the_same_bits_every_time():
+    gen = torch.Generator(device=DEV).manual_seed(10)
+    x, dy = _rand(gen, (9001, 768), BF16), _rand(gen, (9001, 768), BF16)
+    _, mean, rstd = ops.layer_norm_fwd(x, None, None, 1e-6, BF16)
+    first = ops.layer_norm_bwd(dy, x, mean, rstd, None, None, True, True)
+    for _ in range(3):
+        again = ops.layer_norm_bwd(dy, x, mean, rstd, None, None, True, True)
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+@pytest.mark.parametrize("dim", [96, 768, 5000])
+def test_gradients_against_differences(dim):
+    """sum(y * dy) moves by <dx, v> along v: central differences of the fp32 forward in steps of 1/64. Their own errors: 6 ulps of each
+    y per evaluation over the step (2^-24 * 6 * 64 * |y dy| in sum, as independent errors 8 root-sum-squares), and the third
+    derivative, (1/64)^2 times a few times the result."""
+    gen = torch.Generator(device=DEV).manual_seed(11)
+    x, dy, v = (_rand(gen, (23, dim), F32) for _ in range(3))
+    w, b, vw = (_rand(gen, (dim,), F32) for _ in range(3))
+    h = 1.0 / 64
+
+    def f(x, w):
+        return ops.layer_norm_fwd(x, w, b, 1e-6, F32)[0].double() * dy.double()
+
+    y, mean, rstd = ops.layer_norm_fwd(x, w, b, 1e-6, F32)
+    dx, dw, db = ops.layer_norm_bwd(dy, x, mean, rstd, w, None, True, True)
+    noise = 8 * 6 * ref.E / h * float((y.double() * dy.double()).square().sum().sqrt() + (y.double() * dy.double()).abs().sum() / 100)
+    for grad, direction, plus, minus in ((dx, v, f(x + h * v, w), f(x - h * v, w)), (dw, vw, f(x, w + h * vw), f(x, w - h * vw))):
+        num = float((plus - minus).sum() / (2 * h))
+        want = float((grad.double() * direction.double()).sum())
+        size = float((grad.double() * direction.double()).square().sum().sqrt())
+        assert abs(num - want) <= noise + 8 * h * h * (abs(want) + size), (num, want, noise, size)
+
+
+def test_on_another_stream():
+    gen = torch.Generator(device=DEV).manual_seed(12)
+    x = _rand(gen, (5000, 768), BF16)
+    want = ops.layer_norm_fwd(x, None, None, 1e-6, BF16)[0]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        y = ops.layer_norm_fwd(x * 1, None, None, 1e-6, BF16)[0]
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(y, want)
+
+
+def test_refusals():
+    x = torch.randn((4, 64), device=DEV)
+    w = torch.ones(64, device=DEV)
+    m = torch.zeros(4, device=DEV)
+    for call in (lambda: ops.layer_norm_fwd(x.double(), None, None, 1e-6, F32), lambda: ops.layer_norm_fwd(x, w[:63], None, 1e-6, F32),
+                 lambda: ops.layer_norm_fwd(x, w, w.half(), 1e-6, F32), lambda: ops.layer_norm_fwd(x, w, None, 1e-6, torch.int32),
+                 lambda: ops.layer_norm_fwd(x, None, None, -1.0, F32), lambda: ops.layer_norm_fwd(x[:, :0], None, None, 1e-6, F32),
+                 lambda: ops.layer_norm_fwd(x, w.view(1, 64), None, 1e-6, F32), lambda: ops.layer_norm_fwd(x, w.cpu(), None, 1e-6, F32),
+                 lambda: ops.layer_norm_bwd(x[:3], x, m, m, None, None, False, False),
+                 lambda: ops.layer_norm_bwd(x, x, m[:3], m, None, None, False, False),
+                 lambda: ops.layer_norm_bwd(x, x, m, m.half(), None, None, False, False),
+                 lambda: ops.layer_norm_bwd(x, x, m, m, None, x.half(), False, False)):
+        with pytest.raises(RuntimeError):
+            call()
