@@ -213,7 +213,7 @@ def lib() -> ctypes.CDLL:
         L.dopt_linear_act_grad.restype = i32
         L.dopt_linear_weight_grad_workspace_floats.argtypes = [i64, i64, i64]
         L.dopt_linear_weight_grad_workspace_floats.restype = i64
-        L.dopt_linear_weight_grad.argtypes = [vp, i64, vp, i64, i32, i64, i64, i64, vp, vp, vp, vp, vp]
+        L.dopt_linear_weight_grad.argtypes = [vp, i64, vp, i64, i32, i64, i64, i64, vp, vp, vp, vp, vp, vp]
         L.dopt_linear_weight_grad.restype = i32
         _lib = L
     return _lib

@@ -34,6 +34,10 @@ SOURCES = [
     "layer_norm_bwd.hip",
     "dropout.hip",
     "linear_gemm.hip",
+    "linear_big_nt_bf16.hip",
+    "linear_big_nt_f16.hip",
+    "linear_big_kn_bf16.hip",
+    "linear_big_kn_f16.hip",
 ]
 
 ARCH = "gfx950"

@@ -1049,7 +1049,7 @@ int dopt_dw_gemm(const void* dy, int64_t ldd, const void* x_hat, int64_t ldx, co
         mode = dopt::DW_B_PACKED;
     }
     (void)hipGetLastError();
-    dopt::launch_dw_gemm(a, mode, db != nullptr, dw_f32, (uint16_t*)dw_bf16, db, (hipStream_t)stream);
+    dopt::launch_dw_gemm(a, mode, dw_f32, (uint16_t*)dw_bf16, db, nullptr, (hipStream_t)stream);
     return hip_status("dw_gemm launch");
 }
 
@@ -1087,7 +1087,7 @@ int dopt_dw_gemm_any(const void* dy, int64_t ldd, const void* x_hat, int64_t ldx
     a.K = K;
     a.partial = workspace;
     (void)hipGetLastError();
-    if (dopt::launch_dw_gemm(a, dopt::DW_B_BF16, db != nullptr, dw_f32, (uint16_t*)dw_bf16, db, (hipStream_t)stream))
+    if (dopt::launch_dw_gemm(a, dopt::DW_B_BF16, dw_f32, (uint16_t*)dw_bf16, db, nullptr, (hipStream_t)stream))
         return fail(DOPT_EUNSUPPORTED, "no dw_gemm_any kernel for this shape");
     return hip_status("dw_gemm_any launch");
 }
@@ -1242,7 +1242,8 @@ int64_t dopt_linear_weight_grad_workspace_floats(int64_t M, int64_t N, int64_t K
 }
 
 int dopt_linear_weight_grad(const void* dz, int64_t ldz, const void* x, int64_t ldx, int dtype, int64_t M, int64_t N,
-                            int64_t K, float* workspace, float* dw_f32, void* dw_16, float* db, void* stream) {
+                            int64_t K, float* workspace, float* dw_f32, void* dw_16, float* db, void* db_16, void* stream) {
+    if (db && db_16) return fail(DOPT_EINVAL, "linear: one bias gradient, db or db_16");
     if (dtype != DOPT_F16 && dtype != DOPT_BF16)
         return fail(DOPT_EINVAL, "linear: the operands must be DOPT_F16 or DOPT_BF16, got %d", dtype);
     if (!linear_dw_shape(M, N, K))
@@ -1265,7 +1266,7 @@ int dopt_linear_weight_grad(const void* dz, int64_t ldz, const void* x, int64_t 
     a.partial = workspace;
     a.f16 = dtype == DOPT_F16;
     (void)hipGetLastError();
-    if (dopt::launch_dw_gemm(a, dopt::DW_B_BF16, db != nullptr, dw_f32, (uint16_t*)dw_16, db, (hipStream_t)stream))
+    if (dopt::launch_dw_gemm(a, dopt::DW_B_BF16, dw_f32, (uint16_t*)dw_16, db, (uint16_t*)db_16, (hipStream_t)stream))
         return fail(DOPT_EUNSUPPORTED, "no weight-gradient kernel for this shape");
     return hip_status("linear_weight_grad launch");
 }

@@ -25,12 +25,14 @@ struct DwArgs {
     float* partial;           // workspace: [splits][M][N] fp32, then [splits][M] for db; one split: the fp32 result
     uint16_t* out16;          // the bf16 result, of the kernels that write it in place of partial
     float* db_partial;        // set by the launcher
+    uint16_t* db16;           // set by the launcher: the bias gradient's sums in 16 bits, where one split writes them
     bool f16 = false;         // dy, xh and out16 are fp16 (DW_B_BF16 only; M may then be any number below ldd)
 };
 
 int dw_splits(int64_t M, int64_t N, int64_t K);
 int64_t dw_workspace_floats(int64_t M, int64_t N, int64_t K);
 int64_t dw_any_workspace_floats(int64_t M, int64_t N, int64_t K);
-int launch_dw_gemm(DwArgs a, int mode, bool with_db, float* out32, uint16_t* out16, float* db, hipStream_t st);
+// the bias gradient in fp32 (db) or in dy's type (db16, DW_B_BF16 only), at most one of them
+int launch_dw_gemm(DwArgs a, int mode, float* out32, uint16_t* out16, float* db, uint16_t* db16, hipStream_t st);
 
 }  // namespace dopt

@@ -739,7 +739,11 @@ __global__ __launch_bounds__(64 * NW, 1) void dw_gemm_v2_kernel(DwArgs a) {
         for (int ii = 0; ii < TMW; ++ii) {
             const float other = __shfl_xor(dbacc[ii], 32);
             const int64_t m = m0 + wm * RW + ii * 32 + lane;
-            if (lane < 32 && (!RAG || m < a.M)) a.db_partial[(int64_t)split * a.M + m] = dbacc[ii] + other;
+            if (lane < 32 && (!RAG || m < a.M)) {
+                const float sum = dbacc[ii] + other;
+                if (BITS == 0 && a.db16) a.db16[m] = F16 ? to_f16(sum) : to_bf16(sum);
+                else a.db_partial[(int64_t)split * a.M + m] = sum;
+            }
         }
     }
 }
@@ -760,7 +764,7 @@ template <int SUB, bool F16>
 __global__ __launch_bounds__(256) void dw_reduce_kernel(const float* __restrict__ partial, int splits, int64_t MN,
                                                         float* __restrict__ out32, uint16_t* __restrict__ out16,
                                                         const float* __restrict__ dbp, int64_t M,
-                                                        float* __restrict__ db) {
+                                                        float* __restrict__ db, uint16_t* __restrict__ db16) {
     const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int64_t i = (t / SUB) * 4;
     const int j = (int)(t % SUB);
@@ -799,7 +803,7 @@ __global__ __launch_bounds__(256) void dw_reduce_kernel(const float* __restrict_
                 *(uint2*)(out16 + i) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
         }
     }
-    if (db && t < M) {
+    if ((db || db16) && t < M) {
         float d = splits > 0 ? dbp[t] : 0.0f;
         int k = 1;
         for (; k + 3 < splits; k += 4) {
@@ -811,20 +815,21 @@ __global__ __launch_bounds__(256) void dw_reduce_kernel(const float* __restrict_
             d += p3;
         }
         for (; k < splits; ++k) d += dbp[(int64_t)k * M + t];
-        db[t] = d;
+        if (db) db[t] = d;
+        if (db16) db16[t] = F16 ? to_f16(d) : to_bf16(d);
     }
 }
 
 // one launch of the reduce: SUB lanes per output for a wide split count (more loads in flight)
 void launch_dw_reduce(const float* partial, int used, int64_t MN, float* out32, uint16_t* out16, const float* dbp,
-                      int64_t M, float* db, bool f16, hipStream_t st) {
+                      int64_t M, float* db, uint16_t* db16, bool f16, hipStream_t st) {
     const int sub = used > 16 ? 8 : used > 8 ? 4 : used > 4 ? 2 : 1;
     const int64_t threads = std::max<int64_t>(MN / 4 * sub, M);
     const dim3 grid((unsigned)((threads + 255) / 256));
 #define DOPT_RED(S_)                                                                                                          \
     do {                                                                                                                      \
-        if (f16) hipLaunchKernelGGL((dw_reduce_kernel<S_, true>), grid, dim3(256), 0, st, partial, used, MN, out32, out16, dbp, M, db); \
-        else hipLaunchKernelGGL((dw_reduce_kernel<S_, false>), grid, dim3(256), 0, st, partial, used, MN, out32, out16, dbp, M, db);   \
+        if (f16) hipLaunchKernelGGL((dw_reduce_kernel<S_, true>), grid, dim3(256), 0, st, partial, used, MN, out32, out16, dbp, M, db, db16); \
+        else hipLaunchKernelGGL((dw_reduce_kernel<S_, false>), grid, dim3(256), 0, st, partial, used, MN, out32, out16, dbp, M, db, db16);   \
     } while (0)
     if (sub == 8) DOPT_RED(8);
     else if (sub == 4) DOPT_RED(4);
@@ -881,7 +886,8 @@ int64_t dw_any_workspace_floats(int64_t M, int64_t N, int64_t K) {
     return dw_splits(M, N, K) == 1 ? 0 : dw_workspace_floats(M, N, K);
 }
 
-int launch_dw_gemm(DwArgs a, int mode, bool with_db, float* out32, uint16_t* out16, float* db, hipStream_t st) {
+int launch_dw_gemm(DwArgs a, int mode, float* out32, uint16_t* out16, float* db, uint16_t* db16, hipStream_t st) {
+    const bool with_db = db || db16;
     const int splits = dw_splits(a.M, a.N, a.K);
     // the packed codes go through the pipelined kernel for 1/2/4 bits with DMA-aligned arrays
     // (codes 16-byte, scale/min 4-byte aligned); 8-bit codes through the register-decoding kernel
@@ -904,11 +910,13 @@ int launch_dw_gemm(DwArgs a, int mode, bool with_db, float* out32, uint16_t* out
     const bool direct = one && (out32 || o16);
     if (direct) a.partial = out32;
     a.out16 = out16;
+    a.db16 = direct ? db16 : nullptr;
+    if (db16 && !v2 && a.K > 0) return -1;
     const auto reduce = [&](int used) {
         if (!direct)
-            launch_dw_reduce(a.partial, used, a.M * a.N, out32, out16, a.db_partial, a.M, with_db ? db : nullptr, a.f16, st);
+            launch_dw_reduce(a.partial, used, a.M * a.N, out32, out16, a.db_partial, a.M, db, db16, a.f16, st);
         else if (out32 && out16)
-            launch_dw_reduce(out32, used, a.M * a.N, nullptr, out16, nullptr, a.M, nullptr, a.f16, st);
+            launch_dw_reduce(out32, used, a.M * a.N, nullptr, out16, nullptr, a.M, nullptr, nullptr, a.f16, st);
     };
     if (v2) {
         // the transpose-free kernel: 32-token tiles, split at the same token boundaries as the
@@ -978,7 +986,7 @@ int launch_dw_gemm(DwArgs a, int mode, bool with_db, float* out32, uint16_t* out
     }
     if (a.f16 || a.M % BM != 0 || a.N % BN != 0) {
         if (a.K > 0) return -1;  // outside the ragged instances' offsets
-        launch_dw_reduce(a.partial, 0, a.M * a.N, out32, out16, a.partial, a.M, with_db ? db : nullptr, a.f16, st);
+        launch_dw_reduce(a.partial, 0, a.M * a.N, out32, out16, a.partial, a.M, db, db16, a.f16, st);
         return 0;
     }
     const int64_t kts = (a.K + BK - 1) / BK;

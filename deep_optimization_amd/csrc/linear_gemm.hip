@@ -6,6 +6,12 @@
 #include "linear_small.h"
 
 namespace dopt {
+
+void lin_big_nt_bf16(const LinArgs& p, int bm, int n_cu, hipStream_t s);
+void lin_big_nt_f16(const LinArgs& p, int bm, int n_cu, hipStream_t s);
+void lin_big_kn_bf16(const LinArgs& p, int bm, int n_cu, hipStream_t s);
+void lin_big_kn_f16(const LinArgs& p, int bm, int n_cu, hipStream_t s);
+
 namespace {
 
 // compute units of the current device, queried once per device
@@ -22,15 +28,58 @@ int device_cu_count() {
     return n;
 }
 
+// Estimated time (us) of each tile on this part: start + rounds of tiles (of the CUs' slots) * (slabs * step + epilogue), step
+// and epilogue of one tile among the others on its CU.
+struct TileCost {
+    int bm, bn, slots;  // slots: tiles that a CU works on at once
+    float start, step, epilogue;
+};
+enum { T_32x64, T_64x64, T_128x128, T_BIG160, T_BIG256, T_COUNT };
+constexpr TileCost TILE_COST[T_COUNT] = {
+    {32, 64, 2, 2.5f, 0.20f, 0.6f},
+    {64, 64, 2, 2.5f, 0.28f, 1.2f},
+    {128, 128, 2, 3.0f, 0.75f, 5.0f},
+    {160, 256, 1, 4.0f, 0.98f, 5.0f},
+    {256, 256, 1, 4.0f, 1.45f, 9.0f},
+};
+
+int plan(const LinArgs& p, int n_cu, bool big) {
+    const float nk = (float)((p.K + LIN_BK - 1) / LIN_BK);
+    int best = T_32x64;
+    float least = 0.0f;
+    for (int t = 0; t < T_COUNT; ++t) {
+        const TileCost& c = TILE_COST[t];
+        if (t >= T_BIG160 && !big) break;
+        const int64_t tiles = ((p.M + c.bm - 1) / c.bm) * ((p.N + c.bn - 1) / c.bn), slots = (int64_t)n_cu * c.slots;
+        const float rounds = (float)((tiles + slots - 1) / slots);
+        const float us = c.start + rounds * (nk * c.step + c.epilogue);
+        if (t == 0 || us < least) {
+            least = us;
+            best = t;
+        }
+    }
+    return best;
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+
 template <bool KN, bool F16>
 void launch(const LinArgs& p, hipStream_t s) {
     const int n_cu = device_cu_count();
-    const auto tiles = [&](int bm, int bn) { return ((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
     if constexpr (!KN) {
         if (p.M <= 16) return lin_small_launch<8, F16>(p, s);
     }
-    if (tiles(128, 128) >= 2 * n_cu) return lin_gemm_launch<128, 128, 2, 2, KN, F16>(p, s);
-    if (tiles(64, 64) >= n_cu) return lin_gemm_launch<64, 64, 4, 2, KN, F16>(p, s);
+    // what the 256-wide tiles take: whole 16-byte chunks in the results' rows, 32-bit offsets in a tile of them
+    const bool big = p.N % 8 == 0 && p.N < ((int64_t)1 << 21) && p.K > 0 && !p.y_f32 && n_cu >= LIN_XCDS && aligned16(p.y) &&
+                     aligned16(p.pre) && aligned16(p.res) && aligned16(p.aux);
+    const int t = plan(p, n_cu, big);
+    if (t >= T_BIG160) {
+        const int bm = TILE_COST[t].bm;
+        if constexpr (KN) return F16 ? lin_big_kn_f16(p, bm, n_cu, s) : lin_big_kn_bf16(p, bm, n_cu, s);
+        else return F16 ? lin_big_nt_f16(p, bm, n_cu, s) : lin_big_nt_bf16(p, bm, n_cu, s);
+    }
+    if (t == T_128x128) return lin_gemm_launch<128, 128, 2, 2, KN, F16>(p, s);
+    if (t == T_64x64) return lin_gemm_launch<64, 64, 4, 2, KN, F16>(p, s);
     return lin_gemm_launch<32, 64, 4, 2, KN, F16>(p, s);
 }
 

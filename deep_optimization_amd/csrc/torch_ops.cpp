@@ -18,7 +18,8 @@
 // bn_train_fwd, bn_train_bwd (the compressed BatchNorm layers' one-call forward and backward),
 // silu_fwd_quan_pack, silu_bwd_fused_dequan_unpack, gelu_bwd_fused_dequan_unpack
 // (AC/modules/activations/kernel_registration.py:148-237, :295-319), dw_gemm_any (the compressed Linear layer's
-// weight gradient), fp8_gemm_nt, fp8_linear.
+// weight gradient), fp8_gemm_nt, fp8_linear, layer_norm_fwd, layer_norm_bwd, dropout_add_fwd, dropout_bwd,
+// linear_act_fwd, linear_act_bwd (the transformer blocks' operators).
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
@@ -679,6 +680,275 @@ std::tuple<Tensor, Tensor, Tensor> bn_train_bwd(const Tensor& packed_in, const s
     return {dx, dw, db};
 }
 
+// ---------------------------------------------------------------------------- transformer blocks
+bool is_float(ScalarType t) { return t == ScalarType::Float || t == ScalarType::Half || t == ScalarType::BFloat16; }
+
+const void* ptr(const std::optional<Tensor>& t) { return t ? t->data_ptr() : nullptr; }
+
+std::optional<Tensor> contiguous(const std::optional<Tensor>& t) {
+    if (!t) return t;
+    return t->contiguous();
+}
+
+int64_t ln_dim(const char* what, const Tensor& x) {
+    TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1 && is_float(x.scalar_type()), what,
+                ": x must be a float32, float16 or bfloat16 tensor [..., D] with D >= 1, got ", x.sizes(), " ", x.scalar_type());
+    return x.size(-1);
+}
+
+// the parameters' type code (ln_lib._check_params)
+int ln_params(const char* what, int64_t D, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias) {
+    for (const auto& [name, p] : {std::pair<const char*, const std::optional<Tensor>*>{"weight", &weight}, {"bias", &bias}}) {
+        if (!*p) continue;
+        const Tensor& t = **p;
+        TORCH_CHECK(t.numel() == D && t.dim() == 1 && is_float(t.scalar_type()), what, ": ", name,
+                    " must be a float32, float16 or bfloat16 vector of ", D, " values, got ", t.sizes(), " ", t.scalar_type());
+    }
+    TORCH_CHECK(!weight || !bias || weight->scalar_type() == bias->scalar_type(), what, ": weight and bias must have one type");
+    if (!weight && !bias) return DOPT_F32;
+    return dtype_code((weight ? *weight : *bias).scalar_type(), what);
+}
+
+void require_cuda(const std::optional<Tensor>& t) {
+    if (t) require_cuda(*t);
+}
+
+std::tuple<Tensor, Tensor, Tensor> layer_norm_fwd(const Tensor& x_in, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias,
+                                                  double eps, ScalarType out_dtype) {
+    const int64_t D = ln_dim("layer_norm_fwd", x_in);
+    const int code = ln_params("layer_norm_fwd", D, weight, bias);
+    TORCH_CHECK(is_float(out_dtype), "layer_norm_fwd: out_dtype must be float32, float16 or bfloat16, got ", out_dtype);
+    require_cuda(x_in);
+    require_cuda(weight);
+    require_cuda(bias);
+    require_current(x_in);
+    const Tensor x = x_in.contiguous();
+    const auto w = contiguous(weight), b = contiguous(bias);
+    const auto opts = x.options();
+    Tensor y = at::empty(x.sizes(), opts.dtype(out_dtype));
+    Tensor mean = at::empty(x.sizes().slice(0, x.dim() - 1), opts.dtype(at::kFloat)), rstd = at::empty_like(mean);
+    check(dopt_layer_norm_forward(x.data_ptr(), dtype_code(x.scalar_type(), "layer_norm_fwd"), mean.numel(), D, ptr(w), ptr(b), code,
+                                  (float)eps, y.data_ptr(), dtype_code(out_dtype, "layer_norm_fwd"), mean.data_ptr<float>(),
+                                  rstd.data_ptr<float>(), stream_of(x)),
+          "layer_norm_fwd");
+    return {y, mean, rstd};
+}
+
+std::tuple<Tensor, std::optional<Tensor>, std::optional<Tensor>> layer_norm_bwd(
+    const Tensor& dy_in, const Tensor& x_in, const Tensor& mean_in, const Tensor& rstd_in, const std::optional<Tensor>& weight,
+    const std::optional<Tensor>& dresidual, bool weight_grad, bool bias_grad) {
+    const int64_t D = ln_dim("layer_norm_bwd", x_in);
+    const int code = ln_params("layer_norm_bwd", D, weight, std::nullopt);
+    const int64_t rows = x_in.numel() / D;
+    TORCH_CHECK(dy_in.sizes() == x_in.sizes() && is_float(dy_in.scalar_type()),
+                "layer_norm_bwd: dy must be a float32, float16 or bfloat16 tensor of x's shape ", x_in.sizes(), ", got ", dy_in.sizes(), " ",
+                dy_in.scalar_type());
+    for (const Tensor* t : {&mean_in, &rstd_in})
+        TORCH_CHECK(t->numel() == rows && t->scalar_type() == ScalarType::Float, "layer_norm_bwd: ", t == &mean_in ? "mean" : "rstd",
+                    " must hold ", rows, " float32 values, got ", t->sizes(), " ", t->scalar_type());
+    TORCH_CHECK(!dresidual || (dresidual->sizes() == x_in.sizes() && dresidual->scalar_type() == x_in.scalar_type()),
+                "layer_norm_bwd: dresidual must have x's shape and type");
+    for (const Tensor* t : {&dy_in, &x_in, &mean_in, &rstd_in}) require_cuda(*t);
+    require_cuda(weight);
+    require_cuda(dresidual);
+    require_current(x_in);
+    const Tensor dy = dy_in.contiguous(), x = x_in.contiguous(), mean = mean_in.contiguous(), rstd = rstd_in.contiguous();
+    const auto w = contiguous(weight), dr = contiguous(dresidual);
+    const auto f32 = x.options().dtype(at::kFloat);
+    Tensor dx = at::empty(x.sizes(), x.options());
+    std::optional<Tensor> dw, db;
+    Tensor ws;
+    if (weight_grad) dw = at::empty({D}, f32);
+    if (bias_grad) db = at::empty({D}, f32);
+    if (dw || db) ws = at::empty({std::max<int64_t>(dopt_layer_norm_workspace_floats(rows, D), 1)}, f32);
+    check(dopt_layer_norm_backward(dy.data_ptr(), dtype_code(dy.scalar_type(), "layer_norm_bwd"), x.data_ptr(),
+                                   dtype_code(x.scalar_type(), "layer_norm_bwd"), rows, D, mean.data_ptr<float>(), rstd.data_ptr<float>(),
+                                   ptr(w), code, ptr(dr), dx.data_ptr(), ws.defined() ? ws.data_ptr<float>() : nullptr,
+                                   dw ? dw->data_ptr<float>() : nullptr, db ? db->data_ptr<float>() : nullptr, stream_of(x)),
+          "layer_norm_bwd");
+    return {dx, dw, db};
+}
+
+Tensor dropout_launch(const char* what, const Tensor& x_in, const std::optional<Tensor>& residual, double p, int64_t seed, int64_t offset,
+                      const std::optional<Tensor>& step, ScalarType y_dtype) {
+    TORCH_CHECK(is_float(x_in.scalar_type()) && is_float(y_dtype), what, ": input and output must be float32, float16 or bfloat16, got ",
+                x_in.scalar_type(), " and ", y_dtype);
+    TORCH_CHECK(p >= 0.0 && p <= 1.0, what, ": p must lie in [0, 1], got ", p);
+    TORCH_CHECK(!residual || residual->sizes() == x_in.sizes(), what, ": residual must have x's shape ", x_in.sizes());
+    TORCH_CHECK(!step || (step->scalar_type() == ScalarType::Long && step->numel() == 1), what, ": step must be a one-element int64 tensor");
+    require_cuda(x_in);
+    require_cuda(residual);
+    require_cuda(step);
+    require_current(x_in);
+    const Tensor x = x_in.contiguous();
+    const auto r = contiguous(residual);
+    Tensor y = at::empty(x.sizes(), x.options().dtype(y_dtype));
+    check(dopt_dropout(x.data_ptr(), dtype_code(x.scalar_type(), what), ptr(r), x.numel(), p, (uint64_t)seed, (uint64_t)offset,
+                       (const int64_t*)ptr(step), y.data_ptr(), dtype_code(y_dtype, what), stream_of(x)),
+          what);
+    return y;
+}
+
+Tensor dropout_add_fwd(const Tensor& x, const std::optional<Tensor>& residual, double p, int64_t seed, int64_t offset,
+                       const std::optional<Tensor>& step) {
+    return dropout_launch("dropout_add_fwd", x, residual, p, seed, offset, step, (residual ? *residual : x).scalar_type());
+}
+
+Tensor dropout_bwd(const Tensor& dy, double p, int64_t seed, int64_t offset, const std::optional<Tensor>& step, ScalarType out_dtype) {
+    return dropout_launch("dropout_bwd", dy, std::nullopt, p, seed, offset, step, out_dtype);
+}
+
+int lin_act(c10::string_view act) {
+    if (act == "none") return DOPT_LIN_NONE;
+    if (act == "relu") return DOPT_LIN_RELU;
+    if (act == "gelu") return DOPT_LIN_GELU;
+    if (act == "gelu_tanh") return DOPT_LIN_GELU_TANH;
+    TORCH_CHECK_VALUE(act == "silu", "act must be one of none, relu, gelu, gelu_tanh, silu, got '", act, "'");
+    return DOPT_LIN_SILU;
+}
+
+int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
+
+// dy act'(pre) [rows, cols] in rows padded with zeros to a multiple of 8
+Tensor lin_act_grad_rows(const Tensor& dy, const void* pre, int act, int64_t rows, int64_t cols) {
+    Tensor out = at::empty({rows, pad8(cols)}, dy.options());
+    check(dopt_linear_act_grad(dy.data_ptr(), cols, pre, act, dtype_code(dy.scalar_type(), "linear_act"), rows, cols, out.data_ptr(),
+                               pad8(cols), stream_of(dy)),
+          "linear_act");
+    return out;
+}
+
+// t [..., cols] as (tensor, row stride): linear_lib._rows
+std::pair<Tensor, int64_t> lin_rows(const Tensor& t, int64_t rows, int64_t cols) {
+    const auto aligned16 = [](const Tensor& v) { return reinterpret_cast<uintptr_t>(v.data_ptr()) % 16 == 0; };
+    const Tensor t2 = t.dim() == 2 ? t : t.reshape({rows, cols});
+    if (cols % 8 == 0 && t2.stride(1) == 1 && t2.stride(0) >= cols && t2.stride(0) < (1 << 21) && t2.stride(0) % 8 == 0 && aligned16(t2))
+        return {t2, t2.stride(0)};
+    const Tensor c = t2.contiguous();
+    if (cols % 8 == 0 && aligned16(c)) return {c, cols};
+    return {lin_act_grad_rows(c, nullptr, DOPT_LIN_NONE, rows, cols), pad8(cols)};
+}
+
+bool lin_type(ScalarType t) { return t == ScalarType::Half || t == ScalarType::BFloat16; }
+
+void lin_operands(const char* what, const Tensor& x, const Tensor& weight) {
+    TORCH_CHECK(lin_type(x.scalar_type()) && weight.scalar_type() == x.scalar_type() && x.dim() >= 1 && weight.dim() == 2 &&
+                    weight.size(1) == x.size(-1),
+                what, ": x [..., K] and weight [N, K] must both be bfloat16 or float16, got ", x.sizes(), " ", x.scalar_type(), " and ",
+                weight.sizes(), " ", weight.scalar_type());
+}
+
+int64_t lin_leading(const Tensor& x) {
+    int64_t m = 1;
+    for (int64_t d = 0; d + 1 < x.dim(); ++d) m *= x.size(d);
+    return m;
+}
+
+// x's leading sizes and `cols` columns
+c10::SmallVector<int64_t, 6> lin_shape(const Tensor& x, int64_t cols) {
+    c10::SmallVector<int64_t, 6> s(x.sizes().begin(), x.sizes().end());
+    s.back() = cols;
+    return s;
+}
+
+void lin_like(const char* what, const char* name, const Tensor& t, at::IntArrayRef shape, bool type_ok) {
+    TORCH_CHECK(t.sizes() == shape && type_ok, what, ": ", name, " must be ", shape, " in a type that goes with x's, got ", t.sizes(), " ",
+                t.scalar_type());
+}
+
+std::tuple<Tensor, std::optional<Tensor>> linear_act_fwd(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias,
+                                                         const std::optional<Tensor>& residual, c10::string_view act, bool save_pre) {
+    const char* what = "linear_act_fwd";
+    const int code = lin_act(act);
+    lin_operands(what, x, weight);
+    const int64_t M = lin_leading(x), N = weight.size(0), K = weight.size(1);
+    const auto shape = lin_shape(x, N);
+    const ScalarType dt = x.scalar_type();
+    if (bias) lin_like(what, "bias", *bias, {N}, is_float(bias->scalar_type()));
+    if (residual) lin_like(what, "residual", *residual, shape, residual->scalar_type() == dt || residual->scalar_type() == ScalarType::Float);
+    require_cuda(x);
+    require_cuda(weight);
+    require_cuda(bias);
+    require_cuda(residual);
+    require_current(x);
+    const auto [a, lda] = M && K ? lin_rows(x, M, K) : std::pair<Tensor, int64_t>{x, pad8(K)};
+    const auto [b, ldb] = N && K ? lin_rows(weight, N, K) : std::pair<Tensor, int64_t>{weight, pad8(K)};
+    const auto bc = contiguous(bias), r = contiguous(residual);
+    Tensor y = at::empty(shape, x.options().dtype(r ? r->scalar_type() : dt));
+    std::optional<Tensor> pre;
+    if (save_pre) pre = at::empty(shape, x.options());
+    check(dopt_linear_forward(a.data_ptr(), lda, b.data_ptr(), ldb, dtype_code(dt, what), M, N, K, ptr(bc),
+                              bc ? dtype_code(bc->scalar_type(), what) : DOPT_F32, ptr(r), code, y.data_ptr(),
+                              dtype_code(y.scalar_type(), what), pre ? pre->data_ptr() : nullptr, stream_of(x)),
+          what);
+    return {y, pre};
+}
+
+std::tuple<std::optional<Tensor>, std::optional<Tensor>, std::optional<Tensor>> linear_act_bwd(
+    const Tensor& dy, const Tensor& x, const Tensor& weight, const std::optional<Tensor>& pre, c10::string_view act,
+    const std::optional<Tensor>& in_pre, c10::string_view in_act, bool input_grad, bool weight_grad, bool bias_grad, ScalarType grad_dtype) {
+    const char* what = "linear_act_bwd";
+    const int code = lin_act(act), in_code = lin_act(in_act);
+    lin_operands(what, x, weight);
+    const int64_t M = lin_leading(x), N = weight.size(0), K = weight.size(1);
+    const ScalarType dt = x.scalar_type();
+    const auto shape = lin_shape(x, N);
+    lin_like(what, "dy", dy, shape, dy.scalar_type() == dt);
+    TORCH_CHECK(grad_dtype == ScalarType::Float || grad_dtype == dt, what, ": grad_dtype must be float32 or x's type, got ", grad_dtype);
+    TORCH_CHECK((code != DOPT_LIN_NONE) == pre.has_value(), what, ": pre goes with an activation (act '", act, "', pre ",
+                pre ? "given)" : "missing)");
+    TORCH_CHECK((in_code != DOPT_LIN_NONE) == in_pre.has_value(), what, ": in_pre goes with in_act (in_act '", in_act, "', in_pre ",
+                in_pre ? "given)" : "missing)");
+    if (pre) lin_like(what, "pre", *pre, shape, pre->scalar_type() == dt);
+    if (in_pre) lin_like(what, "in_pre", *in_pre, x.sizes(), in_pre->scalar_type() == dt);
+    for (const Tensor* t : {&dy, &x, &weight}) require_cuda(*t);
+    require_cuda(pre);
+    require_cuda(in_pre);
+    require_current(x);
+    const int tc = dtype_code(dt, what);
+    void* const stream = stream_of(x);
+    Tensor dz = dy;
+    int64_t ldz = pad8(N);
+    if (M && N) {
+        if (code != DOPT_LIN_NONE) {
+            const Tensor d = dy.contiguous(), z = pre->contiguous();
+            dz = lin_act_grad_rows(d, z.data_ptr(), code, M, N);
+        } else {
+            std::tie(dz, ldz) = lin_rows(dy, M, N);
+        }
+    }
+    std::optional<Tensor> dx, dw, db;
+    if (input_grad) {
+        dx = at::empty(x.sizes(), x.options());
+        const auto ip = contiguous(in_pre);
+        const auto [w, ldw] = N && K ? lin_rows(weight, N, K) : std::pair<Tensor, int64_t>{weight, pad8(K)};
+        check(dopt_linear_input_grad(dz.data_ptr(), ldz, w.data_ptr(), ldw, tc, M, N, K, ptr(ip), in_code, dx->data_ptr(), stream), what);
+    }
+    if (weight_grad || bias_grad) {
+        const auto opts = x.options().dtype(grad_dtype);
+        if (N == 0 || K == 0) {
+            dw = at::empty({N, K}, opts);
+            db = dz.reshape({M, dz.size(-1)}).narrow(1, 0, N).to(at::kFloat).sum(0).to(grad_dtype);
+        } else {
+            const auto [xr, ldx] = M ? lin_rows(x, M, K) : std::pair<Tensor, int64_t>{x, pad8(K)};
+            const int64_t K8 = pad8(K);
+            const bool f32 = grad_dtype == ScalarType::Float;
+            Tensor ws = at::empty({std::max<int64_t>(dopt_linear_weight_grad_workspace_floats(M, N, K8), 4)}, x.options().dtype(at::kFloat));
+            Tensor d = at::empty({N, K8}, opts);
+            if (bias_grad) db = at::empty({N}, opts);
+            void* const dbp = db ? db->data_ptr() : nullptr;
+            check(dopt_linear_weight_grad(dz.data_ptr(), ldz, xr.data_ptr(), ldx, tc, M, N, K8, ws.data_ptr<float>(),
+                                          f32 ? (float*)d.data_ptr() : nullptr, f32 ? nullptr : d.data_ptr(), f32 ? (float*)dbp : nullptr,
+                                          f32 ? nullptr : dbp, stream),
+                  what);
+            dw = K8 == K ? d : d.narrow(1, 0, K).contiguous();
+        }
+        if (!weight_grad) dw.reset();
+        if (!bias_grad) db.reset();
+    }
+    return {dx, dw, db};
+}
+
 }  // namespace
 
 TORCH_LIBRARY_IMPL(act_lib, CUDA, m) {
@@ -699,4 +969,10 @@ TORCH_LIBRARY_IMPL(act_lib, CUDA, m) {
     m.impl("dw_gemm_any", &dw_gemm_any);
     m.impl("fp8_gemm_nt", &fp8_gemm_nt);
     m.impl("fp8_linear", &fp8_linear);
+    m.impl("layer_norm_fwd", &layer_norm_fwd);
+    m.impl("layer_norm_bwd", &layer_norm_bwd);
+    m.impl("dropout_add_fwd", &dropout_add_fwd);
+    m.impl("dropout_bwd", &dropout_bwd);
+    m.impl("linear_act_fwd", &linear_act_fwd);
+    m.impl("linear_act_bwd", &linear_act_bwd);
 }

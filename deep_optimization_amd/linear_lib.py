@@ -155,20 +155,21 @@ def _linear_act_bwd(dy: Tensor, x: Tensor, weight: Tensor, pre: Optional[Tensor]
     if weight_grad or bias_grad:
         if N == 0 or K == 0:
             dw = torch.empty((N, K), dtype=grad_dtype, device=x.device)
-            db = dz.reshape(M, dz.shape[-1])[:, :N].float().sum(0)
+            db = dz.reshape(M, dz.shape[-1])[:, :N].float().sum(0).to(grad_dtype)
         else:
             xr, ldx = _rows(x, K) if M else (x, _pad8(K))
             K8 = _pad8(K)
             ws = torch.empty(max(int(L.dopt_linear_weight_grad_workspace_floats(M, N, K8)), 4), dtype=torch.float32, device=x.device)
             dw = torch.empty((N, K8), dtype=grad_dtype, device=x.device)
-            db = torch.empty(N, dtype=torch.float32, device=x.device) if bias_grad else None
+            db = torch.empty(N, dtype=grad_dtype, device=x.device) if bias_grad else None
             f32 = grad_dtype == torch.float32
+            dbp = None if db is None else db.data_ptr()
             rc = L.dopt_linear_weight_grad(dz.data_ptr(), ldz, xr.data_ptr(), ldx, dt, M, N, K8, ws.data_ptr(), dw.data_ptr() if f32 else None,
-                                           None if f32 else dw.data_ptr(), None if db is None else db.data_ptr(), stream)
+                                           None if f32 else dw.data_ptr(), dbp if f32 else None, None if f32 else dbp, stream)
             _lib.check(rc, what)
             if K8 != K:
                 dw = dw[:, :K].contiguous()
-    return dx, dw if weight_grad else None, db.to(grad_dtype) if bias_grad else None
+    return dx, dw if weight_grad else None, db if bias_grad else None
 
 
 def _linear_act_bwd_fake(dy, x, weight, pre, act, in_pre, in_act, input_grad, weight_grad, bias_grad, grad_dtype):

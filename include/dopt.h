@@ -486,12 +486,12 @@ int dopt_linear_input_grad(const void* dz, int64_t ldz, const void* weight, int6
  * aligned); pre [rows, cols]. With DOPT_LIN_NONE a copy into padded rows. */
 int dopt_linear_act_grad(const void* dy, int64_t ld_dy, const void* pre, int act, int dtype, int64_t rows, int64_t cols,
                          void* dz, int64_t ld_dz, void* stream);
-/* dw = dz^T x (fp32 dw_f32 and / or dw_16 of the operands' type, [N, K]) and db = sum over rows of dz (fp32 [N], may be
- * NULL): dopt_dw_gemm_any for fp16 or bf16 and any N; K a multiple of 8; the same alignment rules. workspace:
+/* dw = dz^T x (fp32 dw_f32 and / or dw_16 of the operands' type, [N, K]) and the sums of dz over its rows ([N], in fp32
+ * to db or in the operands' type to db_16; one or both NULL): dopt_dw_gemm_any for fp16 or bf16 and any N; K a multiple of 8; the same alignment rules. workspace:
  * dopt_linear_weight_grad_workspace_floats floats (not NULL). */
 int64_t dopt_linear_weight_grad_workspace_floats(int64_t M, int64_t N, int64_t K);
 int dopt_linear_weight_grad(const void* dz, int64_t ldz, const void* x, int64_t ldx, int dtype, int64_t M, int64_t N,
-                            int64_t K, float* workspace, float* dw_f32, void* dw_16, float* db, void* stream);
+                            int64_t K, float* workspace, float* dw_f32, void* dw_16, float* db, void* db_16, void* stream);
 
 /*
  * HIP graph tools for capturing a whole training step (forward, backward, optimizer step) as
