@@ -72,6 +72,8 @@ EXPORTS = (
     "dopt_linear_act_grad",
     "dopt_linear_weight_grad_workspace_floats",
     "dopt_linear_weight_grad",
+    "dopt_linear_tile",
+    "dopt_linear_copy_preferred",
 )
 
 _lib = None
@@ -215,6 +217,10 @@ def lib() -> ctypes.CDLL:
         L.dopt_linear_weight_grad_workspace_floats.restype = i64
         L.dopt_linear_weight_grad.argtypes = [vp, i64, vp, i64, i32, i64, i64, i64, vp, vp, vp, vp, vp, vp]
         L.dopt_linear_weight_grad.restype = i32
+        L.dopt_linear_tile.argtypes = [i32, i64, i64, i64, i32]
+        L.dopt_linear_tile.restype = i32
+        L.dopt_linear_copy_preferred.argtypes = [i32, i64, i64, i64, i64, i32]
+        L.dopt_linear_copy_preferred.restype = i32
         _lib = L
     return _lib
 

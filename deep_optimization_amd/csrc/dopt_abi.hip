@@ -40,7 +40,8 @@ int launch_alam_act_dequant_mul(const DequantArgs& d, int g, int bits, int dy_f3
 int launch_dropout(const void* x, int x_dt, const void* residual, uint64_t n, uint32_t threshold, uint64_t seed,
                    uint64_t offset, const int64_t* step, void* y, int y_dt, hipStream_t s);
 bool lin_shape_fits(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb);
-int launch_linear(const LinArgs& p, bool kn, bool f16, hipStream_t s);
+int launch_linear(const LinArgs& p, int kind, bool f16, hipStream_t s);
+int linear_tile(int kind, int64_t M, int64_t N, int64_t K, bool reg, bool big, float* us);
 int launch_linear_act_grad(const uint16_t* src, int64_t src_ld, const uint16_t* pre, int act, bool f16, int64_t rows,
                            int64_t cols, uint16_t* dst, int64_t ld_dst, hipStream_t s);
 }  // namespace dopt
@@ -1164,6 +1165,65 @@ static int check_linear(int dtype, int64_t M, int64_t N, int64_t K, int64_t lda,
     return DOPT_OK;
 }
 
+// operands of a product's size (the kernels read whole rows): pointers and row strides
+static int check_linear_rows(const void* a, int64_t lda, int64_t a_cols, const void* b, int64_t ldb, int64_t b_cols) {
+    if (!a || !b) return fail(DOPT_EINVAL, "linear: null operand pointer");
+    if (((uintptr_t)a & 1u) || ((uintptr_t)b & 1u)) return fail(DOPT_EINVAL, "linear: operands must lie at whole elements");
+    if (lda < a_cols || ldb < b_cols)
+        return fail(DOPT_EINVAL, "linear: row strides must be at least the row lengths (got %lld for %lld and %lld for %lld)", (long long)lda,
+                    (long long)a_cols, (long long)ldb, (long long)b_cols);
+    return DOPT_OK;
+}
+
+// M, N, K of the sums: LinArgs of each product from the layer's sizes (M rows, N out and K in features)
+static void linear_sizes(int kind, int64_t M, int64_t N, int64_t K, int64_t* m, int64_t* n, int64_t* k) {
+    *m = kind == DOPT_LIN_WEIGHT_GRAD ? N : M;
+    *n = kind == DOPT_LIN_FORWARD ? N : K;
+    *k = kind == DOPT_LIN_FORWARD ? K : kind == DOPT_LIN_INPUT_GRAD ? N : M;
+}
+
+// Estimated time (us) of dopt_dw_gemm_any's kernels: 32-token slabs of each split, and the partials' sum
+static float linear_dw_split_us(int64_t M, int64_t N, int64_t K) {
+    const int splits = dopt::dw_splits(N, K, M);
+    const float slabs = (float)((M + 32 * splits - 1) / (32 * splits));
+    const float step = ((N + 255) / 256) * ((K + 255) / 256) <= 16 ? 0.4f : 1.0f;
+    return 6.0f + slabs * step + (splits > 1 ? 3.0f + (float)splits * (float)N * (float)K * (8.0f / 6.0e6f) : 0.0f);
+}
+
+static bool linear_dw_shape(int64_t M, int64_t N, int64_t K) {
+    return M >= 0 && N > 0 && K > 0 && K % 8 == 0 && N < ((int64_t)1 << 20) && K < ((int64_t)1 << 20);
+}
+
+// whether the weight gradient of aligned operands takes dopt_dw_gemm_any's kernels (their splits of the sum)
+static bool linear_dw_split(int64_t M, int64_t N, int64_t K) {
+    if (!linear_dw_shape(M, N, K)) return false;
+    float us;
+    dopt::linear_tile(DOPT_LIN_WEIGHT_GRAD, N, K, M, false, false, &us);
+    return linear_dw_split_us(M, N, K) < us;
+}
+
+int dopt_linear_tile(int product, int64_t M, int64_t N, int64_t K, int any_rows) {
+    if (product < DOPT_LIN_FORWARD || product > DOPT_LIN_WEIGHT_GRAD || M < 0 || N < 0 || K < 0) return -2;
+    if (product == DOPT_LIN_WEIGHT_GRAD && !any_rows && linear_dw_split(M, N, K)) return 100;
+    int64_t m, n, k;
+    linear_sizes(product, M, N, K, &m, &n, &k);
+    return dopt::linear_tile(product, m, n, k, any_rows != 0, true, nullptr);
+}
+
+int dopt_linear_copy_preferred(int product, int64_t M, int64_t N, int64_t K, int64_t elements, int copies) {
+    if (product < DOPT_LIN_FORWARD || product > DOPT_LIN_WEIGHT_GRAD || M < 0 || N < 0 || K < 0) return 0;
+    int64_t m, n, k;
+    linear_sizes(product, M, N, K, &m, &n, &k);
+    float as_is, aligned;
+    dopt::linear_tile(product, m, n, k, true, true, &as_is);
+    dopt::linear_tile(product, m, n, k, false, true, &aligned);
+    if (product == DOPT_LIN_WEIGHT_GRAD && linear_dw_shape(M, N, (K + 7) / 8 * 8)) {
+        const float split = linear_dw_split_us(M, N, (K + 7) / 8 * 8);
+        if (split < aligned) aligned = split + (K % 8 ? 3.0f : 0.0f);  // (the result's rows are cut to K)
+    }
+    return aligned + (float)copies * 2.5f + (float)elements * (4.0f / 3.0e6f) < as_is;
+}
+
 int dopt_linear_forward(const void* x, int64_t ldx, const void* weight, int64_t ldw, int dtype, int64_t M, int64_t N,
                         int64_t K, const void* bias, int bias_dtype, const void* residual, int act, void* y, int y_dtype,
                         void* pre, void* stream) {
@@ -1173,9 +1233,9 @@ int dopt_linear_forward(const void* x, int64_t ldx, const void* weight, int64_t 
     if (bias)
         if (int rc = check_float(bias_dtype, "linear: the bias's type")) return rc;
     if (M == 0 || N == 0) return ok();
-    if (!y || (K > 0 && (!x || !weight))) return fail(DOPT_EINVAL, "null x/weight/y pointer");
-    if (K > 0 && (!lin_rows(x, ldx, K) || !lin_rows(weight, ldw, K)))
-        return fail(DOPT_EINVAL, "linear: x and weight must be 16-byte aligned, their row strides multiples of 8 and at least K rounded up to one");
+    if (!y) return fail(DOPT_EINVAL, "null y pointer");
+    if (K > 0)
+        if (int rc = check_linear_rows(x, ldx, K, weight, ldw, K)) return rc;
     dopt::LinArgs p{};
     p.A = (const uint16_t*)x;
     p.B = (const uint16_t*)weight;
@@ -1192,7 +1252,7 @@ int dopt_linear_forward(const void* x, int64_t ldx, const void* weight, int64_t 
     p.y_f32 = y_dtype == DOPT_F32;
     p.pre = (uint16_t*)pre;
     (void)hipGetLastError();
-    dopt::launch_linear(p, false, dtype == DOPT_F16, (hipStream_t)stream);
+    dopt::launch_linear(p, dopt::LIN_NT, dtype == DOPT_F16, (hipStream_t)stream);
     return hip_status("linear_forward launch");
 }
 
@@ -1200,10 +1260,10 @@ int dopt_linear_input_grad(const void* dz, int64_t ldz, const void* weight, int6
                            int64_t K, const void* in_pre, int in_act, void* dx, void* stream) {
     if (int rc = check_linear(dtype, M, K, N, ldz, ldw, in_act)) return rc;
     if (M == 0 || K == 0) return ok();
-    if (!dx || (N > 0 && (!dz || !weight))) return fail(DOPT_EINVAL, "null dz/weight/dx pointer");
+    if (!dx) return fail(DOPT_EINVAL, "null dx pointer");
     if (in_act != DOPT_LIN_NONE && !in_pre) return fail(DOPT_EINVAL, "linear: in_act needs in_pre");
-    if (N > 0 && (!lin_rows(dz, ldz, N) || !lin_rows(weight, ldw, K)))
-        return fail(DOPT_EINVAL, "linear: dz and weight must be 16-byte aligned, their row strides multiples of 8 and at least N and K rounded up to one");
+    if (N > 0)
+        if (int rc = check_linear_rows(dz, ldz, N, weight, ldw, K)) return rc;
     dopt::LinArgs p{};
     p.A = (const uint16_t*)dz;
     p.B = (const uint16_t*)weight;
@@ -1216,7 +1276,7 @@ int dopt_linear_input_grad(const void* dz, int64_t ldz, const void* weight, int6
     p.act = in_act;
     p.y = dx;
     (void)hipGetLastError();
-    dopt::launch_linear(p, true, dtype == DOPT_F16, (hipStream_t)stream);
+    dopt::launch_linear(p, dopt::LIN_KN, dtype == DOPT_F16, (hipStream_t)stream);
     return hip_status("linear_input_grad launch");
 }
 
@@ -1225,49 +1285,60 @@ int dopt_linear_act_grad(const void* dy, int64_t ld_dy, const void* pre, int act
     if (int rc = check_linear(dtype, rows, cols, 0, 0, 0, act)) return rc;
     if (rows == 0 || cols == 0) return ok();
     if (!dy || !dz || (act != DOPT_LIN_NONE && !pre)) return fail(DOPT_EINVAL, "null dy/pre/dz pointer");
-    if (ld_dy < cols || !lin_rows(dz, ld_dz, cols))
-        return fail(DOPT_EINVAL, "linear: dz must be 16-byte aligned, its row stride a multiple of 8 and at least cols; dy's at least cols");
+    if (ld_dy < cols || (!lin_rows(dz, ld_dz, cols) && !(ld_dz == cols && ld_dy == cols && act != DOPT_LIN_NONE)))
+        return fail(DOPT_EINVAL, "linear: dz must be 16-byte aligned with a row stride that is a multiple of 8 and at least cols (or, with an "
+                                 "activation, as contiguous as dy); dy's stride must be at least cols");
     (void)hipGetLastError();
     dopt::launch_linear_act_grad((const uint16_t*)dy, ld_dy, (const uint16_t*)pre, act, dtype == DOPT_F16, rows, cols,
                                  (uint16_t*)dz, ld_dz, (hipStream_t)stream);
     return hip_status("linear_act_grad launch");
 }
 
-static bool linear_dw_shape(int64_t M, int64_t N, int64_t K) {
-    return M >= 0 && N > 0 && K > 0 && K % 8 == 0 && N < ((int64_t)1 << 20) && K < ((int64_t)1 << 20);
-}
-
 int64_t dopt_linear_weight_grad_workspace_floats(int64_t M, int64_t N, int64_t K) {
-    return linear_dw_shape(M, N, K) ? dopt::dw_any_workspace_floats(N, K, M) : 0;
+    return linear_dw_split(M, N, K) ? dopt::dw_any_workspace_floats(N, K, M) : 0;
 }
 
 int dopt_linear_weight_grad(const void* dz, int64_t ldz, const void* x, int64_t ldx, int dtype, int64_t M, int64_t N,
                             int64_t K, float* workspace, float* dw_f32, void* dw_16, float* db, void* db_16, void* stream) {
+    if (int rc = check_linear(dtype, N, K, M, ldz, ldx, DOPT_LIN_NONE)) return rc;
     if (db && db_16) return fail(DOPT_EINVAL, "linear: one bias gradient, db or db_16");
-    if (dtype != DOPT_F16 && dtype != DOPT_BF16)
-        return fail(DOPT_EINVAL, "linear: the operands must be DOPT_F16 or DOPT_BF16, got %d", dtype);
-    if (!linear_dw_shape(M, N, K))
-        return fail(DOPT_EUNSUPPORTED, "linear weight gradient needs N >= 1 and K a positive multiple of 8, both below 2^20 (got M=%lld N=%lld K=%lld)",
-                    (long long)M, (long long)N, (long long)K);
-    if ((M > 0 && (!dz || !x)) || !workspace || (!dw_f32 && !dw_16))
-        return fail(DOPT_EINVAL, "null dz/x/workspace/output pointer");
-    if (M > 0 && (!lin_rows(dz, ldz, N) || !lin_rows(x, ldx, K) || ldz >= ((int64_t)1 << 24) || ldx >= ((int64_t)1 << 24)))
-        return fail(DOPT_EINVAL, "linear: dz and x must be 16-byte aligned, their row strides multiples of 8, at least N and K rounded up to one and below 2^24");
-    if (((uintptr_t)workspace & 15u) || (dw_f32 && ((uintptr_t)dw_f32 & 15u)) || (dw_16 && ((uintptr_t)dw_16 & 7u)))
-        return fail(DOPT_EINVAL, "workspace / dw_f32 must be 16-byte and dw_16 8-byte aligned");
-    dopt::DwArgs a{};
-    a.dy = (const uint16_t*)dz;
-    a.ldd = ldz;
-    a.xh = (const uint16_t*)x;
-    a.ldx = ldx;
-    a.M = N;
-    a.N = K;
-    a.K = M;
-    a.partial = workspace;
-    a.f16 = dtype == DOPT_F16;
+    if (!dw_f32 == !dw_16) return fail(DOPT_EINVAL, "linear: one weight gradient, dw_f32 or dw_16");
+    if (N == 0 || K == 0) return fail(DOPT_EINVAL, "linear weight gradient needs N and K >= 1");
+    if (M > 0)
+        if (int rc = check_linear_rows(dz, ldz, N, x, ldx, K)) return rc;
+    const bool whole = M == 0 || (lin_rows(dz, ldz, N) && lin_rows(x, ldx, K));
     (void)hipGetLastError();
-    if (dopt::launch_dw_gemm(a, dopt::DW_B_BF16, dw_f32, (uint16_t*)dw_16, db, (uint16_t*)db_16, (hipStream_t)stream))
-        return fail(DOPT_EUNSUPPORTED, "no weight-gradient kernel for this shape");
+    if (whole && linear_dw_split(M, N, K) && ldz < ((int64_t)1 << 24) && ldx < ((int64_t)1 << 24)) {
+        if (!workspace) return fail(DOPT_EINVAL, "linear: null workspace");
+        if (((uintptr_t)workspace & 15u) || (dw_f32 && ((uintptr_t)dw_f32 & 15u)) || (dw_16 && ((uintptr_t)dw_16 & 7u)))
+            return fail(DOPT_EINVAL, "workspace / dw_f32 must be 16-byte and dw_16 8-byte aligned");
+        dopt::DwArgs a{};
+        a.dy = (const uint16_t*)dz;
+        a.ldd = ldz;
+        a.xh = (const uint16_t*)x;
+        a.ldx = ldx;
+        a.M = N;
+        a.N = K;
+        a.K = M;
+        a.partial = workspace;
+        a.f16 = dtype == DOPT_F16;
+        if (dopt::launch_dw_gemm(a, dopt::DW_B_BF16, dw_f32, (uint16_t*)dw_16, db, (uint16_t*)db_16, (hipStream_t)stream))
+            return fail(DOPT_EUNSUPPORTED, "no weight-gradient kernel for this shape");
+        return hip_status("linear_weight_grad launch");
+    }
+    dopt::LinArgs p{};
+    p.A = (const uint16_t*)dz;
+    p.B = (const uint16_t*)x;
+    p.M = N;
+    p.N = K;
+    p.K = M;
+    p.lda = ldz;
+    p.ldb = ldx;
+    p.y = dw_f32 ? (void*)dw_f32 : dw_16;
+    p.y_f32 = dw_f32 != nullptr;
+    p.db = db;
+    p.db16 = (uint16_t*)db_16;
+    dopt::launch_linear(p, dopt::LIN_TN, dtype == DOPT_F16, (hipStream_t)stream);
     return hip_status("linear_weight_grad launch");
 }
 

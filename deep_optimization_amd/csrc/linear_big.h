@@ -1,5 +1,5 @@
 // The products of linear_gemm.h for large results: persistent workgroups, BM x 256 tiles, one workgroup per CU. Same
-// operands and sums; N a multiple of 8, 16-byte aligned results, no fp32 result.
+// operands and sums; K >= 64, N a multiple of 8, 16-byte aligned results, no fp32 result.
 //
 // 4 waves (2 x 2) of (BM / 2) x 128 as 16 x 16 blocks: at 128 x 128 per wave a slab of 64 K is 128 MFMAs fed by 32 KB
 // of LDS reads, half of what 64 x 64 waves read per flop, and the slab pipeline never drains: the loads of a tile's first
@@ -30,7 +30,6 @@
 namespace dopt {
 
 typedef int lin_v8i_t __attribute__((ext_vector_type(8)));
-typedef uint32_t lin_v4u_t __attribute__((ext_vector_type(4)));
 
 template <int BM, bool KN, bool F16, int ACT>
 __global__ __launch_bounds__(256, 1) void lin_big_kernel(LinArgs p) {
@@ -43,6 +42,7 @@ __global__ __launch_bounds__(256, 1) void lin_big_kernel(LinArgs p) {
     __shared__ __attribute__((aligned(1024))) uint8_t sA1[BM * ROWB];
     __shared__ __attribute__((aligned(1024))) uint8_t sB0[BN * ROWB];
     __shared__ __attribute__((aligned(1024))) uint8_t sB1[BN * ROWB];
+    __shared__ __attribute__((aligned(16))) float s_bias[KN ? 1 : 2][KN ? 4 : BN];  // the columns' bias, of every other tile
 
     // ---- this workgroup's tiles: XCD x owns a contiguous range, its workgroups take every g_x-th of it
     const uint32_t tiles_m = p.tiles_m, tiles_n = p.tiles_n, n_tiles = tiles_m * tiles_n;
@@ -70,82 +70,99 @@ __global__ __launch_bounds__(256, 1) void lin_big_kernel(LinArgs p) {
     const int wm = wave >> 1, wn = wave & 1;
 
     // ---- global -> LDS slab loads: load j of wave w fills rows 8 (4 j + w) + lane / 8, position lane % 8 <- chunk
-    // (lane % 8) ^ f(row). An operand's resource ends with its last row: rows past M (N) read zeros.
+    // (lane % 8) ^ f(row). Rows past M (N) lie past the operand's end and read zeros.
     const int r0 = 8 * wave + (lane >> 3);
     const int lchunk = (lane & 7) ^ ((wave & 1) | (((lane >> 4) & 1) << 1) | (((lane >> 5) & 1) << 2));
     uint32_t offa[LA], offb[LB];
 #pragma unroll
     for (int j = 0; j < LA; ++j) offa[j] = (uint32_t)((32 * j + r0) * lda + lchunk * 8) * 2u;
-    int kcol[KN ? LB : 1];
     if constexpr (KN) {
         constexpr int CPR = BN / 8, RPL = 64 / CPR;  // 32 chunks a row, 2 rows per load
 #pragma unroll
         for (int j = 0; j < LB; ++j) {
             const int k = RPL * (4 * j + wave) + lane / CPR;
-            kcol[j] = ((lane % CPR) ^ ((k & 3) << 2)) * 8;
-            offb[j] = (uint32_t)(k * ldb + kcol[j]) * 2u;
+            offb[j] = (uint32_t)(k * ldb + ((lane % CPR) ^ ((k & 3) << 2)) * 8) * 2u;
         }
     } else {
 #pragma unroll
         for (int j = 0; j < LB; ++j) offb[j] = (uint32_t)((32 * j + r0) * ldb + lchunk * 8) * 2u;
     }
     struct IssueTile {
-        __amdgpu_buffer_rsrc_t ra, rb;
-        int64_t n0;
-        uint32_t dead;  // LIN_OOB past this workgroup's last tile
+        int64_t m0, n0;
+        bool live;  // false past this workgroup's last tile
     };
     auto issue_tile = [&](uint32_t i) __attribute__((always_inline)) {
         IssueTile t;
         uint32_t tm, tn;
-        const bool live = i < my;
-        coords(live ? i : my - 1, tm, tn);
-        const int64_t m0 = (int64_t)tm * BM;
+        t.live = i < my;
+        coords(t.live ? i : my - 1, tm, tn);
+        t.m0 = (int64_t)tm * BM;
         t.n0 = (int64_t)tn * BN;
-        t.dead = live ? 0u : LIN_OOB;
-        const int64_t left_a = min((M - m0) * lda * 2, (int64_t)LIN_RANGE);
-        t.ra = __builtin_amdgcn_make_buffer_rsrc((void*)(p.A + m0 * lda), (short)0, (int)left_a, 0x00020000);
-        if constexpr (!KN) {
-            const int64_t left_b = min((N - t.n0) * ldb * 2, (int64_t)LIN_RANGE);
-            t.rb = __builtin_amdgcn_make_buffer_rsrc((void*)(p.B + t.n0 * ldb), (short)0, (int)left_b, 0x00020000);
-        }
         return t;
     };
     IssueTile cur_t = issue_tile(0), next_t = issue_tile(1);
-    // slab ks of the compute side's tile, or from nk on of the next one; parts: A's loads (1), B's (2) or both
+    // a column's bias for each thread, read a tile ahead (one register, as it lies in memory) and handed to the epilogue
+    // through LDS
+    auto load_bias = [&](int64_t n0) __attribute__((always_inline)) -> uint32_t {
+        uint32_t v = 0;
+        if constexpr (!KN) {
+            if (p.bias && n0 + tid < N) {
+                if (p.bias_dt == DT_F32) v = ((const uint32_t*)p.bias)[n0 + tid];
+                else v = ((const uint16_t*)p.bias)[n0 + tid];
+            }
+        }
+        return v;
+    };
+    auto bias_value = [&](uint32_t v) __attribute__((always_inline)) -> float {
+        return p.bias_dt == DT_F32 ? __uint_as_float(v)
+                                   : p.bias_dt == DT_BF16 ? __uint_as_float(v << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)v);
+    };
+    if constexpr (!KN) s_bias[0][tid] = bias_value(load_bias(cur_t.n0));
+    uint32_t next_bias = load_bias(next_t.n0);
+    // slab ks of the compute side's tile, or from nk on of the next one; parts: A's loads (1), B's (2) or both. The range
+    // of a slab ends with the operand's last element and is empty past K and past the last tile; the lanes' offsets
+    // never change (see linear_gemm.h).
     auto issue = [&](uint8_t* sa, uint8_t* sb, uint32_t ks, int parts = 3) __attribute__((always_inline)) {
         const bool nxt = ks >= nk;
-        const uint32_t dead = nxt ? next_t.dead : cur_t.dead;
         const uint32_t k0 = (nxt ? ks - nk : ks) * LIN_BK;
-        const uint32_t past = (k0 + (uint32_t)lchunk * 8 < K ? 0u : LIN_OOB) | dead;
+        const bool live = (nxt ? next_t.live : cur_t.live) && k0 < K;
         if (parts & 1) {
-            const __amdgpu_buffer_rsrc_t ra = nxt ? next_t.ra : cur_t.ra;
+            const int64_t m0 = nxt ? next_t.m0 : cur_t.m0;
+            const int64_t left = 2 * ((M - 1 - m0) * lda + ((int64_t)K + 7) / 8 * 8 - k0);
+            const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(
+                (void*)(p.A + m0 * lda + k0), (short)0, live ? (int)min(left, (int64_t)LIN_RANGE) : 0, 0x00020000);
 #pragma unroll
             for (int j = 0; j < LA; ++j) {
-                const uint32_t off = offa[j] | past;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lin_lds_t*)(sa + wave * 1024 + j * 4096), 16, off, (int)(2 * k0), 0, 0);
+                const uint32_t off = offa[j];
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lin_lds_t*)(sa + wave * 1024 + j * 4096), 16, off, 0, 0, 0);
             }
         }
         if (parts & 2) {
-            if constexpr (KN) {
-                const int64_t n0 = nxt ? next_t.n0 : cur_t.n0;
-                const int64_t left = k0 < K && !dead ? 2 * ((int64_t)(K - 1 - k0) * ldb + (N + 7) / 8 * 8 - n0) : 0;
-                const int range = left < (int64_t)LIN_RANGE ? (int)left : (int)LIN_RANGE;
-                const __amdgpu_buffer_rsrc_t rk =
-                    __builtin_amdgcn_make_buffer_rsrc((void*)(p.B + (int64_t)k0 * ldb + n0), (short)0, range, 0x00020000);
+            const int64_t n0 = nxt ? next_t.n0 : cur_t.n0;
+            const int64_t left = KN ? 2 * (((int64_t)K - 1 - k0) * ldb + N - n0) : 2 * ((N - 1 - n0) * ldb + ((int64_t)K + 7) / 8 * 8 - k0);
+            const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(
+                (void*)(p.B + (KN ? (int64_t)k0 * ldb + n0 : n0 * ldb + k0)), (short)0, live ? (int)min(left, (int64_t)LIN_RANGE) : 0, 0x00020000);
 #pragma unroll
-                for (int j = 0; j < LB; ++j) {
-                    const uint32_t off = n0 + kcol[j] < N ? offb[j] : LIN_OOB;
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lin_lds_t*)(sb + wave * 1024 + j * 4096), 16, off, 0, 0, 0);
-                }
-            } else {
-                const __amdgpu_buffer_rsrc_t rb = nxt ? next_t.rb : cur_t.rb;
-#pragma unroll
-                for (int j = 0; j < LB; ++j) {
-                    const uint32_t off = offb[j] | past;
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lin_lds_t*)(sb + wave * 1024 + j * 4096), 16, off, (int)(2 * k0), 0, 0);
-                }
+            for (int j = 0; j < LB; ++j) {
+                const uint32_t off = offb[j];
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lin_lds_t*)(sb + wave * 1024 + j * 4096), 16, off, 0, 0, 0);
             }
         }
+    };
+    // the slab that K ends in: what its rows hold past K is zeroed in LDS before its first read (see linear_gemm.h)
+    const uint32_t k_last = K % LIN_BK ? K / LIN_BK : 0xFFFFFFFFu;
+    auto cut = [&](uint8_t* sa, uint8_t* sb) __attribute__((always_inline)) {
+        const int have = (int)(K % LIN_BK) - lchunk * 8;  // of this lane's chunks
+        if (have < 8) {
+#pragma unroll
+            for (int j = 0; j < LA; ++j) lin_cut8(sa + wave * 1024 + j * 4096 + lane * 16, have);
+            if constexpr (!KN) {
+#pragma unroll
+                for (int j = 0; j < LB; ++j) lin_cut8(sb + wave * 1024 + j * 4096 + lane * 16, have);
+            }
+        }
+        __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4));  // lgkmcnt(0)
+        asm volatile("s_barrier" ::: "memory");
     };
 
     // ---- operands
@@ -162,11 +179,11 @@ __global__ __launch_bounds__(256, 1) void lin_big_kernel(LinArgs p) {
     const int cv = lane & 3, cu = (lane & 15) >> 2;
     const int crow = (16 * (lane >> 4) + cu) * (2 * BN), csw = cu << 2;
     auto read_cols = [&](const uint8_t* s, int base) __attribute__((always_inline)) -> lin_v8i_t {
-        const uint8_t* q = s + (crow + ((((base + 4 * cv) >> 3) ^ csw) << 4) + 8 * (cv & 1));
+        const int o = crow + ((((base + 4 * cv) >> 3) ^ csw) << 4) + 8 * (cv & 1);
         lin_v2u_t x[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            x[i] = __builtin_bit_cast(lin_v2u_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lin_lds_v4s_t*)(q + 4 * i * (2 * BN))));
+            x[i] = __builtin_bit_cast(lin_v2u_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lin_lds_v4s_t*)(s + (o + 4 * i * (2 * BN)))));
         return lin_v8i_t{(int)x[0].x, (int)x[0].y, (int)x[1].x, (int)x[1].y, (int)x[2].x, (int)x[2].y, (int)x[3].x, (int)x[3].y};
     };
     auto read_a = [&](const uint8_t* s, int i) __attribute__((always_inline)) { return read_rows(s, WM * wm + 16 * i); };
@@ -213,8 +230,18 @@ __global__ __launch_bounds__(256, 1) void lin_big_kernel(LinArgs p) {
 #pragma unroll
         for (int jp = 0; jp < FN / 2; ++jp) {
             vo[jp] = col0 + 32 * jp + col < N ? (uint32_t)(ln & 15) * pitch + (uint32_t)(32 * jp + col) * 2u : LIN_OOB;
-            if constexpr (!KN) lin_bias8(p, col0 + 32 * jp + col, bias[jp]);
+            if constexpr (!KN) {
+                const float* b = &s_bias[i_tile & 1][WN * wn + 32 * jp + col];
+                const lin_v4f_t x = *(const lin_v4f_t*)b, y = *(const lin_v4f_t*)(b + 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    bias[jp][e] = x[e];
+                    bias[jp][4 + e] = y[e];
+                }
+            }
         }
+        // (read after the next tile's barriers)
+        if constexpr (!KN) s_bias[(i_tile + 1) & 1][tid] = bias_value(next_bias);
         lin_v4u_t side_v[2][FN / 2];
         auto load_side = [&](int i) __attribute__((always_inline)) {
             if (has_res) {
@@ -300,6 +327,9 @@ __global__ __launch_bounds__(256, 1) void lin_big_kernel(LinArgs p) {
         if constexpr (EPI) __builtin_amdgcn_s_waitcnt(WAIT2E);
         else __builtin_amdgcn_s_waitcnt(WAIT2);
         asm volatile("s_barrier" ::: "memory");
+        if constexpr (!LAST) {
+            if (k + 1 == k_last) cut(na, nb);
+        }
         issue(sa, sb, k + 2, 1);
         if constexpr (!LAST) {
 #pragma unroll
@@ -356,6 +386,7 @@ __global__ __launch_bounds__(256, 1) void lin_big_kernel(LinArgs p) {
         read_first(sA0, sB0);
         cur_t = next_t;
         next_t = issue_tile(it + 1);
+        next_bias = load_bias(next_t.n0);
         head();
         slab(sA0, sB0, sA1, sB1, 0, BF{}, BT{});
         head();

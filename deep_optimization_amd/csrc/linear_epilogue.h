@@ -9,18 +9,21 @@
 
 namespace dopt {
 
+enum { LIN_NT = 0, LIN_KN = 1, LIN_TN = 2 };  // the products (linear_gemm.h)
 enum { LIN_NONE = 0, LIN_RELU = 1, LIN_GELU = 2, LIN_GELU_TANH = 3, LIN_SILU = 4 };
 
 struct LinArgs {
-    const uint16_t *A, *B;     // A [M][lda]; B [N][ldb] (NT) or [K][ldb] (KN)
+    const uint16_t *A, *B;     // A [M][lda] (LIN_TN: [K][lda]); B [N][ldb] (LIN_NT) or [K][ldb]
     int64_t M, N, K, lda, ldb;  // K: of the sum
     uint32_t tiles_m, tiles_n;  // set by the launcher
     // the rest: [M][N] rows without padding, or null
     const void* bias;     // [N], of dtype bias_dt
     const void* res;      // of y's type
-    const uint16_t* aux;  // KN: the argument of the activation whose derivative multiplies the result
+    const uint16_t* aux;  // LIN_KN: the argument of the activation whose derivative multiplies the result
     void* y;
     uint16_t* pre;        // the activation's argument
+    float* db;            // LIN_TN: the sums of A's columns, in fp32 or (db16) in the operands' type
+    uint16_t* db16;
     int bias_dt, act, y_f32;
 };
 
@@ -135,12 +138,15 @@ __device__ __forceinline__ void lin_bias8(const LinArgs& p, int64_t n, float* b)
 }
 
 // row m, columns n .. n + 7 (those below N) of the result from the sums v
-template <bool KN, bool F16>
+template <int KIND, bool F16>
 __device__ __forceinline__ void lin_finish8(const LinArgs& p, int64_t m, int64_t n, const float* bias, float* v) {
     constexpr int DT = F16 ? DT_F16 : DT_BF16;
     const int64_t i = m * p.N + n;
     const int have = (int)min((int64_t)8, p.N - n);
-    if constexpr (KN) {
+    if constexpr (KIND == LIN_TN) {
+        if (p.y_f32) lin_store8<DT_F32>(p.y, i, have, v);
+        else lin_store8<DT>(p.y, i, have, v);
+    } else if constexpr (KIND == LIN_KN) {
         if (p.act != LIN_NONE) {
             float z[8];
             lin_load8<DT>(p.aux, i, have, z);

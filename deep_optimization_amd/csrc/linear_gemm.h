@@ -1,22 +1,24 @@
 // The products of a Linear layer in bf16 or fp16 on CDNA4 MFMA, fp32 sums, with the work around them in the epilogue:
 //
-//   NT (forward)         z = sum_k A[m][k] B[n][k] + bias[n];  pre = z;  y = act(z) + residual   (A = x, B = weight)
-//   KN (input gradient)  y = (sum_k A[m][k] B[k][n]) * act'(aux[m][n])                           (A = dz, B = weight)
+//   LIN_NT (forward)          z = sum_k A[m][k] B[n][k] + bias[n];  pre = z;  y = act(z) + residual  (A = x, B = weight)
+//   LIN_KN (input gradient)   y = (sum_k A[m][k] B[k][n]) * act'(aux[m][n])                          (A = dz, B = weight)
+//   LIN_TN (weight gradient)  y = sum_k A[k][m] B[k][n],  db[m] = sum_k A[k][m]                      (A = dz, B = x)
 //
-// Any M, N >= 0; A's rows and B's start at multiples of 16 bytes and hold whole 8-element chunks (a row of K = 13 has
-// 16 elements, the last 3 zero); the results' rows lie at any element.
+// Any M, N >= 0 and result rows at any element. Operands whose rows start at multiples of 16 bytes and lie 16 readable
+// elements apart for a length of 13 (and so on) go straight to LDS (buffer_load ... lds). The REG instances
+// take rows at any element without padding: they load through registers, where the chunk that crosses a row's
+// end is read element by element, one slab further ahead.
 //
 // Tiling: BM x BN for a workgroup of 4 waves (2 x 2) as 16 x 16 blocks of v_mfma_f32_16x16x32; K in slabs of 64 (128
 // bytes a row) through a ring of S LDS stages, S - 1 slabs ahead. A slab goes straight to LDS (buffer_load ... lds);
-// a lane whose row lies past M (N) or whose 8 elements lie past K gets an offset past the resource's range, which
-// reads zeros, so nothing else is masked before the stores. Per slab and wave:
+// a lane whose row lies past M (N) has an offset past the resource's range, which reads zeros. Per slab and wave:
 //   operand reads of half 1 | MFMAs of half 0 | wait: own loads of slab k+1 landed, own reads returned | barrier |
 //   issue slab k+S into slab k's stage | operand reads of slab k+1, half 0 | MFMAs of half 1
 //
 // LDS: 16-byte chunk c of row r lies at c ^ ((r / 2) % 8): the 16 rows that 16 lanes read at once fall into the 16
-// different bank groups of two 128-byte rows. KN: B's slab lies as it is in memory, 64 rows of BN columns, and
+// different bank groups of two 128-byte rows. [K] rows lie in LDS as they are in memory, 64 rows of BN (BM) columns, and
 // ds_read_b64_tr_b16 hands 16 lanes a 4 x 16 block by columns (two make a fragment); chunk c of row r at
-// c ^ (4 (r % 4)) (BN = 64: c ^ (4 ((r / 2) % 2))), which puts those 4 rows on different banks.
+// c ^ (4 (r % 4)) (64 columns: c ^ (4 ((r / 2) % 2))), which puts those 4 rows on different banks.
 //
 // The MFMA takes B's fragment first, so lane l holds row 16 i + l % 16 and columns 16 j + 4 (l / 16) + {0..3} of
 // block (i, j).
@@ -34,6 +36,7 @@ namespace dopt {
 typedef int lin_v4i_t __attribute__((ext_vector_type(4)));
 typedef float lin_v4f_t __attribute__((ext_vector_type(4)));
 typedef uint32_t lin_v2u_t __attribute__((ext_vector_type(2)));
+typedef uint32_t lin_v4u_t __attribute__((ext_vector_type(4)));
 typedef short lin_v4s_t __attribute__((ext_vector_type(4)));
 typedef __bf16 lin_bf16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 lin_f16x8_t __attribute__((ext_vector_type(8)));
@@ -52,6 +55,17 @@ __device__ __forceinline__ lin_v4f_t lin_mfma(const lin_v4i_t& a, const lin_v4i_
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(lin_bf16x8_t, a), __builtin_bit_cast(lin_bf16x8_t, b), c, 0, 0, 0);
 }
 
+// s + the two elements of a dword
+template <bool F16>
+__device__ __forceinline__ float lin_dot_ones(uint32_t w, float s) {
+    if constexpr (F16) {
+        typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, w), __builtin_bit_cast(f16x2_t, 0x3c003c00u), s, false);
+    } else {
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w), __builtin_bit_cast(bf16x2_t, 0x3f803f80u), s, false);
+    }
+}
+
 // The tile of a workgroup: XCD x (workgroup ids x, x + 8, ...) owns a contiguous range of tiles, walked GROUP_M tile
 // rows at a time, so that the rows of A and B that one XCD reads stay in its L2.
 __device__ __forceinline__ void lin_tile(const LinArgs& p, uint32_t bid, uint32_t& tm, uint32_t& tn) {
@@ -66,8 +80,44 @@ __device__ __forceinline__ void lin_tile(const LinArgs& p, uint32_t bid, uint32_
     tn = (t % group) / gsize;
 }
 
-template <int BM, int BN, int S, int PER_CU, bool KN, bool F16>
-__global__ __launch_bounds__(256, PER_CU) void lin_gemm_kernel(LinArgs p) {
+// 8 elements from element i of a matrix of `total` elements on (those past its end read as zeros); rows at any element
+__device__ __forceinline__ lin_v4u_t lin_load8u(const uint16_t* p, int64_t i, int64_t total) {
+    lin_v4u_t v;
+    if (!wave_any(i + 8 > total)) {
+        __builtin_memcpy(&v, p + i, 16);
+    } else {
+        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (i + e < total) w[e >> 1] |= (uint32_t)p[i + e] << (16 * (e & 1));
+        v = lin_v4u_t{w[0], w[1], w[2], w[3]};
+    }
+    return v;
+}
+// the first `have` elements of v, zeros after them
+__device__ __forceinline__ lin_v4u_t lin_keep(const lin_v4u_t& v, int64_t have) {
+    lin_v4u_t r;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) r[k] = v[k] & (have >= 2 * k + 2 ? 0xFFFFFFFFu : have == 2 * k + 1 ? 0xFFFFu : 0u);
+    return r;
+}
+
+// a chunk in LDS, cut to its first `have` elements (all zeros for have <= 0)
+__device__ __forceinline__ void lin_cut8(uint8_t* p, int have) { *(lin_v4u_t*)p = lin_keep(*(const lin_v4u_t*)p, have); }
+
+// position of chunk c of row r of an operand slab that lies in LDS as 64 rows of W columns
+template <int W>
+__device__ __forceinline__ int lin_col_swizzle(int r) {
+    return W == 32 ? 0 : W == 64 ? ((r >> 1) & 1) << 2 : (r & 3) << 2;
+}
+
+// bytes of the smaller of a stage's two operand slabs
+constexpr int wave_part(int bm, int bn) { return (bm < bn ? bm : bn) * 2 * LIN_BK; }
+
+template <int BM, int BN, int S, int KS, int WAVES, int KIND, bool F16, bool REG, bool TAIL>
+__global__ __launch_bounds__(256 * KS, WAVES) void lin_gemm_kernel(LinArgs p) {
+    constexpr bool A_COLS = KIND == LIN_TN, B_COLS = KIND != LIN_NT;  // the operand lies as [K] rows
+    static_assert(!REG || S == 2, "register loads: one slab in registers, two in LDS");
     constexpr int ROWB = 2 * LIN_BK, WM = BM / 2, WN = BN / 2, FM = WM / 16, FN = WN / 16;
     constexpr int LA = BM / 32, LB = BN / 32, LD = LA + LB;  // 1 KB loads per wave and slab
     static_assert(S >= 2 && S <= 4 && (S - 1) * LD < 64, "stages, vmcnt range");
@@ -75,92 +125,177 @@ __global__ __launch_bounds__(256, PER_CU) void lin_gemm_kernel(LinArgs p) {
     const uint32_t K = (uint32_t)p.K;
     // every stage's A and B tiles are LDS objects of their own, so the compiler can tell an operand read from the
     // loads in flight
-    __shared__ __attribute__((aligned(1024))) uint8_t sA0[BM * ROWB];
-    __shared__ __attribute__((aligned(1024))) uint8_t sA1[BM * ROWB];
-    __shared__ __attribute__((aligned(1024))) uint8_t sA2[S > 2 ? BM * ROWB : 16];
-    __shared__ __attribute__((aligned(1024))) uint8_t sA3[S > 3 ? BM * ROWB : 16];
-    __shared__ __attribute__((aligned(1024))) uint8_t sB0[BN * ROWB];
-    __shared__ __attribute__((aligned(1024))) uint8_t sB1[BN * ROWB];
-    __shared__ __attribute__((aligned(1024))) uint8_t sB2[S > 2 ? BN * ROWB : 16];
-    __shared__ __attribute__((aligned(1024))) uint8_t sB3[S > 3 ? BN * ROWB : 16];
+    __shared__ __attribute__((aligned(1024))) uint8_t sA0[KS * BM * ROWB];
+    __shared__ __attribute__((aligned(1024))) uint8_t sA1[KS * BM * ROWB];
+    __shared__ __attribute__((aligned(1024))) uint8_t sA2[S > 2 ? KS * BM * ROWB : 16];
+    __shared__ __attribute__((aligned(1024))) uint8_t sA3[S > 3 ? KS * BM * ROWB : 16];
+    __shared__ __attribute__((aligned(1024))) uint8_t sB0[KS * BN * ROWB];
+    __shared__ __attribute__((aligned(1024))) uint8_t sB1[KS * BN * ROWB];
+    __shared__ __attribute__((aligned(1024))) uint8_t sB2[S > 2 ? KS * BN * ROWB : 16];
+    __shared__ __attribute__((aligned(1024))) uint8_t sB3[S > 3 ? KS * BN * ROWB : 16];
+    // KS > 1: that many groups of 4 waves, each with its own ring, take every KS-th slab
+    const int wave_id = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int group = KS > 1 ? wave_id >> 2 : 0, wave = wave_id & 3;
     auto stage_a = [&](auto i) __attribute__((always_inline)) -> uint8_t* {
         constexpr int I = decltype(i)::value % S;
-        if constexpr (I == 0) return sA0;
-        else if constexpr (I == 1) return sA1;
-        else if constexpr (I == 2) return sA2;
-        else return sA3;
+        if constexpr (I == 0) return sA0 + (KS > 1 ? group * (BM * ROWB) : 0);
+        else if constexpr (I == 1) return sA1 + (KS > 1 ? group * (BM * ROWB) : 0);
+        else if constexpr (I == 2) return sA2 + (KS > 1 ? group * (BM * ROWB) : 0);
+        else return sA3 + (KS > 1 ? group * (BM * ROWB) : 0);
     };
     auto stage_b = [&](auto i) __attribute__((always_inline)) -> uint8_t* {
         constexpr int I = decltype(i)::value % S;
-        if constexpr (I == 0) return sB0;
-        else if constexpr (I == 1) return sB1;
-        else if constexpr (I == 2) return sB2;
-        else return sB3;
+        if constexpr (I == 0) return sB0 + (KS > 1 ? group * (BN * ROWB) : 0);
+        else if constexpr (I == 1) return sB1 + (KS > 1 ? group * (BN * ROWB) : 0);
+        else if constexpr (I == 2) return sB2 + (KS > 1 ? group * (BN * ROWB) : 0);
+        else return sB3 + (KS > 1 ? group * (BN * ROWB) : 0);
     };
 
     uint32_t tm, tn;
     lin_tile(p, blockIdx.x, tm, tn);
     const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave >> 1, wn = wave & 1;
 
     // ---- global -> LDS: load j of wave w fills rows 8 (4 j + w) + lane / 8, position lane % 8 <- chunk
     // (lane % 8) ^ ((row / 2) % 8), where (row / 2) % 8 = 4 (w % 2) + lane / 16
     const int lrow = 8 * wave + (lane >> 3);
     const int lchunk = (lane & 7) ^ (4 * (wave & 1) + (lane >> 4));
-    const __amdgpu_buffer_rsrc_t ra =
-        __builtin_amdgcn_make_buffer_rsrc((void*)(p.A + m0 * lda), (short)0, (int)LIN_RANGE, 0x00020000);
-    const __amdgpu_buffer_rsrc_t rb =
-        __builtin_amdgcn_make_buffer_rsrc((void*)(p.B + (KN ? 0 : n0 * ldb)), (short)0, (int)LIN_RANGE, 0x00020000);
+    // an operand of [K] rows: load j of wave w fills rows k = RPL (4 j + w) + lane / CPR, position lane % CPR <- chunk
+    // (lane % CPR) ^ swizzle(k)
+    constexpr int CPR_A = BM / 8, RPL_A = 64 / CPR_A, CPR_B = BN / 8, RPL_B = 64 / CPR_B;
+    auto krow_a = [&](int j) __attribute__((always_inline)) { return RPL_A * (4 * j + wave) + lane / CPR_A; };
+    auto kcol_a = [&](int j) __attribute__((always_inline)) { return ((lane % CPR_A) ^ lin_col_swizzle<BM>(krow_a(j))) * 8; };
+    auto krow_b = [&](int j) __attribute__((always_inline)) { return RPL_B * (4 * j + wave) + lane / CPR_B; };
+    auto kcol_b = [&](int j) __attribute__((always_inline)) { return ((lane % CPR_B) ^ lin_col_swizzle<BN>(krow_b(j))) * 8; };
     uint32_t offa[LA], offb[LB];
 #pragma unroll
-    for (int j = 0; j < LA; ++j)
-        offa[j] = m0 + 32 * j + lrow < M ? (uint32_t)((32 * j + lrow) * lda + lchunk * 8) * 2u : LIN_OOB;
-    if constexpr (KN) {
-        constexpr int CPR = BN / 8, RPL = 64 / CPR;  // chunks per row, rows per load
+    for (int j = 0; j < LA; ++j) {
+        if constexpr (A_COLS) offa[j] = m0 + kcol_a(j) < M ? (uint32_t)(krow_a(j) * lda + kcol_a(j)) * 2u : LIN_OOB;
+        else offa[j] = m0 + 32 * j + lrow < M ? (uint32_t)((32 * j + lrow) * lda + lchunk * 8) * 2u : LIN_OOB;
+    }
 #pragma unroll
-        for (int j = 0; j < LB; ++j) {
-            const int k = RPL * (4 * j + wave) + lane / CPR;
-            const int sw = CPR == 8 ? ((k >> 1) & 1) << 2 : (k & 3) << 2;
-            const int col = ((lane % CPR) ^ sw) * 8;
-            offb[j] = n0 + col < N ? (uint32_t)(k * ldb + col) * 2u : LIN_OOB;
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < LB; ++j)
-            offb[j] = n0 + 32 * j + lrow < N ? (uint32_t)((32 * j + lrow) * ldb + lchunk * 8) * 2u : LIN_OOB;
+    for (int j = 0; j < LB; ++j) {
+        if constexpr (B_COLS) offb[j] = n0 + kcol_b(j) < N ? (uint32_t)(krow_b(j) * ldb + kcol_b(j)) * 2u : LIN_OOB;
+        else offb[j] = n0 + 32 * j + lrow < N ? (uint32_t)((32 * j + lrow) * ldb + lchunk * 8) * 2u : LIN_OOB;
     }
     // (the LDS offsets carry a zero that the compiler cannot see through: a read that it could prove disjoint from
     // the one load it records per LDS object would wait for every load in flight)
     int opaque0;
     asm volatile("s_mov_b32 %0, 0" : "=s"(opaque0));
+    // A slab's part of an operand. The lanes' offsets never change: an address in a register that is soon overwritten by
+    // an operand read would make the compiler wait for the load there.
+    // TAIL (K is no multiple of 64): the range of the slab that K ends in ends with the operand's last element; its base
+    // steps, where rows of K otherwise keep theirs and step in soffset. A slab past K loads the last one again, which
+    // nobody multiplies (KS > 1: zeros, which are).
+    const uint32_t n_slabs = (K + LIN_BK - 1) / LIN_BK, k_end = TAIL ? K / LIN_BK : 0xFFFFFFFFu;
+    const auto slab_range = [&](int64_t left, uint32_t ks) __attribute__((always_inline)) {
+        const int range = TAIL ? (int)max((int64_t)0, min(left, (int64_t)LIN_RANGE)) : (int)LIN_RANGE;
+        return KS > 1 ? range & -(int)(ks < n_slabs) : range;
+    };
+    auto rows_slab = [&](const uint16_t* base, int64_t ld, int64_t rows, int64_t r0, uint32_t ks) __attribute__((always_inline)) {
+        const int64_t k0 = TAIL && ks == k_end ? (int64_t)ks * LIN_BK : 0;
+        const int range = slab_range(2 * ((rows - 1 - r0) * ld + ((int64_t)K + 7) / 8 * 8 - k0), ks);
+        return __builtin_amdgcn_make_buffer_rsrc((void*)(base + r0 * ld + k0), (short)0, range, 0x00020000);
+    };
+    auto cols_slab = [&](const uint16_t* base, int64_t ld, int64_t cols, int64_t c0, uint32_t ks) __attribute__((always_inline)) {
+        const int64_t k0 = (int64_t)ks * LIN_BK;
+        const int range = slab_range(2 * (((int64_t)K - 1 - k0) * ld + (cols + 7) / 8 * 8 - c0), ks);
+        return __builtin_amdgcn_make_buffer_rsrc((void*)(base + k0 * ld + c0), (short)0, range, 0x00020000);
+    };
+    // REG: two slabs on their way to LDS. A lane whose row or columns lie past the matrix reads row or column 0 (its
+    // results are not stored); what lies past K is zeroed on the way to LDS.
+    lin_v4u_t va[2][REG ? LA : 1], vb[2][REG ? LB : 1];
+    const uint16_t *pa[REG ? LA : 1], *pb[REG ? LB : 1];  // this group's next slab's chunks
+    if constexpr (REG) {
+        const int64_t k0 = (int64_t)group * LIN_BK;
+#pragma unroll
+        for (int j = 0; j < LA; ++j)
+            pa[j] = p.A + (A_COLS ? (k0 + krow_a(j)) * lda + (offa[j] != LIN_OOB ? m0 + kcol_a(j) : 0)
+                                  : (offa[j] != LIN_OOB ? m0 + 32 * j + lrow : 0) * lda + k0 + lchunk * 8);
+#pragma unroll
+        for (int j = 0; j < LB; ++j)
+            pb[j] = p.B + (B_COLS ? (k0 + krow_b(j)) * ldb + (offb[j] != LIN_OOB ? n0 + kcol_b(j) : 0)
+                                  : (offb[j] != LIN_OOB ? n0 + 32 * j + lrow : 0) * ldb + k0 + lchunk * 8);
+    }
+    auto load_regs = [&](auto set, uint32_t k) __attribute__((always_inline)) {
+        if constexpr (REG) {
+            constexpr int Q = decltype(set)::value & 1;
+            const int64_t k0 = ((int64_t)k * KS + group) * LIN_BK;
+            // a chunk may run past its row's end, but with 8 rows (or elements of a row) more behind this slab not past
+            // the matrix's
+            if (k0 + LIN_BK + 8 < (int64_t)K) {
+#pragma unroll
+                for (int j = 0; j < LA; ++j) __builtin_memcpy(&va[Q][j], pa[j], 16);
+#pragma unroll
+                for (int j = 0; j < LB; ++j) __builtin_memcpy(&vb[Q][j], pb[j], 16);
+            } else {
+                const int64_t total_a = A_COLS ? ((int64_t)K - 1) * lda + M : (M - 1) * lda + K;
+                const int64_t total_b = B_COLS ? ((int64_t)K - 1) * ldb + N : (N - 1) * ldb + K;
+#pragma unroll
+                for (int j = 0; j < LA; ++j)
+                    va[Q][j] = lin_load8u(p.A, k0 + (A_COLS ? krow_a(j) : lchunk * 8) < (int64_t)K ? pa[j] - p.A : 0, total_a);
+#pragma unroll
+                for (int j = 0; j < LB; ++j)
+                    vb[Q][j] = lin_load8u(p.B, k0 + (B_COLS ? krow_b(j) : lchunk * 8) < (int64_t)K ? pb[j] - p.B : 0, total_b);
+            }
+#pragma unroll
+            for (int j = 0; j < LA; ++j) pa[j] += KS * LIN_BK * (A_COLS ? lda : 1);
+#pragma unroll
+            for (int j = 0; j < LB; ++j) pb[j] += KS * LIN_BK * (B_COLS ? ldb : 1);
+        }
+    };
+    auto write_regs = [&](auto set, uint8_t* sa, uint8_t* sb, uint32_t k) __attribute__((always_inline)) {
+        if constexpr (REG) {
+            constexpr int Q = decltype(set)::value & 1;
+            const int64_t k0 = ((int64_t)k * KS + group) * LIN_BK;
+            if (k0 + LIN_BK > (int64_t)K) {
+#pragma unroll
+                for (int j = 0; j < LA; ++j)
+                    va[Q][j] = lin_keep(va[Q][j], A_COLS ? (k0 + krow_a(j) < (int64_t)K ? 8 : 0) : (int64_t)K - k0 - lchunk * 8);
+#pragma unroll
+                for (int j = 0; j < LB; ++j)
+                    vb[Q][j] = lin_keep(vb[Q][j], B_COLS ? (k0 + krow_b(j) < (int64_t)K ? 8 : 0) : (int64_t)K - k0 - lchunk * 8);
+            }
+#pragma unroll
+            for (int j = 0; j < LA; ++j) *(lin_v4u_t*)(sa + wave * 1024 + j * 4096 + lane * 16) = va[Q][j];
+#pragma unroll
+            for (int j = 0; j < LB; ++j) *(lin_v4u_t*)(sb + wave * 1024 + j * 4096 + lane * 16) = vb[Q][j];
+        }
+    };
     auto issue = [&](uint8_t* sa, uint8_t* sb, uint32_t k) __attribute__((always_inline)) {
         uint8_t *da = sa + opaque0, *db = sb + opaque0;
-        const uint32_t k0 = k * LIN_BK;
-        const uint32_t past = k0 + (uint32_t)lchunk * 8 < K ? 0u : LIN_OOB;
+        const uint32_t want = k * KS + group, ks = KS > 1 ? want : min(want, n_slabs - 1);
+        const int step = TAIL && ks == k_end ? 0 : (int)(2 * LIN_BK * ks);
+        const __amdgpu_buffer_rsrc_t ra = A_COLS ? cols_slab(p.A, lda, M, m0, ks) : rows_slab(p.A, lda, M, m0, ks);
+        const __amdgpu_buffer_rsrc_t rb = B_COLS ? cols_slab(p.B, ldb, N, n0, ks) : rows_slab(p.B, ldb, N, n0, ks);
 #pragma unroll
         for (int j = 0; j < LA; ++j) {
-            const uint32_t off = offa[j] | past;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lin_lds_t*)(da + wave * 1024 + j * 4096), 16, off, (int)(2 * k0), 0, 0);
+            const uint32_t off = offa[j];
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lin_lds_t*)(da + wave * 1024 + j * 4096), 16, off, A_COLS ? 0 : step, 0, 0);
         }
-        if constexpr (KN) {
-            // the range ends with B's last row: rows past it read zeros
-            const int64_t left = k0 < K ? 2 * ((int64_t)(K - 1 - k0) * ldb + (N + 7) / 8 * 8 - n0) : 0;
-            const int range = left < (int64_t)LIN_RANGE ? (int)left : (int)LIN_RANGE;
-            const __amdgpu_buffer_rsrc_t rk =
-                __builtin_amdgcn_make_buffer_rsrc((void*)(p.B + (int64_t)k0 * ldb + n0), (short)0, range, 0x00020000);
 #pragma unroll
-            for (int j = 0; j < LB; ++j) {
-                const uint32_t off = offb[j];
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lin_lds_t*)(db + wave * 1024 + j * 4096), 16, off, 0, 0, 0);
-            }
-        } else {
+        for (int j = 0; j < LB; ++j) {
+            const uint32_t off = offb[j];
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lin_lds_t*)(db + wave * 1024 + j * 4096), 16, off, B_COLS ? 0 : step, 0, 0);
+        }
+    };
+    // The slab that K ends in, once it is in LDS and before its first read: what its rows hold past K (what lies between
+    // rows, the next row) is zeroed, each lane its own chunks. (Operands of [K] rows end there by their range.)
+    auto cut = [&](uint8_t* sa, uint8_t* sb, uint32_t k) __attribute__((always_inline)) {
+        if constexpr (TAIL && KIND != LIN_TN) {
+            if (k != k_end / KS) return;  // the same for the whole workgroup
+            const int have = (int)(K % LIN_BK) - lchunk * 8;  // of this lane's chunks
+            if (k * KS + group == k_end && have < 8) {
 #pragma unroll
-            for (int j = 0; j < LB; ++j) {
-                const uint32_t off = offb[j] | past;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lin_lds_t*)(db + wave * 1024 + j * 4096), 16, off, (int)(2 * k0), 0, 0);
+                for (int j = 0; j < LA; ++j) lin_cut8(sa + wave * 1024 + j * 4096 + lane * 16, have);
+                if constexpr (!B_COLS) {
+#pragma unroll
+                    for (int j = 0; j < LB; ++j) lin_cut8(sb + wave * 1024 + j * 4096 + lane * 16, have);
+                }
             }
+            __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+            asm volatile("s_barrier" ::: "memory");
         }
     };
 
@@ -170,13 +305,14 @@ __global__ __launch_bounds__(256, PER_CU) void lin_gemm_kernel(LinArgs p) {
     auto read_rows = [&](const uint8_t* s, int base, int h) __attribute__((always_inline)) -> lin_v4i_t {
         return *(const lin_v4i_t*)(s + ((base + orow) * ROWB + ((4 * h + (lane >> 4)) ^ sw) * 16));
     };
-    // KN: source lane 4 u + v of a group of 16 names row 32 h + 8 (l / 16) + 4 r + u and columns 4 v .. + 3
+    // [K] rows: source lane 4 u + v of a group of 16 names row 32 h + 8 (l / 16) + 4 r + u and columns 4 v .. + 3
     const int crow = 8 * (lane >> 4) + ((lane & 15) >> 2), cv = lane & 3;
-    const int csw = BN == 64 ? ((crow >> 1) & 1) << 2 : (crow & 3) << 2;
-    auto read_cols = [&](const uint8_t* s, int base, int h) __attribute__((always_inline)) -> lin_v4i_t {
-        const uint8_t* q = s + ((32 * h + crow) * (2 * BN) + ((((base + 4 * cv) >> 3) ^ csw) << 4) + 8 * (cv & 1));
-        const lin_v4s_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lin_lds_v4s_t*)q);
-        const lin_v4s_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lin_lds_v4s_t*)(q + 4 * (2 * BN)));
+    auto read_cols = [&](const uint8_t* s, auto width, int base, int h) __attribute__((always_inline)) -> lin_v4i_t {
+        constexpr int PITCH_B = 2 * decltype(width)::value;
+        // (one addition to the LDS object: past a depth of them the compiler no longer knows which object a read is of)
+        const int o = crow * PITCH_B + ((((base + 4 * cv) >> 3) ^ lin_col_swizzle<decltype(width)::value>(crow)) << 4) + 8 * (cv & 1);
+        const lin_v4s_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lin_lds_v4s_t*)(s + (o + 32 * h * PITCH_B)));
+        const lin_v4s_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lin_lds_v4s_t*)(s + (o + (32 * h + 4) * PITCH_B)));
         const lin_v2u_t a = __builtin_bit_cast(lin_v2u_t, x), b = __builtin_bit_cast(lin_v2u_t, y);
         return lin_v4i_t{(int)a.x, (int)a.y, (int)b.x, (int)b.y};
     };
@@ -185,27 +321,40 @@ __global__ __launch_bounds__(256, PER_CU) void lin_gemm_kernel(LinArgs p) {
     for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = lin_v4f_t{0.0f, 0.0f, 0.0f, 0.0f};
+    float col_sum[FM] = {};  // LIN_TN: the sums of A's columns, each lane its own K
     lin_v4i_t a0[FM], b0[FN], a1[FM], b1[FN];
     auto read_half = [&](const uint8_t* sa, const uint8_t* sb, int h, lin_v4i_t* a, lin_v4i_t* b) __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < FN; ++j) b[j] = KN ? read_cols(sb, WN * wn + 16 * j, h) : read_rows(sb, WN * wn + 16 * j, h);
+        for (int j = 0; j < FN; ++j) {
+            if constexpr (B_COLS) b[j] = read_cols(sb, std::integral_constant<int, BN>{}, WN * wn + 16 * j, h);
+            else b[j] = read_rows(sb, WN * wn + 16 * j, h);
+        }
 #pragma unroll
-        for (int i = 0; i < FM; ++i) a[i] = read_rows(sa, WM * wm + 16 * i, h);
+        for (int i = 0; i < FM; ++i) {
+            if constexpr (A_COLS) a[i] = read_cols(sa, std::integral_constant<int, BM>{}, WM * wm + 16 * i, h);
+            else a[i] = read_rows(sa, WM * wm + 16 * i, h);
+        }
     };
     auto mma = [&](const lin_v4i_t* a, const lin_v4i_t* b) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < FM; ++i)
 #pragma unroll
             for (int j = 0; j < FN; ++j) acc[i][j] = lin_mfma<F16>(b[j], a[i], acc[i][j]);
+        if constexpr (KIND == LIN_TN) {
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) col_sum[i] = lin_dot_ones<F16>((uint32_t)a[i][q], col_sum[i]);
+        }
     };
-    constexpr int NM = FM * FN, NR = FM + (KN ? 2 : 1) * FN;  // MFMAs and LDS reads per half
+    constexpr int NM = FM * FN, NR = (A_COLS ? 2 : 1) * FM + (B_COLS ? 2 : 1) * FN;  // MFMAs and LDS reads per half
     constexpr int RPM = (NR + NM - 1) / NM;
     constexpr int W = (S - 2) * LD, WAIT = (W & 15) | ((W >> 4) << 14) | (7 << 4);  // vmcnt(W), lgkmcnt(0)
     auto slab = [&](uint32_t k, auto at) __attribute__((always_inline)) {
         constexpr int I = decltype(at)::value;
         using Next = std::integral_constant<int, I + 1>;
         uint8_t *sa = stage_a(at), *sb = stage_b(at);
-        const uint8_t *na = stage_a(Next{}), *nb = stage_b(Next{});
+        uint8_t *na = stage_a(Next{}), *nb = stage_b(Next{});
         read_half(sa, sb, 1, a1, b1);
         mma(a0, b0);
 #pragma unroll
@@ -213,11 +362,22 @@ __global__ __launch_bounds__(256, PER_CU) void lin_gemm_kernel(LinArgs p) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);    // one MFMA
             __builtin_amdgcn_sched_group_barrier(0x100, RPM, 0);  // LDS reads
         }
-        __builtin_amdgcn_s_waitcnt(WAIT);
-        asm volatile("s_barrier" ::: "memory");
-        issue(sa, sb, k + S);
+        if constexpr (REG) {
+            // every wave's reads of slab k and writes of slab k+1 are complete: slab k+2 from the registers into slab
+            // k's stage, slab k+4 into those registers
+            __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+            asm volatile("s_barrier" ::: "memory");
+            write_regs(at, sa, sb, k + 2);
+            load_regs(at, k + 4);
+        } else {
+            __builtin_amdgcn_s_waitcnt(WAIT);
+            asm volatile("s_barrier" ::: "memory");
+            cut(na, nb, k + 1);
+            issue(sa, sb, k + S);
+        }
         read_half(na, nb, 0, a0, b0);
         mma(a1, b1);
+        if constexpr (REG) return;
 #pragma unroll
         for (int q = 0; q < NM; ++q) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
@@ -230,15 +390,26 @@ __global__ __launch_bounds__(256, PER_CU) void lin_gemm_kernel(LinArgs p) {
     using I2 = std::integral_constant<int, 2>;
     using I3 = std::integral_constant<int, 3>;
 
-    const uint32_t nk = (K + LIN_BK - 1) / LIN_BK;
+    const uint32_t nk = ((K + LIN_BK - 1) / LIN_BK + KS - 1) / KS;  // slabs of a group (those past K are zeros)
     if (nk > 0) {
-        issue(stage_a(I0{}), stage_b(I0{}), 0);
-        issue(stage_a(I1{}), stage_b(I1{}), 1);
-        if constexpr (S > 2) issue(stage_a(I2{}), stage_b(I2{}), 2);
-        if constexpr (S > 3) issue(stage_a(I3{}), stage_b(I3{}), 3);
-        constexpr int W0 = (S - 1) * LD;
-        __builtin_amdgcn_s_waitcnt((W0 & 15) | ((W0 >> 4) << 14) | (7 << 4));
+        if constexpr (REG) {
+            load_regs(I0{}, 0);
+            load_regs(I1{}, 1);
+            write_regs(I0{}, stage_a(I0{}), stage_b(I0{}), 0);
+            load_regs(I0{}, 2);
+            write_regs(I1{}, stage_a(I1{}), stage_b(I1{}), 1);
+            load_regs(I1{}, 3);
+            __builtin_amdgcn_s_waitcnt(0xC07F);
+        } else {
+            issue(stage_a(I0{}), stage_b(I0{}), 0);
+            issue(stage_a(I1{}), stage_b(I1{}), 1);
+            if constexpr (S > 2) issue(stage_a(I2{}), stage_b(I2{}), 2);
+            if constexpr (S > 3) issue(stage_a(I3{}), stage_b(I3{}), 3);
+            constexpr int W0 = (S - 1) * LD;
+            __builtin_amdgcn_s_waitcnt((W0 & 15) | ((W0 >> 4) << 14) | (7 << 4));
+        }
         asm volatile("s_barrier" ::: "memory");
+        cut(stage_a(I0{}), stage_b(I0{}), 0);
         read_half(stage_a(I0{}), stage_b(I0{}), 0, a0, b0);
         uint32_t k = 0;
         for (; k + S <= nk; k += S) {
@@ -260,11 +431,58 @@ __global__ __launch_bounds__(256, PER_CU) void lin_gemm_kernel(LinArgs p) {
     // ---- epilogue: up to 32 rows of the wave's tile at a time through LDS in fp32, then 8 columns of a row per lane
     constexpr int PITCH = WN + 4, RB = WM < 32 ? WM : 32;  // floats per staged row, rows at a time
     static_assert(RB * PITCH * 4 <= BM * ROWB && RB * PITCH * 4 <= BN * ROWB, "a wave's rows fit one LDS array");
-    float* st = (float*)(wave == 0 ? sA0 : wave == 1 ? sA1 : wave == 2 ? sB0 : sB1);
+    uint8_t* const mine = wave == 0 ? sA0 : wave == 1 ? sA1 : wave == 2 ? sB0 : sB1;
+    if constexpr (KS > 1) {
+        // the groups' sums, added in order by the first
+        constexpr int PART = wave_part(BM, BN), AREA = FM * FN * 1024 + (KIND == LIN_TN ? FM * 256 : 0);
+        static_assert(AREA <= PART && FM <= 4, "a wave's sums fit its part of an LDS array");
+        const int stride = wave < 2 ? BM * ROWB : BN * ROWB;
+        if (group > 0) {
+            uint8_t* out = mine + group * stride;
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) *(lin_v4f_t*)(out + (i * FN + j) * 1024 + lane * 16) = acc[i][j];
+            if constexpr (KIND == LIN_TN) {
+#pragma unroll
+                for (int i = 0; i < FM; ++i) *(float*)(out + FM * FN * 1024 + i * 256 + lane * 4) = col_sum[i];
+            }
+        }
+        __syncthreads();
+        if (group > 0) return;
+#pragma unroll
+        for (int g = 1; g < KS; ++g) {
+            const uint8_t* in = mine + g * stride;
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] += *(const lin_v4f_t*)(in + (i * FN + j) * 1024 + lane * 16);
+            if constexpr (KIND == LIN_TN) {
+#pragma unroll
+                for (int i = 0; i < FM; ++i) col_sum[i] += *(const float*)(in + FM * FN * 1024 + i * 256 + lane * 4);
+            }
+        }
+    }
+    float* st = (float*)mine;
     constexpr int CPR = WN / 8, RPI = 64 / CPR;  // chunks per row, rows per step
     const int64_t row0 = m0 + WM * wm, n = n0 + WN * wn + 8 * (lane % CPR);
     float bias[8];
-    lin_bias8(p, n, bias);
+    if constexpr (KIND == LIN_NT) lin_bias8(p, n, bias);
+    if constexpr (KIND == LIN_TN) {
+        // the four 16-lane groups hold different K of a column
+        if (tn == 0 && wn == 0 && (p.db || p.db16)) {
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+                float s = col_sum[i] + __shfl_xor(col_sum[i], 16);
+                s += __shfl_xor(s, 32);
+                const int64_t m = row0 + 16 * i + lane;
+                if (lane < 16 && m < M) {
+                    if (p.db) p.db[m] = s;
+                    else store1(p.db16, F16 ? DT_F16 : DT_BF16, m, s);
+                }
+            }
+        }
+    }
 #pragma unroll 1
     for (int i = 0; i < WM / RB; ++i) {
 #pragma unroll
@@ -285,18 +503,21 @@ __global__ __launch_bounds__(256, PER_CU) void lin_gemm_kernel(LinArgs p) {
             const lin_v4f_t x = *(const lin_v4f_t*)src, y = *(const lin_v4f_t*)(src + 4);
             float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
             const int64_t m = row0 + i * RB + row;
-            if (m < M && n < N) lin_finish8<KN, F16>(p, m, n, bias, v);
+            if (m < M && n < N) lin_finish8<KIND, F16>(p, m, n, bias, v);
         }
         __builtin_amdgcn_s_waitcnt(0xC07F);
         __builtin_amdgcn_wave_barrier();
     }
 }
 
-template <int BM, int BN, int S, int PER_CU, bool KN, bool F16>
+// KS: groups of 4 waves that share a tile's slabs; WAVES: waves per SIMD that the registers leave room for
+template <int BM, int BN, int S, int KS, int WAVES, int KIND, bool F16, bool REG = false>
 inline void lin_gemm_launch(LinArgs p, hipStream_t s) {
     p.tiles_m = (uint32_t)((p.M + BM - 1) / BM);
     p.tiles_n = (uint32_t)((p.N + BN - 1) / BN);
-    hipLaunchKernelGGL((lin_gemm_kernel<BM, BN, S, PER_CU, KN, F16>), dim3(p.tiles_m * p.tiles_n), dim3(256), 0, s, p);
+    const dim3 grid(p.tiles_m * p.tiles_n), block(256 * KS);
+    if (REG || p.K % LIN_BK == 0) hipLaunchKernelGGL((lin_gemm_kernel<BM, BN, S, KS, WAVES, KIND, F16, REG, false>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((lin_gemm_kernel<BM, BN, S, KS, WAVES, KIND, F16, REG, !REG>), grid, block, 0, s, p);
 }
 
 }  // namespace dopt

@@ -28,70 +28,102 @@ int device_cu_count() {
     return n;
 }
 
-// Estimated time (us) of each tile on this part: start + rounds of tiles (of the CUs' slots) * (slabs * step + epilogue), step
-// and epilogue of one tile among the others on its CU.
+// Estimated time (us) of each tile on this part, fitted to sweeps of every kernel over some 80 shapes from 72 x 72 x 72 to
+// 8192^3 and 25216 x 3072 x 768: start + slabs * (the larger of a lone tile's step and its share of a CU's throughput) + an
+// epilogue per tile of a CU. slots: tiles that a CU works on at once. The steps by product (forward, input gradient,
+// weight gradient: its operands are the long ones and come from memory, not from an L2). The REG tiles read rows
+// at any element.
 struct TileCost {
-    int bm, bn, slots;  // slots: tiles that a CU works on at once
-    float start, step, epilogue;
+    int bm, bn, slots;
+    float start, epilogue;
+    float alone[3], shared[3];
 };
-enum { T_32x64, T_64x64, T_128x128, T_BIG160, T_BIG256, T_COUNT };
+enum { T_32x64, T_64x64, T_64x64_4, T_128x64, T_128x128, T_BIG160, T_BIG256, T_REG32x64, T_REG64x64, T_COUNT };
 constexpr TileCost TILE_COST[T_COUNT] = {
-    {32, 64, 2, 2.5f, 0.20f, 0.6f},
-    {64, 64, 2, 2.5f, 0.28f, 1.2f},
-    {128, 128, 2, 3.0f, 0.75f, 5.0f},
-    {160, 256, 1, 4.0f, 0.98f, 5.0f},
-    {256, 256, 1, 4.0f, 1.45f, 9.0f},
+    {32, 64, 3, 3.9f, 0.35f, {0.085f, 0.100f, 0.160f}, {0.130f, 0.150f, 0.165f}},
+    {64, 64, 2, 3.9f, 0.70f, {0.140f, 0.160f, 0.195f}, {0.175f, 0.200f, 0.215f}},
+    {64, 64, 4, 3.9f, 0.35f, {0.340f, 0.360f, 0.410f}, {0.175f, 0.200f, 0.210f}},
+    {128, 64, 2, 4.2f, 1.00f, {0.230f, 0.250f, 0.335f}, {0.290f, 0.300f, 0.370f}},
+    {128, 128, 2, 5.0f, 2.40f, {0.600f, 0.580f, 0.550f}, {0.460f, 0.460f, 0.520f}},
+    {160, 256, 1, 6.0f, 3.80f, {0.920f, 0.920f, 0.0f}, {0.920f, 0.920f, 0.0f}},
+    {256, 256, 1, 6.0f, 5.80f, {1.430f, 1.430f, 0.0f}, {1.430f, 1.430f, 0.0f}},
+    {32, 64, 4, 4.2f, 0.50f, {0.210f, 0.300f, 0.350f}, {0.160f, 0.200f, 0.220f}},
+    {64, 64, 3, 4.4f, 0.80f, {0.300f, 0.380f, 0.400f}, {0.255f, 0.270f, 0.300f}},
 };
 
-int plan(const LinArgs& p, int n_cu, bool big) {
-    const float nk = (float)((p.K + LIN_BK - 1) / LIN_BK);
-    int best = T_32x64;
+float estimate(const TileCost& c, int kind, int64_t M, int64_t N, int64_t K, int n_cu, float extras) {
+    const float nk = (float)((K + LIN_BK - 1) / LIN_BK);
+    const int64_t tiles = ((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn), per_cu = (tiles + n_cu - 1) / n_cu;
+    const float rounds = (float)((per_cu + c.slots - 1) / c.slots);
+    return c.start + nk * std::max(c.alone[kind] * rounds, c.shared[kind] * (float)per_cu) + c.epilogue * extras * (float)per_cu;
+}
+
+// the tile with the least estimate: of the REG ones where rows lie at any element, else of the others (the 256-wide ones
+// if `big`). extras: what an epilogue costs beside a plain one.
+int plan(int kind, int64_t M, int64_t N, int64_t K, int n_cu, bool reg, bool big, float extras, float* us) {
+    int best = -1;
     float least = 0.0f;
-    for (int t = 0; t < T_COUNT; ++t) {
-        const TileCost& c = TILE_COST[t];
-        if (t >= T_BIG160 && !big) break;
-        const int64_t tiles = ((p.M + c.bm - 1) / c.bm) * ((p.N + c.bn - 1) / c.bn), slots = (int64_t)n_cu * c.slots;
-        const float rounds = (float)((tiles + slots - 1) / slots);
-        const float us = c.start + rounds * (nk * c.step + c.epilogue);
-        if (t == 0 || us < least) {
-            least = us;
+    for (int t = reg ? T_REG32x64 : 0; t < (reg ? T_COUNT : big && kind != LIN_TN ? T_REG32x64 : T_BIG160); ++t) {
+        const float e = estimate(TILE_COST[t], kind, M, N, K, n_cu, extras);
+        if (best < 0 || e < least) {
+            least = e;
             best = t;
         }
     }
+    if (us) *us = least;
     return best;
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
-template <bool KN, bool F16>
+// rows that the loads to LDS take: 16-byte aligned, with whole chunks
+bool whole_rows(const void* p, int64_t ld, int64_t cols) { return aligned16(p) && ld % 8 == 0 && ld >= (cols + 7) / 8 * 8; }
+
+template <int KIND, bool F16>
 void launch(const LinArgs& p, hipStream_t s) {
     const int n_cu = device_cu_count();
-    if constexpr (!KN) {
-        if (p.M <= 16) return lin_small_launch<8, F16>(p, s);
+    const bool reg = !whole_rows(p.A, p.lda, KIND == LIN_TN ? p.M : p.K) || !whole_rows(p.B, p.ldb, KIND == LIN_NT ? p.K : p.N);
+    if constexpr (KIND == LIN_NT) {
+        if (p.M <= 16) {
+            if (reg) lin_small_launch<8, F16, true>(p, s);
+            else lin_small_launch<8, F16, false>(p, s);
+            return;
+        }
     }
     // what the 256-wide tiles take: whole 16-byte chunks in the results' rows, 32-bit offsets in a tile of them
-    const bool big = p.N % 8 == 0 && p.N < ((int64_t)1 << 21) && p.K > 0 && !p.y_f32 && n_cu >= LIN_XCDS && aligned16(p.y) &&
+    const bool big = p.N % 8 == 0 && p.N < ((int64_t)1 << 21) && p.K >= LIN_BK && !p.y_f32 && n_cu >= LIN_XCDS && aligned16(p.y) &&
                      aligned16(p.pre) && aligned16(p.res) && aligned16(p.aux);
-    const int t = plan(p, n_cu, big);
-    if (t >= T_BIG160) {
-        const int bm = TILE_COST[t].bm;
-        if constexpr (KN) return F16 ? lin_big_kn_f16(p, bm, n_cu, s) : lin_big_kn_bf16(p, bm, n_cu, s);
-        else return F16 ? lin_big_nt_f16(p, bm, n_cu, s) : lin_big_nt_bf16(p, bm, n_cu, s);
+    const float extras = 1.0f + (p.pre ? 0.6f : 0.0f) + (p.res || p.aux ? 0.6f : 0.0f) + (p.act != LIN_NONE ? 0.4f : 0.0f);
+    const int t = plan(KIND, p.M, p.N, p.K, n_cu, reg, big, extras, nullptr);
+    if constexpr (KIND != LIN_TN) {
+        if (t == T_BIG160 || t == T_BIG256) {
+            const int bm = TILE_COST[t].bm;
+            if constexpr (KIND == LIN_KN) return F16 ? lin_big_kn_f16(p, bm, n_cu, s) : lin_big_kn_bf16(p, bm, n_cu, s);
+            else return F16 ? lin_big_nt_f16(p, bm, n_cu, s) : lin_big_nt_bf16(p, bm, n_cu, s);
+        }
     }
-    if (t == T_128x128) return lin_gemm_launch<128, 128, 2, 2, KN, F16>(p, s);
-    if (t == T_64x64) return lin_gemm_launch<64, 64, 4, 2, KN, F16>(p, s);
-    return lin_gemm_launch<32, 64, 4, 2, KN, F16>(p, s);
+    switch (t) {
+        case T_32x64: return lin_gemm_launch<32, 64, 4, 1, 3, KIND, F16>(p, s);
+        case T_64x64: return lin_gemm_launch<64, 64, 4, 1, 2, KIND, F16>(p, s);
+        case T_64x64_4: return lin_gemm_launch<64, 64, 2, 1, 4, KIND, F16>(p, s);
+        case T_128x64: return lin_gemm_launch<128, 64, 3, 1, 2, KIND, F16>(p, s);
+        case T_REG32x64: return lin_gemm_launch<32, 64, 2, 1, 4, KIND, F16, true>(p, s);
+        case T_REG64x64: return lin_gemm_launch<64, 64, 2, 1, 3, KIND, F16, true>(p, s);
+        default: return lin_gemm_launch<128, 128, 2, 1, 2, KIND, F16>(p, s);
+    }
 }
 
-// dst[r][c] = src[r][c] act'(pre[r][c]) for c < cols, 0 for the columns up to ld_dst; 8 columns a lane. Both sources
-// have rows of src_ld elements (pre: cols), dst's are aligned.
+// dst[r][c] = src[r][c] act'(pre[r][c]) for c < cols, 0 for the columns up to ld_dst; 8 columns a lane. The source has
+// rows of src_ld elements (pre: cols), dst's are aligned.
 template <bool F16>
 __global__ __launch_bounds__(256) void lin_act_grad_kernel(const uint16_t* src, int64_t src_ld, const uint16_t* pre, int act,
                                                            int64_t rows, int64_t cols, uint16_t* dst, int64_t ld_dst) {
     constexpr int DT = F16 ? DT_F16 : DT_BF16;
-    const int64_t cpr = ld_dst / 8, total = rows * cpr;
-    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total; q += (int64_t)gridDim.x * 256) {
-        const int64_t r = q / cpr, c = (q - r * cpr) * 8;
+    const uint64_t cpr = (uint64_t)ld_dst / 8, total = (uint64_t)rows * cpr;
+    for (uint64_t q = (uint64_t)blockIdx.x * 256 + threadIdx.x; q < total; q += (uint64_t)gridDim.x * 256) {
+        // (32-bit division where it does)
+        const int64_t r = total >> 32 ? (int64_t)(q / cpr) : (int64_t)((uint32_t)q / (uint32_t)cpr);
+        const int64_t c = ((int64_t)q - r * (int64_t)cpr) * 8;
         const int have = (int)std::min<int64_t>(8, cols - c);
         float v[8];
         lin_load8<DT>(src, r * src_ld + c, have, v);
@@ -104,6 +136,20 @@ __global__ __launch_bounds__(256) void lin_act_grad_kernel(const uint16_t* src, 
     }
 }
 
+// the same without rows: n elements
+template <bool F16>
+__global__ __launch_bounds__(256) void lin_act_grad_flat_kernel(const uint16_t* src, const uint16_t* pre, int act, int64_t n, uint16_t* dst) {
+    constexpr int DT = F16 ? DT_F16 : DT_BF16;
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (int64_t)gridDim.x * 2048) {
+        const int have = (int)std::min<int64_t>(8, n - i);
+        float v[8], z[8];
+        lin_load8<DT>(src, i, have, v);
+        lin_load8<DT>(pre, i, have, z);
+        lin_act_grad8(act, z, v);
+        lin_store8<DT>(dst, i, have, v);
+    }
+}
+
 }  // namespace
 
 // A's and B's offsets of one tile and slab stay within a buffer resource, a grid's work-items below 2^32
@@ -113,24 +159,36 @@ bool lin_shape_fits(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb) {
            (M + 127) / 128 < most / ((N + 127) / 128 + 1);
 }
 
-int launch_linear(const LinArgs& p, bool kn, bool f16, hipStream_t s) {
+int launch_linear(const LinArgs& p, int kind, bool f16, hipStream_t s) {
     if (p.M == 0 || p.N == 0) return 0;
-    if (kn) {
-        if (f16) launch<true, true>(p, s);
-        else launch<true, false>(p, s);
-    } else {
-        if (f16) launch<false, true>(p, s);
-        else launch<false, false>(p, s);
-    }
+    if (kind == LIN_KN) f16 ? launch<LIN_KN, true>(p, s) : launch<LIN_KN, false>(p, s);
+    else if (kind == LIN_TN) f16 ? launch<LIN_TN, true>(p, s) : launch<LIN_TN, false>(p, s);
+    else f16 ? launch<LIN_NT, true>(p, s) : launch<LIN_NT, false>(p, s);
     return 0;
+}
+
+// The tile that a product gets (an index of TILE_COST; -1: the kernel of at most 16 rows) and its estimate. M, N, K as in
+// LinArgs; reg: an operand's rows lie at any element.
+int linear_tile(int kind, int64_t M, int64_t N, int64_t K, bool reg, bool big, float* us) {
+    const int n_cu = device_cu_count();
+    if (kind == LIN_NT && M <= 16) {
+        // 16 columns a workgroup, 8 slabs at a time
+        const float rounds = (float)((N + 16 * 2 * n_cu - 1) / (16 * 2 * n_cu));
+        if (us) *us = 3.5f + rounds * (float)((K + 511) / 512) * (reg ? 0.45f : 0.40f);
+        return -1;
+    }
+    return plan(kind, M, N, K, n_cu, reg, big && N % 8 == 0 && K >= LIN_BK, 1.0f, us);
 }
 
 int launch_linear_act_grad(const uint16_t* src, int64_t src_ld, const uint16_t* pre, int act, bool f16, int64_t rows,
                            int64_t cols, uint16_t* dst, int64_t ld_dst, hipStream_t s) {
-    const int64_t chunks = rows * (ld_dst / 8);
+    const bool flat = src_ld == cols && ld_dst == cols && act != LIN_NONE;
+    const int64_t n = rows * cols, chunks = flat ? (n + 7) / 8 : rows * (ld_dst / 8);
     if (chunks == 0) return 0;
     const dim3 grid((uint32_t)std::min<int64_t>((chunks + 255) / 256, 1 << 20));
-    if (f16) hipLaunchKernelGGL(lin_act_grad_kernel<true>, grid, dim3(256), 0, s, src, src_ld, pre, act, rows, cols, dst, ld_dst);
+    if (flat && f16) hipLaunchKernelGGL(lin_act_grad_flat_kernel<true>, grid, dim3(256), 0, s, src, pre, act, n, dst);
+    else if (flat) hipLaunchKernelGGL(lin_act_grad_flat_kernel<false>, grid, dim3(256), 0, s, src, pre, act, n, dst);
+    else if (f16) hipLaunchKernelGGL(lin_act_grad_kernel<true>, grid, dim3(256), 0, s, src, src_ld, pre, act, rows, cols, dst, ld_dst);
     else hipLaunchKernelGGL(lin_act_grad_kernel<false>, grid, dim3(256), 0, s, src, src_ld, pre, act, rows, cols, dst, ld_dst);
     return 0;
 }

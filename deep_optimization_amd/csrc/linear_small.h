@@ -1,5 +1,5 @@
 // The forward product of at most 16 rows (single tokens): a workgroup computes a 16 x 16 tile and its NW waves split K
-// between them. Same operands, result and edges as lin_gemm_kernel<.., KN = false>.
+// between them. Same operands, result and edges as the LIN_NT form of lin_gemm_kernel.
 //
 // What bounds it is the weight's bytes and latency. Each wave walks the K chunks w, w + NW, ... of 64 elements with its
 // operands straight from memory to registers (a fragment is 16 rows x 128 bytes; LDS would save nothing), the next
@@ -11,7 +11,8 @@
 
 namespace dopt {
 
-template <int NW, bool F16>
+// REG: rows at any element without padding, as in linear_gemm.h.
+template <int NW, bool F16, bool REG>
 __global__ __launch_bounds__(64 * NW) void lin_small_kernel(LinArgs p) {
     constexpr int PITCH = 20;  // floats per LDS row
     __shared__ __attribute__((aligned(16))) float part[NW][16 * PITCH];
@@ -32,9 +33,25 @@ __global__ __launch_bounds__(64 * NW) void lin_small_kernel(LinArgs p) {
     auto load = [&](Frags& f, uint32_t k0) __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+            if constexpr (REG) {
+                const int64_t k = (int64_t)k0 + 32 * h + kb, left = (int64_t)K - k;
+                const bool in_b = n0 + row < p.N && left > 0, in_a = row < p.M && left > 0;
+                f.b[h] = __builtin_bit_cast(lin_v4i_t, lin_load8u(p.B, in_b ? (n0 + row) * p.ldb + k : 0, (p.N - 1) * p.ldb + K));
+                f.a[h] = __builtin_bit_cast(lin_v4i_t, lin_load8u(p.A, in_a ? row * p.lda + k : 0, (p.M - 1) * p.lda + K));
+                if (k0 + LIN_BK > K) {
+                    f.b[h] = __builtin_bit_cast(lin_v4i_t, lin_keep(__builtin_bit_cast(lin_v4u_t, f.b[h]), left));
+                    f.a[h] = __builtin_bit_cast(lin_v4i_t, lin_keep(__builtin_bit_cast(lin_v4u_t, f.a[h]), left));
+                }
+                continue;
+            }
             const uint32_t past = k0 + 32 * h + kb < K ? 0u : LIN_OOB;
             f.b[h] = __builtin_bit_cast(lin_v4i_t, __builtin_amdgcn_raw_buffer_load_b128(rb, (offb + 64 * h) | past, (int)(2 * k0), 0));
             f.a[h] = __builtin_bit_cast(lin_v4i_t, __builtin_amdgcn_raw_buffer_load_b128(ra, (offa + 64 * h) | past, (int)(2 * k0), 0));
+            if (K % 8 && k0 + LIN_BK > K) {
+                const int64_t left = (int64_t)K - k0 - 32 * h - kb;
+                f.b[h] = __builtin_bit_cast(lin_v4i_t, lin_keep(__builtin_bit_cast(lin_v4u_t, f.b[h]), left));
+                f.a[h] = __builtin_bit_cast(lin_v4i_t, lin_keep(__builtin_bit_cast(lin_v4u_t, f.a[h]), left));
+            }
         }
     };
     lin_v4f_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -73,13 +90,13 @@ __global__ __launch_bounds__(64 * NW) void lin_small_kernel(LinArgs p) {
             for (int e = 0; e < 8; ++e) v[e] += part[w][r * PITCH + c + e];
         float bias[8];
         lin_bias8(p, n0 + c, bias);
-        lin_finish8<false, F16>(p, r, n0 + c, bias, v);
+        lin_finish8<LIN_NT, F16>(p, r, n0 + c, bias, v);
     }
 }
 
-template <int NW, bool F16>
+template <int NW, bool F16, bool REG>
 inline void lin_small_launch(const LinArgs& p, hipStream_t s) {
-    hipLaunchKernelGGL((lin_small_kernel<NW, F16>), dim3((uint32_t)((p.N + 15) / 16)), dim3(64 * NW), 0, s, p);
+    hipLaunchKernelGGL((lin_small_kernel<NW, F16, REG>), dim3((uint32_t)((p.N + 15) / 16)), dim3(64 * NW), 0, s, p);
 }
 
 }  // namespace dopt

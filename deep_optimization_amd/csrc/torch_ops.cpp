@@ -809,24 +809,41 @@ int lin_act(c10::string_view act) {
 
 int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
 
-// dy act'(pre) [rows, cols] in rows padded with zeros to a multiple of 8
-Tensor lin_act_grad_rows(const Tensor& dy, const void* pre, int act, int64_t rows, int64_t cols) {
-    Tensor out = at::empty({rows, pad8(cols)}, dy.options());
-    check(dopt_linear_act_grad(dy.data_ptr(), cols, pre, act, dtype_code(dy.scalar_type(), "linear_act"), rows, cols, out.data_ptr(),
-                               pad8(cols), stream_of(dy)),
+// dy act'(pre) of dy [rows, cols] at stride ld, in rows padded with zeros to a multiple of 8 or contiguous
+Tensor lin_act_grad_rows(const Tensor& dy, int64_t ld, const void* pre, int act, int64_t rows, int64_t cols, bool padded) {
+    const int64_t width = padded ? pad8(cols) : cols;
+    Tensor out = at::empty({rows, width}, dy.options());
+    check(dopt_linear_act_grad(dy.data_ptr(), ld, pre, act, dtype_code(dy.scalar_type(), "linear_act"), rows, cols, out.data_ptr(), width,
+                               stream_of(dy)),
           "linear_act");
     return out;
 }
 
-// t [..., cols] as (tensor, row stride): linear_lib._rows
-std::pair<Tensor, int64_t> lin_rows(const Tensor& t, int64_t rows, int64_t cols) {
-    const auto aligned16 = [](const Tensor& v) { return reinterpret_cast<uintptr_t>(v.data_ptr()) % 16 == 0; };
-    const Tensor t2 = t.dim() == 2 ? t : t.reshape({rows, cols});
-    if (cols % 8 == 0 && t2.stride(1) == 1 && t2.stride(0) >= cols && t2.stride(0) < (1 << 21) && t2.stride(0) % 8 == 0 && aligned16(t2))
-        return {t2, t2.stride(0)};
-    const Tensor c = t2.contiguous();
-    if (cols % 8 == 0 && aligned16(c)) return {c, cols};
-    return {lin_act_grad_rows(c, nullptr, DOPT_LIN_NONE, rows, cols), pad8(cols)};
+struct LinRows {
+    Tensor t;
+    int64_t ld;
+    bool whole;  // the kernels read its rows in whole 16-byte chunks
+};
+
+// t [..., cols] as a matrix with contiguous rows: linear_lib._rows
+LinRows lin_rows(const Tensor& t, int64_t rows, int64_t cols) {
+    Tensor t2 = t.dim() == 2 ? t : t.reshape({rows, cols});
+    if (t2.stride(1) != 1 || t2.stride(0) < cols || t2.stride(0) >= (1 << 21)) t2 = t2.contiguous();
+    const int64_t ld = rows <= 1 ? cols : t2.stride(0);
+    const bool whole = ld % 8 == 0 && ld >= pad8(cols) && reinterpret_cast<uintptr_t>(t2.data_ptr()) % 16 == 0;
+    if (whole && cols % 8 && (size_t)(t2.storage_offset() + (rows - 1) * ld + pad8(cols)) * 2 > t2.storage().nbytes())
+        return {lin_act_grad_rows(t2, ld, nullptr, DOPT_LIN_NONE, rows, cols, true), pad8(cols), true};  // the last row's last chunk is not all there
+    return {t2, ld, whole};
+}
+
+// the operands as the product's kernels read them: linear_lib._operands
+void lin_operands_of(int product, int64_t M, int64_t N, int64_t K, LinRows& a, int64_t a_rows, int64_t a_cols, LinRows& b, int64_t b_rows,
+                     int64_t b_cols) {
+    const int copies = (a.whole ? 0 : 1) + (b.whole ? 0 : 1);
+    const int64_t elements = (a.whole ? 0 : a_rows * a_cols) + (b.whole ? 0 : b_rows * b_cols);
+    if (!copies || !dopt_linear_copy_preferred(product, M, N, K, elements, copies)) return;
+    if (!a.whole) a = {lin_act_grad_rows(a.t, a.ld, nullptr, DOPT_LIN_NONE, a_rows, a_cols, true), pad8(a_cols), true};
+    if (!b.whole) b = {lin_act_grad_rows(b.t, b.ld, nullptr, DOPT_LIN_NONE, b_rows, b_cols, true), pad8(b_cols), true};
 }
 
 bool lin_type(ScalarType t) { return t == ScalarType::Half || t == ScalarType::BFloat16; }
@@ -871,13 +888,17 @@ std::tuple<Tensor, std::optional<Tensor>> linear_act_fwd(const Tensor& x, const 
     require_cuda(bias);
     require_cuda(residual);
     require_current(x);
-    const auto [a, lda] = M && K ? lin_rows(x, M, K) : std::pair<Tensor, int64_t>{x, pad8(K)};
-    const auto [b, ldb] = N && K ? lin_rows(weight, N, K) : std::pair<Tensor, int64_t>{weight, pad8(K)};
+    LinRows a{x, K, true}, b{weight, K, true};
+    if (M && N && K) {
+        a = lin_rows(x, M, K);
+        b = lin_rows(weight, N, K);
+        lin_operands_of(DOPT_LIN_FORWARD, M, N, K, a, M, K, b, N, K);
+    }
     const auto bc = contiguous(bias), r = contiguous(residual);
     Tensor y = at::empty(shape, x.options().dtype(r ? r->scalar_type() : dt));
     std::optional<Tensor> pre;
     if (save_pre) pre = at::empty(shape, x.options());
-    check(dopt_linear_forward(a.data_ptr(), lda, b.data_ptr(), ldb, dtype_code(dt, what), M, N, K, ptr(bc),
+    check(dopt_linear_forward(a.t.data_ptr(), a.ld, b.t.data_ptr(), b.ld, dtype_code(dt, what), M, N, K, ptr(bc),
                               bc ? dtype_code(bc->scalar_type(), what) : DOPT_F32, ptr(r), code, y.data_ptr(),
                               dtype_code(y.scalar_type(), what), pre ? pre->data_ptr() : nullptr, stream_of(x)),
           what);
@@ -907,39 +928,53 @@ std::tuple<std::optional<Tensor>, std::optional<Tensor>, std::optional<Tensor>> 
     require_current(x);
     const int tc = dtype_code(dt, what);
     void* const stream = stream_of(x);
+    const bool empty = M == 0 || N == 0 || K == 0;
     Tensor dz = dy;
-    int64_t ldz = pad8(N);
-    if (M && N) {
-        if (code != DOPT_LIN_NONE) {
-            const Tensor d = dy.contiguous(), z = pre->contiguous();
-            dz = lin_act_grad_rows(d, z.data_ptr(), code, M, N);
-        } else {
-            std::tie(dz, ldz) = lin_rows(dy, M, N);
-        }
+    if (code != DOPT_LIN_NONE && M && N) {
+        const Tensor d = dy.contiguous(), z = pre->contiguous();
+        // (padded where a product that reads dz is going to want it so)
+        const bool padded = N % 8 != 0 && K != 0 &&
+                            dopt_linear_copy_preferred(input_grad ? DOPT_LIN_INPUT_GRAD : DOPT_LIN_WEIGHT_GRAD, M, N, K, 0, 0);
+        dz = lin_act_grad_rows(d, N, z.data_ptr(), code, M, N, padded).narrow(1, 0, N);
     }
+    LinRows dzr{dz, N, true};
+    if (!empty) dzr = lin_rows(dz, M, N);
     std::optional<Tensor> dx, dw, db;
     if (input_grad) {
         dx = at::empty(x.sizes(), x.options());
         const auto ip = contiguous(in_pre);
-        const auto [w, ldw] = N && K ? lin_rows(weight, N, K) : std::pair<Tensor, int64_t>{weight, pad8(K)};
-        check(dopt_linear_input_grad(dz.data_ptr(), ldz, w.data_ptr(), ldw, tc, M, N, K, ptr(ip), in_code, dx->data_ptr(), stream), what);
+        LinRows a = dzr, b{weight, K, true};
+        if (!empty) {
+            b = lin_rows(weight, N, K);
+            lin_operands_of(DOPT_LIN_INPUT_GRAD, M, N, K, a, M, N, b, N, K);
+        }
+        check(dopt_linear_input_grad(a.t.data_ptr(), a.ld, b.t.data_ptr(), b.ld, tc, M, N, K, ptr(ip), in_code, dx->data_ptr(), stream), what);
     }
     if (weight_grad || bias_grad) {
         const auto opts = x.options().dtype(grad_dtype);
         if (N == 0 || K == 0) {
             dw = at::empty({N, K}, opts);
-            db = dz.reshape({M, dz.size(-1)}).narrow(1, 0, N).to(at::kFloat).sum(0).to(grad_dtype);
+            db = dz.reshape({M, N}).to(at::kFloat).sum(0).to(grad_dtype);
         } else {
-            const auto [xr, ldx] = M ? lin_rows(x, M, K) : std::pair<Tensor, int64_t>{x, pad8(K)};
-            const int64_t K8 = pad8(K);
+            LinRows a = dzr, b{x, K, true};
+            if (!empty) {
+                b = lin_rows(x, M, K);
+                lin_operands_of(DOPT_LIN_WEIGHT_GRAD, M, N, K, a, M, N, b, M, K);
+            }
+            // the kernels that split the sum write whole chunks of a row
+            int64_t K8 = pad8(K);
+            if (K8 != K && (!a.whole || !b.whole || dopt_linear_tile(DOPT_LIN_WEIGHT_GRAD, M, N, K8, 0) != 100)) K8 = K;
             const bool f32 = grad_dtype == ScalarType::Float;
-            Tensor ws = at::empty({std::max<int64_t>(dopt_linear_weight_grad_workspace_floats(M, N, K8), 4)}, x.options().dtype(at::kFloat));
+            const int64_t floats = dopt_linear_weight_grad_workspace_floats(M, N, K8);
+            Tensor ws;
+            if (floats > 0) ws = at::empty({floats}, x.options().dtype(at::kFloat));
             Tensor d = at::empty({N, K8}, opts);
             if (bias_grad) db = at::empty({N}, opts);
             void* const dbp = db ? db->data_ptr() : nullptr;
-            check(dopt_linear_weight_grad(dz.data_ptr(), ldz, xr.data_ptr(), ldx, tc, M, N, K8, ws.data_ptr<float>(),
-                                          f32 ? (float*)d.data_ptr() : nullptr, f32 ? nullptr : d.data_ptr(), f32 ? (float*)dbp : nullptr,
-                                          f32 ? nullptr : dbp, stream),
+            // (a pointer that is not null where nothing is written to it)
+            check(dopt_linear_weight_grad(a.t.data_ptr(), a.ld, b.t.data_ptr(), b.ld, tc, M, N, K8,
+                                          floats > 0 ? ws.data_ptr<float>() : (float*)d.data_ptr(), f32 ? (float*)d.data_ptr() : nullptr,
+                                          f32 ? nullptr : d.data_ptr(), f32 ? (float*)dbp : nullptr, f32 ? nullptr : dbp, stream),
                   what);
             dw = K8 == K ? d : d.narrow(1, 0, K).contiguous();
         }

@@ -19,8 +19,9 @@ gradient of the pre-activation in one pass. dz is rounded to x's type for the pr
 instructions of that type). dweight and dbias come in ``grad_dtype`` (float32 or x's type; both are summed in fp32);
 what is not asked for is None, and bias_grad alone still runs the weight gradient's product, which sums dz on its way.
 
-Rows of x may be strided (x[:, 0] of a [B, T, K] tensor) where the stride is a multiple of 8 elements and the rows start
-at 16 bytes; other layouts, and operands whose K (N) is no multiple of 8, are copied into aligned rows first.
+Rows may be strided (x[:, 0] of a [B, T, K] tensor) and lie at any element. Where they start at multiples of 16 bytes
+and hold whole 16-byte chunks the faster kernels read them; others are read through registers, or copied into
+aligned rows first where that is estimated to be faster (dopt_linear_copy_preferred).
 """
 from __future__ import annotations
 
@@ -47,22 +48,35 @@ def _pad8(n: int) -> int:
 
 
 def _rows(t: Tensor, cols: int):
-    """t [..., cols] as (tensor, row stride): rows at 16-byte aligned addresses that hold whole 8-element chunks, zero
-    past ``cols``."""
+    """t [..., cols] as (matrix with contiguous rows, row stride, whether the kernels read its rows in whole 16-byte chunks)."""
     t2 = t.reshape(-1, cols) if t.dim() != 2 else t
-    if cols % 8 == 0 and t2.stride(1) == 1 and cols <= t2.stride(0) < 1 << 21 and t2.stride(0) % 8 == 0 and t2.data_ptr() % 16 == 0:
-        return t2, int(t2.stride(0))
-    t2 = t2.contiguous()
-    if cols % 8 == 0 and t2.data_ptr() % 16 == 0:
-        return t2, cols
-    return _act_grad_rows(t2, None, "none"), _pad8(cols)
+    if t2.stride(1) != 1 or not cols <= t2.stride(0) < 1 << 21:
+        t2 = t2.contiguous()
+    rows = t2.shape[0]
+    ld = cols if rows <= 1 else int(t2.stride(0))
+    whole = ld % 8 == 0 and ld >= _pad8(cols) and t2.data_ptr() % 16 == 0
+    if whole and cols % 8 and (t2.storage_offset() + (rows - 1) * ld + _pad8(cols)) * 2 > t2.untyped_storage().nbytes():
+        return _act_grad_rows(t2, ld, None, "none", True), _pad8(cols), True  # the last row's last chunk is not all there
+    return t2, ld, whole
 
 
-def _act_grad_rows(dy: Tensor, pre: Optional[Tensor], act: str) -> Tensor:
-    """dy act'(pre) [rows, cols] in rows padded with zeros to a multiple of 8."""
+def _operands(product: int, M: int, N: int, K: int, *operands):
+    """(tensor, columns) pairs as the product's kernels read them: [(tensor, row stride)]. Operands whose rows lie at any
+    element stay where they are, or are copied into aligned rows where that is estimated to be faster."""
+    rows = [_rows(t, cols) for t, cols in operands]
+    loose = [i for i, r in enumerate(rows) if not r[2]]
+    if loose and _lib.lib().dopt_linear_copy_preferred(product, M, N, K, sum(rows[i][0].numel() for i in loose), len(loose)):
+        for i in loose:
+            cols = operands[i][1]
+            rows[i] = (_act_grad_rows(rows[i][0], rows[i][1], None, "none", True), _pad8(cols), True)
+    return [(t, ld) for t, ld, _ in rows]
+
+
+def _act_grad_rows(dy: Tensor, ld: int, pre: Optional[Tensor], act: str, padded: bool) -> Tensor:
+    """dy act'(pre) of dy [rows, cols], in rows padded with zeros to a multiple of 8 or contiguous."""
     rows, cols = dy.shape
-    out = torch.empty((rows, _pad8(cols)), dtype=dy.dtype, device=dy.device)
-    rc = _lib.lib().dopt_linear_act_grad(dy.data_ptr(), cols, None if pre is None else pre.data_ptr(), _act_code(act),
+    out = torch.empty((rows, _pad8(cols) if padded else cols), dtype=dy.dtype, device=dy.device)
+    rc = _lib.lib().dopt_linear_act_grad(dy.data_ptr(), ld, None if pre is None else pre.data_ptr(), _act_code(act),
                                          _DTYPE_CODE[dy.dtype], rows, cols, out.data_ptr(), out.shape[1], _stream(dy))
     _lib.check(rc, "linear_act")
     return out
@@ -94,8 +108,7 @@ def _linear_act_fwd(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual:
     if residual is not None:
         _check_like(what, "residual", residual, shape, (x.dtype, torch.float32))
     _require_cuda(x, weight, bias, residual)
-    a, lda = _rows(x, K) if M and K else (x, _pad8(K))
-    b, ldb = _rows(weight, K) if N and K else (weight, _pad8(K))
+    (a, lda), (b, ldb) = _operands(0, M, N, K, (x, K), (weight, K)) if M and N and K else ((x, K), (weight, K))
     bias = None if bias is None else bias.contiguous()
     residual = None if residual is None else residual.contiguous()
     y = torch.empty(shape, dtype=x.dtype if residual is None else residual.dtype, device=x.device)
@@ -136,35 +149,37 @@ def _linear_act_bwd(dy: Tensor, x: Tensor, weight: Tensor, pre: Optional[Tensor]
         _check_like(what, "in_pre", in_pre, x.shape, (x.dtype,))
     _require_cuda(dy, x, weight, pre, in_pre)
     L, dt, stream = _lib.lib(), _DTYPE_CODE[x.dtype], _stream(x)
-    if M and N:
-        if code:
-            dz = _act_grad_rows(dy.contiguous().view(M, N), pre.contiguous(), act)
-            ldz = _pad8(N)
-        else:
-            dz, ldz = _rows(dy, N)
-    else:
-        dz, ldz = dy, _pad8(N)
+    empty = M == 0 or N == 0 or K == 0
+    dz, cols = dy, N
+    if code and M and N:
+        # (padded where a product that reads dz is going to want it so)
+        want = (0 if K == 0 else 1 if input_grad else 2)
+        padded = N % 8 != 0 and want != 0 and bool(L.dopt_linear_copy_preferred(want, M, N, K, 0, 0))
+        dz = _act_grad_rows(dy.contiguous().view(M, N), N, pre.contiguous(), act, padded)[:, :N]
     dx = dw = db = None
     if input_grad:
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         in_pre = None if in_pre is None else in_pre.contiguous()
-        w, ldw = _rows(weight, K) if N and K else (weight, _pad8(K))
-        rc = L.dopt_linear_input_grad(dz.data_ptr(), ldz, w.data_ptr(), ldw, dt, M, N, K, None if in_pre is None else in_pre.data_ptr(),
+        (a, lda), (b, ldb) = _operands(1, M, N, K, (dz, N), (weight, K)) if not empty else ((dz, N), (weight, K))
+        rc = L.dopt_linear_input_grad(a.data_ptr(), lda, b.data_ptr(), ldb, dt, M, N, K, None if in_pre is None else in_pre.data_ptr(),
                                       in_code, dx.data_ptr(), stream)
         _lib.check(rc, what)
     if weight_grad or bias_grad:
         if N == 0 or K == 0:
             dw = torch.empty((N, K), dtype=grad_dtype, device=x.device)
-            db = dz.reshape(M, dz.shape[-1])[:, :N].float().sum(0).to(grad_dtype)
+            db = dz.reshape(M, N).float().sum(0).to(grad_dtype)
         else:
-            xr, ldx = _rows(x, K) if M else (x, _pad8(K))
+            (a, lda), (b, ldb) = _operands(2, M, N, K, (dz, N), (x, K)) if not empty else ((dz, N), (x, K))
+            # the kernels that split the sum write whole chunks of a row
             K8 = _pad8(K)
+            if K8 != K and (lda % 8 or ldb % 8 or ldb < K8 or a.data_ptr() % 16 or b.data_ptr() % 16 or L.dopt_linear_tile(2, M, N, K8, 0) != 100):
+                K8 = K
             ws = torch.empty(max(int(L.dopt_linear_weight_grad_workspace_floats(M, N, K8)), 4), dtype=torch.float32, device=x.device)
             dw = torch.empty((N, K8), dtype=grad_dtype, device=x.device)
             db = torch.empty(N, dtype=grad_dtype, device=x.device) if bias_grad else None
             f32 = grad_dtype == torch.float32
             dbp = None if db is None else db.data_ptr()
-            rc = L.dopt_linear_weight_grad(dz.data_ptr(), ldz, xr.data_ptr(), ldx, dt, M, N, K8, ws.data_ptr(), dw.data_ptr() if f32 else None,
+            rc = L.dopt_linear_weight_grad(a.data_ptr(), lda, b.data_ptr(), ldb, dt, M, N, K8, ws.data_ptr(), dw.data_ptr() if f32 else None,
                                            None if f32 else dw.data_ptr(), dbp if f32 else None, None if f32 else dbp, stream)
             _lib.check(rc, what)
             if K8 != K:

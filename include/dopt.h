@@ -470,28 +470,39 @@ int dopt_dropout(const void* x, int x_dtype, const void* residual, int64_t n, do
 #define DOPT_LIN_GELU_TANH 3 /* the tanh form */
 #define DOPT_LIN_SILU 4
 
+/* the layer's three products: M rows, N out and K in features */
+#define DOPT_LIN_FORWARD 0     /* x [M, K] weight^T [K, N] */
+#define DOPT_LIN_INPUT_GRAD 1  /* dz [M, N] weight [N, K] */
+#define DOPT_LIN_WEIGHT_GRAD 2 /* dz^T [N, M] x [M, K] */
+
 /* z = x weight^T + bias, y = act(z) + residual, pre = z: x [M, ldx], weight [N, ldw], both fp16 or bf16 (dtype), sums and
  * epilogue in fp32, each result rounded once. bias [N] of bias_dtype, residual [M, N] of y's type, pre [M, N] of
- * the operands' type; each may be NULL. y [M, N]: the operands' type or fp32. x and weight: 16-byte aligned, strides
- * multiples of 8 (below 2^21) that are at least K rounded up to one; where K is not a multiple of 8 the elements up to
- * that are read and must be zero. */
+ * the operands' type; each may be NULL. y [M, N]: the operands' type or fp32; results overlap no operand. Row strides
+ * below 2^21. x and weight may lie at any element; where both are 16-byte aligned with strides that are multiples of 8 and
+ * at least K rounded up to one, the faster kernels run (which read each row, the last one too, up to that length). */
 int dopt_linear_forward(const void* x, int64_t ldx, const void* weight, int64_t ldw, int dtype, int64_t M, int64_t N,
                         int64_t K, const void* bias, int bias_dtype, const void* residual, int act, void* y, int y_dtype,
                         void* pre, void* stream);
-/* dx = (dz weight) * in_act'(in_pre): dz [M, ldz] (N columns, zeros up to a multiple of 8), weight [N, ldw] as in the
- * forward call (K columns), dx and in_pre [M, K]. in_act DOPT_LIN_NONE: dx = dz weight, in_pre is not read. */
+/* dx = (dz weight) * in_act'(in_pre): dz [M, ldz], weight [N, ldw], dx and in_pre [M, K]. in_act DOPT_LIN_NONE: dx =
+ * dz weight, in_pre is not read. The same alignment rules (dz's rows hold N elements, weight's K). */
 int dopt_linear_input_grad(const void* dz, int64_t ldz, const void* weight, int64_t ldw, int dtype, int64_t M, int64_t N,
                            int64_t K, const void* in_pre, int in_act, void* dx, void* stream);
-/* dz[r][c] = dy[r][c] * act'(pre[r][c]) for c < cols, 0 for the columns up to ld_dz (a multiple of 8, dz 16-byte
- * aligned); pre [rows, cols]. With DOPT_LIN_NONE a copy into padded rows. */
+/* dz[r][c] = dy[r][c] * act'(pre[r][c]) for c < cols, 0 for the columns up to ld_dz; pre [rows, cols]. dz 16-byte aligned
+ * with ld_dz a multiple of 8, or contiguous as dy is. With DOPT_LIN_NONE a copy into padded rows. */
 int dopt_linear_act_grad(const void* dy, int64_t ld_dy, const void* pre, int act, int dtype, int64_t rows, int64_t cols,
                          void* dz, int64_t ld_dz, void* stream);
-/* dw = dz^T x (fp32 dw_f32 and / or dw_16 of the operands' type, [N, K]) and the sums of dz over its rows ([N], in fp32
- * to db or in the operands' type to db_16; one or both NULL): dopt_dw_gemm_any for fp16 or bf16 and any N; K a multiple of 8; the same alignment rules. workspace:
- * dopt_linear_weight_grad_workspace_floats floats (not NULL). */
+/* dw = dz^T x (fp32 to dw_f32 or the operands' type to dw_16, [N, K]) and the sums of dz over its rows ([N], fp32 to db or
+ * the operands' type to db_16; NULL: none): dz [M, ldz], x [M, ldx], the same alignment rules. workspace:
+ * dopt_linear_weight_grad_workspace_floats floats (0: it may be NULL). Sums in an order that the sizes fix. */
 int64_t dopt_linear_weight_grad_workspace_floats(int64_t M, int64_t N, int64_t K);
 int dopt_linear_weight_grad(const void* dz, int64_t ldz, const void* x, int64_t ldx, int dtype, int64_t M, int64_t N,
                             int64_t K, float* workspace, float* dw_f32, void* dw_16, float* db, void* db_16, void* stream);
+/* Which tile a product gets (an index of the launcher's table; -1: the kernel of at most 16 rows; 100: dopt_dw_gemm_any's
+ * kernels; -2: bad arguments); any_rows: an operand's rows lie at any element. */
+int dopt_linear_tile(int product, int64_t M, int64_t N, int64_t K, int any_rows);
+/* Whether copying operands that lie at any element into aligned rows (`copies` of them, of `elements` elements together)
+ * is estimated to be faster than reading them as they lie. */
+int dopt_linear_copy_preferred(int product, int64_t M, int64_t N, int64_t K, int64_t elements, int copies);
 
 /*
  * HIP graph tools for capturing a whole training step (forward, backward, optimizer step) as

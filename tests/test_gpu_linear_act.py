@@ -57,7 +57,9 @@ def check_bwd(M, K, N, dt, act="none", in_act="none", grad=None, seed=0, parts=(
 # the smallest, odd and whole sizes: single tokens, edges of every tile, K of a few slabs and their remainders
 SIZES = [(1, 8, 8), (1, 768, 1000), (2, 24, 3), (16, 64, 16), (16, 1000, 33), (17, 72, 31), (31, 128, 64), (33, 40, 65), (64, 64, 64),
          (100, 192, 200), (129, 256, 127), (197, 768, 768), (300, 520, 1000), (985, 384, 1536), (2000, 333, 129), (77, 1, 5), (5, 5, 1),
-         (130, 13, 258), (1, 1, 1), (40, 4097, 24), (1, 777, 10), (4100, 136, 2056)]
+         (130, 13, 258), (1, 1, 1), (40, 4097, 24), (1, 777, 10), (4100, 136, 2056), (3000, 1000, 1000), (2600, 2504, 1000), (700, 999, 1001),
+         (6000, 1001, 2047), (8200, 520, 776), (8200, 3000, 264), (12000, 64, 264), (5000, 72, 1544), (30000, 24, 40), (20000, 9, 17),
+         (64, 100, 3000), (600, 3001, 600), (73, 73, 73), (72, 71, 70), (513, 65, 66)]
 
 
 @gpu
