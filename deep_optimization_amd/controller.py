@@ -82,8 +82,9 @@ _BATCHNORM = (nn.BatchNorm2d, nn.SyncBatchNorm)
 
 
 class _Tracer:
-    """torch.fx tracer that keeps this library's compressed layers as leaves, so a model that
-    already holds them traces (their forward is an autograd Function, not traceable ops)."""
+    """torch.fx tracer that keeps this library's compressed layers, and its transformer block layers, as
+    leaves, so a model that already holds them traces (their forward is an autograd Function, not
+    traceable ops)."""
 
     @staticmethod
     def make():
@@ -92,13 +93,17 @@ class _Tracer:
         from .layers import DOConv1d, DOConv2d, DOConv3d, DOLinear
         from .modules.activations import DOGELU, DOReLU_Variance, DOSiLU
         from .modules.normalization import DOBatchNorm2d, DOSyncBatchNorm2d
+        from .vit import FusedBlock
+        from .modules import transformer
 
+        block_layers = (transformer.LayerNorm, transformer.LinearAct, transformer.Mlp, transformer.DropoutAdd,
+                        transformer.DropoutRng, FusedBlock)
         compressed = (DOLinear, DOConv1d, DOConv2d, DOConv3d, DOGELU, DOReLU_Variance, DOSiLU, DOBatchNorm2d,
                       DOSyncBatchNorm2d, DOBatchNormReLU2d)
 
         class Tracer(fx.Tracer):
             def is_leaf_module(self, m, qualname):
-                return isinstance(m, compressed) or super().is_leaf_module(m, qualname)
+                return isinstance(m, compressed + block_layers) or super().is_leaf_module(m, qualname)
 
         return Tracer(), compressed
 

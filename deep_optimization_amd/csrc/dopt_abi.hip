@@ -1309,7 +1309,7 @@ int dopt_linear_weight_grad(const void* dz, int64_t ldz, const void* x, int64_t 
     const bool whole = M == 0 || (lin_rows(dz, ldz, N) && lin_rows(x, ldx, K));
     (void)hipGetLastError();
     if (whole && linear_dw_split(M, N, K) && ldz < ((int64_t)1 << 24) && ldx < ((int64_t)1 << 24)) {
-        if (!workspace) return fail(DOPT_EINVAL, "linear: null workspace");
+        if (!workspace && dopt::dw_any_workspace_floats(N, K, M) > 0) return fail(DOPT_EINVAL, "linear: null workspace");
         if (((uintptr_t)workspace & 15u) || (dw_f32 && ((uintptr_t)dw_f32 & 15u)) || (dw_16 && ((uintptr_t)dw_16 & 7u)))
             return fail(DOPT_EINVAL, "workspace / dw_f32 must be 16-byte and dw_16 8-byte aligned");
         dopt::DwArgs a{};

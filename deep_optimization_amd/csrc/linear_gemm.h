@@ -111,11 +111,8 @@ __device__ __forceinline__ int lin_col_swizzle(int r) {
     return W == 32 ? 0 : W == 64 ? ((r >> 1) & 1) << 2 : (r & 3) << 2;
 }
 
-// bytes of the smaller of a stage's two operand slabs
-constexpr int wave_part(int bm, int bn) { return (bm < bn ? bm : bn) * 2 * LIN_BK; }
-
-template <int BM, int BN, int S, int KS, int WAVES, int KIND, bool F16, bool REG, bool TAIL>
-__global__ __launch_bounds__(256 * KS, WAVES) void lin_gemm_kernel(LinArgs p) {
+template <int BM, int BN, int S, int WAVES, int KIND, bool F16, bool REG, bool TAIL>
+__global__ __launch_bounds__(256, WAVES) void lin_gemm_kernel(LinArgs p) {
     constexpr bool A_COLS = KIND == LIN_TN, B_COLS = KIND != LIN_NT;  // the operand lies as [K] rows
     static_assert(!REG || S == 2, "register loads: one slab in registers, two in LDS");
     constexpr int ROWB = 2 * LIN_BK, WM = BM / 2, WN = BN / 2, FM = WM / 16, FN = WN / 16;
@@ -125,30 +122,28 @@ __global__ __launch_bounds__(256 * KS, WAVES) void lin_gemm_kernel(LinArgs p) {
     const uint32_t K = (uint32_t)p.K;
     // every stage's A and B tiles are LDS objects of their own, so the compiler can tell an operand read from the
     // loads in flight
-    __shared__ __attribute__((aligned(1024))) uint8_t sA0[KS * BM * ROWB];
-    __shared__ __attribute__((aligned(1024))) uint8_t sA1[KS * BM * ROWB];
-    __shared__ __attribute__((aligned(1024))) uint8_t sA2[S > 2 ? KS * BM * ROWB : 16];
-    __shared__ __attribute__((aligned(1024))) uint8_t sA3[S > 3 ? KS * BM * ROWB : 16];
-    __shared__ __attribute__((aligned(1024))) uint8_t sB0[KS * BN * ROWB];
-    __shared__ __attribute__((aligned(1024))) uint8_t sB1[KS * BN * ROWB];
-    __shared__ __attribute__((aligned(1024))) uint8_t sB2[S > 2 ? KS * BN * ROWB : 16];
-    __shared__ __attribute__((aligned(1024))) uint8_t sB3[S > 3 ? KS * BN * ROWB : 16];
-    // KS > 1: that many groups of 4 waves, each with its own ring, take every KS-th slab
-    const int wave_id = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int group = KS > 1 ? wave_id >> 2 : 0, wave = wave_id & 3;
+    __shared__ __attribute__((aligned(1024))) uint8_t sA0[BM * ROWB];
+    __shared__ __attribute__((aligned(1024))) uint8_t sA1[BM * ROWB];
+    __shared__ __attribute__((aligned(1024))) uint8_t sA2[S > 2 ? BM * ROWB : 16];
+    __shared__ __attribute__((aligned(1024))) uint8_t sA3[S > 3 ? BM * ROWB : 16];
+    __shared__ __attribute__((aligned(1024))) uint8_t sB0[BN * ROWB];
+    __shared__ __attribute__((aligned(1024))) uint8_t sB1[BN * ROWB];
+    __shared__ __attribute__((aligned(1024))) uint8_t sB2[S > 2 ? BN * ROWB : 16];
+    __shared__ __attribute__((aligned(1024))) uint8_t sB3[S > 3 ? BN * ROWB : 16];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     auto stage_a = [&](auto i) __attribute__((always_inline)) -> uint8_t* {
         constexpr int I = decltype(i)::value % S;
-        if constexpr (I == 0) return sA0 + (KS > 1 ? group * (BM * ROWB) : 0);
-        else if constexpr (I == 1) return sA1 + (KS > 1 ? group * (BM * ROWB) : 0);
-        else if constexpr (I == 2) return sA2 + (KS > 1 ? group * (BM * ROWB) : 0);
-        else return sA3 + (KS > 1 ? group * (BM * ROWB) : 0);
+        if constexpr (I == 0) return sA0;
+        else if constexpr (I == 1) return sA1;
+        else if constexpr (I == 2) return sA2;
+        else return sA3;
     };
     auto stage_b = [&](auto i) __attribute__((always_inline)) -> uint8_t* {
         constexpr int I = decltype(i)::value % S;
-        if constexpr (I == 0) return sB0 + (KS > 1 ? group * (BN * ROWB) : 0);
-        else if constexpr (I == 1) return sB1 + (KS > 1 ? group * (BN * ROWB) : 0);
-        else if constexpr (I == 2) return sB2 + (KS > 1 ? group * (BN * ROWB) : 0);
-        else return sB3 + (KS > 1 ? group * (BN * ROWB) : 0);
+        if constexpr (I == 0) return sB0;
+        else if constexpr (I == 1) return sB1;
+        else if constexpr (I == 2) return sB2;
+        else return sB3;
     };
 
     uint32_t tm, tn;
@@ -187,41 +182,39 @@ __global__ __launch_bounds__(256 * KS, WAVES) void lin_gemm_kernel(LinArgs p) {
     // an operand read would make the compiler wait for the load there.
     // TAIL (K is no multiple of 64): the range of the slab that K ends in ends with the operand's last element; its base
     // steps, where rows of K otherwise keep theirs and step in soffset. A slab past K loads the last one again, which
-    // nobody multiplies (KS > 1: zeros, which are).
+    // nobody multiplies.
     const uint32_t n_slabs = (K + LIN_BK - 1) / LIN_BK, k_end = TAIL ? K / LIN_BK : 0xFFFFFFFFu;
-    const auto slab_range = [&](int64_t left, uint32_t ks) __attribute__((always_inline)) {
-        const int range = TAIL ? (int)max((int64_t)0, min(left, (int64_t)LIN_RANGE)) : (int)LIN_RANGE;
-        return KS > 1 ? range & -(int)(ks < n_slabs) : range;
+    const auto slab_range = [&](int64_t left) __attribute__((always_inline)) {
+        return TAIL ? (int)max((int64_t)0, min(left, (int64_t)LIN_RANGE)) : (int)LIN_RANGE;
     };
     auto rows_slab = [&](const uint16_t* base, int64_t ld, int64_t rows, int64_t r0, uint32_t ks) __attribute__((always_inline)) {
         const int64_t k0 = TAIL && ks == k_end ? (int64_t)ks * LIN_BK : 0;
-        const int range = slab_range(2 * ((rows - 1 - r0) * ld + ((int64_t)K + 7) / 8 * 8 - k0), ks);
+        const int range = slab_range(2 * ((rows - 1 - r0) * ld + ((int64_t)K + 7) / 8 * 8 - k0));
         return __builtin_amdgcn_make_buffer_rsrc((void*)(base + r0 * ld + k0), (short)0, range, 0x00020000);
     };
     auto cols_slab = [&](const uint16_t* base, int64_t ld, int64_t cols, int64_t c0, uint32_t ks) __attribute__((always_inline)) {
         const int64_t k0 = (int64_t)ks * LIN_BK;
-        const int range = slab_range(2 * (((int64_t)K - 1 - k0) * ld + (cols + 7) / 8 * 8 - c0), ks);
+        const int range = slab_range(2 * (((int64_t)K - 1 - k0) * ld + (cols + 7) / 8 * 8 - c0));
         return __builtin_amdgcn_make_buffer_rsrc((void*)(base + k0 * ld + c0), (short)0, range, 0x00020000);
     };
     // REG: two slabs on their way to LDS. A lane whose row or columns lie past the matrix reads row or column 0 (its
     // results are not stored); what lies past K is zeroed on the way to LDS.
     lin_v4u_t va[2][REG ? LA : 1], vb[2][REG ? LB : 1];
-    const uint16_t *pa[REG ? LA : 1], *pb[REG ? LB : 1];  // this group's next slab's chunks
+    const uint16_t *pa[REG ? LA : 1], *pb[REG ? LB : 1];  // the next slab's chunks
     if constexpr (REG) {
-        const int64_t k0 = (int64_t)group * LIN_BK;
 #pragma unroll
         for (int j = 0; j < LA; ++j)
-            pa[j] = p.A + (A_COLS ? (k0 + krow_a(j)) * lda + (offa[j] != LIN_OOB ? m0 + kcol_a(j) : 0)
-                                  : (offa[j] != LIN_OOB ? m0 + 32 * j + lrow : 0) * lda + k0 + lchunk * 8);
+            pa[j] = p.A + (A_COLS ? krow_a(j) * lda + (offa[j] != LIN_OOB ? m0 + kcol_a(j) : 0)
+                                  : (offa[j] != LIN_OOB ? m0 + 32 * j + lrow : 0) * lda + lchunk * 8);
 #pragma unroll
         for (int j = 0; j < LB; ++j)
-            pb[j] = p.B + (B_COLS ? (k0 + krow_b(j)) * ldb + (offb[j] != LIN_OOB ? n0 + kcol_b(j) : 0)
-                                  : (offb[j] != LIN_OOB ? n0 + 32 * j + lrow : 0) * ldb + k0 + lchunk * 8);
+            pb[j] = p.B + (B_COLS ? krow_b(j) * ldb + (offb[j] != LIN_OOB ? n0 + kcol_b(j) : 0)
+                                  : (offb[j] != LIN_OOB ? n0 + 32 * j + lrow : 0) * ldb + lchunk * 8);
     }
     auto load_regs = [&](auto set, uint32_t k) __attribute__((always_inline)) {
         if constexpr (REG) {
             constexpr int Q = decltype(set)::value & 1;
-            const int64_t k0 = ((int64_t)k * KS + group) * LIN_BK;
+            const int64_t k0 = (int64_t)k * LIN_BK;
             // a chunk may run past its row's end, but with 8 rows (or elements of a row) more behind this slab not past
             // the matrix's
             if (k0 + LIN_BK + 8 < (int64_t)K) {
@@ -240,15 +233,15 @@ __global__ __launch_bounds__(256 * KS, WAVES) void lin_gemm_kernel(LinArgs p) {
                     vb[Q][j] = lin_load8u(p.B, k0 + (B_COLS ? krow_b(j) : lchunk * 8) < (int64_t)K ? pb[j] - p.B : 0, total_b);
             }
 #pragma unroll
-            for (int j = 0; j < LA; ++j) pa[j] += KS * LIN_BK * (A_COLS ? lda : 1);
+            for (int j = 0; j < LA; ++j) pa[j] += LIN_BK * (A_COLS ? lda : 1);
 #pragma unroll
-            for (int j = 0; j < LB; ++j) pb[j] += KS * LIN_BK * (B_COLS ? ldb : 1);
+            for (int j = 0; j < LB; ++j) pb[j] += LIN_BK * (B_COLS ? ldb : 1);
         }
     };
     auto write_regs = [&](auto set, uint8_t* sa, uint8_t* sb, uint32_t k) __attribute__((always_inline)) {
         if constexpr (REG) {
             constexpr int Q = decltype(set)::value & 1;
-            const int64_t k0 = ((int64_t)k * KS + group) * LIN_BK;
+            const int64_t k0 = (int64_t)k * LIN_BK;
             if (k0 + LIN_BK > (int64_t)K) {
 #pragma unroll
                 for (int j = 0; j < LA; ++j)
@@ -265,7 +258,7 @@ __global__ __launch_bounds__(256 * KS, WAVES) void lin_gemm_kernel(LinArgs p) {
     };
     auto issue = [&](uint8_t* sa, uint8_t* sb, uint32_t k) __attribute__((always_inline)) {
         uint8_t *da = sa + opaque0, *db = sb + opaque0;
-        const uint32_t want = k * KS + group, ks = KS > 1 ? want : min(want, n_slabs - 1);
+        const uint32_t ks = min(k, n_slabs - 1);
         const int step = TAIL && ks == k_end ? 0 : (int)(2 * LIN_BK * ks);
         const __amdgpu_buffer_rsrc_t ra = A_COLS ? cols_slab(p.A, lda, M, m0, ks) : rows_slab(p.A, lda, M, m0, ks);
         const __amdgpu_buffer_rsrc_t rb = B_COLS ? cols_slab(p.B, ldb, N, n0, ks) : rows_slab(p.B, ldb, N, n0, ks);
@@ -284,9 +277,9 @@ __global__ __launch_bounds__(256 * KS, WAVES) void lin_gemm_kernel(LinArgs p) {
     // rows, the next row) is zeroed, each lane its own chunks. (Operands of [K] rows end there by their range.)
     auto cut = [&](uint8_t* sa, uint8_t* sb, uint32_t k) __attribute__((always_inline)) {
         if constexpr (TAIL && KIND != LIN_TN) {
-            if (k != k_end / KS) return;  // the same for the whole workgroup
+            if (k != k_end) return;  // the same for the whole workgroup
             const int have = (int)(K % LIN_BK) - lchunk * 8;  // of this lane's chunks
-            if (k * KS + group == k_end && have < 8) {
+            if (have < 8) {
 #pragma unroll
                 for (int j = 0; j < LA; ++j) lin_cut8(sa + wave * 1024 + j * 4096 + lane * 16, have);
                 if constexpr (!B_COLS) {
@@ -390,8 +383,7 @@ __global__ __launch_bounds__(256 * KS, WAVES) void lin_gemm_kernel(LinArgs p) {
     using I2 = std::integral_constant<int, 2>;
     using I3 = std::integral_constant<int, 3>;
 
-    const uint32_t nk = ((K + LIN_BK - 1) / LIN_BK + KS - 1) / KS;  // slabs of a group (those past K are zeros)
-    if (nk > 0) {
+    if (n_slabs > 0) {
         if constexpr (REG) {
             load_regs(I0{}, 0);
             load_regs(I1{}, 1);
@@ -412,16 +404,16 @@ __global__ __launch_bounds__(256 * KS, WAVES) void lin_gemm_kernel(LinArgs p) {
         cut(stage_a(I0{}), stage_b(I0{}), 0);
         read_half(stage_a(I0{}), stage_b(I0{}), 0, a0, b0);
         uint32_t k = 0;
-        for (; k + S <= nk; k += S) {
+        for (; k + S <= n_slabs; k += S) {
             slab(k, I0{});
             slab(k + 1, I1{});
             if constexpr (S > 2) slab(k + 2, I2{});
             if constexpr (S > 3) slab(k + 3, I3{});
         }
-        if (k < nk) slab(k, I0{});
-        if (S > 2 && k + 1 < nk) slab(k + 1, I1{});
+        if (k < n_slabs) slab(k, I0{});
+        if (S > 2 && k + 1 < n_slabs) slab(k + 1, I1{});
         if constexpr (S > 3) {
-            if (k + 2 < nk) slab(k + 2, I2{});
+            if (k + 2 < n_slabs) slab(k + 2, I2{});
         }
     }
     // the trailing loads land and every wave's operand reads return before LDS is used again
@@ -431,39 +423,7 @@ __global__ __launch_bounds__(256 * KS, WAVES) void lin_gemm_kernel(LinArgs p) {
     // ---- epilogue: up to 32 rows of the wave's tile at a time through LDS in fp32, then 8 columns of a row per lane
     constexpr int PITCH = WN + 4, RB = WM < 32 ? WM : 32;  // floats per staged row, rows at a time
     static_assert(RB * PITCH * 4 <= BM * ROWB && RB * PITCH * 4 <= BN * ROWB, "a wave's rows fit one LDS array");
-    uint8_t* const mine = wave == 0 ? sA0 : wave == 1 ? sA1 : wave == 2 ? sB0 : sB1;
-    if constexpr (KS > 1) {
-        // the groups' sums, added in order by the first
-        constexpr int PART = wave_part(BM, BN), AREA = FM * FN * 1024 + (KIND == LIN_TN ? FM * 256 : 0);
-        static_assert(AREA <= PART && FM <= 4, "a wave's sums fit its part of an LDS array");
-        const int stride = wave < 2 ? BM * ROWB : BN * ROWB;
-        if (group > 0) {
-            uint8_t* out = mine + group * stride;
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j) *(lin_v4f_t*)(out + (i * FN + j) * 1024 + lane * 16) = acc[i][j];
-            if constexpr (KIND == LIN_TN) {
-#pragma unroll
-                for (int i = 0; i < FM; ++i) *(float*)(out + FM * FN * 1024 + i * 256 + lane * 4) = col_sum[i];
-            }
-        }
-        __syncthreads();
-        if (group > 0) return;
-#pragma unroll
-        for (int g = 1; g < KS; ++g) {
-            const uint8_t* in = mine + g * stride;
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] += *(const lin_v4f_t*)(in + (i * FN + j) * 1024 + lane * 16);
-            if constexpr (KIND == LIN_TN) {
-#pragma unroll
-                for (int i = 0; i < FM; ++i) col_sum[i] += *(const float*)(in + FM * FN * 1024 + i * 256 + lane * 4);
-            }
-        }
-    }
-    float* st = (float*)mine;
+    float* const st = (float*)(wave == 0 ? sA0 : wave == 1 ? sA1 : wave == 2 ? sB0 : sB1);
     constexpr int CPR = WN / 8, RPI = 64 / CPR;  // chunks per row, rows per step
     const int64_t row0 = m0 + WM * wm, n = n0 + WN * wn + 8 * (lane % CPR);
     float bias[8];
@@ -510,14 +470,14 @@ __global__ __launch_bounds__(256 * KS, WAVES) void lin_gemm_kernel(LinArgs p) {
     }
 }
 
-// KS: groups of 4 waves that share a tile's slabs; WAVES: waves per SIMD that the registers leave room for
-template <int BM, int BN, int S, int KS, int WAVES, int KIND, bool F16, bool REG = false>
+// WAVES: waves per SIMD that the registers leave room for
+template <int BM, int BN, int S, int WAVES, int KIND, bool F16, bool REG = false>
 inline void lin_gemm_launch(LinArgs p, hipStream_t s) {
     p.tiles_m = (uint32_t)((p.M + BM - 1) / BM);
     p.tiles_n = (uint32_t)((p.N + BN - 1) / BN);
-    const dim3 grid(p.tiles_m * p.tiles_n), block(256 * KS);
-    if (REG || p.K % LIN_BK == 0) hipLaunchKernelGGL((lin_gemm_kernel<BM, BN, S, KS, WAVES, KIND, F16, REG, false>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((lin_gemm_kernel<BM, BN, S, KS, WAVES, KIND, F16, REG, !REG>), grid, block, 0, s, p);
+    const dim3 grid(p.tiles_m * p.tiles_n), block(256);
+    if (REG || p.K % LIN_BK == 0) hipLaunchKernelGGL((lin_gemm_kernel<BM, BN, S, WAVES, KIND, F16, REG, false>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((lin_gemm_kernel<BM, BN, S, WAVES, KIND, F16, REG, !REG>), grid, block, 0, s, p);
 }
 
 }  // namespace dopt

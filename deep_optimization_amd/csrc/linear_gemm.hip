@@ -103,13 +103,13 @@ void launch(const LinArgs& p, hipStream_t s) {
         }
     }
     switch (t) {
-        case T_32x64: return lin_gemm_launch<32, 64, 4, 1, 3, KIND, F16>(p, s);
-        case T_64x64: return lin_gemm_launch<64, 64, 4, 1, 2, KIND, F16>(p, s);
-        case T_64x64_4: return lin_gemm_launch<64, 64, 2, 1, 4, KIND, F16>(p, s);
-        case T_128x64: return lin_gemm_launch<128, 64, 3, 1, 2, KIND, F16>(p, s);
-        case T_REG32x64: return lin_gemm_launch<32, 64, 2, 1, 4, KIND, F16, true>(p, s);
-        case T_REG64x64: return lin_gemm_launch<64, 64, 2, 1, 3, KIND, F16, true>(p, s);
-        default: return lin_gemm_launch<128, 128, 2, 1, 2, KIND, F16>(p, s);
+        case T_32x64: return lin_gemm_launch<32, 64, 4, 3, KIND, F16>(p, s);
+        case T_64x64: return lin_gemm_launch<64, 64, 4, 2, KIND, F16>(p, s);
+        case T_64x64_4: return lin_gemm_launch<64, 64, 2, 4, KIND, F16>(p, s);
+        case T_128x64: return lin_gemm_launch<128, 64, 3, 2, KIND, F16>(p, s);
+        case T_REG32x64: return lin_gemm_launch<32, 64, 2, 4, KIND, F16, true>(p, s);
+        case T_REG64x64: return lin_gemm_launch<64, 64, 2, 3, KIND, F16, true>(p, s);
+        default: return lin_gemm_launch<128, 128, 2, 2, KIND, F16>(p, s);
     }
 }
 

@@ -1,0 +1,266 @@
+"""Layers of a pre-norm transformer block on the layer norm, dropout and linear operators (``ln_lib``, ``dropout_lib``,
+``linear_lib``). No counterparts in the reference, whose transformer models use torch's modules.
+
+Functional forms, differentiable, on the GPU:
+
+    layer_norm(x, weight, bias, eps)                      in the autocast dtype under autocast, else in x's
+    layer_norm_residual(x, weight, bias, eps)             (layer_norm(x), x); its backward adds the gradient that reaches x
+                                                          past the norm while it writes the norm's own
+    linear_act(x, weight, bias, residual, act)            act(x weight^T + bias) + residual
+    mlp(x, w1, b1, w2, b2, residual, act)                 act(x w1^T + b1) w2^T + b2 + residual; its backward hands the first
+                                                          layer the gradient of its pre-activation in one pass
+    dropout_add(x, residual, p, seed, offset, step)       residual + dropout(x)
+
+and as modules with torch's parameter names: LayerNorm, LinearAct, Mlp, DropoutAdd (with DropoutRng, the count that gives
+every pass of a model its own masks). Products run in bf16 or fp16: of that type, or under autocast.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch import Tensor, nn
+from torch.amp import custom_bwd, custom_fwd
+from torch.autograd import Function
+
+from .. import dropout_lib, linear_lib, ln_lib  # noqa: F401  (registers torch.ops.act_lib.*)
+from .ops import _compute_dtype
+
+_U63 = (1 << 63) - 1
+
+
+def _grad(*tensors: Optional[Tensor]) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _to(t: Optional[Tensor], dtype: torch.dtype) -> Optional[Tensor]:
+    return None if t is None else t.to(dtype)
+
+
+def _product_operands(x: Tensor, *weights: Tensor):
+    """x and weights in the products' type: the autocast dtype, else x's."""
+    dt = _compute_dtype() or x.dtype
+    return (x.to(dt), *(w.to(dt) for w in weights))
+
+
+def _grad_dtype(param: Tensor, operand: Tensor) -> torch.dtype:
+    return operand.dtype if param.dtype == operand.dtype else torch.float32
+
+
+class _LayerNorm(Function):
+    @staticmethod
+    @custom_fwd(device_type="cuda")
+    def forward(ctx, x, weight, bias, eps, residual):
+        y, mean, rstd = torch.ops.act_lib.layer_norm_fwd(x, weight, bias, eps, _compute_dtype() or x.dtype)
+        ctx.save_for_backward(x, mean, rstd, weight)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.set_materialize_grads(False)
+        return (y, x.view_as(x)) if residual else y
+
+    @staticmethod
+    @custom_bwd(device_type="cuda")
+    def backward(ctx, dy, dresidual=None):
+        x, mean, rstd, weight = ctx.saved_tensors
+        _, need_w, need_b, _, _ = ctx.needs_input_grad
+        if dy is None:
+            return dresidual, None, None, None, None
+        dx, dw, db = torch.ops.act_lib.layer_norm_bwd(dy, x, mean, rstd, weight, dresidual, need_w, need_b)
+        return dx, _to(dw, weight.dtype) if need_w else None, _to(db, ctx.bias_dtype) if need_b else None, None, None
+
+
+def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5) -> Tensor:
+    return _LayerNorm.apply(x, weight, bias, eps, False)
+
+
+def layer_norm_residual(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5):
+    return _LayerNorm.apply(x, weight, bias, eps, True)
+
+
+class _LinearAct(Function):
+    @staticmethod
+    @custom_fwd(device_type="cuda")
+    def forward(ctx, x, weight, bias, residual, act):
+        xc, wc = _product_operands(x, weight)
+        y, pre = torch.ops.act_lib.linear_act_fwd(xc, wc, bias, residual, act, act != "none")
+        ctx.save_for_backward(xc, wc, pre)
+        ctx.act, ctx.x_dtype, ctx.param = act, x.dtype, (weight.dtype, None if bias is None else bias.dtype)
+        ctx.grad_dtype = _grad_dtype(weight, wc)
+        return y
+
+    @staticmethod
+    @custom_bwd(device_type="cuda")
+    def backward(ctx, dy):
+        x, weight, pre = ctx.saved_tensors
+        need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
+        dx, dw, db = torch.ops.act_lib.linear_act_bwd(dy.to(x.dtype), x, weight, pre, ctx.act, None, "none", need_x, need_w, need_b,
+                                                      ctx.grad_dtype)
+        return (_to(dx, ctx.x_dtype), _to(dw, ctx.param[0]), _to(db, ctx.param[1]) if need_b else None, dy if need_r else None, None)
+
+
+def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, residual: Optional[Tensor] = None, act: str = "none") -> Tensor:
+    if not _grad(x, weight, bias, residual):
+        xc, wc = _product_operands(x, weight)
+        return torch.ops.act_lib.linear_act_fwd(xc, wc, bias, residual, act, False)[0]
+    return _LinearAct.apply(x, weight, bias, residual, act)
+
+
+class _Mlp(Function):
+    @staticmethod
+    @custom_fwd(device_type="cuda")
+    def forward(ctx, x, w1, b1, w2, b2, residual, act):
+        xc, w1c, w2c = _product_operands(x, w1, w2)
+        h, pre = torch.ops.act_lib.linear_act_fwd(xc, w1c, b1, None, act, act != "none")
+        y, _ = torch.ops.act_lib.linear_act_fwd(h, w2c, b2, residual, "none", False)
+        ctx.save_for_backward(xc, w1c, w2c, h, pre)
+        ctx.act, ctx.x_dtype = act, x.dtype
+        ctx.param = tuple(None if t is None else t.dtype for t in (w1, b1, w2, b2))
+        ctx.grad_dtypes = _grad_dtype(w1, w1c), _grad_dtype(w2, w2c)
+        return y
+
+    @staticmethod
+    @custom_bwd(device_type="cuda")
+    def backward(ctx, dy):
+        x, w1, w2, h, pre = ctx.saved_tensors
+        need_x, need_w1, need_b1, need_w2, need_b2, need_r, _ = ctx.needs_input_grad
+        first = need_x or need_w1 or need_b1
+        dz, dw2, db2 = torch.ops.act_lib.linear_act_bwd(dy.to(x.dtype), h, w2, None, "none", pre, ctx.act, first, need_w2, need_b2,
+                                                        ctx.grad_dtypes[1])
+        dx = dw1 = db1 = None
+        if first:
+            dx, dw1, db1 = torch.ops.act_lib.linear_act_bwd(dz, x, w1, None, "none", None, "none", need_x, need_w1, need_b1,
+                                                            ctx.grad_dtypes[0])
+        t1, u1, t2, u2 = ctx.param
+        return (_to(dx, ctx.x_dtype), _to(dw1, t1), _to(db1, u1) if need_b1 else None, _to(dw2, t2), _to(db2, u2) if need_b2 else None,
+                dy if need_r else None, None)
+
+
+def mlp(x: Tensor, w1: Tensor, b1: Optional[Tensor], w2: Tensor, b2: Optional[Tensor], residual: Optional[Tensor] = None,
+        act: str = "gelu") -> Tensor:
+    if not _grad(x, w1, b1, w2, b2, residual):
+        xc, w1c, w2c = _product_operands(x, w1, w2)
+        h = torch.ops.act_lib.linear_act_fwd(xc, w1c, b1, None, act, False)[0]
+        return torch.ops.act_lib.linear_act_fwd(h, w2c, b2, residual, "none", False)[0]
+    return _Mlp.apply(x, w1, b1, w2, b2, residual, act)
+
+
+class _DropoutAdd(Function):
+    @staticmethod
+    def forward(ctx, x, residual, p, seed, offset, step):
+        ctx.save_for_backward(step)
+        ctx.args, ctx.x_dtype = (p, seed, offset), x.dtype
+        return torch.ops.act_lib.dropout_add_fwd(x, residual, p, seed, offset, step)
+
+    @staticmethod
+    def backward(ctx, dy):
+        (step,) = ctx.saved_tensors
+        need_x, need_r = ctx.needs_input_grad[:2]
+        dx = torch.ops.act_lib.dropout_bwd(dy, *ctx.args, step, ctx.x_dtype) if need_x else None
+        return dx, dy if need_r else None, None, None, None, None
+
+
+def dropout_add(x: Tensor, residual: Optional[Tensor], p: float, seed: int, offset: int = 0, step: Optional[Tensor] = None) -> Tensor:
+    return _DropoutAdd.apply(x, residual, p, seed, offset, step)
+
+
+class LayerNorm(nn.LayerNorm):
+    """torch.nn.LayerNorm over the last axis. ``residual(x)`` is (norm(x), x) for x + f(norm(x))."""
+
+    def __init__(self, dim: int, eps: float = 1e-5, **kw):
+        super().__init__(dim, eps, **kw)
+        if len(self.normalized_shape) != 1:
+            raise ValueError(f"LayerNorm normalizes the last axis only, got {self.normalized_shape}")
+
+    def forward(self, x):
+        return layer_norm(x, self.weight, self.bias, self.eps)
+
+    def residual(self, x):
+        return layer_norm_residual(x, self.weight, self.bias, self.eps)
+
+
+class LinearAct(nn.Module):
+    """act(x weight^T + bias) + residual with torch.nn.Linear's parameters and initialisation."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, act: str = "none", device=None, dtype=None):
+        super().__init__()
+        linear_lib._act_code(act)
+        plain = nn.Linear(in_features, out_features, bias, device=device, dtype=dtype)
+        self.in_features, self.out_features, self.act = in_features, out_features, act
+        self.weight, self.bias = plain.weight, plain.bias
+
+    def forward(self, x, residual=None):
+        return linear_act(x, self.weight, self.bias, residual, self.act)
+
+    def extra_repr(self):
+        return f"{self.in_features}, {self.out_features}, bias={self.bias is not None}, act={self.act!r}"
+
+
+class DropoutRng(nn.Module):
+    """The masks of a model's dropout layers: a seed, and a count of passes that lies on the device, so that a captured
+    step draws new masks on every replay. Call it once at the start of a pass, on the input: it returns that and steps the
+    count. Every layer has an offset of its own (``site``). ``step`` is part of the state dict; the seed is not: ranks that
+    train on different data each give their own (default: from torch's initial seed)."""
+
+    def __init__(self, seed: Optional[int] = None):
+        super().__init__()
+        # (not the quantizer's default key: both use the same generator)
+        self.seed = (torch.initial_seed() ^ 0x64726F70 if seed is None else seed) & _U63
+        self.register_buffer("step", torch.zeros(1, dtype=torch.int64))
+        self.current = None
+        self.sites = 0
+
+    def site(self) -> int:
+        self.sites += 1
+        return (self.sites - 1) << 40
+
+    def forward(self, x):
+        if self.training:
+            # (a tensor of its own, which the pass's backward reads whatever passes follow)
+            self.current = self.step + 1
+            self.step.copy_(self.current)
+        return x
+
+
+class DropoutAdd(nn.Module):
+    """residual + dropout(x), in residual's type (x's without one)."""
+
+    def __init__(self, p: float, rng: DropoutRng):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"p must lie in [0, 1], got {p}")
+        self.p, self.offset = float(p), rng.site()
+        self._rng = (rng,)  # (not a submodule of every layer)
+
+    def forward(self, x, residual=None):
+        if not self.training or self.p == 0.0:
+            return x if residual is None else residual + x.to(residual.dtype)
+        rng = self._rng[0]
+        if rng.current is None:
+            raise RuntimeError("DropoutAdd: call the model's DropoutRng at the start of the pass")
+        return dropout_add(x, residual, self.p, rng.seed, self.offset, rng.current)
+
+    def extra_repr(self):
+        return f"p={self.p}"
+
+
+class Mlp(nn.Module):
+    """fc2(act(fc1(x))) + residual; with a dropout rate after the activation and after fc2."""
+
+    def __init__(self, dim: int, hidden: int, act: str = "gelu", drop: float = 0.0, rng: Optional[DropoutRng] = None):
+        super().__init__()
+        self.fc1 = LinearAct(dim, hidden, act=act)
+        self.fc2 = LinearAct(hidden, dim)
+        if drop:
+            if rng is None:
+                raise ValueError("Mlp: a dropout rate needs a DropoutRng")
+            self.drop1, self.drop2 = DropoutAdd(drop, rng), DropoutAdd(drop, rng)
+        else:
+            self.drop1 = self.drop2 = None
+
+    def forward(self, x, residual=None):
+        if self.drop1 is not None and self.training:
+            return self.drop2(self.fc2(self.drop1(self.fc1(x))), residual)
+        return mlp(x, self.fc1.weight, self.fc1.bias, self.fc2.weight, self.fc2.bias, residual, self.fc1.act)
+
+
+__all__ = ["layer_norm", "layer_norm_residual", "linear_act", "mlp", "dropout_add", "LayerNorm", "LinearAct", "DropoutRng", "DropoutAdd",
+           "Mlp"]
