@@ -69,7 +69,7 @@ EXPORTS = (
     "dopt_dropout",
     "dopt_linear_forward",
     "dopt_linear_input_grad",
-    "dopt_linear_act_grad",
+    "dopt_linear_layout",
     "dopt_linear_weight_grad_workspace_floats",
     "dopt_linear_weight_grad",
     "dopt_linear_tile",
@@ -77,6 +77,12 @@ EXPORTS = (
 )
 
 _lib = None
+
+
+class LinearRows(ctypes.Structure):
+    """dopt_linear_rows: a matrix that dopt_linear_layout lays out."""
+    _fields_ = [("src", ctypes.c_void_p), ("ld_src", ctypes.c_int64), ("pre", ctypes.c_void_p), ("rows", ctypes.c_int64),
+                ("cols", ctypes.c_int64), ("dst", ctypes.c_void_p), ("ld_dst", ctypes.c_int64), ("act", ctypes.c_int)]
 
 
 class DoptError(RuntimeError):
@@ -211,8 +217,8 @@ def lib() -> ctypes.CDLL:
         L.dopt_linear_forward.restype = i32
         L.dopt_linear_input_grad.argtypes = [vp, i64, vp, i64, i32, i64, i64, i64, vp, i32, vp, vp]
         L.dopt_linear_input_grad.restype = i32
-        L.dopt_linear_act_grad.argtypes = [vp, i64, vp, i32, i32, i64, i64, vp, i64, vp]
-        L.dopt_linear_act_grad.restype = i32
+        L.dopt_linear_layout.argtypes = [ctypes.POINTER(LinearRows), i32, i32, vp]
+        L.dopt_linear_layout.restype = i32
         L.dopt_linear_weight_grad_workspace_floats.argtypes = [i64, i64, i64]
         L.dopt_linear_weight_grad_workspace_floats.restype = i64
         L.dopt_linear_weight_grad.argtypes = [vp, i64, vp, i64, i32, i64, i64, i64, vp, vp, vp, vp, vp, vp]

@@ -42,8 +42,7 @@ int launch_dropout(const void* x, int x_dt, const void* residual, uint64_t n, ui
 bool lin_shape_fits(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb);
 int launch_linear(const LinArgs& p, int kind, bool f16, hipStream_t s);
 int linear_tile(int kind, int64_t M, int64_t N, int64_t K, bool reg, bool big, float* us);
-int launch_linear_act_grad(const uint16_t* src, int64_t src_ld, const uint16_t* pre, int act, bool f16, int64_t rows,
-                           int64_t cols, uint16_t* dst, int64_t ld_dst, hipStream_t s);
+int launch_linear_rows(LinRowItems items, bool f16, hipStream_t s);
 }  // namespace dopt
 
 namespace {
@@ -1210,7 +1209,7 @@ int dopt_linear_tile(int product, int64_t M, int64_t N, int64_t K, int any_rows)
     return dopt::linear_tile(product, m, n, k, any_rows != 0, true, nullptr);
 }
 
-int dopt_linear_copy_preferred(int product, int64_t M, int64_t N, int64_t K, int64_t elements, int copies) {
+int dopt_linear_copy_preferred(int product, int64_t M, int64_t N, int64_t K, int64_t elements, int launches) {
     if (product < DOPT_LIN_FORWARD || product > DOPT_LIN_WEIGHT_GRAD || M < 0 || N < 0 || K < 0) return 0;
     int64_t m, n, k;
     linear_sizes(product, M, N, K, &m, &n, &k);
@@ -1221,7 +1220,7 @@ int dopt_linear_copy_preferred(int product, int64_t M, int64_t N, int64_t K, int
         const float split = linear_dw_split_us(M, N, (K + 7) / 8 * 8);
         if (split < aligned) aligned = split + (K % 8 ? 3.0f : 0.0f);  // (the result's rows are cut to K)
     }
-    return aligned + (float)copies * 2.5f + (float)elements * (4.0f / 3.0e6f) < as_is;
+    return aligned + (float)launches * 2.5f + (float)elements * (4.0f / 3.0e6f) < as_is;
 }
 
 int dopt_linear_forward(const void* x, int64_t ldx, const void* weight, int64_t ldw, int dtype, int64_t M, int64_t N,
@@ -1280,18 +1279,26 @@ int dopt_linear_input_grad(const void* dz, int64_t ldz, const void* weight, int6
     return hip_status("linear_input_grad launch");
 }
 
-int dopt_linear_act_grad(const void* dy, int64_t ld_dy, const void* pre, int act, int dtype, int64_t rows, int64_t cols,
-                         void* dz, int64_t ld_dz, void* stream) {
-    if (int rc = check_linear(dtype, rows, cols, 0, 0, 0, act)) return rc;
-    if (rows == 0 || cols == 0) return ok();
-    if (!dy || !dz || (act != DOPT_LIN_NONE && !pre)) return fail(DOPT_EINVAL, "null dy/pre/dz pointer");
-    if (ld_dy < cols || (!lin_rows(dz, ld_dz, cols) && !(ld_dz == cols && ld_dy == cols && act != DOPT_LIN_NONE)))
-        return fail(DOPT_EINVAL, "linear: dz must be 16-byte aligned with a row stride that is a multiple of 8 and at least cols (or, with an "
-                                 "activation, as contiguous as dy); dy's stride must be at least cols");
+int dopt_linear_layout(const dopt_linear_rows* rows, int n, int dtype, void* stream) {
+    if (n < 0 || n > dopt::LIN_ROW_ITEMS || (n > 0 && !rows)) return fail(DOPT_EINVAL, "linear: 0 to %d matrices, got %d", dopt::LIN_ROW_ITEMS, n);
+    dopt::LinRowItems items{};
+    for (int k = 0; k < n; ++k) {
+        const dopt_linear_rows& r = rows[k];
+        if (int rc = check_linear(dtype, 0, 0, 0, 0, 0, r.act)) return rc;
+        if (r.rows < 0 || r.cols < 0)
+            return fail(DOPT_EINVAL, "linear: sizes must be >= 0 (got %lld, %lld)", (long long)r.rows, (long long)r.cols);
+        if (r.rows == 0 || r.cols == 0) continue;
+        if (!r.src || !r.dst || (r.act != DOPT_LIN_NONE && !r.pre)) return fail(DOPT_EINVAL, "linear: null src/pre/dst pointer");
+        if (r.ld_src < r.cols || r.ld_dst < r.cols || !aligned16(r.dst) || (r.rows > 1 && r.ld_dst % 8 != 0))
+            return fail(DOPT_EINVAL, "linear: src's rows must lie at least cols apart, dst's in 16-byte aligned rows of at least cols elements");
+        if (r.ld_src >= ((int64_t)1 << 44) / r.rows || r.ld_dst >= ((int64_t)1 << 44) / r.rows)
+            return fail(DOPT_EUNSUPPORTED, "linear: matrices below 2^44 elements");
+        items.item[items.n++] = {(const uint16_t*)r.src, r.ld_src, (const uint16_t*)r.pre, r.rows, r.cols, (uint16_t*)r.dst, r.ld_dst, r.act, 0};
+    }
+    if (items.n == 0) return ok();
     (void)hipGetLastError();
-    dopt::launch_linear_act_grad((const uint16_t*)dy, ld_dy, (const uint16_t*)pre, act, dtype == DOPT_F16, rows, cols,
-                                 (uint16_t*)dz, ld_dz, (hipStream_t)stream);
-    return hip_status("linear_act_grad launch");
+    dopt::launch_linear_rows(items, dtype == DOPT_F16, (hipStream_t)stream);
+    return hip_status("linear_layout launch");
 }
 
 int64_t dopt_linear_weight_grad_workspace_floats(int64_t M, int64_t N, int64_t K) {

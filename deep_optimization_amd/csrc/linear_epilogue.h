@@ -27,6 +27,25 @@ struct LinArgs {
     int bias_dt, act, y_f32;
 };
 
+// Rows laid out for the products: dst[r][c] = src[r][c] act'(pre[r][c]) for c < cols, 0 for the columns up to ld_dst (act
+// LIN_NONE: a copy). src rows ld_src elements apart, pre [rows][cols] contiguous, dst 16-byte aligned with ld_dst a multiple
+// of 8 (or one row).
+struct LinRowItem {
+    const uint16_t* src;
+    int64_t ld_src;
+    const uint16_t* pre;
+    int64_t rows, cols;
+    uint16_t* dst;
+    int64_t ld_dst;
+    int act;
+    uint32_t blocks;  // set by the launcher
+};
+constexpr int LIN_ROW_ITEMS = 4;
+struct LinRowItems {
+    LinRowItem item[LIN_ROW_ITEMS];
+    int n;
+};
+
 // GELU through the normal distribution's upper tail: with a = |z| and Q(a) = 1 - Phi(a),
 //   gelu(z) = max(z, 0) - a Q(a),  Q(a) = t P(t) e^{-a^2 / 2} / 2,  t = 1 / (1 + c a)
 // (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26, whose erf is within 1.5e-7: nothing cancels

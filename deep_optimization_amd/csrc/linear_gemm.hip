@@ -113,40 +113,45 @@ void launch(const LinArgs& p, hipStream_t s) {
     }
 }
 
-// dst[r][c] = src[r][c] act'(pre[r][c]) for c < cols, 0 for the columns up to ld_dst; 8 columns a lane. The source has
-// rows of src_ld elements (pre: cols), dst's are aligned.
-template <bool F16>
-__global__ __launch_bounds__(256) void lin_act_grad_kernel(const uint16_t* src, int64_t src_ld, const uint16_t* pre, int act,
-                                                           int64_t rows, int64_t cols, uint16_t* dst, int64_t ld_dst) {
-    constexpr int DT = F16 ? DT_F16 : DT_BF16;
-    const uint64_t cpr = (uint64_t)ld_dst / 8, total = (uint64_t)rows * cpr;
-    for (uint64_t q = (uint64_t)blockIdx.x * 256 + threadIdx.x; q < total; q += (uint64_t)gridDim.x * 256) {
-        // (32-bit division where it does)
-        const int64_t r = total >> 32 ? (int64_t)(q / cpr) : (int64_t)((uint32_t)q / (uint32_t)cpr);
-        const int64_t c = ((int64_t)q - r * (int64_t)cpr) * 8;
-        const int have = (int)std::min<int64_t>(8, cols - c);
-        float v[8];
-        lin_load8<DT>(src, r * src_ld + c, have, v);
-        if (act != LIN_NONE) {
-            float z[8];
-            lin_load8<DT>(pre, r * cols + c, have, z);
-            lin_act_grad8(act, z, v);
-        }
-        lin_store8<DT>(dst, r * ld_dst + c, 8, v);
+// Elements i .. i + 7 of rows at any element, those from `have` on as zeros; `total` elements exist from p on. One vector load,
+// which may reach into the next row, where that lies in the matrix.
+template <int DT>
+__device__ __forceinline__ void lin_load_row8(const uint16_t* p, int64_t i, int64_t total, int have, float* f) {
+    if (i + 8 <= total) {
+        lin_load8<DT>(p, i, 8, f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = e < have ? f[e] : 0.0f;
+    } else {
+        lin_load8<DT>(p, i, have, f);
     }
 }
 
-// the same without rows: n elements
+// Every item's rows (linear_epilogue.h), 8 columns a lane; an item's blocks follow the ones before it. Memory-bound: 2 bytes
+// read (4 with an activation) and 2 written an element; 25216 x 3072 with GELU 114 us, 4.1 TB/s. The backward of a layer
+// whose sizes are no multiples of 8 hands up to three operands to one launch: 2001 rows of 333 -> 1001 9.0 us, in three
+// launches 15.0.
 template <bool F16>
-__global__ __launch_bounds__(256) void lin_act_grad_flat_kernel(const uint16_t* src, const uint16_t* pre, int act, int64_t n, uint16_t* dst) {
+__global__ __launch_bounds__(256) void lin_rows_kernel(LinRowItems items) {
     constexpr int DT = F16 ? DT_F16 : DT_BF16;
-    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (int64_t)gridDim.x * 2048) {
-        const int have = (int)std::min<int64_t>(8, n - i);
-        float v[8], z[8];
-        lin_load8<DT>(src, i, have, v);
-        lin_load8<DT>(pre, i, have, z);
-        lin_act_grad8(act, z, v);
-        lin_store8<DT>(dst, i, have, v);
+    uint32_t block = blockIdx.x;
+    int k = 0;
+    while (k + 1 < items.n && block >= items.item[k].blocks) block -= items.item[k++].blocks;
+    const LinRowItem p = items.item[k];
+    const uint64_t cpr = (uint64_t)(p.ld_dst + 7) / 8, total = (uint64_t)p.rows * cpr;
+    const int64_t src_total = (p.rows - 1) * p.ld_src + p.cols;
+    for (uint64_t q = (uint64_t)block * 256 + threadIdx.x; q < total; q += (uint64_t)p.blocks * 256) {
+        // (one row: contiguous matrices; 32-bit division where it does)
+        const int64_t r = p.rows == 1 ? 0 : total >> 32 ? (int64_t)(q / cpr) : (int64_t)((uint32_t)q / (uint32_t)cpr);
+        const int64_t c = ((int64_t)q - r * (int64_t)cpr) * 8;
+        const int have = (int)max((int64_t)0, min((int64_t)8, p.cols - c));
+        float v[8];
+        lin_load_row8<DT>(p.src, r * p.ld_src + c, src_total, have, v);
+        if (p.act != LIN_NONE) {
+            float z[8];
+            lin_load_row8<DT>(p.pre, r * p.cols + c, p.rows * p.cols, have, z);
+            lin_act_grad8(p.act, z, v);
+        }
+        lin_store8<DT>(p.dst, r * p.ld_dst + c, (int)min((int64_t)8, p.ld_dst - c), v);
     }
 }
 
@@ -180,16 +185,17 @@ int linear_tile(int kind, int64_t M, int64_t N, int64_t K, bool reg, bool big, f
     return plan(kind, M, N, K, n_cu, reg, big && N % 8 == 0 && K >= LIN_BK, 1.0f, us);
 }
 
-int launch_linear_act_grad(const uint16_t* src, int64_t src_ld, const uint16_t* pre, int act, bool f16, int64_t rows,
-                           int64_t cols, uint16_t* dst, int64_t ld_dst, hipStream_t s) {
-    const bool flat = src_ld == cols && ld_dst == cols && act != LIN_NONE;
-    const int64_t n = rows * cols, chunks = flat ? (n + 7) / 8 : rows * (ld_dst / 8);
-    if (chunks == 0) return 0;
-    const dim3 grid((uint32_t)std::min<int64_t>((chunks + 255) / 256, 1 << 20));
-    if (flat && f16) hipLaunchKernelGGL(lin_act_grad_flat_kernel<true>, grid, dim3(256), 0, s, src, pre, act, n, dst);
-    else if (flat) hipLaunchKernelGGL(lin_act_grad_flat_kernel<false>, grid, dim3(256), 0, s, src, pre, act, n, dst);
-    else if (f16) hipLaunchKernelGGL(lin_act_grad_kernel<true>, grid, dim3(256), 0, s, src, src_ld, pre, act, rows, cols, dst, ld_dst);
-    else hipLaunchKernelGGL(lin_act_grad_kernel<false>, grid, dim3(256), 0, s, src, src_ld, pre, act, rows, cols, dst, ld_dst);
+int launch_linear_rows(LinRowItems items, bool f16, hipStream_t s) {
+    uint32_t blocks = 0;
+    for (int k = 0; k < items.n; ++k) {
+        LinRowItem& p = items.item[k];
+        const int64_t chunks = p.rows * ((p.ld_dst + 7) / 8);
+        p.blocks = (uint32_t)std::min<int64_t>((chunks + 255) / 256, 1 << 20);
+        blocks += p.blocks;
+    }
+    if (blocks == 0) return 0;
+    if (f16) hipLaunchKernelGGL(lin_rows_kernel<true>, dim3(blocks), dim3(256), 0, s, items);
+    else hipLaunchKernelGGL(lin_rows_kernel<false>, dim3(blocks), dim3(256), 0, s, items);
     return 0;
 }
 

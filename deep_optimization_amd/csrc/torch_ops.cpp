@@ -21,6 +21,7 @@
 // weight gradient), fp8_gemm_nt, fp8_linear, layer_norm_fwd, layer_norm_bwd, dropout_add_fwd, dropout_bwd,
 // linear_act_fwd, linear_act_bwd (the transformer blocks' operators).
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPFunctions.h>
@@ -30,6 +31,7 @@
 #include <cstdint>
 #include <optional>
 #include <tuple>
+#include <utility>
 
 #include "dopt.h"
 
@@ -709,6 +711,11 @@ int ln_params(const char* what, int64_t D, const std::optional<Tensor>& weight, 
     return dtype_code((weight ? *weight : *bias).scalar_type(), what);
 }
 
+// a contiguous tensor on like's device (not through the dispatcher: a call on one token is as long as its host work)
+Tensor fresh(at::IntArrayRef sizes, ScalarType dtype, const Tensor& like) {
+    return at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt);
+}
+
 void require_cuda(const std::optional<Tensor>& t) {
     if (t) require_cuda(*t);
 }
@@ -724,9 +731,9 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_fwd(const Tensor& x_in, const std:
     require_current(x_in);
     const Tensor x = x_in.contiguous();
     const auto w = contiguous(weight), b = contiguous(bias);
-    const auto opts = x.options();
-    Tensor y = at::empty(x.sizes(), opts.dtype(out_dtype));
-    Tensor mean = at::empty(x.sizes().slice(0, x.dim() - 1), opts.dtype(at::kFloat)), rstd = at::empty_like(mean);
+    Tensor y = fresh(x.sizes(), out_dtype, x);
+    const auto rows = x.sizes().slice(0, x.dim() - 1);
+    Tensor mean = fresh(rows, at::kFloat, x), rstd = fresh(rows, at::kFloat, x);
     check(dopt_layer_norm_forward(x.data_ptr(), dtype_code(x.scalar_type(), "layer_norm_fwd"), mean.numel(), D, ptr(w), ptr(b), code,
                                   (float)eps, y.data_ptr(), dtype_code(out_dtype, "layer_norm_fwd"), mean.data_ptr<float>(),
                                   rstd.data_ptr<float>(), stream_of(x)),
@@ -754,13 +761,12 @@ std::tuple<Tensor, std::optional<Tensor>, std::optional<Tensor>> layer_norm_bwd(
     require_current(x_in);
     const Tensor dy = dy_in.contiguous(), x = x_in.contiguous(), mean = mean_in.contiguous(), rstd = rstd_in.contiguous();
     const auto w = contiguous(weight), dr = contiguous(dresidual);
-    const auto f32 = x.options().dtype(at::kFloat);
-    Tensor dx = at::empty(x.sizes(), x.options());
+    Tensor dx = fresh(x.sizes(), x.scalar_type(), x);
     std::optional<Tensor> dw, db;
     Tensor ws;
-    if (weight_grad) dw = at::empty({D}, f32);
-    if (bias_grad) db = at::empty({D}, f32);
-    if (dw || db) ws = at::empty({std::max<int64_t>(dopt_layer_norm_workspace_floats(rows, D), 1)}, f32);
+    if (weight_grad) dw = fresh({D}, at::kFloat, x);
+    if (bias_grad) db = fresh({D}, at::kFloat, x);
+    if (dw || db) ws = fresh({std::max<int64_t>(dopt_layer_norm_workspace_floats(rows, D), 1)}, at::kFloat, x);
     check(dopt_layer_norm_backward(dy.data_ptr(), dtype_code(dy.scalar_type(), "layer_norm_bwd"), x.data_ptr(),
                                    dtype_code(x.scalar_type(), "layer_norm_bwd"), rows, D, mean.data_ptr<float>(), rstd.data_ptr<float>(),
                                    ptr(w), code, ptr(dr), dx.data_ptr(), ws.defined() ? ws.data_ptr<float>() : nullptr,
@@ -782,7 +788,7 @@ Tensor dropout_launch(const char* what, const Tensor& x_in, const std::optional<
     require_current(x_in);
     const Tensor x = x_in.contiguous();
     const auto r = contiguous(residual);
-    Tensor y = at::empty(x.sizes(), x.options().dtype(y_dtype));
+    Tensor y = fresh(x.sizes(), y_dtype, x);
     check(dopt_dropout(x.data_ptr(), dtype_code(x.scalar_type(), what), ptr(r), x.numel(), p, (uint64_t)seed, (uint64_t)offset,
                        (const int64_t*)ptr(step), y.data_ptr(), dtype_code(y_dtype, what), stream_of(x)),
           what);
@@ -809,41 +815,63 @@ int lin_act(c10::string_view act) {
 
 int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
 
-// dy act'(pre) of dy [rows, cols] at stride ld, in rows padded with zeros to a multiple of 8 or contiguous
-Tensor lin_act_grad_rows(const Tensor& dy, int64_t ld, const void* pre, int act, int64_t rows, int64_t cols, bool padded) {
-    const int64_t width = padded ? pad8(cols) : cols;
-    Tensor out = at::empty({rows, width}, dy.options());
-    check(dopt_linear_act_grad(dy.data_ptr(), ld, pre, act, dtype_code(dy.scalar_type(), "linear_act"), rows, cols, out.data_ptr(), width,
-                               stream_of(dy)),
-          "linear_act");
-    return out;
-}
-
+// An operand [rows, cols] as the products read it: contiguous rows `ld` apart, `whole` where they hold whole 16-byte chunks.
+// `copy`: it is going to be laid out again; `written`: it is an activation's gradient, which is written anyway.
+// (linear_lib._Rows)
 struct LinRows {
     Tensor t;
-    int64_t ld;
-    bool whole;  // the kernels read its rows in whole 16-byte chunks
+    int64_t rows, cols, ld;
+    bool whole, copy = false, written;
+
+    LinRows(const Tensor& from, int64_t rows, int64_t cols, bool written = false)
+        : t(from.dim() == 2 ? from : from.reshape({rows, cols})), rows(rows), cols(cols), written(written) {
+        if (t.stride(1) != 1 || t.stride(0) < cols || t.stride(0) >= (1 << 21)) t = t.contiguous();
+        ld = rows <= 1 ? cols : t.stride(0);
+        whole = written ? cols % 8 == 0
+                        : ld % 8 == 0 && ld >= pad8(cols) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
+                              (cols % 8 == 0 || (size_t)(t.storage_offset() + (rows - 1) * ld + pad8(cols)) * 2 <= t.storage().nbytes());
+    }
+    bool loose() const { return !(whole || copy); }
 };
 
-// t [..., cols] as a matrix with contiguous rows: linear_lib._rows
-LinRows lin_rows(const Tensor& t, int64_t rows, int64_t cols) {
-    Tensor t2 = t.dim() == 2 ? t : t.reshape({rows, cols});
-    if (t2.stride(1) != 1 || t2.stride(0) < cols || t2.stride(0) >= (1 << 21)) t2 = t2.contiguous();
-    const int64_t ld = rows <= 1 ? cols : t2.stride(0);
-    const bool whole = ld % 8 == 0 && ld >= pad8(cols) && reinterpret_cast<uintptr_t>(t2.data_ptr()) % 16 == 0;
-    if (whole && cols % 8 && (size_t)(t2.storage_offset() + (rows - 1) * ld + pad8(cols)) * 2 > t2.storage().nbytes())
-        return {lin_act_grad_rows(t2, ld, nullptr, DOPT_LIN_NONE, rows, cols, true), pad8(cols), true};  // the last row's last chunk is not all there
-    return {t2, ld, whole};
+// marks the loose ones of a product's operands for a copy into aligned rows, where that is estimated to be faster;
+// launched: others are laid out anyway, by the same launch (linear_lib._plan)
+void lin_plan(int product, int64_t M, int64_t N, int64_t K, LinRows& a, LinRows& b, bool launched) {
+    int64_t elements = 0;
+    bool copies = false;
+    for (const LinRows* r : {&a, &b})
+        if (r->loose() && !r->written) {
+            elements += r->rows * r->cols;
+            copies = true;
+        }
+    if (!(a.loose() || b.loose()) || !dopt_linear_copy_preferred(product, M, N, K, elements, copies && !launched)) return;
+    for (LinRows* r : {&a, &b})
+        if (r->loose()) r->copy = true;
 }
 
-// the operands as the product's kernels read them: linear_lib._operands
-void lin_operands_of(int product, int64_t M, int64_t N, int64_t K, LinRows& a, int64_t a_rows, int64_t a_cols, LinRows& b, int64_t b_rows,
-                     int64_t b_cols) {
-    const int copies = (a.whole ? 0 : 1) + (b.whole ? 0 : 1);
-    const int64_t elements = (a.whole ? 0 : a_rows * a_cols) + (b.whole ? 0 : b_rows * b_cols);
-    if (!copies || !dopt_linear_copy_preferred(product, M, N, K, elements, copies)) return;
-    if (!a.whole) a = {lin_act_grad_rows(a.t, a.ld, nullptr, DOPT_LIN_NONE, a_rows, a_cols, true), pad8(a_cols), true};
-    if (!b.whole) b = {lin_act_grad_rows(b.t, b.ld, nullptr, DOPT_LIN_NONE, b_rows, b_cols, true), pad8(b_cols), true};
+// one launch that lays out those operands that are marked; `pre`, `act`: of the one that is written (linear_lib._layout)
+void lin_layout(std::initializer_list<LinRows*> operands, const void* pre, int act, ScalarType dt, void* stream) {
+    dopt_linear_rows items[4];
+    Tensor sources[4];
+    int n = 0;
+    for (LinRows* r : operands) {
+        if (!r->copy && !r->written) continue;
+        r->copy |= r->cols % 8 != 0 && r->ld != r->cols;  // (unpadded rows are written as one)
+        const int64_t width = r->copy ? pad8(r->cols) : r->cols;
+        Tensor out = fresh({r->rows, width}, dt, r->t);
+        dopt_linear_rows& d = items[n++];
+        d = {r->t.data_ptr(), r->ld, r->written ? pre : nullptr, r->rows, r->cols, out.data_ptr(), width, r->written ? act : DOPT_LIN_NONE};
+        if (width == r->cols && width == r->ld) {  // a contiguous matrix as one row
+            d.rows = 1;
+            d.cols = d.ld_src = d.ld_dst = r->rows * r->cols;
+        }
+        // (a source that was made contiguous lives until the launch: the next result could take its memory)
+        sources[n - 1] = std::exchange(r->t, out);
+        r->whole = width % 8 == 0;
+        r->ld = width;
+        r->copy = false;
+    }
+    if (n) check(dopt_linear_layout(items, n, dtype_code(dt, "linear_act"), stream), "linear_act");
 }
 
 bool lin_type(ScalarType t) { return t == ScalarType::Half || t == ScalarType::BFloat16; }
@@ -888,16 +916,15 @@ std::tuple<Tensor, std::optional<Tensor>> linear_act_fwd(const Tensor& x, const 
     require_cuda(bias);
     require_cuda(residual);
     require_current(x);
-    LinRows a{x, K, true}, b{weight, K, true};
+    LinRows a(x, M, K), b(weight, N, K);
     if (M && N && K) {
-        a = lin_rows(x, M, K);
-        b = lin_rows(weight, N, K);
-        lin_operands_of(DOPT_LIN_FORWARD, M, N, K, a, M, K, b, N, K);
+        lin_plan(DOPT_LIN_FORWARD, M, N, K, a, b, false);
+        lin_layout({&a, &b}, nullptr, DOPT_LIN_NONE, dt, stream_of(x));
     }
     const auto bc = contiguous(bias), r = contiguous(residual);
-    Tensor y = at::empty(shape, x.options().dtype(r ? r->scalar_type() : dt));
+    Tensor y = fresh(shape, r ? r->scalar_type() : dt, x);
     std::optional<Tensor> pre;
-    if (save_pre) pre = at::empty(shape, x.options());
+    if (save_pre) pre = fresh(shape, dt, x);
     check(dopt_linear_forward(a.t.data_ptr(), a.ld, b.t.data_ptr(), b.ld, dtype_code(dt, what), M, N, K, ptr(bc),
                               bc ? dtype_code(bc->scalar_type(), what) : DOPT_F32, ptr(r), code, y.data_ptr(),
                               dtype_code(y.scalar_type(), what), pre ? pre->data_ptr() : nullptr, stream_of(x)),
@@ -929,51 +956,38 @@ std::tuple<std::optional<Tensor>, std::optional<Tensor>, std::optional<Tensor>> 
     const int tc = dtype_code(dt, what);
     void* const stream = stream_of(x);
     const bool empty = M == 0 || N == 0 || K == 0;
-    Tensor dz = dy;
-    if (code != DOPT_LIN_NONE && M && N) {
-        const Tensor d = dy.contiguous(), z = pre->contiguous();
-        // (padded where a product that reads dz is going to want it so)
-        const bool padded = N % 8 != 0 && K != 0 &&
-                            dopt_linear_copy_preferred(input_grad ? DOPT_LIN_INPUT_GRAD : DOPT_LIN_WEIGHT_GRAD, M, N, K, 0, 0);
-        dz = lin_act_grad_rows(d, N, z.data_ptr(), code, M, N, padded).narrow(1, 0, N);
+    // dz is dy, or written by the launch that lays out the operands whose rows the products do better to read aligned
+    const bool z = code != DOPT_LIN_NONE && M && N;
+    LinRows dz(dy, M, N, z), w(weight, N, K), xr(x, M, K);
+    if (!empty) {
+        if (input_grad) lin_plan(DOPT_LIN_INPUT_GRAD, M, N, K, dz, w, z);
+        if (weight_grad || bias_grad) lin_plan(DOPT_LIN_WEIGHT_GRAD, M, N, K, dz, xr, z || dz.copy || w.copy);
     }
-    LinRows dzr{dz, N, true};
-    if (!empty) dzr = lin_rows(dz, M, N);
+    const auto p = contiguous(pre);
+    lin_layout({&dz, &w, &xr}, ptr(p), code, dt, stream);
     std::optional<Tensor> dx, dw, db;
     if (input_grad) {
-        dx = at::empty(x.sizes(), x.options());
+        dx = fresh(x.sizes(), dt, x);
         const auto ip = contiguous(in_pre);
-        LinRows a = dzr, b{weight, K, true};
-        if (!empty) {
-            b = lin_rows(weight, N, K);
-            lin_operands_of(DOPT_LIN_INPUT_GRAD, M, N, K, a, M, N, b, N, K);
-        }
-        check(dopt_linear_input_grad(a.t.data_ptr(), a.ld, b.t.data_ptr(), b.ld, tc, M, N, K, ptr(ip), in_code, dx->data_ptr(), stream), what);
+        check(dopt_linear_input_grad(dz.t.data_ptr(), dz.ld, w.t.data_ptr(), w.ld, tc, M, N, K, ptr(ip), in_code, dx->data_ptr(), stream), what);
     }
     if (weight_grad || bias_grad) {
-        const auto opts = x.options().dtype(grad_dtype);
         if (N == 0 || K == 0) {
-            dw = at::empty({N, K}, opts);
-            db = dz.reshape({M, N}).to(at::kFloat).sum(0).to(grad_dtype);
+            dw = fresh({N, K}, grad_dtype, x);
+            db = dz.t.reshape({M, N}).to(at::kFloat).sum(0).to(grad_dtype);
         } else {
-            LinRows a = dzr, b{x, K, true};
-            if (!empty) {
-                b = lin_rows(x, M, K);
-                lin_operands_of(DOPT_LIN_WEIGHT_GRAD, M, N, K, a, M, N, b, M, K);
-            }
             // the kernels that split the sum write whole chunks of a row
             int64_t K8 = pad8(K);
-            if (K8 != K && (!a.whole || !b.whole || dopt_linear_tile(DOPT_LIN_WEIGHT_GRAD, M, N, K8, 0) != 100)) K8 = K;
+            if (K8 != K && !(dz.whole && xr.whole && dopt_linear_tile(DOPT_LIN_WEIGHT_GRAD, M, N, K8, 0) == 100)) K8 = K;
             const bool f32 = grad_dtype == ScalarType::Float;
             const int64_t floats = dopt_linear_weight_grad_workspace_floats(M, N, K8);
             Tensor ws;
-            if (floats > 0) ws = at::empty({floats}, x.options().dtype(at::kFloat));
-            Tensor d = at::empty({N, K8}, opts);
-            if (bias_grad) db = at::empty({N}, opts);
+            if (floats > 0) ws = fresh({floats}, ScalarType::Float, x);
+            Tensor d = fresh({N, K8}, grad_dtype, x);
+            if (bias_grad) db = fresh({N}, grad_dtype, x);
             void* const dbp = db ? db->data_ptr() : nullptr;
-            // (a pointer that is not null where nothing is written to it)
-            check(dopt_linear_weight_grad(a.t.data_ptr(), a.ld, b.t.data_ptr(), b.ld, tc, M, N, K8,
-                                          floats > 0 ? ws.data_ptr<float>() : (float*)d.data_ptr(), f32 ? (float*)d.data_ptr() : nullptr,
+            check(dopt_linear_weight_grad(dz.t.data_ptr(), dz.ld, xr.t.data_ptr(), xr.ld, tc, M, N, K8,
+                                          floats > 0 ? ws.data_ptr<float>() : nullptr, f32 ? (float*)d.data_ptr() : nullptr,
                                           f32 ? nullptr : d.data_ptr(), f32 ? (float*)dbp : nullptr, f32 ? nullptr : dbp, stream),
                   what);
             dw = K8 == K ? d : d.narrow(1, 0, K).contiguous();

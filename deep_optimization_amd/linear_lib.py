@@ -47,39 +47,55 @@ def _pad8(n: int) -> int:
     return (n + 7) // 8 * 8
 
 
-def _rows(t: Tensor, cols: int):
-    """t [..., cols] as (matrix with contiguous rows, row stride, whether the kernels read its rows in whole 16-byte chunks)."""
-    t2 = t.reshape(-1, cols) if t.dim() != 2 else t
-    if t2.stride(1) != 1 or not cols <= t2.stride(0) < 1 << 21:
-        t2 = t2.contiguous()
-    rows = t2.shape[0]
-    ld = cols if rows <= 1 else int(t2.stride(0))
-    whole = ld % 8 == 0 and ld >= _pad8(cols) and t2.data_ptr() % 16 == 0
-    if whole and cols % 8 and (t2.storage_offset() + (rows - 1) * ld + _pad8(cols)) * 2 > t2.untyped_storage().nbytes():
-        return _act_grad_rows(t2, ld, None, "none", True), _pad8(cols), True  # the last row's last chunk is not all there
-    return t2, ld, whole
+class _Rows:
+    """An operand [rows, cols] as the products read it: contiguous rows ``ld`` apart, ``whole`` where they hold whole 16-byte
+    chunks. ``copy``: it is going to be laid out again; ``written``: it is an activation's gradient, which is written anyway."""
+
+    def __init__(self, t: Tensor, rows: int, cols: int, written: bool = False):
+        t2 = t.reshape(rows, cols) if t.dim() != 2 else t
+        if t2.stride(1) != 1 or not cols <= t2.stride(0) < 1 << 21:
+            t2 = t2.contiguous()
+        self.t, self.rows, self.cols, self.copy, self.written = t2, rows, cols, False, written
+        self.ld = cols if rows <= 1 else int(t2.stride(0))
+        if written:
+            self.whole = cols % 8 == 0
+            return
+        # (the last row's last chunk must be there too)
+        self.whole = self.ld % 8 == 0 and self.ld >= _pad8(cols) and t2.data_ptr() % 16 == 0 and (
+            cols % 8 == 0 or (t2.storage_offset() + (rows - 1) * self.ld + _pad8(cols)) * 2 <= t2.untyped_storage().nbytes())
+
+    @property
+    def loose(self) -> bool:
+        return not (self.whole or self.copy)
 
 
-def _operands(product: int, M: int, N: int, K: int, *operands):
-    """(tensor, columns) pairs as the product's kernels read them: [(tensor, row stride)]. Operands whose rows lie at any
-    element stay where they are, or are copied into aligned rows where that is estimated to be faster."""
-    rows = [_rows(t, cols) for t, cols in operands]
-    loose = [i for i, r in enumerate(rows) if not r[2]]
-    if loose and _lib.lib().dopt_linear_copy_preferred(product, M, N, K, sum(rows[i][0].numel() for i in loose), len(loose)):
-        for i in loose:
-            cols = operands[i][1]
-            rows[i] = (_act_grad_rows(rows[i][0], rows[i][1], None, "none", True), _pad8(cols), True)
-    return [(t, ld) for t, ld, _ in rows]
+def _plan(product: int, M: int, N: int, K: int, a: _Rows, b: _Rows, launched: bool) -> None:
+    """Marks the loose ones of a product's operands for a copy into aligned rows, where that is estimated to be faster;
+    ``launched``: others are laid out anyway, by the same launch."""
+    loose = [r for r in (a, b) if r.loose]
+    copies = [r for r in loose if not r.written]
+    if loose and _lib.lib().dopt_linear_copy_preferred(product, M, N, K, sum(r.rows * r.cols for r in copies), int(bool(copies) and not launched)):
+        for r in loose:
+            r.copy = True
 
 
-def _act_grad_rows(dy: Tensor, ld: int, pre: Optional[Tensor], act: str, padded: bool) -> Tensor:
-    """dy act'(pre) of dy [rows, cols], in rows padded with zeros to a multiple of 8 or contiguous."""
-    rows, cols = dy.shape
-    out = torch.empty((rows, _pad8(cols) if padded else cols), dtype=dy.dtype, device=dy.device)
-    rc = _lib.lib().dopt_linear_act_grad(dy.data_ptr(), ld, None if pre is None else pre.data_ptr(), _act_code(act),
-                                         _DTYPE_CODE[dy.dtype], rows, cols, out.data_ptr(), out.shape[1], _stream(dy))
-    _lib.check(rc, "linear_act")
-    return out
+def _layout(items, dtype: torch.dtype, stream) -> None:
+    """One launch that lays out [(operand, pre, act)]; each then holds its new rows. With an activation the rows become dy act'(pre),
+    padded only where a copy is marked."""
+    if not items:
+        return
+    rows = (_lib.LinearRows * len(items))()
+    for d, (r, pre, act) in zip(rows, items):
+        r.copy |= r.cols % 8 != 0 and r.ld != r.cols  # (unpadded rows are written as one)
+        width = _pad8(r.cols) if r.copy else r.cols
+        out = torch.empty((r.rows, width), dtype=dtype, device=r.t.device)
+        n, cols, src, dst = r.rows, r.cols, r.ld, width
+        if width == cols == r.ld:  # a contiguous matrix as one row
+            n, cols, src, dst = 1, n * cols, n * cols, n * cols
+        d.src, d.ld_src, d.pre, d.rows, d.cols, d.dst, d.ld_dst, d.act = (r.t.data_ptr(), src, None if pre is None else pre.data_ptr(), n,
+                                                                          cols, out.data_ptr(), dst, act)
+        r.t, r.ld, r.whole, r.copy = out, width, width % 8 == 0, False
+    _lib.check(_lib.lib().dopt_linear_layout(rows, len(items), _DTYPE_CODE[dtype], stream), "linear_act")
 
 
 def _check_operands(what: str, x: Tensor, weight: Tensor):
@@ -108,13 +124,16 @@ def _linear_act_fwd(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual:
     if residual is not None:
         _check_like(what, "residual", residual, shape, (x.dtype, torch.float32))
     _require_cuda(x, weight, bias, residual)
-    (a, lda), (b, ldb) = _operands(0, M, N, K, (x, K), (weight, K)) if M and N and K else ((x, K), (weight, K))
+    a, b = _Rows(x, M, K), _Rows(weight, N, K)
+    if M and N and K:
+        _plan(0, M, N, K, a, b, False)
+        _layout([(r, None, 0) for r in (a, b) if r.copy], x.dtype, _stream(x))
     bias = None if bias is None else bias.contiguous()
     residual = None if residual is None else residual.contiguous()
     y = torch.empty(shape, dtype=x.dtype if residual is None else residual.dtype, device=x.device)
     pre = torch.empty(shape, dtype=x.dtype, device=x.device) if save_pre else None
     rc = _lib.lib().dopt_linear_forward(
-        a.data_ptr(), lda, b.data_ptr(), ldb, _DTYPE_CODE[x.dtype], M, N, K, None if bias is None else bias.data_ptr(),
+        a.t.data_ptr(), a.ld, b.t.data_ptr(), b.ld, _DTYPE_CODE[x.dtype], M, N, K, None if bias is None else bias.data_ptr(),
         _lib.F32 if bias is None else _DTYPE_CODE[bias.dtype], None if residual is None else residual.data_ptr(), code,
         y.data_ptr(), _DTYPE_CODE[y.dtype], None if pre is None else pre.data_ptr(), _stream(x))
     _lib.check(rc, what)
@@ -150,36 +169,38 @@ def _linear_act_bwd(dy: Tensor, x: Tensor, weight: Tensor, pre: Optional[Tensor]
     _require_cuda(dy, x, weight, pre, in_pre)
     L, dt, stream = _lib.lib(), _DTYPE_CODE[x.dtype], _stream(x)
     empty = M == 0 or N == 0 or K == 0
-    dz, cols = dy, N
-    if code and M and N:
-        # (padded where a product that reads dz is going to want it so)
-        want = (0 if K == 0 else 1 if input_grad else 2)
-        padded = N % 8 != 0 and want != 0 and bool(L.dopt_linear_copy_preferred(want, M, N, K, 0, 0))
-        dz = _act_grad_rows(dy.contiguous().view(M, N), N, pre.contiguous(), act, padded)[:, :N]
+    # dz is dy, or written by the launch that lays out the operands whose rows the products do better to read aligned
+    z = code != 0 and M > 0 and N > 0
+    dz, w, xr = _Rows(dy, M, N, z), _Rows(weight, N, K), _Rows(x, M, K)
+    if not empty:
+        if input_grad:
+            _plan(1, M, N, K, dz, w, z)
+        if weight_grad or bias_grad:
+            _plan(2, M, N, K, dz, xr, z or dz.copy or w.copy)
+    pre = None if pre is None else pre.contiguous()
+    _layout([(r, p, a) for r, p, a in ((dz, pre, code), (w, None, 0), (xr, None, 0)) if r.copy or r.written], x.dtype, stream)
     dx = dw = db = None
     if input_grad:
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         in_pre = None if in_pre is None else in_pre.contiguous()
-        (a, lda), (b, ldb) = _operands(1, M, N, K, (dz, N), (weight, K)) if not empty else ((dz, N), (weight, K))
-        rc = L.dopt_linear_input_grad(a.data_ptr(), lda, b.data_ptr(), ldb, dt, M, N, K, None if in_pre is None else in_pre.data_ptr(),
+        rc = L.dopt_linear_input_grad(dz.t.data_ptr(), dz.ld, w.t.data_ptr(), w.ld, dt, M, N, K, None if in_pre is None else in_pre.data_ptr(),
                                       in_code, dx.data_ptr(), stream)
         _lib.check(rc, what)
     if weight_grad or bias_grad:
         if N == 0 or K == 0:
             dw = torch.empty((N, K), dtype=grad_dtype, device=x.device)
-            db = dz.reshape(M, N).float().sum(0).to(grad_dtype)
+            db = dz.t.reshape(M, N).float().sum(0).to(grad_dtype)
         else:
-            (a, lda), (b, ldb) = _operands(2, M, N, K, (dz, N), (x, K)) if not empty else ((dz, N), (x, K))
             # the kernels that split the sum write whole chunks of a row
             K8 = _pad8(K)
-            if K8 != K and (lda % 8 or ldb % 8 or ldb < K8 or a.data_ptr() % 16 or b.data_ptr() % 16 or L.dopt_linear_tile(2, M, N, K8, 0) != 100):
+            if K8 != K and not (dz.whole and xr.whole and L.dopt_linear_tile(2, M, N, K8, 0) == 100):
                 K8 = K
             ws = torch.empty(max(int(L.dopt_linear_weight_grad_workspace_floats(M, N, K8)), 4), dtype=torch.float32, device=x.device)
             dw = torch.empty((N, K8), dtype=grad_dtype, device=x.device)
             db = torch.empty(N, dtype=grad_dtype, device=x.device) if bias_grad else None
             f32 = grad_dtype == torch.float32
             dbp = None if db is None else db.data_ptr()
-            rc = L.dopt_linear_weight_grad(a.data_ptr(), lda, b.data_ptr(), ldb, dt, M, N, K8, ws.data_ptr(), dw.data_ptr() if f32 else None,
+            rc = L.dopt_linear_weight_grad(dz.t.data_ptr(), dz.ld, xr.t.data_ptr(), xr.ld, dt, M, N, K8, ws.data_ptr(), dw.data_ptr() if f32 else None,
                                            None if f32 else dw.data_ptr(), dbp if f32 else None, None if f32 else dbp, stream)
             _lib.check(rc, what)
             if K8 != K:

@@ -487,10 +487,19 @@ int dopt_linear_forward(const void* x, int64_t ldx, const void* weight, int64_t 
  * dz weight, in_pre is not read. The same alignment rules (dz's rows hold N elements, weight's K). */
 int dopt_linear_input_grad(const void* dz, int64_t ldz, const void* weight, int64_t ldw, int dtype, int64_t M, int64_t N,
                            int64_t K, const void* in_pre, int in_act, void* dx, void* stream);
-/* dz[r][c] = dy[r][c] * act'(pre[r][c]) for c < cols, 0 for the columns up to ld_dz; pre [rows, cols]. dz 16-byte aligned
- * with ld_dz a multiple of 8, or contiguous as dy is. With DOPT_LIN_NONE a copy into padded rows. */
-int dopt_linear_act_grad(const void* dy, int64_t ld_dy, const void* pre, int act, int dtype, int64_t rows, int64_t cols,
-                         void* dz, int64_t ld_dz, void* stream);
+/* Rows laid out for the products, up to 4 matrices in one launch: dst[r][c] = src[r][c] * act'(pre[r][c]) for c < cols, 0 for the
+ * columns up to ld_dst; with DOPT_LIN_NONE a copy (pre is not read). src's rows ld_src elements apart, at any element; pre
+ * [rows, cols] contiguous; dst 16-byte aligned with ld_dst a multiple of 8, or one row (a contiguous matrix as a whole). */
+typedef struct {
+    const void* src;
+    int64_t ld_src;
+    const void* pre;
+    int64_t rows, cols;
+    void* dst;
+    int64_t ld_dst;
+    int act;
+} dopt_linear_rows;
+int dopt_linear_layout(const dopt_linear_rows* rows, int n, int dtype, void* stream);
 /* dw = dz^T x (fp32 to dw_f32 or the operands' type to dw_16, [N, K]) and the sums of dz over its rows ([N], fp32 to db or
  * the operands' type to db_16; NULL: none): dz [M, ldz], x [M, ldx], the same alignment rules. workspace:
  * dopt_linear_weight_grad_workspace_floats floats (0: it may be NULL). Sums in an order that the sizes fix. */
@@ -500,9 +509,9 @@ int dopt_linear_weight_grad(const void* dz, int64_t ldz, const void* x, int64_t 
 /* Which tile a product gets (an index of the launcher's table; -1: the kernel of at most 16 rows; 100: dopt_dw_gemm_any's
  * kernels; -2: bad arguments); any_rows: an operand's rows lie at any element. */
 int dopt_linear_tile(int product, int64_t M, int64_t N, int64_t K, int any_rows);
-/* Whether copying operands that lie at any element into aligned rows (`copies` of them, of `elements` elements together)
- * is estimated to be faster than reading them as they lie. */
-int dopt_linear_copy_preferred(int product, int64_t M, int64_t N, int64_t K, int64_t elements, int copies);
+/* Whether a product is estimated to run faster on aligned rows than on operands that lie at any element, where laying those out
+ * again takes `launches` more launches and `elements` elements of copying. */
+int dopt_linear_copy_preferred(int product, int64_t M, int64_t N, int64_t K, int64_t elements, int launches);
 
 /*
  * HIP graph tools for capturing a whole training step (forward, backward, optimizer step) as

@@ -74,9 +74,15 @@ def test_c_entries_refuse_before_any_launch():
     wg = lambda **k: L.dopt_linear_weight_grad(*{**dict(dz=AT, ldz=8, x=AT, ldx=8, dt=BF, M=2, N=8, K=8, ws=AT, dw=AT, dw16=None, db=None, db16=None, s=None), **k}.values())  # noqa: E731
     for k in (dict(dz=None), dict(x=None), dict(ldz=7), dict(ldx=7), dict(dt=FP), dict(M=-1), dict(N=0), dict(dw=None), dict(dw16=AT), dict(db=AT, db16=AT)):
         _refused(wg(**k))
-    ag = lambda **k: L.dopt_linear_act_grad(*{**dict(dy=AT, ld=8, pre=AT, act=2, dt=BF, rows=2, cols=8, dz=AT, ldz=8, s=None), **k}.values())  # noqa: E731
-    for k in (dict(dy=None), dict(dz=None), dict(pre=None), dict(ld=7), dict(ldz=7), dict(act=7), dict(dt=FP), dict(rows=-1), dict(act=0, pre=None, ldz=9)):
-        _refused(ag(**k))
+    def lay(n=1, dt=BF, **k):
+        r = _lib.LinearRows(*{**dict(src=AT, ld=8, pre=AT, rows=2, cols=8, dst=AT, ldd=8, act=2), **k}.values())
+        return L.dopt_linear_layout(ctypes.byref(r), n, dt, None)
+
+    for k in (dict(src=None), dict(dst=None), dict(pre=None), dict(ld=7), dict(ldd=7), dict(ldd=9), dict(act=7), dict(act=-1), dict(dt=FP),
+              dict(rows=-1), dict(cols=-1), dict(n=5), dict(n=-1), dict(dst=ODD), dict(rows=1 << 40, ld=32, ldd=32)):
+        _refused(lay(**k))
+    _refused(L.dopt_linear_layout(None, 1, BF, None))
+    assert lay(n=0) == 0 and lay(rows=0, src=None, dst=None) == 0
     # nothing to do is no error
     assert ln(rows=0, x=None, y=None, mean=None, rstd=None) == 0 and dr(n=0, x=None, y=None) == 0 and fw(M=0, y=None) == 0 and dg(M=0, dx=None) == 0
 
