@@ -69,6 +69,7 @@ EXPORTS = (
     "dopt_dropout",
     "dopt_linear_forward",
     "dopt_linear_input_grad",
+    "dopt_linear_layout_workspace_floats",
     "dopt_linear_layout",
     "dopt_linear_weight_grad_workspace_floats",
     "dopt_linear_weight_grad",
@@ -82,7 +83,8 @@ _lib = None
 class LinearRows(ctypes.Structure):
     """dopt_linear_rows: a matrix that dopt_linear_layout lays out."""
     _fields_ = [("src", ctypes.c_void_p), ("ld_src", ctypes.c_int64), ("pre", ctypes.c_void_p), ("rows", ctypes.c_int64),
-                ("cols", ctypes.c_int64), ("dst", ctypes.c_void_p), ("ld_dst", ctypes.c_int64), ("act", ctypes.c_int)]
+                ("cols", ctypes.c_int64), ("dst", ctypes.c_void_p), ("ld_dst", ctypes.c_int64), ("act", ctypes.c_int),
+                ("sum_dtype", ctypes.c_int), ("sum", ctypes.c_void_p), ("workspace", ctypes.c_void_p)]
 
 
 class DoptError(RuntimeError):
@@ -217,6 +219,8 @@ def lib() -> ctypes.CDLL:
         L.dopt_linear_forward.restype = i32
         L.dopt_linear_input_grad.argtypes = [vp, i64, vp, i64, i32, i64, i64, i64, vp, i32, vp, vp]
         L.dopt_linear_input_grad.restype = i32
+        L.dopt_linear_layout_workspace_floats.argtypes = [i64, i64]
+        L.dopt_linear_layout_workspace_floats.restype = i64
         L.dopt_linear_layout.argtypes = [ctypes.POINTER(LinearRows), i32, i32, vp]
         L.dopt_linear_layout.restype = i32
         L.dopt_linear_weight_grad_workspace_floats.argtypes = [i64, i64, i64]

@@ -42,7 +42,9 @@ int launch_dropout(const void* x, int x_dt, const void* residual, uint64_t n, ui
 bool lin_shape_fits(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb);
 int launch_linear(const LinArgs& p, int kind, bool f16, hipStream_t s);
 int linear_tile(int kind, int64_t M, int64_t N, int64_t K, bool reg, bool big, float* us);
+int linear_sum_groups(int64_t rows, int64_t cols);
 int launch_linear_rows(LinRowItems items, bool f16, hipStream_t s);
+int launch_linear_sum(const float* partial, int groups, int64_t cols, void* sum, int dt, hipStream_t s);
 }  // namespace dopt
 
 namespace {
@@ -1279,25 +1281,57 @@ int dopt_linear_input_grad(const void* dz, int64_t ldz, const void* weight, int6
     return hip_status("linear_input_grad launch");
 }
 
+int64_t dopt_linear_layout_workspace_floats(int64_t rows, int64_t cols) {
+    if (rows <= 0 || cols <= 0 || cols >= ((int64_t)1 << 26)) return 0;
+    const int groups = dopt::linear_sum_groups(rows, cols);
+    return groups == 1 ? 0 : groups * cols;
+}
+
 int dopt_linear_layout(const dopt_linear_rows* rows, int n, int dtype, void* stream) {
     if (n < 0 || n > dopt::LIN_ROW_ITEMS || (n > 0 && !rows)) return fail(DOPT_EINVAL, "linear: 0 to %d matrices, got %d", dopt::LIN_ROW_ITEMS, n);
     dopt::LinRowItems items{};
+    bool sums = false;
     for (int k = 0; k < n; ++k) {
         const dopt_linear_rows& r = rows[k];
         if (int rc = check_linear(dtype, 0, 0, 0, 0, 0, r.act)) return rc;
         if (r.rows < 0 || r.cols < 0)
             return fail(DOPT_EINVAL, "linear: sizes must be >= 0 (got %lld, %lld)", (long long)r.rows, (long long)r.cols);
+        if (r.sum) {
+            if (r.sum_dtype != dtype && r.sum_dtype != DOPT_F32)
+                return fail(DOPT_EINVAL, "linear: the sums have the operands' type or DOPT_F32, got %d", r.sum_dtype);
+            if (r.cols >= ((int64_t)1 << 26)) return fail(DOPT_EUNSUPPORTED, "linear: sums of fewer than 2^26 columns");
+            sums |= r.cols > 0;
+        }
         if (r.rows == 0 || r.cols == 0) continue;
-        if (!r.src || !r.dst || (r.act != DOPT_LIN_NONE && !r.pre)) return fail(DOPT_EINVAL, "linear: null src/pre/dst pointer");
-        if (r.ld_src < r.cols || r.ld_dst < r.cols || !aligned16(r.dst) || (r.rows > 1 && r.ld_dst % 8 != 0))
-            return fail(DOPT_EINVAL, "linear: src's rows must lie at least cols apart, dst's in 16-byte aligned rows of at least cols elements");
+        if (!r.src || !r.dst || (r.act != DOPT_LIN_NONE && !r.pre) || (r.sum && !r.workspace && dopt_linear_layout_workspace_floats(r.rows, r.cols) > 0))
+            return fail(DOPT_EINVAL, "linear: null src/pre/dst/workspace pointer");
+        if (r.ld_src < r.cols || r.ld_dst < r.cols || ((uintptr_t)r.src & 1u) || ((uintptr_t)r.pre & 1u) || ((uintptr_t)r.dst & 1u))
+            return fail(DOPT_EINVAL, "linear: src's and dst's rows must lie at whole elements, at least cols apart");
         if (r.ld_src >= ((int64_t)1 << 44) / r.rows || r.ld_dst >= ((int64_t)1 << 44) / r.rows)
             return fail(DOPT_EUNSUPPORTED, "linear: matrices below 2^44 elements");
-        items.item[items.n++] = {(const uint16_t*)r.src, r.ld_src, (const uint16_t*)r.pre, r.rows, r.cols, (uint16_t*)r.dst, r.ld_dst, r.act, 0};
+        dopt::LinRowItem item{};
+        item.src = (const uint16_t*)r.src;
+        item.ld_src = r.ld_src;
+        item.pre = (const uint16_t*)r.pre;
+        item.rows = r.rows;
+        item.cols = r.cols;
+        item.dst = (uint16_t*)r.dst;
+        item.ld_dst = r.ld_dst;
+        item.act = r.act;
+        item.sum = r.sum;
+        item.sum_dt = r.sum_dtype;
+        item.partial = r.workspace;
+        items.item[items.n++] = item;
     }
-    if (items.n == 0) return ok();
+    if (items.n == 0 && !sums) return ok();
     (void)hipGetLastError();
     dopt::launch_linear_rows(items, dtype == DOPT_F16, (hipStream_t)stream);
+    for (int k = 0; k < n; ++k) {
+        const dopt_linear_rows& r = rows[k];
+        const int groups = r.rows > 0 ? dopt::linear_sum_groups(r.rows, r.cols) : 0;
+        if (r.sum && r.cols > 0 && groups != 1)  // (no rows: zeros)
+            dopt::launch_linear_sum(r.workspace, groups, r.cols, r.sum, r.sum_dtype, (hipStream_t)stream);
+    }
     return hip_status("linear_layout launch");
 }
 

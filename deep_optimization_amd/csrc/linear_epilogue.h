@@ -28,8 +28,8 @@ struct LinArgs {
 };
 
 // Rows laid out for the products: dst[r][c] = src[r][c] act'(pre[r][c]) for c < cols, 0 for the columns up to ld_dst (act
-// LIN_NONE: a copy). src rows ld_src elements apart, pre [rows][cols] contiguous, dst 16-byte aligned with ld_dst a multiple
-// of 8 (or one row).
+// LIN_NONE: a copy), and with `sum` the columns' sums of it before its rounding; partial: [groups][cols] where those are not 1. src rows ld_src and dst rows
+// ld_dst elements apart, pre [rows][cols] contiguous.
 struct LinRowItem {
     const uint16_t* src;
     int64_t ld_src;
@@ -38,7 +38,12 @@ struct LinRowItem {
     uint16_t* dst;
     int64_t ld_dst;
     int act;
-    uint32_t blocks;  // set by the launcher
+    void* sum;  // [cols] of sum_dt
+    int sum_dt;
+    float* partial;
+    // set by the launcher
+    int lg;
+    uint32_t groups, blocks;
 };
 constexpr int LIN_ROW_ITEMS = 4;
 struct LinRowItems {

@@ -127,24 +127,29 @@ __device__ __forceinline__ void lin_load_row8(const uint16_t* p, int64_t i, int6
 }
 
 // Every item's rows (linear_epilogue.h), 8 columns a lane; an item's blocks follow the ones before it. Memory-bound: 2 bytes
-// read (4 with an activation) and 2 written an element; 25216 x 3072 with GELU 114 us, 4.1 TB/s. The backward of a layer
-// whose sizes are no multiples of 8 hands up to three operands to one launch: 2001 rows of 333 -> 1001 9.0 us, in three
+// read (4 with an activation) and 2 written an element; 25216 x 3072 with GELU and sums 103 us, 4.5 TB/s. The backward of a
+// layer whose sizes are no multiples of 8 hands up to three operands to one launch: 2001 rows of 333 -> 1001 9.8 us, in three
 // launches 15.0.
+//
+// An item with sums walks its rows in strips of 2^lg chunks of columns: a block takes every groups-th (1024 >> lg) rows of one,
+// its threads add their 8 columns in fp32 over the rows they take, and the threads of equal columns meet over the lanes of
+// a wave and then over the waves in LDS, in an order that the sizes fix. The sums are of the fp32 values: the bias gradient is then
+// as exact as its own rounding, where the sum of the rounded dz that the weight gradient's product makes on its way is off by up
+// to half a rounding more.
+constexpr int ROWS_THREADS = 1024;
 template <bool F16>
-__global__ __launch_bounds__(256) void lin_rows_kernel(LinRowItems items) {
+__global__ __launch_bounds__(ROWS_THREADS, 8) void lin_rows_kernel(LinRowItems items) {
     constexpr int DT = F16 ? DT_F16 : DT_BF16;
+    __shared__ __attribute__((aligned(16))) float meet[ROWS_THREADS / 64][32 * 8];
     uint32_t block = blockIdx.x;
     int k = 0;
     while (k + 1 < items.n && block >= items.item[k].blocks) block -= items.item[k++].blocks;
     const LinRowItem p = items.item[k];
-    const uint64_t cpr = (uint64_t)(p.ld_dst + 7) / 8, total = (uint64_t)p.rows * cpr;
+    const uint64_t cpr = (uint64_t)(p.ld_dst + 7) / 8;
     const int64_t src_total = (p.rows - 1) * p.ld_src + p.cols;
-    for (uint64_t q = (uint64_t)block * 256 + threadIdx.x; q < total; q += (uint64_t)p.blocks * 256) {
-        // (one row: contiguous matrices; 32-bit division where it does)
-        const int64_t r = p.rows == 1 ? 0 : total >> 32 ? (int64_t)(q / cpr) : (int64_t)((uint32_t)q / (uint32_t)cpr);
-        const int64_t c = ((int64_t)q - r * (int64_t)cpr) * 8;
+    // the 8 columns from c on of row r: stored, and left in v in fp32
+    const auto chunk = [&](int64_t r, int64_t c, float* v) __attribute__((always_inline)) {
         const int have = (int)max((int64_t)0, min((int64_t)8, p.cols - c));
-        float v[8];
         lin_load_row8<DT>(p.src, r * p.ld_src + c, src_total, have, v);
         if (p.act != LIN_NONE) {
             float z[8];
@@ -152,6 +157,65 @@ __global__ __launch_bounds__(256) void lin_rows_kernel(LinRowItems items) {
             lin_act_grad8(p.act, z, v);
         }
         lin_store8<DT>(p.dst, r * p.ld_dst + c, (int)min((int64_t)8, p.ld_dst - c), v);
+    };
+    if (p.sum) {
+        const int across = 1 << p.lg, x = threadIdx.x & (across - 1), y = threadIdx.x >> p.lg, tall = ROWS_THREADS >> p.lg;
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+        const uint32_t strip = block / p.groups, group = block % p.groups;
+        const int64_t c = ((int64_t)strip * across + x) * 8;
+        float sum[8] = {};
+        if (c < p.ld_dst) {
+#pragma unroll 1
+            for (int64_t r = (int64_t)group * tall + y; r < p.rows; r += (int64_t)p.groups * tall) {
+                float v[8];
+                chunk(r, c, v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum[e] += v[e];
+            }
+        }
+        for (int d = across; d < 64; d <<= 1)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[e] += __shfl_xor(sum[e], d);
+        if (lane < across) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) meet[wave][lane * 8 + e] = sum[e];
+        }
+        __syncthreads();
+        const int64_t at = (int64_t)strip * across * 8 + threadIdx.x;
+        if ((int)threadIdx.x < across * 8 && at < p.cols) {
+            float s = meet[0][threadIdx.x];
+#pragma unroll
+            for (int q = 1; q < ROWS_THREADS / 64; ++q) s += meet[q][threadIdx.x];
+            if (p.groups == 1) store1(p.sum, p.sum_dt, at, s);
+            else p.partial[group * p.cols + at] = s;
+        }
+        return;
+    }
+    const uint64_t total = (uint64_t)p.rows * cpr;
+    for (uint64_t q = (uint64_t)block * ROWS_THREADS + threadIdx.x; q < total; q += (uint64_t)p.blocks * ROWS_THREADS) {
+        // (one row: contiguous matrices; 32-bit division where it does)
+        const int64_t r = p.rows == 1 ? 0 : total >> 32 ? (int64_t)(q / cpr) : (int64_t)((uint32_t)q / (uint32_t)cpr);
+        float v[8];
+        chunk(r, ((int64_t)q - r * (int64_t)cpr) * 8, v);
+    }
+}
+
+// The sums of the partial rows: a workgroup takes 64 columns, its 16 waves every 16th row; the waves' sums are added in order.
+__global__ __launch_bounds__(1024) void lin_sum_kernel(const float* partial, int groups, int64_t cols, void* sum, int dt) {
+    __shared__ float part[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+    float s = 0.0f;
+    if (c < cols) {
+#pragma unroll 8
+        for (int g = wave; g < groups; g += 16) s += partial[g * cols + c];
+    }
+    part[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && c < cols) {
+#pragma unroll
+        for (int k = 1; k < 16; ++k) s += part[k][lane];
+        store1(sum, dt, c, s);
     }
 }
 
@@ -185,17 +249,42 @@ int linear_tile(int kind, int64_t M, int64_t N, int64_t K, bool reg, bool big, f
     return plan(kind, M, N, K, n_cu, reg, big && N % 8 == 0 && K >= LIN_BK, 1.0f, us);
 }
 
+namespace {
+// Few rows take strips of 4 chunks, one block each, which writes the result: the whole call is 6.8 us at 64 x 1024 and 8.4 at 512 x
+// 3072, where wide strips and lin_sum_kernel's launch take 9.9 and 10.4. Past that a block reads its strip for too long
+// (2001 x 1001: 21.0 us against 10.3).
+constexpr int64_t SUM_ROWS = 512;
+}  // namespace
+
+// partial rows of the sums of a [rows, cols] item: one, or as many as make 512 blocks (two a CU) of 32 rows x 32 chunks at a time
+int linear_sum_groups(int64_t rows, int64_t cols) {
+    if (rows <= SUM_ROWS) return 1;
+    const int64_t strips = (cols + 255) / 256;
+    return (int)std::max<int64_t>(1, std::min<int64_t>((rows + 31) / 32, 512 / std::max<int64_t>(strips, 1)));
+}
+
 int launch_linear_rows(LinRowItems items, bool f16, hipStream_t s) {
     uint32_t blocks = 0;
     for (int k = 0; k < items.n; ++k) {
         LinRowItem& p = items.item[k];
-        const int64_t chunks = p.rows * ((p.ld_dst + 7) / 8);
-        p.blocks = (uint32_t)std::min<int64_t>((chunks + 255) / 256, 1 << 20);
+        const int64_t cpr = (p.ld_dst + 7) / 8;
+        if (p.sum) {
+            p.groups = (uint32_t)linear_sum_groups(p.rows, p.cols);
+            p.lg = p.groups == 1 ? 2 : 5;
+            p.blocks = (uint32_t)((cpr + (1 << p.lg) - 1) >> p.lg) * p.groups;
+        } else {
+            p.blocks = (uint32_t)std::min<int64_t>((p.rows * cpr + ROWS_THREADS - 1) / ROWS_THREADS, 1 << 20);
+        }
         blocks += p.blocks;
     }
     if (blocks == 0) return 0;
-    if (f16) hipLaunchKernelGGL(lin_rows_kernel<true>, dim3(blocks), dim3(256), 0, s, items);
-    else hipLaunchKernelGGL(lin_rows_kernel<false>, dim3(blocks), dim3(256), 0, s, items);
+    if (f16) hipLaunchKernelGGL(lin_rows_kernel<true>, dim3(blocks), dim3(ROWS_THREADS), 0, s, items);
+    else hipLaunchKernelGGL(lin_rows_kernel<false>, dim3(blocks), dim3(ROWS_THREADS), 0, s, items);
+    return 0;
+}
+
+int launch_linear_sum(const float* partial, int groups, int64_t cols, void* sum, int dt, hipStream_t s) {
+    hipLaunchKernelGGL(lin_sum_kernel, dim3((uint32_t)((cols + 63) / 64)), dim3(1024), 0, s, partial, groups, cols, sum, dt);
     return 0;
 }
 

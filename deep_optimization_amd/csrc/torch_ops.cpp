@@ -849,19 +849,26 @@ void lin_plan(int product, int64_t M, int64_t N, int64_t K, LinRows& a, LinRows&
         if (r->loose()) r->copy = true;
 }
 
-// one launch that lays out those operands that are marked; `pre`, `act`: of the one that is written (linear_lib._layout)
-void lin_layout(std::initializer_list<LinRows*> operands, const void* pre, int act, ScalarType dt, void* stream) {
+// one launch that lays out those operands that are marked; `pre`, `act`, `sum`: of the one that is written
+// (linear_lib._layout)
+void lin_layout(std::initializer_list<LinRows*> operands, const void* pre, int act, const std::optional<Tensor>& sum, ScalarType dt, void* stream) {
     dopt_linear_rows items[4];
-    Tensor sources[4];
+    Tensor sources[4], space;
     int n = 0;
     for (LinRows* r : operands) {
         if (!r->copy && !r->written) continue;
-        r->copy |= r->cols % 8 != 0 && r->ld != r->cols;  // (unpadded rows are written as one)
         const int64_t width = r->copy ? pad8(r->cols) : r->cols;
         Tensor out = fresh({r->rows, width}, dt, r->t);
         dopt_linear_rows& d = items[n++];
-        d = {r->t.data_ptr(), r->ld, r->written ? pre : nullptr, r->rows, r->cols, out.data_ptr(), width, r->written ? act : DOPT_LIN_NONE};
-        if (width == r->cols && width == r->ld) {  // a contiguous matrix as one row
+        d = {r->t.data_ptr(), r->ld, r->written ? pre : nullptr, r->rows, r->cols, out.data_ptr(), width, r->written ? act : DOPT_LIN_NONE,
+             0, nullptr, nullptr};
+        if (r->written && sum) {
+            const int64_t floats = dopt_linear_layout_workspace_floats(r->rows, r->cols);
+            if (floats > 0) space = fresh({floats}, at::kFloat, r->t);
+            d.sum = sum->data_ptr();
+            d.sum_dtype = dtype_code(sum->scalar_type(), "linear_act");
+            d.workspace = floats > 0 ? space.data_ptr<float>() : nullptr;
+        } else if (width == r->cols && width == r->ld) {  // a contiguous matrix as one row
             d.rows = 1;
             d.cols = d.ld_src = d.ld_dst = r->rows * r->cols;
         }
@@ -919,7 +926,7 @@ std::tuple<Tensor, std::optional<Tensor>> linear_act_fwd(const Tensor& x, const 
     LinRows a(x, M, K), b(weight, N, K);
     if (M && N && K) {
         lin_plan(DOPT_LIN_FORWARD, M, N, K, a, b, false);
-        lin_layout({&a, &b}, nullptr, DOPT_LIN_NONE, dt, stream_of(x));
+        lin_layout({&a, &b}, nullptr, DOPT_LIN_NONE, std::nullopt, dt, stream_of(x));
     }
     const auto bc = contiguous(bias), r = contiguous(residual);
     Tensor y = fresh(shape, r ? r->scalar_type() : dt, x);
@@ -957,24 +964,27 @@ std::tuple<std::optional<Tensor>, std::optional<Tensor>, std::optional<Tensor>> 
     void* const stream = stream_of(x);
     const bool empty = M == 0 || N == 0 || K == 0;
     // dz is dy, or written by the launch that lays out the operands whose rows the products do better to read aligned
-    const bool z = code != DOPT_LIN_NONE && M && N;
+    // (and, where no product sums it, or only once it is rounded, for its sums)
+    std::optional<Tensor> db, sum;
+    if (bias_grad) db = fresh({N}, grad_dtype, x);
+    if (db && (code != DOPT_LIN_NONE || K == 0 || M == 0)) sum = db;
+    const bool z = (code != DOPT_LIN_NONE && M && N) || sum;
     LinRows dz(dy, M, N, z), w(weight, N, K), xr(x, M, K);
     if (!empty) {
         if (input_grad) lin_plan(DOPT_LIN_INPUT_GRAD, M, N, K, dz, w, z);
-        if (weight_grad || bias_grad) lin_plan(DOPT_LIN_WEIGHT_GRAD, M, N, K, dz, xr, z || dz.copy || w.copy);
+        if (weight_grad || (db && !sum)) lin_plan(DOPT_LIN_WEIGHT_GRAD, M, N, K, dz, xr, z || dz.copy || w.copy);
     }
     const auto p = contiguous(pre);
-    lin_layout({&dz, &w, &xr}, ptr(p), code, dt, stream);
-    std::optional<Tensor> dx, dw, db;
+    lin_layout({&dz, &w, &xr}, ptr(p), code, sum, dt, stream);
+    std::optional<Tensor> dx, dw;
     if (input_grad) {
         dx = fresh(x.sizes(), dt, x);
         const auto ip = contiguous(in_pre);
         check(dopt_linear_input_grad(dz.t.data_ptr(), dz.ld, w.t.data_ptr(), w.ld, tc, M, N, K, ptr(ip), in_code, dx->data_ptr(), stream), what);
     }
-    if (weight_grad || bias_grad) {
+    if (weight_grad || (db && !sum)) {
         if (N == 0 || K == 0) {
             dw = fresh({N, K}, grad_dtype, x);
-            db = dz.t.reshape({M, N}).to(at::kFloat).sum(0).to(grad_dtype);
         } else {
             // the kernels that split the sum write whole chunks of a row
             int64_t K8 = pad8(K);
@@ -984,8 +994,7 @@ std::tuple<std::optional<Tensor>, std::optional<Tensor>, std::optional<Tensor>> 
             Tensor ws;
             if (floats > 0) ws = fresh({floats}, ScalarType::Float, x);
             Tensor d = fresh({N, K8}, grad_dtype, x);
-            if (bias_grad) db = fresh({N}, grad_dtype, x);
-            void* const dbp = db ? db->data_ptr() : nullptr;
+            void* const dbp = db && !sum ? db->data_ptr() : nullptr;
             check(dopt_linear_weight_grad(dz.t.data_ptr(), dz.ld, xr.t.data_ptr(), xr.ld, tc, M, N, K8,
                                           floats > 0 ? ws.data_ptr<float>() : nullptr, f32 ? (float*)d.data_ptr() : nullptr,
                                           f32 ? nullptr : d.data_ptr(), f32 ? (float*)dbp : nullptr, f32 ? nullptr : dbp, stream),
@@ -993,7 +1002,6 @@ std::tuple<std::optional<Tensor>, std::optional<Tensor>, std::optional<Tensor>> 
             dw = K8 == K ? d : d.narrow(1, 0, K).contiguous();
         }
         if (!weight_grad) dw.reset();
-        if (!bias_grad) db.reset();
     }
     return {dx, dw, db};
 }

@@ -16,8 +16,9 @@ y in residual's type (x's without one). pre [..., N] in x's type.
 Backward: dy and pre [..., N] in x's type. With ``in_act`` other than "none", x is in_act(in_pre), the output of the
 activation that feeds the layer, and dx is the gradient of in_pre [..., K]: an MLP's second layer hands its first one the
 gradient of the pre-activation in one pass. dz is rounded to x's type for the products (both read it on matrix
-instructions of that type). dweight and dbias come in ``grad_dtype`` (float32 or x's type; both are summed in fp32);
-what is not asked for is None, and bias_grad alone still runs the weight gradient's product, which sums dz on its way.
+instructions of that type); dbias is the sum of dz before that rounding. dweight and dbias come in ``grad_dtype`` (float32 or
+x's type; both are summed in fp32); what is not asked for is None, and without an activation bias_grad alone still runs the weight
+gradient's product, which sums dy on its way.
 
 Rows may be strided (x[:, 0] of a [B, T, K] tensor) and lie at any element. Where they start at multiples of 16 bytes
 and hold whole 16-byte chunks the faster kernels read them; others are read through registers, or copied into
@@ -80,18 +81,24 @@ def _plan(product: int, M: int, N: int, K: int, a: _Rows, b: _Rows, launched: bo
 
 
 def _layout(items, dtype: torch.dtype, stream) -> None:
-    """One launch that lays out [(operand, pre, act)]; each then holds its new rows. With an activation the rows become dy act'(pre),
-    padded only where a copy is marked."""
+    """One launch that lays out [(operand, pre, act, sum)]; each then holds its new rows. With an activation the rows become dy act'(pre),
+    padded only where a copy is marked; ``sum`` (or None) receives their columns' sums."""
     if not items:
         return
-    rows = (_lib.LinearRows * len(items))()
-    for d, (r, pre, act) in zip(rows, items):
-        r.copy |= r.cols % 8 != 0 and r.ld != r.cols  # (unpadded rows are written as one)
+    rows, kept = (_lib.LinearRows * len(items))(), []
+    for d, (r, pre, act, total) in zip(rows, items):
         width = _pad8(r.cols) if r.copy else r.cols
         out = torch.empty((r.rows, width), dtype=dtype, device=r.t.device)
         n, cols, src, dst = r.rows, r.cols, r.ld, width
-        if width == cols == r.ld:  # a contiguous matrix as one row
+        space = None
+        if total is not None:
+            floats = int(_lib.lib().dopt_linear_layout_workspace_floats(n, cols))
+            space = torch.empty(floats, dtype=torch.float32, device=r.t.device) if floats else None
+            d.sum, d.sum_dtype, d.workspace = total.data_ptr(), _DTYPE_CODE[total.dtype], None if space is None else space.data_ptr()
+        elif width == cols == r.ld:  # a contiguous matrix as one row
             n, cols, src, dst = 1, n * cols, n * cols, n * cols
+        # (what the launch reads lives until then: the next result could take its memory)
+        kept.append((r.t, space))
         d.src, d.ld_src, d.pre, d.rows, d.cols, d.dst, d.ld_dst, d.act = (r.t.data_ptr(), src, None if pre is None else pre.data_ptr(), n,
                                                                           cols, out.data_ptr(), dst, act)
         r.t, r.ld, r.whole, r.copy = out, width, width % 8 == 0, False
@@ -127,7 +134,7 @@ def _linear_act_fwd(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual:
     a, b = _Rows(x, M, K), _Rows(weight, N, K)
     if M and N and K:
         _plan(0, M, N, K, a, b, False)
-        _layout([(r, None, 0) for r in (a, b) if r.copy], x.dtype, _stream(x))
+        _layout([(r, None, 0, None) for r in (a, b) if r.copy], x.dtype, _stream(x))
     bias = None if bias is None else bias.contiguous()
     residual = None if residual is None else residual.contiguous()
     y = torch.empty(shape, dtype=x.dtype if residual is None else residual.dtype, device=x.device)
@@ -170,26 +177,29 @@ def _linear_act_bwd(dy: Tensor, x: Tensor, weight: Tensor, pre: Optional[Tensor]
     L, dt, stream = _lib.lib(), _DTYPE_CODE[x.dtype], _stream(x)
     empty = M == 0 or N == 0 or K == 0
     # dz is dy, or written by the launch that lays out the operands whose rows the products do better to read aligned
-    z = code != 0 and M > 0 and N > 0
+    # (and, where no product sums it, or only once it is rounded, for its sums)
+    db = torch.empty(N, dtype=grad_dtype, device=x.device) if bias_grad else None
+    summed = db is not None and (code != 0 or K == 0 or M == 0)
+    z = (code != 0 and M > 0 and N > 0) or summed
     dz, w, xr = _Rows(dy, M, N, z), _Rows(weight, N, K), _Rows(x, M, K)
     if not empty:
         if input_grad:
             _plan(1, M, N, K, dz, w, z)
-        if weight_grad or bias_grad:
+        if weight_grad or (bias_grad and not summed):
             _plan(2, M, N, K, dz, xr, z or dz.copy or w.copy)
     pre = None if pre is None else pre.contiguous()
-    _layout([(r, p, a) for r, p, a in ((dz, pre, code), (w, None, 0), (xr, None, 0)) if r.copy or r.written], x.dtype, stream)
-    dx = dw = db = None
+    _layout([(r, p, a, s) for r, p, a, s in ((dz, pre, code, db if summed else None), (w, None, 0, None), (xr, None, 0, None))
+             if r.copy or r.written], x.dtype, stream)
+    dx = dw = None
     if input_grad:
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         in_pre = None if in_pre is None else in_pre.contiguous()
         rc = L.dopt_linear_input_grad(dz.t.data_ptr(), dz.ld, w.t.data_ptr(), w.ld, dt, M, N, K, None if in_pre is None else in_pre.data_ptr(),
                                       in_code, dx.data_ptr(), stream)
         _lib.check(rc, what)
-    if weight_grad or bias_grad:
+    if weight_grad or (bias_grad and not summed):
         if N == 0 or K == 0:
             dw = torch.empty((N, K), dtype=grad_dtype, device=x.device)
-            db = dz.t.reshape(M, N).float().sum(0).to(grad_dtype)
         else:
             # the kernels that split the sum write whole chunks of a row
             K8 = _pad8(K)
@@ -197,15 +207,14 @@ def _linear_act_bwd(dy: Tensor, x: Tensor, weight: Tensor, pre: Optional[Tensor]
                 K8 = K
             ws = torch.empty(max(int(L.dopt_linear_weight_grad_workspace_floats(M, N, K8)), 4), dtype=torch.float32, device=x.device)
             dw = torch.empty((N, K8), dtype=grad_dtype, device=x.device)
-            db = torch.empty(N, dtype=grad_dtype, device=x.device) if bias_grad else None
             f32 = grad_dtype == torch.float32
-            dbp = None if db is None else db.data_ptr()
+            dbp = None if db is None or summed else db.data_ptr()
             rc = L.dopt_linear_weight_grad(dz.t.data_ptr(), dz.ld, xr.t.data_ptr(), xr.ld, dt, M, N, K8, ws.data_ptr(), dw.data_ptr() if f32 else None,
                                            None if f32 else dw.data_ptr(), dbp if f32 else None, None if f32 else dbp, stream)
             _lib.check(rc, what)
             if K8 != K:
                 dw = dw[:, :K].contiguous()
-    return dx, dw if weight_grad else None, db if bias_grad else None
+    return dx, dw if weight_grad else None, db
 
 
 def _linear_act_bwd_fake(dy, x, weight, pre, act, in_pre, in_act, input_grad, weight_grad, bias_grad, grad_dtype):

@@ -488,8 +488,10 @@ int dopt_linear_forward(const void* x, int64_t ldx, const void* weight, int64_t 
 int dopt_linear_input_grad(const void* dz, int64_t ldz, const void* weight, int64_t ldw, int dtype, int64_t M, int64_t N,
                            int64_t K, const void* in_pre, int in_act, void* dx, void* stream);
 /* Rows laid out for the products, up to 4 matrices in one launch: dst[r][c] = src[r][c] * act'(pre[r][c]) for c < cols, 0 for the
- * columns up to ld_dst; with DOPT_LIN_NONE a copy (pre is not read). src's rows ld_src elements apart, at any element; pre
- * [rows, cols] contiguous; dst 16-byte aligned with ld_dst a multiple of 8, or one row (a contiguous matrix as a whole). */
+ * columns up to ld_dst; with DOPT_LIN_NONE a copy (pre is not read). src's and dst's rows ld_src and ld_dst elements apart, at
+ * any element; pre [rows, cols] contiguous. sum (or NULL): the columns' sums of the fp32 values before their rounding, [cols] of
+ * sum_dtype (dtype or DOPT_F32), in an order that the sizes fix; workspace: dopt_linear_layout_workspace_floats floats (0: it may
+ * be NULL; else the sums take a second launch). */
 typedef struct {
     const void* src;
     int64_t ld_src;
@@ -497,8 +499,11 @@ typedef struct {
     int64_t rows, cols;
     void* dst;
     int64_t ld_dst;
-    int act;
+    int act, sum_dtype;
+    void* sum;
+    float* workspace;
 } dopt_linear_rows;
+int64_t dopt_linear_layout_workspace_floats(int64_t rows, int64_t cols);
 int dopt_linear_layout(const dopt_linear_rows* rows, int n, int dtype, void* stream);
 /* dw = dz^T x (fp32 to dw_f32 or the operands' type to dw_16, [N, K]) and the sums of dz over its rows ([N], fp32 to db or
  * the operands' type to db_16; NULL: none): dz [M, ldz], x [M, ldx], the same alignment rules. workspace:

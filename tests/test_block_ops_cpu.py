@@ -75,14 +75,15 @@ def test_c_entries_refuse_before_any_launch():
     for k in (dict(dz=None), dict(x=None), dict(ldz=7), dict(ldx=7), dict(dt=FP), dict(M=-1), dict(N=0), dict(dw=None), dict(dw16=AT), dict(db=AT, db16=AT)):
         _refused(wg(**k))
     def lay(n=1, dt=BF, **k):
-        r = _lib.LinearRows(*{**dict(src=AT, ld=8, pre=AT, rows=2, cols=8, dst=AT, ldd=8, act=2), **k}.values())
+        r = _lib.LinearRows(*{**dict(src=AT, ld=8, pre=AT, rows=2, cols=8, dst=AT, ldd=8, act=2, sdt=BF, sum=AT, ws=AT), **k}.values())
         return L.dopt_linear_layout(ctypes.byref(r), n, dt, None)
 
-    for k in (dict(src=None), dict(dst=None), dict(pre=None), dict(ld=7), dict(ldd=7), dict(ldd=9), dict(act=7), dict(act=-1), dict(dt=FP),
-              dict(rows=-1), dict(cols=-1), dict(n=5), dict(n=-1), dict(dst=ODD), dict(rows=1 << 40, ld=32, ldd=32)):
+    for k in (dict(src=None), dict(dst=None), dict(pre=None), dict(ld=7), dict(ldd=7), dict(act=7), dict(act=-1), dict(dt=FP),
+              dict(rows=-1), dict(cols=-1), dict(n=5), dict(n=-1), dict(src=ODD), dict(pre=ODD), dict(dst=ODD),
+              dict(rows=1 << 40, ld=32, ldd=32), dict(rows=5000, ws=None), dict(sdt=I8), dict(sdt=_lib.F16), dict(cols=1 << 26, ld=1 << 26, ldd=1 << 26)):
         _refused(lay(**k))
     _refused(L.dopt_linear_layout(None, 1, BF, None))
-    assert lay(n=0) == 0 and lay(rows=0, src=None, dst=None) == 0
+    assert lay(n=0) == 0 and lay(rows=0, src=None, dst=None, sum=None) == 0
     # nothing to do is no error
     assert ln(rows=0, x=None, y=None, mean=None, rstd=None) == 0 and dr(n=0, x=None, y=None) == 0 and fw(M=0, y=None) == 0 and dg(M=0, dx=None) == 0
 

@@ -211,3 +211,21 @@ def test_refusals():
                  lambda: bwd(dy, x, w, None, "none", None, "none", True, True, True, F16)):
         with pytest.raises(RuntimeError):
             call()
+
+
+@gpu
+@pytest.mark.parametrize("M,N", [(1, 8), (3, 13), (64, 2048), (333, 1001), (20000, 40), (5000, 2311), (9, 9000)])
+@pytest.mark.parametrize("dt", [BF16, F16], ids=IDS.get)
+def test_the_bias_gradient_is_the_sum_before_rounding(M, N, dt):
+    """With an activation, dbias in fp32 is within the fp32 sums' bound, which the sum of a rounded dz is not; rows as they lie in
+    a larger tensor, too."""
+    gen = torch.Generator(device=DEV).manual_seed(M + N)
+    x, w = _rand(gen, (M, 16), dt), _rand(gen, (N, 16), dt)
+    wide, pre = _rand(gen, (M, N + 5), dt), _rand(gen, (M, N), dt)
+    for dy in (wide[:, :N].contiguous(), wide[:, 2:N + 2]):
+        for act in ("gelu", "silu", "relu"):
+            db = ops.linear_act_bwd(dy, x, w, pre, act, None, "none", False, False, True, F32)[2]
+            terms = dy.double() * ref.act_grad(pre.double(), act)
+            ref.close(db, terms.sum(0), (M + 8) * ref.E * terms.abs().sum(0) + ref.ACT_ERR * dy.double().abs().sum(0), act)
+            full = ops.linear_act_bwd(dy, x, w, pre, act, None, "none", True, True, True, F32)
+            assert torch.equal(full[2], db)
