@@ -73,6 +73,7 @@ EXPORTS = (
     "dopt_linear_layout",
     "dopt_linear_weight_grad_workspace_floats",
     "dopt_linear_weight_grad",
+    "dopt_linear_backward",
     "dopt_linear_tile",
     "dopt_linear_copy_preferred",
 )
@@ -227,6 +228,8 @@ def lib() -> ctypes.CDLL:
         L.dopt_linear_weight_grad_workspace_floats.restype = i64
         L.dopt_linear_weight_grad.argtypes = [vp, i64, vp, i64, i32, i64, i64, i64, vp, vp, vp, vp, vp, vp]
         L.dopt_linear_weight_grad.restype = i32
+        L.dopt_linear_backward.argtypes = [vp, i64, vp, i64, vp, i64, i32, i64, i64, i64, vp, i32, vp, vp, vp, vp, vp, vp, vp]
+        L.dopt_linear_backward.restype = i32
         L.dopt_linear_tile.argtypes = [i32, i64, i64, i64, i32]
         L.dopt_linear_tile.restype = i32
         L.dopt_linear_copy_preferred.argtypes = [i32, i64, i64, i64, i64, i32]

@@ -42,6 +42,8 @@ int launch_dropout(const void* x, int x_dt, const void* residual, uint64_t n, ui
 bool lin_shape_fits(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb);
 int launch_linear(const LinArgs& p, int kind, bool f16, hipStream_t s);
 int linear_tile(int kind, int64_t M, int64_t N, int64_t K, bool reg, bool big, float* us);
+int linear_pair(int64_t M, int64_t N, int64_t K, bool reg, float* us);
+int launch_linear_pair(const LinArgs& dx, const LinArgs& dw, int tile, bool f16, hipStream_t s);
 int linear_sum_groups(int64_t rows, int64_t cols);
 int launch_linear_rows(LinRowItems items, bool f16, hipStream_t s);
 int launch_linear_sum(const float* partial, int groups, int64_t cols, void* sum, int dt, hipStream_t s);
@@ -1257,14 +1259,17 @@ int dopt_linear_forward(const void* x, int64_t ldx, const void* weight, int64_t 
     return hip_status("linear_forward launch");
 }
 
-int dopt_linear_input_grad(const void* dz, int64_t ldz, const void* weight, int64_t ldw, int dtype, int64_t M, int64_t N,
-                           int64_t K, const void* in_pre, int in_act, void* dx, void* stream) {
+static int check_input_grad(const void* dz, int64_t ldz, const void* weight, int64_t ldw, int dtype, int64_t M, int64_t N, int64_t K,
+                            const void* in_pre, int in_act, void* dx) {
     if (int rc = check_linear(dtype, M, K, N, ldz, ldw, in_act)) return rc;
-    if (M == 0 || K == 0) return ok();
+    if (M == 0 || K == 0) return DOPT_OK;
     if (!dx) return fail(DOPT_EINVAL, "null dx pointer");
     if (in_act != DOPT_LIN_NONE && !in_pre) return fail(DOPT_EINVAL, "linear: in_act needs in_pre");
-    if (N > 0)
-        if (int rc = check_linear_rows(dz, ldz, N, weight, ldw, K)) return rc;
+    return N > 0 ? check_linear_rows(dz, ldz, N, weight, ldw, K) : DOPT_OK;
+}
+
+static dopt::LinArgs input_grad_args(const void* dz, int64_t ldz, const void* weight, int64_t ldw, int64_t M, int64_t N, int64_t K,
+                                     const void* in_pre, int in_act, void* dx) {
     dopt::LinArgs p{};
     p.A = (const uint16_t*)dz;
     p.B = (const uint16_t*)weight;
@@ -1276,6 +1281,14 @@ int dopt_linear_input_grad(const void* dz, int64_t ldz, const void* weight, int6
     p.aux = (const uint16_t*)in_pre;
     p.act = in_act;
     p.y = dx;
+    return p;
+}
+
+int dopt_linear_input_grad(const void* dz, int64_t ldz, const void* weight, int64_t ldw, int dtype, int64_t M, int64_t N,
+                           int64_t K, const void* in_pre, int in_act, void* dx, void* stream) {
+    if (int rc = check_input_grad(dz, ldz, weight, ldw, dtype, M, N, K, in_pre, in_act, dx)) return rc;
+    if (M == 0 || K == 0) return ok();
+    const dopt::LinArgs p = input_grad_args(dz, ldz, weight, ldw, M, N, K, in_pre, in_act, dx);
     (void)hipGetLastError();
     dopt::launch_linear(p, dopt::LIN_KN, dtype == DOPT_F16, (hipStream_t)stream);
     return hip_status("linear_input_grad launch");
@@ -1339,14 +1352,35 @@ int64_t dopt_linear_weight_grad_workspace_floats(int64_t M, int64_t N, int64_t K
     return linear_dw_split(M, N, K) ? dopt::dw_any_workspace_floats(N, K, M) : 0;
 }
 
-int dopt_linear_weight_grad(const void* dz, int64_t ldz, const void* x, int64_t ldx, int dtype, int64_t M, int64_t N,
-                            int64_t K, float* workspace, float* dw_f32, void* dw_16, float* db, void* db_16, void* stream) {
+static int check_weight_grad(const void* dz, int64_t ldz, const void* x, int64_t ldx, int dtype, int64_t M, int64_t N, int64_t K,
+                             const float* dw_f32, const void* dw_16, const float* db, const void* db_16) {
     if (int rc = check_linear(dtype, N, K, M, ldz, ldx, DOPT_LIN_NONE)) return rc;
     if (db && db_16) return fail(DOPT_EINVAL, "linear: one bias gradient, db or db_16");
     if (!dw_f32 == !dw_16) return fail(DOPT_EINVAL, "linear: one weight gradient, dw_f32 or dw_16");
     if (N == 0 || K == 0) return fail(DOPT_EINVAL, "linear weight gradient needs N and K >= 1");
-    if (M > 0)
-        if (int rc = check_linear_rows(dz, ldz, N, x, ldx, K)) return rc;
+    return M > 0 ? check_linear_rows(dz, ldz, N, x, ldx, K) : DOPT_OK;
+}
+
+static dopt::LinArgs weight_grad_args(const void* dz, int64_t ldz, const void* x, int64_t ldx, int64_t M, int64_t N, int64_t K, float* dw_f32,
+                                      void* dw_16, float* db, void* db_16) {
+    dopt::LinArgs p{};
+    p.A = (const uint16_t*)dz;
+    p.B = (const uint16_t*)x;
+    p.M = N;
+    p.N = K;
+    p.K = M;
+    p.lda = ldz;
+    p.ldb = ldx;
+    p.y = dw_f32 ? (void*)dw_f32 : dw_16;
+    p.y_f32 = dw_f32 != nullptr;
+    p.db = db;
+    p.db16 = (uint16_t*)db_16;
+    return p;
+}
+
+int dopt_linear_weight_grad(const void* dz, int64_t ldz, const void* x, int64_t ldx, int dtype, int64_t M, int64_t N,
+                            int64_t K, float* workspace, float* dw_f32, void* dw_16, float* db, void* db_16, void* stream) {
+    if (int rc = check_weight_grad(dz, ldz, x, ldx, dtype, M, N, K, dw_f32, dw_16, db, db_16)) return rc;
     const bool whole = M == 0 || (lin_rows(dz, ldz, N) && lin_rows(x, ldx, K));
     (void)hipGetLastError();
     if (whole && linear_dw_split(M, N, K) && ldz < ((int64_t)1 << 24) && ldx < ((int64_t)1 << 24)) {
@@ -1367,20 +1401,33 @@ int dopt_linear_weight_grad(const void* dz, int64_t ldz, const void* x, int64_t 
             return fail(DOPT_EUNSUPPORTED, "no weight-gradient kernel for this shape");
         return hip_status("linear_weight_grad launch");
     }
-    dopt::LinArgs p{};
-    p.A = (const uint16_t*)dz;
-    p.B = (const uint16_t*)x;
-    p.M = N;
-    p.N = K;
-    p.K = M;
-    p.lda = ldz;
-    p.ldb = ldx;
-    p.y = dw_f32 ? (void*)dw_f32 : dw_16;
-    p.y_f32 = dw_f32 != nullptr;
-    p.db = db;
-    p.db16 = (uint16_t*)db_16;
+    const dopt::LinArgs p = weight_grad_args(dz, ldz, x, ldx, M, N, K, dw_f32, dw_16, db, db_16);
     dopt::launch_linear(p, dopt::LIN_TN, dtype == DOPT_F16, (hipStream_t)stream);
     return hip_status("linear_weight_grad launch");
+}
+
+int dopt_linear_backward(const void* dz, int64_t ldz, const void* x, int64_t ldx, const void* weight, int64_t ldw, int dtype, int64_t M,
+                         int64_t N, int64_t K, const void* in_pre, int in_act, void* dx, float* workspace, float* dw_f32, void* dw_16,
+                         float* db, void* db_16, void* stream) {
+    if (int rc = check_input_grad(dz, ldz, weight, ldw, dtype, M, N, K, in_pre, in_act, dx)) return rc;
+    if (int rc = check_weight_grad(dz, ldz, x, ldx, dtype, M, N, K, dw_f32, dw_16, db, db_16)) return rc;
+    if (M > 0) {
+        const bool whole_x = lin_rows(dz, ldz, N) && lin_rows(weight, ldw, K), whole_w = lin_rows(dz, ldz, N) && lin_rows(x, ldx, K);
+        float one, ux, uw;
+        const int tile = dopt::linear_pair(M, N, K, !whole_x, &one);
+        dopt::linear_tile(DOPT_LIN_INPUT_GRAD, M, K, N, !whole_x, true, &ux);
+        dopt::linear_tile(DOPT_LIN_WEIGHT_GRAD, N, K, M, !whole_w, false, &uw);
+        if (whole_w && linear_dw_split(M, N, K)) uw = std::min(uw, linear_dw_split_us(M, N, K));
+        if (whole_x == whole_w && one < ux + uw) {
+            (void)hipGetLastError();
+            dopt::launch_linear_pair(input_grad_args(dz, ldz, weight, ldw, M, N, K, in_pre, in_act, dx),
+                                     weight_grad_args(dz, ldz, x, ldx, M, N, K, dw_f32, dw_16, db, db_16), tile, dtype == DOPT_F16,
+                                     (hipStream_t)stream);
+            return hip_status("linear_backward launch");
+        }
+    }
+    if (int rc = dopt_linear_input_grad(dz, ldz, weight, ldw, dtype, M, N, K, in_pre, in_act, dx, stream)) return rc;
+    return dopt_linear_weight_grad(dz, ldz, x, ldx, dtype, M, N, K, workspace, dw_f32, dw_16, db, db_16, stream);
 }
 
 int dopt_graph_node_counts(void* graph, int64_t* counts, int n_counts) {

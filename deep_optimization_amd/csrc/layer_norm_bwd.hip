@@ -16,7 +16,8 @@ namespace {
 
 constexpr int LNB_THREADS = 1024, LNB_GROUPS = 256;
 
-template <int DTX, int DTY, int TPR, int ACC>
+// PARAMS: with the parameters' sums.
+template <int DTX, int DTY, int TPR, int ACC, bool PARAMS = true>
 __global__ __launch_bounds__(LNB_THREADS) void ln_bwd_kernel(LnBwdArgs p) {
     constexpr int RPW = LNB_THREADS / TPR;  // rows at a time
     __shared__ float red[TPR > 64 ? 2 * LNB_THREADS / 64 : 1];
@@ -24,7 +25,7 @@ __global__ __launch_bounds__(LNB_THREADS) void ln_bwd_kernel(LnBwdArgs p) {
     const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, dim = p.dim;
     const float inv = 1.0f / (float)dim;
     LnCol col[ACC];
-    float w[ACC][4], dw[ACC][4] = {}, db[ACC][4] = {};
+    float w[ACC][4], dw[PARAMS ? ACC : 1][4] = {}, db[PARAMS ? ACC : 1][4] = {};
 #pragma unroll
     for (int a = 0; a < ACC; ++a) {
         col[a] = ln_col<TPR>(a, t, dim);
@@ -56,9 +57,9 @@ __global__ __launch_bounds__(LNB_THREADS) void ln_bwd_kernel(LnBwdArgs p) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 xh[a][e] = (xh[a][e] - mean) * rstd;
-                if (live) {
-                    dw[a][e] = __builtin_fmaf(g[a][e], xh[a][e], dw[a][e]);
-                    db[a][e] += g[a][e];
+                if (PARAMS && live) {
+                    dw[PARAMS ? a : 0][e] = __builtin_fmaf(g[a][e], xh[a][e], dw[PARAMS ? a : 0][e]);
+                    db[PARAMS ? a : 0][e] += g[a][e];
                 }
                 g[a][e] *= w[a][e];
                 const float q = e >= col[a].first ? g[a][e] : 0.0f;
@@ -79,11 +80,13 @@ __global__ __launch_bounds__(LNB_THREADS) void ln_bwd_kernel(LnBwdArgs p) {
             store4<DTX>(p.dx, row * dim + col[a].at, d);
         }
     }
+    if constexpr (!PARAMS) return;
     if (!p.partial) return;
     // the RPW lanes of equal columns, by halves
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
         float(*v)[4] = part ? db : dw;
+        if constexpr (!PARAMS) break;
 #pragma unroll
         for (int h = RPW / 2; h > 0; h >>= 1) {
             __syncthreads();
@@ -111,6 +114,42 @@ __global__ __launch_bounds__(LNB_THREADS) void ln_bwd_kernel(LnBwdArgs p) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (e >= col[a].first) out[col[a].at + e] = v[a][e];
+        }
+    }
+}
+
+// The parameters' sums alone, for rows that are too wide for a lane to hold its columns' sums beside its row: a block takes
+// 256 columns of every groups-th 4 rows, a wave a row at a time, and reads dy and x a second time.
+template <int DTX, int DTY>
+__global__ __launch_bounds__(256) void ln_col_sum_kernel(LnBwdArgs p, int groups) {
+    __shared__ __attribute__((aligned(16))) float meet[4][2][256];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, dim = p.dim;
+    const uint32_t strip = blockIdx.x / groups, group = blockIdx.x % groups;
+    const LnCol col = ln_col<64>(strip, lane, dim);
+    float dw[4] = {}, db[4] = {};
+#pragma unroll 4
+    for (int64_t row = (int64_t)group * 4 + wave; row < p.rows; row += (int64_t)groups * 4) {
+        float x[4], d[4];
+        widen4<DTX>(load4<DTX>(p.x, row * dim + col.at), x);
+        widen4<DTY>(load4<DTY>(p.dy, row * dim + col.at), d);
+        const float mean = p.mean[row], rstd = p.rstd[row];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            dw[e] = __builtin_fmaf(d[e], (x[e] - mean) * rstd, dw[e]);
+            db[e] += d[e];
+        }
+    }
+    *(float4*)&meet[wave][0][lane * 4] = make_float4(dw[0], dw[1], dw[2], dw[3]);
+    *(float4*)&meet[wave][1][lane * 4] = make_float4(db[0], db[1], db[2], db[3]);
+    __syncthreads();
+    if (wave < 2) {  // a wave for each of the two
+        float* out = p.partial + ((int64_t)group * 2 + wave) * dim;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float sum = meet[0][wave][lane * 4 + e];
+#pragma unroll
+            for (int q = 1; q < 4; ++q) sum += meet[q][wave][lane * 4 + e];
+            if (e >= col.first) out[col.at + e] = sum;
         }
     }
 }
@@ -168,9 +207,15 @@ __global__ __launch_bounds__(1024) void ln_param_kernel(const float* partial, in
     }
 }
 
-// widths past this (and under 4) go through ln_bwd_any_kernel: with 3 accesses a lane over 1024 lanes the row, its
-// columns' sums and the weight no longer fit the 128 registers that 16 waves a CU leave (26 spilled)
-constexpr int LNB_MAX_DIM = 8192;
+// Widths past this take the parameters' sums in a kernel of their own: the row, its columns' sums and the weight no longer fit
+// the 128 registers that 16 waves a CU leave (3 accesses a lane over 1024 lanes spilled 26). 452 x 15232 in fp16 with a
+// residual: WIDE_US us, through ln_bwd_any_kernel with its sums in memory 85.6.
+constexpr int LNB_MAX_DIM = 8192, LNB_WIDE_DIM = 16384;
+
+// partial rows of ln_col_sum_kernel: some 1024 blocks
+int wide_groups(int64_t rows, int dim) {
+    return (int)std::max<int64_t>(1, std::min<int64_t>((rows + 3) / 4, 1024 / ((dim + 255) / 256)));
+}
 
 int rows_at_a_time(int dim) { return dim < 4 ? 1 : dim <= 768 ? 16 : dim <= 3072 ? 4 : 1; }
 
@@ -185,7 +230,13 @@ void pick(const LnBwdArgs& a, int64_t groups, hipStream_t s) {
     else if (d <= 2048) hipLaunchKernelGGL((ln_bwd_kernel<DTX, DTY, 256, 2>), g, b, 0, s, a);
     else if (d <= 3072) hipLaunchKernelGGL((ln_bwd_kernel<DTX, DTY, 256, 3>), g, b, 0, s, a);
     else if (d <= 4096) hipLaunchKernelGGL((ln_bwd_kernel<DTX, DTY, 1024, 1>), g, b, 0, s, a);
-    else hipLaunchKernelGGL((ln_bwd_kernel<DTX, DTY, 1024, 2>), g, b, 0, s, a);
+    else if (d <= LNB_MAX_DIM) hipLaunchKernelGGL((ln_bwd_kernel<DTX, DTY, 1024, 2>), g, b, 0, s, a);
+    else {
+        const dim3 rows((uint32_t)std::min<int64_t>(a.rows, 2 * LNB_GROUPS));
+        if (d <= 12288) hipLaunchKernelGGL((ln_bwd_kernel<DTX, DTY, 1024, 3, false>), rows, b, 0, s, a);
+        else if (d <= LNB_WIDE_DIM) hipLaunchKernelGGL((ln_bwd_kernel<DTX, DTY, 1024, 4, false>), rows, b, 0, s, a);
+        if (a.partial) hipLaunchKernelGGL((ln_col_sum_kernel<DTX, DTY>), dim3((uint32_t)(groups * ((d + 255) / 256))), dim3(256), 0, s, a, (int)groups);
+    }
 }
 
 template <int DTX>
@@ -198,6 +249,7 @@ void pick_dy(const LnBwdArgs& a, int dy_dt, int64_t groups, hipStream_t s) {
 }  // namespace
 
 int64_t layer_norm_groups(int64_t rows, int dim) {
+    if (dim > LNB_MAX_DIM) return rows > 0 ? wide_groups(rows, dim) : 0;
     const int64_t r = rows_at_a_time(dim);
     return std::min<int64_t>((rows + r - 1) / r, LNB_GROUPS);
 }
@@ -205,11 +257,17 @@ int64_t layer_norm_groups(int64_t rows, int dim) {
 int launch_layer_norm_bwd(const LnBwdArgs& a, int x_dt, int dy_dt, float* dweight, float* dbias, hipStream_t s) {
     const int64_t groups = layer_norm_groups(a.rows, a.dim);
     if (groups > 0) {
-        if (a.dim < 4 || a.dim > LNB_MAX_DIM)
-            hipLaunchKernelGGL(ln_bwd_any_kernel, dim3((uint32_t)groups), dim3(LNB_THREADS), 0, s, a, x_dt, dy_dt);
-        else if (x_dt == DT_F32) pick_dy<DT_F32>(a, dy_dt, groups, s);
-        else if (x_dt == DT_F16) pick_dy<DT_F16>(a, dy_dt, groups, s);
-        else pick_dy<DT_BF16>(a, dy_dt, groups, s);
+        if (a.dim < 4 || a.dim > LNB_WIDE_DIM) {
+            LnBwdArgs any = a;
+            if (a.dim >= 4) any.partial = nullptr;
+            const int64_t grid = a.dim < 4 ? groups : std::min<int64_t>(a.rows, 2 * LNB_GROUPS);
+            hipLaunchKernelGGL(ln_bwd_any_kernel, dim3((uint32_t)grid), dim3(LNB_THREADS), 0, s, any, x_dt, dy_dt);
+        }
+        if (a.dim >= 4) {
+            if (x_dt == DT_F32) pick_dy<DT_F32>(a, dy_dt, groups, s);
+            else if (x_dt == DT_F16) pick_dy<DT_F16>(a, dy_dt, groups, s);
+            else pick_dy<DT_BF16>(a, dy_dt, groups, s);
+        }
     }
     if (dweight || dbias)  // (no rows: zeros)
         hipLaunchKernelGGL(ln_param_kernel, dim3((uint32_t)((2 * (int64_t)a.dim + 63) / 64)), dim3(1024), 0, s, a.partial,

@@ -111,8 +111,9 @@ __device__ __forceinline__ int lin_col_swizzle(int r) {
     return W == 32 ? 0 : W == 64 ? ((r >> 1) & 1) << 2 : (r & 3) << 2;
 }
 
-template <int BM, int BN, int S, int WAVES, int KIND, bool F16, bool REG, bool TAIL>
-__global__ __launch_bounds__(256, WAVES) void lin_gemm_kernel(LinArgs p) {
+template <int BM, int BN, int S, int KIND, bool F16, bool REG, bool TAIL>
+__device__ __forceinline__ void lin_gemm_tile(const LinArgs& p, uint32_t bid, uint8_t* sA0, uint8_t* sA1, uint8_t* sA2, uint8_t* sA3,
+                                              uint8_t* sB0, uint8_t* sB1, uint8_t* sB2, uint8_t* sB3) {
     constexpr bool A_COLS = KIND == LIN_TN, B_COLS = KIND != LIN_NT;  // the operand lies as [K] rows
     static_assert(!REG || S == 2, "register loads: one slab in registers, two in LDS");
     constexpr int ROWB = 2 * LIN_BK, WM = BM / 2, WN = BN / 2, FM = WM / 16, FN = WN / 16;
@@ -120,16 +121,6 @@ __global__ __launch_bounds__(256, WAVES) void lin_gemm_kernel(LinArgs p) {
     static_assert(S >= 2 && S <= 4 && (S - 1) * LD < 64, "stages, vmcnt range");
     const int64_t M = p.M, N = p.N, lda = p.lda, ldb = p.ldb;
     const uint32_t K = (uint32_t)p.K;
-    // every stage's A and B tiles are LDS objects of their own, so the compiler can tell an operand read from the
-    // loads in flight
-    __shared__ __attribute__((aligned(1024))) uint8_t sA0[BM * ROWB];
-    __shared__ __attribute__((aligned(1024))) uint8_t sA1[BM * ROWB];
-    __shared__ __attribute__((aligned(1024))) uint8_t sA2[S > 2 ? BM * ROWB : 16];
-    __shared__ __attribute__((aligned(1024))) uint8_t sA3[S > 3 ? BM * ROWB : 16];
-    __shared__ __attribute__((aligned(1024))) uint8_t sB0[BN * ROWB];
-    __shared__ __attribute__((aligned(1024))) uint8_t sB1[BN * ROWB];
-    __shared__ __attribute__((aligned(1024))) uint8_t sB2[S > 2 ? BN * ROWB : 16];
-    __shared__ __attribute__((aligned(1024))) uint8_t sB3[S > 3 ? BN * ROWB : 16];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     auto stage_a = [&](auto i) __attribute__((always_inline)) -> uint8_t* {
         constexpr int I = decltype(i)::value % S;
@@ -147,7 +138,7 @@ __global__ __launch_bounds__(256, WAVES) void lin_gemm_kernel(LinArgs p) {
     };
 
     uint32_t tm, tn;
-    lin_tile(p, blockIdx.x, tm, tn);
+    lin_tile(p, bid, tm, tn);
     const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
     const int lane = threadIdx.x & 63;
     const int wm = wave >> 1, wn = wave & 1;
@@ -470,7 +461,35 @@ __global__ __launch_bounds__(256, WAVES) void lin_gemm_kernel(LinArgs p) {
     }
 }
 
+// Every stage's A and B tiles are LDS objects of their own, so the compiler can tell an operand read from the loads in flight.
+#define LIN_STAGES(BM, BN, S)                                                                    \
+    __shared__ __attribute__((aligned(1024))) uint8_t sA0[(BM) * 2 * LIN_BK];                     \
+    __shared__ __attribute__((aligned(1024))) uint8_t sA1[(BM) * 2 * LIN_BK];                     \
+    __shared__ __attribute__((aligned(1024))) uint8_t sA2[(S) > 2 ? (BM) * 2 * LIN_BK : 16];      \
+    __shared__ __attribute__((aligned(1024))) uint8_t sA3[(S) > 3 ? (BM) * 2 * LIN_BK : 16];      \
+    __shared__ __attribute__((aligned(1024))) uint8_t sB0[(BN) * 2 * LIN_BK];                     \
+    __shared__ __attribute__((aligned(1024))) uint8_t sB1[(BN) * 2 * LIN_BK];                     \
+    __shared__ __attribute__((aligned(1024))) uint8_t sB2[(S) > 2 ? (BN) * 2 * LIN_BK : 16];      \
+    __shared__ __attribute__((aligned(1024))) uint8_t sB3[(S) > 3 ? (BN) * 2 * LIN_BK : 16]
+
 // WAVES: waves per SIMD that the registers leave room for
+template <int BM, int BN, int S, int WAVES, int KIND, bool F16, bool REG, bool TAIL>
+__global__ __launch_bounds__(256, WAVES) void lin_gemm_kernel(LinArgs p) {
+    LIN_STAGES(BM, BN, S);
+    lin_gemm_tile<BM, BN, S, KIND, F16, REG, TAIL>(p, blockIdx.x, sA0, sA1, sA2, sA3, sB0, sB1, sB2, sB3);
+}
+// Both products of a backward pass, the input gradient's tiles in the first workgroups: two products that leave CUs idle run beside
+// each other and take one launch.
+template <int BM, int BN, int S, int WAVES, bool F16, bool REG>
+__global__ __launch_bounds__(256, WAVES) void lin_pair_kernel(LinArgs dx, LinArgs dw) {
+    LIN_STAGES(BM, BN, S);
+    const uint32_t first = dx.tiles_m * dx.tiles_n;
+    if (blockIdx.x < first)
+        lin_gemm_tile<BM, BN, S, LIN_KN, F16, REG, !REG>(dx, blockIdx.x, sA0, sA1, sA2, sA3, sB0, sB1, sB2, sB3);
+    else
+        lin_gemm_tile<BM, BN, S, LIN_TN, F16, REG, !REG>(dw, blockIdx.x - first, sA0, sA1, sA2, sA3, sB0, sB1, sB2, sB3);
+}
+
 template <int BM, int BN, int S, int WAVES, int KIND, bool F16, bool REG = false>
 inline void lin_gemm_launch(LinArgs p, hipStream_t s) {
     p.tiles_m = (uint32_t)((p.M + BM - 1) / BM);
@@ -478,6 +497,16 @@ inline void lin_gemm_launch(LinArgs p, hipStream_t s) {
     const dim3 grid(p.tiles_m * p.tiles_n), block(256);
     if (REG || p.K % LIN_BK == 0) hipLaunchKernelGGL((lin_gemm_kernel<BM, BN, S, WAVES, KIND, F16, REG, false>), grid, block, 0, s, p);
     else hipLaunchKernelGGL((lin_gemm_kernel<BM, BN, S, WAVES, KIND, F16, REG, !REG>), grid, block, 0, s, p);
+}
+
+template <int BM, int BN, int S, int WAVES, bool F16, bool REG>
+inline void lin_pair_launch(LinArgs dx, LinArgs dw, hipStream_t s) {
+    for (LinArgs* p : {&dx, &dw}) {
+        p->tiles_m = (uint32_t)((p->M + BM - 1) / BM);
+        p->tiles_n = (uint32_t)((p->N + BN - 1) / BN);
+    }
+    const dim3 grid(dx.tiles_m * dx.tiles_n + dw.tiles_m * dw.tiles_n), block(256);
+    hipLaunchKernelGGL((lin_pair_kernel<BM, BN, S, WAVES, F16, REG>), grid, block, 0, s, dx, dw);
 }
 
 }  // namespace dopt

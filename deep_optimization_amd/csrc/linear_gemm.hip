@@ -1,6 +1,7 @@
 // Launchers of a Linear layer's products: which tile a shape gets, the activation's gradient, rows laid out again.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "linear_gemm.h"
 #include "linear_small.h"
@@ -261,6 +262,41 @@ int linear_sum_groups(int64_t rows, int64_t cols) {
     if (rows <= SUM_ROWS) return 1;
     const int64_t strips = (cols + 255) / 256;
     return (int)std::max<int64_t>(1, std::min<int64_t>((rows + 31) / 32, 512 / std::max<int64_t>(strips, 1)));
+}
+
+// The tile (of TILE_COST) that both products of a backward pass take in one launch, and its estimate; M rows, N out, K in.
+int linear_pair(int64_t M, int64_t N, int64_t K, bool reg, float* us) {
+    const int n_cu = device_cu_count();
+    const float kx = (float)((N + LIN_BK - 1) / LIN_BK), kw = (float)((M + LIN_BK - 1) / LIN_BK);
+    int best = -1;
+    for (int t = reg ? T_REG32x64 : 0; t < (reg ? T_COUNT : T_128x64); ++t) {
+        const TileCost& c = TILE_COST[t];
+        const auto tiles = [&](int64_t m, int64_t n) { return (float)((m + c.bm - 1) / c.bm) * (float)((n + c.bn - 1) / c.bn); };
+        const float tx = tiles(M, K), tw = tiles(N, K), per_cu = std::ceil((tx + tw) / (float)n_cu);
+        const float alone = std::max(kx * c.alone[LIN_KN], kw * c.alone[LIN_TN]) * std::ceil(per_cu / (float)c.slots);
+        const float shared = (tx * kx * c.shared[LIN_KN] + tw * kw * c.shared[LIN_TN]) / (tx + tw) * per_cu;
+        const float e = c.start + std::max(alone, shared) + c.epilogue * per_cu;
+        if (best < 0 || e < *us) {
+            best = t;
+            *us = e;
+        }
+    }
+    return best;
+}
+
+int launch_linear_pair(const LinArgs& dx, const LinArgs& dw, int tile, bool f16, hipStream_t s) {
+#define LIN_PAIR(...) (f16 ? lin_pair_launch<__VA_ARGS__, true, false>(dx, dw, s) : lin_pair_launch<__VA_ARGS__, false, false>(dx, dw, s))
+#define LIN_PAIR_REG(...) (f16 ? lin_pair_launch<__VA_ARGS__, true, true>(dx, dw, s) : lin_pair_launch<__VA_ARGS__, false, true>(dx, dw, s))
+    switch (tile) {
+        case T_32x64: LIN_PAIR(32, 64, 4, 3); break;
+        case T_64x64: LIN_PAIR(64, 64, 4, 2); break;
+        case T_64x64_4: LIN_PAIR(64, 64, 2, 4); break;
+        case T_REG32x64: LIN_PAIR_REG(32, 64, 2, 4); break;
+        default: LIN_PAIR_REG(64, 64, 2, 3); break;
+    }
+#undef LIN_PAIR
+#undef LIN_PAIR_REG
+    return 0;
 }
 
 int launch_linear_rows(LinRowItems items, bool f16, hipStream_t s) {

@@ -977,32 +977,37 @@ std::tuple<std::optional<Tensor>, std::optional<Tensor>, std::optional<Tensor>> 
     const auto p = contiguous(pre);
     lin_layout({&dz, &w, &xr}, ptr(p), code, sum, dt, stream);
     std::optional<Tensor> dx, dw;
+    std::optional<Tensor> ip;
     if (input_grad) {
         dx = fresh(x.sizes(), dt, x);
-        const auto ip = contiguous(in_pre);
-        check(dopt_linear_input_grad(dz.t.data_ptr(), dz.ld, w.t.data_ptr(), w.ld, tc, M, N, K, ptr(ip), in_code, dx->data_ptr(), stream), what);
+        ip = contiguous(in_pre);
     }
+    int64_t K8 = K;
+    Tensor ws;
     if (weight_grad || (db && !sum)) {
-        if (N == 0 || K == 0) {
-            dw = fresh({N, K}, grad_dtype, x);
-        } else {
-            // the kernels that split the sum write whole chunks of a row
-            int64_t K8 = pad8(K);
-            if (K8 != K && !(dz.whole && xr.whole && dopt_linear_tile(DOPT_LIN_WEIGHT_GRAD, M, N, K8, 0) == 100)) K8 = K;
-            const bool f32 = grad_dtype == ScalarType::Float;
-            const int64_t floats = dopt_linear_weight_grad_workspace_floats(M, N, K8);
-            Tensor ws;
-            if (floats > 0) ws = fresh({floats}, ScalarType::Float, x);
-            Tensor d = fresh({N, K8}, grad_dtype, x);
-            void* const dbp = db && !sum ? db->data_ptr() : nullptr;
-            check(dopt_linear_weight_grad(dz.t.data_ptr(), dz.ld, xr.t.data_ptr(), xr.ld, tc, M, N, K8,
-                                          floats > 0 ? ws.data_ptr<float>() : nullptr, f32 ? (float*)d.data_ptr() : nullptr,
-                                          f32 ? nullptr : d.data_ptr(), f32 ? (float*)dbp : nullptr, f32 ? nullptr : dbp, stream),
-                  what);
-            dw = K8 == K ? d : d.narrow(1, 0, K).contiguous();
-        }
-        if (!weight_grad) dw.reset();
+        // the kernels that split the sum write whole chunks of a row
+        if (K % 8 && N && dz.whole && xr.whole && dopt_linear_tile(DOPT_LIN_WEIGHT_GRAD, M, N, pad8(K), 0) == 100) K8 = pad8(K);
+        dw = fresh({N, K8}, grad_dtype, x);
+        const int64_t floats = dopt_linear_weight_grad_workspace_floats(M, N, K8);
+        if (floats > 0) ws = fresh({floats}, at::kFloat, x);
     }
+    const bool f32 = grad_dtype == ScalarType::Float, with_dw = dw && N && K;
+    float* const wsp = ws.defined() ? ws.data_ptr<float>() : nullptr;
+    void *const dwp = dw ? dw->data_ptr() : nullptr, *const dbp = db && !sum ? db->data_ptr() : nullptr;
+    float *const dw32 = f32 ? (float*)dwp : nullptr, *const db32 = f32 ? (float*)dbp : nullptr;
+    void *const dw16 = f32 ? nullptr : dwp, *const db16 = f32 ? nullptr : dbp;
+    if (dx && with_dw && K8 == K) {
+        check(dopt_linear_backward(dz.t.data_ptr(), dz.ld, xr.t.data_ptr(), xr.ld, w.t.data_ptr(), w.ld, tc, M, N, K, ptr(ip), in_code,
+                                   dx->data_ptr(), wsp, dw32, dw16, db32, db16, stream),
+              what);
+    } else {
+        if (dx)
+            check(dopt_linear_input_grad(dz.t.data_ptr(), dz.ld, w.t.data_ptr(), w.ld, tc, M, N, K, ptr(ip), in_code, dx->data_ptr(), stream), what);
+        if (with_dw)
+            check(dopt_linear_weight_grad(dz.t.data_ptr(), dz.ld, xr.t.data_ptr(), xr.ld, tc, M, N, K8, wsp, dw32, dw16, db32, db16, stream), what);
+    }
+    if (K8 != K) dw = dw->narrow(1, 0, K).contiguous();
+    if (!weight_grad) dw.reset();
     return {dx, dw, db};
 }
 

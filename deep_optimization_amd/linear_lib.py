@@ -191,29 +191,32 @@ def _linear_act_bwd(dy: Tensor, x: Tensor, weight: Tensor, pre: Optional[Tensor]
     _layout([(r, p, a, s) for r, p, a, s in ((dz, pre, code, db if summed else None), (w, None, 0, None), (xr, None, 0, None))
              if r.copy or r.written], x.dtype, stream)
     dx = dw = None
+    dx_args = dw_args = ()
     if input_grad:
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         in_pre = None if in_pre is None else in_pre.contiguous()
-        rc = L.dopt_linear_input_grad(dz.t.data_ptr(), dz.ld, w.t.data_ptr(), w.ld, dt, M, N, K, None if in_pre is None else in_pre.data_ptr(),
-                                      in_code, dx.data_ptr(), stream)
-        _lib.check(rc, what)
+        dx_args = (None if in_pre is None else in_pre.data_ptr(), in_code, dx.data_ptr())
+    K8 = K
     if weight_grad or (bias_grad and not summed):
-        if N == 0 or K == 0:
-            dw = torch.empty((N, K), dtype=grad_dtype, device=x.device)
-        else:
-            # the kernels that split the sum write whole chunks of a row
+        # the kernels that split the sum write whole chunks of a row
+        if K % 8 and N and dz.whole and xr.whole and L.dopt_linear_tile(2, M, N, _pad8(K), 0) == 100:
             K8 = _pad8(K)
-            if K8 != K and not (dz.whole and xr.whole and L.dopt_linear_tile(2, M, N, K8, 0) == 100):
-                K8 = K
+        dw = torch.empty((N, K8), dtype=grad_dtype, device=x.device)
+        if N and K:
             ws = torch.empty(max(int(L.dopt_linear_weight_grad_workspace_floats(M, N, K8)), 4), dtype=torch.float32, device=x.device)
-            dw = torch.empty((N, K8), dtype=grad_dtype, device=x.device)
             f32 = grad_dtype == torch.float32
             dbp = None if db is None or summed else db.data_ptr()
-            rc = L.dopt_linear_weight_grad(dz.t.data_ptr(), dz.ld, xr.t.data_ptr(), xr.ld, dt, M, N, K8, ws.data_ptr(), dw.data_ptr() if f32 else None,
-                                           None if f32 else dw.data_ptr(), dbp if f32 else None, None if f32 else dbp, stream)
-            _lib.check(rc, what)
-            if K8 != K:
-                dw = dw[:, :K].contiguous()
+            dw_args = (ws.data_ptr(), dw.data_ptr() if f32 else None, None if f32 else dw.data_ptr(), dbp if f32 else None, None if f32 else dbp)
+    if dx_args and dw_args and K8 == K:
+        _lib.check(L.dopt_linear_backward(dz.t.data_ptr(), dz.ld, xr.t.data_ptr(), xr.ld, w.t.data_ptr(), w.ld, dt, M, N, K, *dx_args, *dw_args,
+                                          stream), what)
+    else:
+        if dx_args:
+            _lib.check(L.dopt_linear_input_grad(dz.t.data_ptr(), dz.ld, w.t.data_ptr(), w.ld, dt, M, N, K, *dx_args, stream), what)
+        if dw_args:
+            _lib.check(L.dopt_linear_weight_grad(dz.t.data_ptr(), dz.ld, xr.t.data_ptr(), xr.ld, dt, M, N, K8, *dw_args, stream), what)
+    if K8 != K:
+        dw = dw[:, :K].contiguous()
     return dx, dw if weight_grad else None, db
 
 

@@ -511,6 +511,10 @@ int dopt_linear_layout(const dopt_linear_rows* rows, int n, int dtype, void* str
 int64_t dopt_linear_weight_grad_workspace_floats(int64_t M, int64_t N, int64_t K);
 int dopt_linear_weight_grad(const void* dz, int64_t ldz, const void* x, int64_t ldx, int dtype, int64_t M, int64_t N,
                             int64_t K, float* workspace, float* dw_f32, void* dw_16, float* db, void* db_16, void* stream);
+/* Both of the above, in one launch where that is estimated to be faster (two products that leave much of the GPU idle). */
+int dopt_linear_backward(const void* dz, int64_t ldz, const void* x, int64_t ldx, const void* weight, int64_t ldw, int dtype, int64_t M,
+                         int64_t N, int64_t K, const void* in_pre, int in_act, void* dx, float* workspace, float* dw_f32, void* dw_16,
+                         float* db, void* db_16, void* stream);
 /* Which tile a product gets (an index of the launcher's table; -1: the kernel of at most 16 rows; 100: dopt_dw_gemm_any's
  * kernels; -2: bad arguments); any_rows: an operand's rows lie at any element. */
 int dopt_linear_tile(int product, int64_t M, int64_t N, int64_t K, int any_rows);

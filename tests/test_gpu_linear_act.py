@@ -229,3 +229,15 @@ def test_the_bias_gradient_is_the_sum_before_rounding(M, N, dt):
             ref.close(db, terms.sum(0), (M + 8) * ref.E * terms.abs().sum(0) + ref.ACT_ERR * dy.double().abs().sum(0), act)
             full = ops.linear_act_bwd(dy, x, w, pre, act, None, "none", True, True, True, F32)
             assert torch.equal(full[2], db)
+
+
+@gpu
+@pytest.mark.parametrize("M,K,N", [(1, 8, 8), (9, 117, 128), (33, 64, 64), (70, 200, 72), (197, 384, 384), (394, 768, 768), (985, 384, 1536), (640, 1000, 77),
+                                   (300, 301, 303), (61, 1537, 63)])
+@pytest.mark.parametrize("dt", [BF16, F16], ids=IDS.get)
+def test_small_backward_products_together(M, K, N, dt):
+    """Both products of a small layer go out in one launch: their results, with every epilogue, and in fp32."""
+    for act, in_act in (("none", "none"), ("none", "gelu"), ("relu", "silu")):
+        for grad in (F32, dt):
+            check_bwd(M, K, N, dt, act, in_act, grad)
+    check_bwd(M, K, N, dt, "none", "gelu_tanh", dt, parts=(True, True, False))
