@@ -1413,12 +1413,12 @@ int dopt_linear_backward(const void* dz, int64_t ldz, const void* x, int64_t ldx
     if (int rc = check_weight_grad(dz, ldz, x, ldx, dtype, M, N, K, dw_f32, dw_16, db, db_16)) return rc;
     if (M > 0) {
         const bool whole_x = lin_rows(dz, ldz, N) && lin_rows(weight, ldw, K), whole_w = lin_rows(dz, ldz, N) && lin_rows(x, ldx, K);
-        float one, ux, uw;
+        float one = 0.0f, ux, uw;
         const int tile = dopt::linear_pair(M, N, K, !whole_x, &one);
         dopt::linear_tile(DOPT_LIN_INPUT_GRAD, M, K, N, !whole_x, true, &ux);
         dopt::linear_tile(DOPT_LIN_WEIGHT_GRAD, N, K, M, !whole_w, false, &uw);
         if (whole_w && linear_dw_split(M, N, K)) uw = std::min(uw, linear_dw_split_us(M, N, K));
-        if (whole_x == whole_w && one < ux + uw) {
+        if (tile >= 0 && whole_x == whole_w && one < ux + uw) {
             (void)hipGetLastError();
             dopt::launch_linear_pair(input_grad_args(dz, ldz, weight, ldw, M, N, K, in_pre, in_act, dx),
                                      weight_grad_args(dz, ldz, x, ldx, M, N, K, dw_f32, dw_16, db, db_16), tile, dtype == DOPT_F16,

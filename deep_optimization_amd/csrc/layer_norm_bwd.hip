@@ -209,7 +209,7 @@ __global__ __launch_bounds__(1024) void ln_param_kernel(const float* partial, in
 
 // Widths past this take the parameters' sums in a kernel of their own: the row, its columns' sums and the weight no longer fit
 // the 128 registers that 16 waves a CU leave (3 accesses a lane over 1024 lanes spilled 26). 452 x 15232 in fp16 with a
-// residual: WIDE_US us, through ln_bwd_any_kernel with its sums in memory 85.6.
+// residual: 22 us, through ln_bwd_any_kernel with its sums in memory 85.6.
 constexpr int LNB_MAX_DIM = 8192, LNB_WIDE_DIM = 16384;
 
 // partial rows of ln_col_sum_kernel: some 1024 blocks

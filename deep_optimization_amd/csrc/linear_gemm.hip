@@ -264,7 +264,9 @@ int linear_sum_groups(int64_t rows, int64_t cols) {
     return (int)std::max<int64_t>(1, std::min<int64_t>((rows + 31) / 32, 512 / std::max<int64_t>(strips, 1)));
 }
 
-// The tile (of TILE_COST) that both products of a backward pass take in one launch, and its estimate; M rows, N out, K in.
+// The tile (of TILE_COST) that both products of a backward pass take in one launch, and its estimate; M rows, N out, K in. -1: none
+// holds both products' tiles on the CUs at once. (Past that one launch is slower than two: 4437 rows of 1088 -> 1025 60 us
+// in 1479 tiles, in two launches 50; 985 of 384 -> 1536 in 528 tiles 12.2 against 15.4.)
 int linear_pair(int64_t M, int64_t N, int64_t K, bool reg, float* us) {
     const int n_cu = device_cu_count();
     const float kx = (float)((N + LIN_BK - 1) / LIN_BK), kw = (float)((M + LIN_BK - 1) / LIN_BK);
@@ -273,7 +275,8 @@ int linear_pair(int64_t M, int64_t N, int64_t K, bool reg, float* us) {
         const TileCost& c = TILE_COST[t];
         const auto tiles = [&](int64_t m, int64_t n) { return (float)((m + c.bm - 1) / c.bm) * (float)((n + c.bn - 1) / c.bn); };
         const float tx = tiles(M, K), tw = tiles(N, K), per_cu = std::ceil((tx + tw) / (float)n_cu);
-        const float alone = std::max(kx * c.alone[LIN_KN], kw * c.alone[LIN_TN]) * std::ceil(per_cu / (float)c.slots);
+        if (per_cu > (float)c.slots) continue;
+        const float alone = std::max(kx * c.alone[LIN_KN], kw * c.alone[LIN_TN]);
         const float shared = (tx * kx * c.shared[LIN_KN] + tw * kw * c.shared[LIN_TN]) / (tx + tw) * per_cu;
         const float e = c.start + std::max(alone, shared) + c.epilogue * per_cu;
         if (best < 0 || e < *us) {
