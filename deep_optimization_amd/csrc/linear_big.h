@@ -18,7 +18,8 @@
 //
 // Fragments: lane l of fragment i has row 16 i + l % 16, chunks 2 (l / 16) and + 1 of the slab's 8 (16 elements of K), one
 // chunk for each of two MFMAs; A and B share that order of K. LDS chunk c of row r at c ^ f(r), f(r) = r3 | r1 << 1 |
-// r2 << 2 (rn: bit n of r), which spreads the two chunks that 64 lanes read over all banks. KN as in linear_gemm.h.
+// r2 << 2 (rn: bit n of r), which spreads the two chunks that 64 lanes read over all banks. KN as in linear_gemm.h, with row bit 4 where it has
+// bit 3: 16 lanes' rows lie 16 apart here.
 //
 // Epilogue, from registers: blocks j and j + 1 of a fragment row exchange halves (v_permlane16_swap), after which a lane
 // holds 8 consecutive columns of its row and 16 lanes' rows cover 64 contiguous bytes each; bias, activation and
@@ -81,7 +82,7 @@ __global__ __launch_bounds__(256, 1) void lin_big_kernel(LinArgs p) {
 #pragma unroll
         for (int j = 0; j < LB; ++j) {
             const int k = RPL * (4 * j + wave) + lane / CPR;
-            offb[j] = (uint32_t)(k * ldb + ((lane % CPR) ^ ((k & 3) << 2)) * 8) * 2u;
+            offb[j] = (uint32_t)(k * ldb + ((lane % CPR) ^ (((k & 3) << 2) | (((k >> 4) & 1) << 1))) * 8) * 2u;
         }
     } else {
 #pragma unroll
@@ -177,7 +178,7 @@ __global__ __launch_bounds__(256, 1) void lin_big_kernel(LinArgs p) {
     };
     // KN: source lane 4 u + v of a group of 16 names row 16 (l / 16) + 4 q + u (q = 0..3) and columns 4 v .. + 3
     const int cv = lane & 3, cu = (lane & 15) >> 2;
-    const int crow = (16 * (lane >> 4) + cu) * (2 * BN), csw = cu << 2;
+    const int crow = (16 * (lane >> 4) + cu) * (2 * BN), csw = cu << 2 | ((lane >> 4) & 1) << 1;
     auto read_cols = [&](const uint8_t* s, int base) __attribute__((always_inline)) -> lin_v8i_t {
         const int o = crow + ((((base + 4 * cv) >> 3) ^ csw) << 4) + 8 * (cv & 1);
         lin_v2u_t x[4];

@@ -18,7 +18,8 @@
 // LDS: 16-byte chunk c of row r lies at c ^ ((r / 2) % 8): the 16 rows that 16 lanes read at once fall into the 16
 // different bank groups of two 128-byte rows. [K] rows lie in LDS as they are in memory, 64 rows of BN (BM) columns, and
 // ds_read_b64_tr_b16 hands 16 lanes a 4 x 16 block by columns (two make a fragment); chunk c of row r at
-// c ^ (4 (r % 4)) (64 columns: c ^ (4 ((r / 2) % 2))), which puts those 4 rows on different banks.
+// c ^ (4 (r % 4)) ^ (2 ((r / 8) % 2)) (64 columns: c ^ (4 ((r / 2) % 2)) ^ ..): the first puts those 4 rows on different
+// banks, the second those of the next 16 lanes, 8 rows on, which the hardware serves together with them.
 //
 // The MFMA takes B's fragment first, so lane l holds row 16 i + l % 16 and columns 16 j + 4 (l / 16) + {0..3} of
 // block (i, j).
@@ -108,7 +109,7 @@ __device__ __forceinline__ void lin_cut8(uint8_t* p, int have) { *(lin_v4u_t*)p 
 // position of chunk c of row r of an operand slab that lies in LDS as 64 rows of W columns
 template <int W>
 __device__ __forceinline__ int lin_col_swizzle(int r) {
-    return W == 32 ? 0 : W == 64 ? ((r >> 1) & 1) << 2 : (r & 3) << 2;
+    return (W == 32 ? 0 : W == 64 ? ((r >> 1) & 1) << 2 : (r & 3) << 2) ^ ((r >> 3) & 1) << 1;
 }
 
 template <int BM, int BN, int S, int KIND, bool F16, bool REG, bool TAIL>
