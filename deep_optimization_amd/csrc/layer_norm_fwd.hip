@@ -6,6 +6,9 @@
 // accesses of 4 elements each; the lanes of a launch keep their columns' weight and bias in registers over all the
 // rows they take. Rows of other widths (under 4, over 16384) go through ln_fwd_any_kernel, which reads
 // x three times, the second and third time mostly from the caches.
+//
+// Bound by memory: 25216 x 768 in bf16 13.8 us, 5.6 TB/s (part of it from the cache behind the L2s; a copy of 2 GiB runs
+// at 5.0). One row is bound by its launch: 2.3 us in the kernel, 6.2 the whole call.
 #include <algorithm>
 
 #include "layer_norm.h"

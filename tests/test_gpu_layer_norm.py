@@ -61,6 +61,14 @@ def test_every_pair_of_types(x_dt, y_dt, dim):
         _check((19, dim), x_dt, y_dt, p_dt, dim + 1)
 
 
+@pytest.mark.parametrize("x_dt", [F32, F16, BF16], ids=["xf32", "xf16", "xbf16"])
+@pytest.mark.parametrize("y_dt", [F32, F16, BF16], ids=["yf32", "yf16", "ybf16"])
+def test_every_pair_of_types_of_the_widest_rows_in_registers(x_dt, y_dt):
+    """The backward pass without the parameters' sums, and those in a kernel of their own: more rows than its blocks take at once."""
+    _check((19, 16000), x_dt, y_dt, BF16, 3)
+    _check((700, 9001), x_dt, y_dt, F32, 4, dres=False)
+
+
 @pytest.mark.parametrize("rows", [1, 2, 15, 16, 17, 4095, 4096, 4097, 20001])
 @pytest.mark.parametrize("dim", [64, 768, 1100])
 def test_rows(rows, dim):
@@ -190,3 +198,23 @@ def test_refusals():
                  lambda: ops.layer_norm_bwd(x, x, m, m, None, x.half(), False, False)):
         with pytest.raises(RuntimeError):
             call()
+
+
+def test_past_32_bit_element_offsets():
+    """More than 2^31 elements: the last rows, and parameter gradients to which only the last row gives."""
+    rows, dim = 2_800_001, 768
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.ones((rows, dim), device=DEV, dtype=BF16)
+    x[-5:] = _rand(gen, (5, dim), BF16)
+    y, mean, rstd = ops.layer_norm_fwd(x, None, None, 1e-5, BF16)
+    wy, _, _, tol, _, _ = ref.layer_norm(x[-5:], None, None, 1e-5)
+    ref.close(y[-5:], wy, tol, "y")
+    assert not y[:-5].any() and (mean[:-5] == 1).all()
+    dy = torch.zeros((rows, dim), device=DEV, dtype=BF16)
+    dy[-1] = _rand(gen, (dim,), BF16)
+    dx, dw, db = ops.layer_norm_bwd(dy, x, mean, rstd, None, None, True, True)
+    wx, ww, wb, tx, tw, tb = ref.layer_norm_grads(dy[-1:], x[-1:], mean[-1:], rstd[-1:], None, None)
+    ref.close(dx[-1:], wx, tx, "dx")
+    ref.close(dw, ww, tw, "dweight")
+    ref.close(db, wb, tb, "dbias")
+    assert not dx[:-1].any()

@@ -241,3 +241,72 @@ def test_small_backward_products_together(M, K, N, dt):
         for grad in (F32, dt):
             check_bwd(M, K, N, dt, act, in_act, grad)
     check_bwd(M, K, N, dt, "none", "gelu_tanh", dt, parts=(True, True, False))
+
+
+# sizes (M rows, columns of the result, terms of the sum) that take the persistent 160- and 256-high tiles (5 and 6 of the launchers'
+# table) whatever their epilogue: a tile for each CU, a remainder of 8 terms; and two tiles and whole slabs
+LARGE = {5: [(2624, 3592, 264), (5264, 1544, 264)], 6: [(4736, 2824, 264), (6144, 4096, 512)]}
+
+
+@gpu
+@pytest.mark.parametrize("tile", sorted(LARGE))
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dt", [BF16, F16], ids=IDS.get)
+def test_large_tiles(tile, act, dt):
+    from deep_optimization_amd import _lib
+
+    taken = []
+    for M, N, K in LARGE[tile]:
+        taken += [_lib.lib().dopt_linear_tile(0, M, N, K, 0), _lib.lib().dopt_linear_tile(1, M, K, N, 0)]
+        check_fwd(M, K, N, dt, act, bias=dt, pre=True, res=dt)
+        check_fwd(M, K, N, dt, act, bias=F32)
+        check_bwd(M, N, K, dt, "none", act, parts=(True, False, False))
+    assert taken.count(tile) >= 2, taken
+
+
+@gpu
+@pytest.mark.parametrize("dt", [BF16, F16], ids=IDS.get)
+def test_the_128_high_tiles_with_a_remainder(dt):
+    check_fwd(1000, 776, 1032, dt, bias=None)
+
+
+@gpu
+@pytest.mark.parametrize("dt", [BF16, F16], ids=IDS.get)
+def test_large_tiles_cut_rows_that_end_inside_a_chunk(dt):
+    """Rows of 261 (and 515) in a pitch of whole chunks, NaN in what lies between them."""
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    for M, N, K in ((2624, 3592, 261), (4736, 2824, 261), (6144, 4096, 515), (300, 200, 77), (1000, 1032, 773), (40, 64, 13)):
+        pitch = (K + 7) // 8 * 8
+        x, w = _rand(gen, (M, pitch), dt), _rand(gen, (N, pitch), dt, K ** -0.5)
+        x[:, K:], w[:, K:] = float("nan"), float("nan")
+        check_fwd(M, K, N, dt, "none", bias=None, x=x[:, :K], weight=w[:, :K])
+        dy = _rand(gen, (M, pitch), dt)
+        dy[:, K:] = float("nan")
+        check_bwd(M, N, K, dt, parts=(True, False, False), dy=dy[:, :K])
+
+
+@gpu
+def test_past_32_bit_element_offsets():
+    """x and dx of more than 2^31 elements: the last rows' results, and a weight gradient to which only the last row gives."""
+    M, K, N = 2_800_001, 768, 64
+    gen = torch.Generator(device=DEV).manual_seed(9)
+    x = torch.zeros((M, K), device=DEV, dtype=BF16)
+    x[-300:] = _rand(gen, (300, K), BF16)
+    w, dy = _rand(gen, (N, K), BF16, K ** -0.5), _rand(gen, (M, N), BF16)
+    y, pre = ops.linear_act_fwd(x, w, None, None, "gelu", True)
+    wy, wz, ty, tz = ref.linear_fwd(x[-300:], w, None, None, "gelu")
+    ref.close(y[-300:], wy, ty, "y")
+    ref.close(pre[-300:], wz, tz, "pre")
+    assert not y[:-300].any()
+    x[:-1] = 0
+    dx, dw, db = ops.linear_act_bwd(dy, x, w, None, "none", x, "relu", True, True, True, F32)
+    rows = dy[-300:].double() @ w.double()
+    assert not dx[:-1].any()
+    ref.close(dx[-1:], rows[-1:] * (x[-1:] > 0), (N + 8) * ref.E * (dy[-1:].double().abs() @ w.double().abs()), "dx")
+    ref.close(dw, dy[-1:].double().t() @ x[-1:].double(), 0.0, "dweight")
+    ref.close(db, dy.double().sum(0), (M + 8) * ref.E * dy.double().abs().sum(0), "dbias")
+    del x, dx
+    dz = ops.linear_act_bwd(torch.ones((M, K), device=DEV, dtype=BF16), torch.zeros((M, 8), device=DEV, dtype=BF16),
+                            torch.zeros((K, 8), device=DEV, dtype=BF16), torch.ones((M, K), device=DEV, dtype=BF16), "relu", None, "none",
+                            False, False, True, F32)[2]
+    assert (dz == M).all()  # (sums of ones, exact in fp32)
