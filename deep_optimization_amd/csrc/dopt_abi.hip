@@ -1125,7 +1125,8 @@ int dopt_layer_norm_forward(const void* x, int x_dtype, int64_t rows, int64_t di
 
 int64_t dopt_layer_norm_workspace_floats(int64_t rows, int64_t dim) {
     if (rows < 0 || dim < 1 || dim >= ((int64_t)1 << 30)) return 0;
-    return dopt::layer_norm_groups(rows, (int)dim) * 2 * dim;
+    const int64_t groups = dopt::layer_norm_groups(rows, (int)dim);
+    return groups == 1 && dim >= 4 ? 0 : groups * 2 * dim;
 }
 
 int dopt_layer_norm_backward(const void* dy, int dy_dtype, const void* x, int x_dtype, int64_t rows, int64_t dim,
@@ -1133,10 +1134,11 @@ int dopt_layer_norm_backward(const void* dy, int dy_dtype, const void* x, int x_
                              const void* dresidual, void* dx, float* workspace, float* dweight, float* dbias, void* stream) {
     if (int rc = check_layer_norm(rows, dim, x_dtype, dy_dtype, weight, param_dtype)) return rc;
     if (rows > 0 && (!dy || !x || !mean || !rstd || !dx)) return fail(DOPT_EINVAL, "null dy/x/mean/rstd/dx pointer");
-    if ((dweight || dbias) && rows > 0 && !workspace) return fail(DOPT_EINVAL, "the parameter gradients need a workspace");
-    const dopt::LnBwdArgs a{dy, x, mean, rstd, weight, dresidual, dx, dweight || dbias ? workspace : nullptr, rows, (int)dim, param_dtype};
+    if ((dweight || dbias) && !workspace && dopt_layer_norm_workspace_floats(rows, dim) > 0)
+        return fail(DOPT_EINVAL, "the parameter gradients need a workspace");
+    const dopt::LnBwdArgs a{dy, x, mean, rstd, weight, dresidual, dx, workspace, dweight, dbias, rows, (int)dim, param_dtype};
     (void)hipGetLastError();
-    dopt::launch_layer_norm_bwd(a, x_dtype, dy_dtype, dweight, dbias, (hipStream_t)stream);
+    dopt::launch_layer_norm_bwd(a, x_dtype, dy_dtype, (hipStream_t)stream);
     return hip_status("layer_norm_backward launch");
 }
 

@@ -26,16 +26,17 @@ struct LnBwdArgs {
     const void* weight;  // may be null
     const void* dres;    // of x's dtype, may be null
     void* dx;            // of x's dtype
-    float* partial;      // [groups][2][dim]; null: no parameter gradients
+    float* partial;      // [groups][2][dim] where those are not 1
+    float *dweight, *dbias;  // may be null
     int64_t rows;
     int dim;
     int param_dt;
 };
 
 int launch_layer_norm_fwd(const LnFwdArgs& a, int x_dt, hipStream_t s);
-// workgroups of the backward pass: the rows of its partial sums
+// rows of partial sums that the backward pass joins; 1: its kernels write the sums themselves
 int64_t layer_norm_groups(int64_t rows, int dim);
-int launch_layer_norm_bwd(const LnBwdArgs& a, int x_dt, int dy_dt, float* dweight, float* dbias, hipStream_t s);
+int launch_layer_norm_bwd(const LnBwdArgs& a, int x_dt, int dy_dt, hipStream_t s);
 
 // ------------------------------------------------------------------------------------------ device
 // How a row lies on its lanes: access a of lane t holds the 4 elements from 4 (a TPR + t) on. The access that
@@ -131,13 +132,30 @@ __device__ __forceinline__ float wave_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// The sums over the TPR lanes of a row of NV values. TPR = 64: one wave. Larger: the row's waves meet in
+// v + the lane's that CTRL names
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
+}
+
+// The sums over the TPR lanes of a row of NV values. TPR = 16 or 32: 4 or 2 rows a wave. TPR = 64: one wave. Larger: the row's waves meet in
 // LDS (`red`: NV floats for each wave of the workgroup) and each lane adds the wave sums in order. Two barriers, so
 // that a following call may write `red` again: every wave of the workgroup takes part.
 template <int TPR, int NV>
 __device__ __forceinline__ void row_sums(float* v, float* red) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) v[k] = wave_sum(v[k]);
+    for (int k = 0; k < NV; ++k) {
+        if constexpr (TPR >= 64) {
+            v[k] = wave_sum(v[k]);
+        } else {
+            // lanes 1 and 2 apart, the other half of 8, of 16, of 32
+            v[k] = add_dpp<0xB1>(v[k]);
+            v[k] = add_dpp<0x4E>(v[k]);
+            v[k] = add_dpp<0x141>(v[k]);
+            v[k] = add_dpp<0x140>(v[k]);
+            if constexpr (TPR == 32) v[k] += __shfl_xor(v[k], 16);
+        }
+    }
     if constexpr (TPR > 64) {
         constexpr int W = TPR / 64;
         const int wave = threadIdx.x / 64;

@@ -11,7 +11,8 @@
 // Bound by memory: 25216 x 768 in bf16 with a residual 31.7 us, 4.9 TB/s, the rate of a large copy, and 4.7 in
 // ln_param_kernel (1.6 MB of partial rows; latency). 6304 x 591 in fp32 12.3 + 4.0 us, 3.6 TB/s: a wave takes one or two rows
 // there, one after the other; reading the next row ahead needs more than the 128 registers that 16 waves leave (41
-// spilled). Sizes of a few rows are bound by the two launches (11 us a call).
+// spilled). 302592 x 64 in bf16 26.7 us (4.4 TB/s), with a whole wave
+// a row 67. A few hundred rows are bound by the two launches (10-11 us a call).
 #include <algorithm>
 
 #include "layer_norm.h"
@@ -86,7 +87,7 @@ __global__ __launch_bounds__(LNB_THREADS) void ln_bwd_kernel(LnBwdArgs p) {
         }
     }
     if constexpr (!PARAMS) return;
-    if (!p.partial) return;
+    if (!p.dweight && !p.dbias) return;
     // the RPW lanes of equal columns, by halves
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
@@ -113,7 +114,8 @@ __global__ __launch_bounds__(LNB_THREADS) void ln_bwd_kernel(LnBwdArgs p) {
             }
         }
         if (sub == 0) {
-            float* out = p.partial + ((int64_t)blockIdx.x * 2 + part) * dim;
+            float* out = gridDim.x == 1 ? (part ? p.dbias : p.dweight) : p.partial + ((int64_t)blockIdx.x * 2 + part) * dim;
+            if (!out) continue;
 #pragma unroll
             for (int a = 0; a < ACC; ++a)
 #pragma unroll
@@ -148,7 +150,8 @@ __global__ __launch_bounds__(256) void ln_col_sum_kernel(LnBwdArgs p, int groups
     *(float4*)&meet[wave][1][lane * 4] = make_float4(db[0], db[1], db[2], db[3]);
     __syncthreads();
     if (wave < 2) {  // a wave for each of the two
-        float* out = p.partial + ((int64_t)group * 2 + wave) * dim;
+        float* out = groups == 1 ? (wave ? p.dbias : p.dweight) : p.partial + ((int64_t)group * 2 + wave) * dim;
+        if (!out) return;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             float sum = meet[0][wave][lane * 4 + e];
@@ -217,18 +220,25 @@ __global__ __launch_bounds__(1024) void ln_param_kernel(const float* partial, in
 // residual: 22 us, through ln_bwd_any_kernel with its sums in memory 85.6.
 constexpr int LNB_MAX_DIM = 8192, LNB_WIDE_DIM = 16384;
 
+// Few rows stay in one workgroup, which then writes the parameters' gradients: up to 4 rounds of it take less than a second
+// launch does (8 x 256 in bf16 6.3 us a call, in two launches 10.3).
+constexpr int LNB_ROUNDS = 4;
+
 // partial rows of ln_col_sum_kernel: some 1024 blocks
 int wide_groups(int64_t rows, int dim) {
+    if (rows <= 4 * LNB_ROUNDS) return 1;
     return (int)std::max<int64_t>(1, std::min<int64_t>((rows + 3) / 4, 1024 / ((dim + 255) / 256)));
 }
 
-int rows_at_a_time(int dim) { return dim < 4 ? 1 : dim <= 768 ? 16 : dim <= 3072 ? 4 : 1; }
+int rows_at_a_time(int dim) { return dim < 4 ? 1 : dim <= 64 ? 64 : dim <= 128 ? 32 : dim <= 768 ? 16 : dim <= 3072 ? 4 : 1; }
 
 template <int DTX, int DTY>
 void pick(const LnBwdArgs& a, int64_t groups, hipStream_t s) {
     const int d = a.dim;
     const dim3 g((uint32_t)groups), b(LNB_THREADS);
-    if (d <= 256) hipLaunchKernelGGL((ln_bwd_kernel<DTX, DTY, 64, 1>), g, b, 0, s, a);
+    if (d <= 64) hipLaunchKernelGGL((ln_bwd_kernel<DTX, DTY, 16, 1>), g, b, 0, s, a);
+    else if (d <= 128) hipLaunchKernelGGL((ln_bwd_kernel<DTX, DTY, 32, 1>), g, b, 0, s, a);
+    else if (d <= 256) hipLaunchKernelGGL((ln_bwd_kernel<DTX, DTY, 64, 1>), g, b, 0, s, a);
     else if (d <= 512) hipLaunchKernelGGL((ln_bwd_kernel<DTX, DTY, 64, 2>), g, b, 0, s, a);
     else if (d <= 768) hipLaunchKernelGGL((ln_bwd_kernel<DTX, DTY, 64, 3>), g, b, 0, s, a);
     else if (d <= 1024) hipLaunchKernelGGL((ln_bwd_kernel<DTX, DTY, 256, 1>), g, b, 0, s, a);
@@ -240,7 +250,7 @@ void pick(const LnBwdArgs& a, int64_t groups, hipStream_t s) {
         const dim3 rows((uint32_t)std::min<int64_t>(a.rows, 2 * LNB_GROUPS));
         if (d <= 12288) hipLaunchKernelGGL((ln_bwd_kernel<DTX, DTY, 1024, 3, false>), rows, b, 0, s, a);
         else if (d <= LNB_WIDE_DIM) hipLaunchKernelGGL((ln_bwd_kernel<DTX, DTY, 1024, 4, false>), rows, b, 0, s, a);
-        if (a.partial) hipLaunchKernelGGL((ln_col_sum_kernel<DTX, DTY>), dim3((uint32_t)(groups * ((d + 255) / 256))), dim3(256), 0, s, a, (int)groups);
+        if (a.dweight || a.dbias) hipLaunchKernelGGL((ln_col_sum_kernel<DTX, DTY>), dim3((uint32_t)(groups * ((d + 255) / 256))), dim3(256), 0, s, a, (int)groups);
     }
 }
 
@@ -256,15 +266,16 @@ void pick_dy(const LnBwdArgs& a, int dy_dt, int64_t groups, hipStream_t s) {
 int64_t layer_norm_groups(int64_t rows, int dim) {
     if (dim > LNB_MAX_DIM) return rows > 0 ? wide_groups(rows, dim) : 0;
     const int64_t r = rows_at_a_time(dim);
+    if (dim >= 4 && rows > 0 && rows <= r * LNB_ROUNDS) return 1;
     return std::min<int64_t>((rows + r - 1) / r, LNB_GROUPS);
 }
 
-int launch_layer_norm_bwd(const LnBwdArgs& a, int x_dt, int dy_dt, float* dweight, float* dbias, hipStream_t s) {
+int launch_layer_norm_bwd(const LnBwdArgs& a, int x_dt, int dy_dt, hipStream_t s) {
     const int64_t groups = layer_norm_groups(a.rows, a.dim);
     if (groups > 0) {
         if (a.dim < 4 || a.dim > LNB_WIDE_DIM) {
             LnBwdArgs any = a;
-            if (a.dim >= 4) any.partial = nullptr;
+            if (a.dim >= 4 || !(a.dweight || a.dbias)) any.partial = nullptr;
             const int64_t grid = a.dim < 4 ? groups : std::min<int64_t>(a.rows, 2 * LNB_GROUPS);
             hipLaunchKernelGGL(ln_bwd_any_kernel, dim3((uint32_t)grid), dim3(LNB_THREADS), 0, s, any, x_dt, dy_dt);
         }
@@ -274,9 +285,9 @@ int launch_layer_norm_bwd(const LnBwdArgs& a, int x_dt, int dy_dt, float* dweigh
             else pick_dy<DT_BF16>(a, dy_dt, groups, s);
         }
     }
-    if (dweight || dbias)  // (no rows: zeros)
+    if ((a.dweight || a.dbias) && !(groups == 1 && a.dim >= 4))  // (no rows: zeros)
         hipLaunchKernelGGL(ln_param_kernel, dim3((uint32_t)((2 * (int64_t)a.dim + 63) / 64)), dim3(1024), 0, s, a.partial,
-                           (int)groups, a.dim, dweight, dbias);
+                           (int)groups, a.dim, a.dweight, a.dbias);
     return 0;
 }
 

@@ -2,13 +2,14 @@
 //
 // A row's elements stay in registers: one read of x, the mean, then the squares of the differences from it (two
 // sums one after the other; E[x^2] - mean^2 would lose the variance of a row whose mean is large), one write of y.
-// All in fp32. TPR lanes hold a row (one wave up to 1024 elements, then 4 and 16 waves up to 4096 and 16384), ACC
+// All in fp32. TPR lanes hold a row (16 and 32 up to 64 and 128 elements, one wave up to 1024, then 4 and 16 waves up to 4096 and 16384), ACC
 // accesses of 4 elements each; the lanes of a launch keep their columns' weight and bias in registers over all the
 // rows they take. Rows of other widths (under 4, over 16384) go through ln_fwd_any_kernel, which reads
 // x three times, the second and third time mostly from the caches.
 //
 // Bound by memory: 25216 x 768 in bf16 13.8 us, 5.6 TB/s (part of it from the cache behind the L2s; a copy of 2 GiB runs
-// at 5.0). One row is bound by its launch: 2.3 us in the kernel, 6.2 the whole call.
+// at 5.0). 302592 x 64 18.4 us, 4.2 TB/s, with a whole wave a row 56.5. One row is bound by its launch: 2.3 us in the kernel, 6.2
+// the whole call.
 #include <algorithm>
 
 #include "layer_norm.h"
@@ -128,7 +129,9 @@ void launch(const LnFwdArgs& a, hipStream_t s) {
 template <int DTX>
 void pick(const LnFwdArgs& a, hipStream_t s) {
     const int d = a.dim;
-    if (d <= 256) launch<DTX, 64, 1>(a, s);
+    if (d <= 64) launch<DTX, 16, 1>(a, s);
+    else if (d <= 128) launch<DTX, 32, 1>(a, s);
+    else if (d <= 256) launch<DTX, 64, 1>(a, s);
     else if (d <= 512) launch<DTX, 64, 2>(a, s);
     else if (d <= 768) launch<DTX, 64, 3>(a, s);
     else if (d <= 1024) launch<DTX, 64, 4>(a, s);

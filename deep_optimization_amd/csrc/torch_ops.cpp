@@ -766,7 +766,7 @@ std::tuple<Tensor, std::optional<Tensor>, std::optional<Tensor>> layer_norm_bwd(
     Tensor ws;
     if (weight_grad) dw = fresh({D}, at::kFloat, x);
     if (bias_grad) db = fresh({D}, at::kFloat, x);
-    if (dw || db) ws = fresh({std::max<int64_t>(dopt_layer_norm_workspace_floats(rows, D), 1)}, at::kFloat, x);
+    if (const int64_t floats = dw || db ? dopt_layer_norm_workspace_floats(rows, D) : 0) ws = fresh({floats}, at::kFloat, x);
     check(dopt_layer_norm_backward(dy.data_ptr(), dtype_code(dy.scalar_type(), "layer_norm_bwd"), x.data_ptr(),
                                    dtype_code(x.scalar_type(), "layer_norm_bwd"), rows, D, mean.data_ptr<float>(), rstd.data_ptr<float>(),
                                    ptr(w), code, ptr(dr), dx.data_ptr(), ws.defined() ? ws.data_ptr<float>() : nullptr,

@@ -89,9 +89,8 @@ def _layer_norm_bwd(dy: Tensor, x: Tensor, mean: Tensor, rstd: Tensor, weight: O
     dx = torch.empty_like(x)
     dw = torch.empty(D, dtype=torch.float32, device=x.device) if weight_grad else None
     db = torch.empty(D, dtype=torch.float32, device=x.device) if bias_grad else None
-    ws = None
-    if weight_grad or bias_grad:
-        ws = torch.empty(max(int(L.dopt_layer_norm_workspace_floats(rows, D)), 1), dtype=torch.float32, device=x.device)
+    floats = int(L.dopt_layer_norm_workspace_floats(rows, D)) if weight_grad or bias_grad else 0
+    ws = torch.empty(floats, dtype=torch.float32, device=x.device) if floats else None
     rc = L.dopt_layer_norm_backward(dy.data_ptr(), _DTYPE_CODE[dy.dtype], x.data_ptr(), _DTYPE_CODE[x.dtype], rows, D,
                                     mean.data_ptr(), rstd.data_ptr(), _ptr(weight), code, _ptr(dresidual), dx.data_ptr(),
                                     _ptr(ws), _ptr(dw), _ptr(db), _stream(x))

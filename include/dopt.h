@@ -447,7 +447,7 @@ int dopt_dw_gemm_any(const void* dy, int64_t ldd, const void* x_hat, int64_t ldx
  * Backward, with xh = (x - mean) * rstd and g = dy * weight:
  *   dx = rstd * (g - avg(g) - xh * avg(g * xh)) + dresidual,  dweight = sum dy * xh,  dbias = sum dy (over rows)
  * dx and dresidual (NULL: none) are of x's type, dweight and dbias (fp32 [dim], either may be NULL) come from partial
- * sums in `workspace` (dopt_layer_norm_workspace_floats floats; may be NULL without them) in a fixed order. */
+ * sums in `workspace` (dopt_layer_norm_workspace_floats floats; may be NULL where that is 0 or without them) in a fixed order. */
 int dopt_layer_norm_forward(const void* x, int x_dtype, int64_t rows, int64_t dim, const void* weight, const void* bias,
                             int param_dtype, float eps, void* y, int y_dtype, float* mean, float* rstd, void* stream);
 int64_t dopt_layer_norm_workspace_floats(int64_t rows, int64_t dim);

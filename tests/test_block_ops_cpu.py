@@ -59,7 +59,7 @@ def test_c_entries_refuse_before_any_launch():
     for k in (dict(x=None), dict(xd=I8), dict(rows=-1), dict(dim=0), dict(y=None), dict(yd=I8), dict(mean=None), dict(rstd=None), dict(w=AT, pd=I8)):
         _refused(ln(**k))
     lb = lambda **k: L.dopt_layer_norm_backward(*{**dict(dy=AT, dyd=BF, x=AT, xd=BF, rows=2, dim=8, mean=AT, rstd=AT, w=None, pd=FP, res=None, dx=AT, ws=AT, dw=AT, db=AT, s=None), **k}.values())  # noqa: E731
-    for k in (dict(dy=None), dict(dyd=I8), dict(x=None), dict(rows=-1), dict(dim=0), dict(mean=None), dict(dx=None), dict(ws=None)):
+    for k in (dict(dy=None), dict(dyd=I8), dict(x=None), dict(rows=-1), dict(dim=0), dict(mean=None), dict(dx=None), dict(rows=5000, ws=None)):
         _refused(lb(**k))
     dr = lambda **k: L.dopt_dropout(*{**dict(x=AT, xd=BF, res=None, n=8, p=0.5, seed=0, off=0, step=None, y=AT, yd=BF, s=None), **k}.values())  # noqa: E731
     for k in (dict(x=None), dict(xd=I8), dict(n=-1), dict(p=-0.1), dict(p=1.5), dict(p=float("nan")), dict(y=None), dict(yd=I8)):

@@ -200,6 +200,21 @@ def test_refusals():
             call()
 
 
+@pytest.mark.parametrize("x_dt", [F32, F16, BF16], ids=["xf32", "xf16", "xbf16"])
+@pytest.mark.parametrize("y_dt", [F32, F16, BF16], ids=["yf32", "yf16", "ybf16"])
+def test_rows_of_a_part_of_a_wave(x_dt, y_dt):
+    """Several rows a wave: counts around those of a wave, a workgroup and the grid, and one bad row among them."""
+    for rows, dim in ((1, 64), (3, 60), (64, 64), (65, 17), (16385, 64), (16400, 33), (31, 128), (33, 100), (8193, 96)):
+        _check((rows, dim), x_dt, y_dt, BF16, rows + dim)
+    x = torch.randn((67, 48), device=DEV).to(x_dt)
+    clean, _, _ = ops.layer_norm_fwd(x, None, None, 1e-6, y_dt)
+    x[34, 5] = float("nan")
+    y, mean, rstd = ops.layer_norm_fwd(x, None, None, 1e-6, y_dt)
+    dx, _, _ = ops.layer_norm_bwd(torch.ones_like(y), x, mean, rstd, None, None, False, False)
+    rest = [r for r in range(67) if r != 34]
+    assert torch.isnan(y[34]).all() and torch.equal(y[rest], clean[rest]) and torch.isnan(dx[34]).all() and torch.isfinite(dx[rest]).all()
+
+
 def test_past_32_bit_element_offsets():
     """More than 2^31 elements: the last rows, and parameter gradients to which only the last row gives."""
     rows, dim = 2_800_001, 768
