@@ -1,7 +1,7 @@
 """Layers of a pre-norm transformer block on the layer norm, dropout and linear operators (``ln_lib``, ``dropout_lib``,
 ``linear_lib``). No counterparts in the reference, whose transformer models use torch's modules.
 
-Functional forms, differentiable, on the GPU:
+Functional forms on the GPU, differentiable in reverse mode (forward mode raises):
 
     layer_norm(x, weight, bias, eps)                      in the autocast dtype under autocast, else in x's
     layer_norm_residual(x, weight, bias, eps)             (layer_norm(x), x); its backward adds the gradient that reaches x
@@ -21,6 +21,7 @@ from typing import Optional
 import torch
 from torch import Tensor, nn
 from torch.amp import custom_bwd, custom_fwd
+from torch.autograd import forward_ad
 from torch.autograd import Function
 
 from .. import dropout_lib, linear_lib, ln_lib  # noqa: F401  (registers torch.ops.act_lib.*)
@@ -29,8 +30,13 @@ from .ops import _compute_dtype
 _U63 = (1 << 63) - 1
 
 
-def _grad(*tensors: Optional[Tensor]) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def _differentiated(*tensors: Optional[Tensor]) -> bool:
+    """Whether a call on these goes through its autograd Function: one that does not would lose the tangents of forward mode, which
+    ask for no gradient (the Functions refuse them, and functorch's transforms)."""
+    if torch._C._are_functorch_transforms_active():
+        return True
+    grad = torch.is_grad_enabled()
+    return any(t is not None and (grad and t.requires_grad or forward_ad.unpack_dual(t).tangent is not None) for t in tensors)
 
 
 def _to(t: Optional[Tensor], dtype: torch.dtype) -> Optional[Tensor]:
@@ -98,7 +104,7 @@ class _LinearAct(Function):
 
 
 def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, residual: Optional[Tensor] = None, act: str = "none") -> Tensor:
-    if not _grad(x, weight, bias, residual):
+    if not _differentiated(x, weight, bias, residual):
         xc, wc = _product_operands(x, weight)
         return torch.ops.act_lib.linear_act_fwd(xc, wc, bias, residual, act, False)[0]
     return _LinearAct.apply(x, weight, bias, residual, act)
@@ -136,7 +142,7 @@ class _Mlp(Function):
 
 def mlp(x: Tensor, w1: Tensor, b1: Optional[Tensor], w2: Tensor, b2: Optional[Tensor], residual: Optional[Tensor] = None,
         act: str = "gelu") -> Tensor:
-    if not _grad(x, w1, b1, w2, b2, residual):
+    if not _differentiated(x, w1, b1, w2, b2, residual):
         xc, w1c, w2c = _product_operands(x, w1, w2)
         h = torch.ops.act_lib.linear_act_fwd(xc, w1c, b1, None, act, False)[0]
         return torch.ops.act_lib.linear_act_fwd(h, w2c, b2, residual, "none", False)[0]

@@ -1,0 +1,95 @@
+"""The transformer block layers (modules/transformer.py) as autograd and torch.nn see them, on the CPU: stand-in operators, plain
+torch behind the same schemas, take the kernels' place while a test runs."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fw
+
+import deep_optimization_amd  # noqa: F401
+from deep_optimization_amd.modules import transformer as T
+from tests import block_reference as ref
+
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def _layer_norm_fwd(x, weight, bias, eps, out_dtype):
+    y, mean, rstd = ref.layer_norm(x, weight, bias, eps)[:3]
+    return y.to(out_dtype), mean.float(), rstd.float()
+
+
+def _layer_norm_bwd(dy, x, mean, rstd, weight, dresidual, weight_grad, bias_grad):
+    dx, dw, db = ref.layer_norm_grads(dy, x, mean, rstd, weight, dresidual)[:3]
+    return dx.to(x.dtype), dw.float() if weight_grad else None, db.float() if bias_grad else None
+
+
+def _linear_act_fwd(x, weight, bias, residual, act, save_pre):
+    y, z = ref.linear_fwd(x, weight, bias, residual, act)[:2]
+    return y.to(x.dtype if residual is None else residual.dtype), z.to(x.dtype) if save_pre else None
+
+
+def _linear_act_bwd(dy, x, weight, pre, act, in_pre, in_act, input_grad, weight_grad, bias_grad, grad_dtype):
+    dx, dw, db = ref.linear_bwd(dy, x, weight, pre, act, in_pre, in_act)[:3]
+    return (dx.to(x.dtype) if input_grad else None, dw.to(grad_dtype) if weight_grad else None, db.to(grad_dtype) if bias_grad else None)
+
+
+def _dropout(x, p, seed, offset, step):
+    keep = torch.from_numpy(ref.kept(x.numel(), p, seed, offset + (0 if step is None else int(step)))).view(x.shape)
+    return torch.where(keep, x.double() * ref.scale(p), 0.0)
+
+
+def _dropout_add_fwd(x, residual, p, seed, offset, step):
+    y = _dropout(x, p, seed, offset, step)
+    return y.to(x.dtype) if residual is None else (y + residual.double()).to(residual.dtype)
+
+
+def _dropout_bwd(dy, p, seed, offset, step, out_dtype):
+    return _dropout(dy, p, seed, offset, step).to(out_dtype)
+
+
+@pytest.fixture(autouse=True)
+def stand_ins():
+    lib = torch.library.Library("act_lib", "IMPL")
+    for f in (_layer_norm_fwd, _layer_norm_bwd, _linear_act_fwd, _linear_act_bwd, _dropout_add_fwd, _dropout_bwd):
+        def opaque(*args, f=f):  # (as a kernel: autograd sees nothing of what is inside)
+            with torch.no_grad():
+                return f(*(fw.unpack_dual(a).primal if isinstance(a, torch.Tensor) else a for a in args))
+
+        lib.impl(f.__name__[1:], opaque, "CPU")
+    yield
+    lib._destroy()
+
+
+def _rand(seed, *shape, dtype=BF16):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+def _calls():
+    """(name, function of one tensor, its shape) of every differentiable function, in that argument."""
+    w, w1, w2, x = _rand(1, 6, 8), _rand(2, 12, 8), _rand(3, 6, 12), _rand(4, 5, 8)
+    return [("layer_norm", lambda t: T.layer_norm(t, None, None), (5, 8)),
+            ("layer_norm_residual", lambda t: sum(T.layer_norm_residual(t, None, None)), (5, 8)),
+            ("linear_act", lambda t: T.linear_act(t, w, None, None, "gelu"), (5, 8)),
+            ("linear_act weight", lambda t: T.linear_act(x, t, None, None, "none"), (6, 8)),
+            ("linear_act bias", lambda t: T.linear_act(x, w, t, None, "silu"), (6,)),
+            ("linear_act residual", lambda t: T.linear_act(x, w, None, t, "none"), (5, 6)),
+            ("mlp", lambda t: T.mlp(t, w1, None, w2, None, None, "gelu"), (5, 8)),
+            ("mlp weight", lambda t: T.mlp(x, w1, None, t, None, None, "gelu"), (6, 12)),
+            ("dropout_add", lambda t: T.dropout_add(t, t, 0.5, 3), (5, 8))]
+
+
+CALLS = pytest.mark.parametrize("i", range(9), ids=[c[0].replace(" ", "_") for c in _calls()])
+
+
+@CALLS
+def test_forward_mode_raises(i):
+    """No function has a forward-mode derivative: a tangent that reaches one is an error, not a zero."""
+    _, f, shape = _calls()[i]
+    t, d = _rand(7, *shape), _rand(8, *shape)
+    for grad in (True, False):
+        with torch.set_grad_enabled(grad):
+            with fw.dual_level(), pytest.raises((NotImplementedError, RuntimeError)):
+                f(fw.make_dual(t, d))
+            with pytest.raises((NotImplementedError, RuntimeError)):
+                torch.func.jvp(f, (t,), (d,))
+            with pytest.raises((NotImplementedError, RuntimeError)):  # (a tangent of an outer level)
+                torch.func.jvp(lambda v: torch.func.jvp(lambda s: s * f(v).float().sum(), (torch.ones(()),), (torch.ones(()),))[1], (t,), (d,))
+    assert f(t).shape == f(t.clone().requires_grad_()).shape
