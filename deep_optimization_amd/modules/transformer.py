@@ -1,7 +1,7 @@
 """Layers of a pre-norm transformer block on the layer norm, dropout and linear operators (``ln_lib``, ``dropout_lib``,
 ``linear_lib``). No counterparts in the reference, whose transformer models use torch's modules.
 
-Functional forms on the GPU, differentiable in reverse mode (forward mode raises):
+Functional forms on the GPU, differentiable once in reverse mode (forward mode and second derivatives raise):
 
     layer_norm(x, weight, bias, eps)                      in the autocast dtype under autocast, else in x's
     layer_norm_residual(x, weight, bias, eps)             (layer_norm(x), x); its backward adds the gradient that reaches x
@@ -16,6 +16,7 @@ every pass of a model its own masks). Products run in bf16 or fp16: of that type
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
@@ -37,6 +38,25 @@ def _differentiated(*tensors: Optional[Tensor]) -> bool:
         return True
     grad = torch.is_grad_enabled()
     return any(t is not None and (grad and t.requires_grad or forward_ad.unpack_dual(t).tangent is not None) for t in tensors)
+
+
+def _first_order(backward):
+    """For the backward of a Function: the operators that compute it have no derivatives, so a graph of it (create_graph) is refused, as
+    is a tangent that comes in. Not an error that waits until the results are differentiated, as torch's once_differentiable: a
+    search for some tensors' gradients would pass that by, and add nothing."""
+    @functools.wraps(backward)
+    def guarded(ctx, *grads):
+        if any(g is not None and forward_ad.unpack_dual(g).tangent is not None for g in grads):
+            raise NotImplementedError("the transformer layers' gradients have no forward-mode derivatives")
+        if not torch.is_grad_enabled():
+            return backward(ctx, *grads)
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if any(g is not None and not any(g is d for d in grads) for g in out):  # (an incoming one that is handed on has its own graph)
+            raise RuntimeError("the transformer layers' gradients cannot be differentiated again (create_graph=True)")
+        return out
+
+    return guarded
 
 
 def _to(t: Optional[Tensor], dtype: torch.dtype) -> Optional[Tensor]:
@@ -65,6 +85,7 @@ class _LayerNorm(Function):
 
     @staticmethod
     @custom_bwd(device_type="cuda")
+    @_first_order
     def backward(ctx, dy, dresidual=None):
         x, mean, rstd, weight = ctx.saved_tensors
         _, need_w, need_b, _, _ = ctx.needs_input_grad
@@ -95,6 +116,7 @@ class _LinearAct(Function):
 
     @staticmethod
     @custom_bwd(device_type="cuda")
+    @_first_order
     def backward(ctx, dy):
         x, weight, pre = ctx.saved_tensors
         need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
@@ -125,6 +147,7 @@ class _Mlp(Function):
 
     @staticmethod
     @custom_bwd(device_type="cuda")
+    @_first_order
     def backward(ctx, dy):
         x, w1, w2, h, pre = ctx.saved_tensors
         need_x, need_w1, need_b1, need_w2, need_b2, need_r, _ = ctx.needs_input_grad
@@ -157,6 +180,7 @@ class _DropoutAdd(Function):
         return torch.ops.act_lib.dropout_add_fwd(x, residual, p, seed, offset, step)
 
     @staticmethod
+    @_first_order
     def backward(ctx, dy):
         (step,) = ctx.saved_tensors
         need_x, need_r = ctx.needs_input_grad[:2]

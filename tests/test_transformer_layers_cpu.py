@@ -93,3 +93,30 @@ def test_forward_mode_raises(i):
             with pytest.raises((NotImplementedError, RuntimeError)):  # (a tangent of an outer level)
                 torch.func.jvp(lambda v: torch.func.jvp(lambda s: s * f(v).float().sum(), (torch.ones(()),), (torch.ones(()),))[1], (t,), (d,))
     assert f(t).shape == f(t.clone().requires_grad_()).shape
+
+
+@CALLS
+@pytest.mark.parametrize("loss", [lambda y: y.float().sum(), lambda y: y.float().pow(2).sum()], ids=["sum", "squares"])
+def test_double_backward_raises(i, loss):
+    """A graph of a gradient is an error, not one whose derivative is zero; a residual's gradient, which is the one that came in, has it."""
+    name, f, shape = _calls()[i]
+    t = _rand(7, *shape).requires_grad_()
+    assert torch.autograd.grad(loss(f(t)), t)[0].shape == t.shape
+    if name == "linear_act residual":
+        g, = torch.autograd.grad(f(t).float().pow(2).sum(), t, create_graph=True)  # 2 y
+        assert torch.equal(torch.autograd.grad(g.float().pow(2).sum(), t)[0], 4 * g)
+        return
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(loss(f(t)), t, create_graph=True)
+    with pytest.raises(RuntimeError):
+        loss(f(t)).backward(create_graph=True)
+
+
+@CALLS
+def test_forward_over_reverse_raises(i):
+    """A tangent of the gradient that comes in is not lost in a backward pass either."""
+    _, f, shape = _calls()[i]
+    t = _rand(7, *shape).requires_grad_()
+    y = f(t)
+    with fw.dual_level(), pytest.raises((NotImplementedError, RuntimeError)):
+        torch.autograd.grad(y, t, fw.make_dual(torch.ones_like(y), torch.ones_like(y)))
