@@ -69,8 +69,10 @@ def _product_operands(x: Tensor, *weights: Tensor):
     return (x.to(dt), *(w.to(dt) for w in weights))
 
 
-def _grad_dtype(param: Tensor, operand: Tensor) -> torch.dtype:
-    return operand.dtype if param.dtype == operand.dtype else torch.float32
+def _grad_dtype(operand: Tensor, *params) -> torch.dtype:
+    """What a product's parameter gradients come in, of (parameter's type, whether it needs one): the operands' type where
+    all that need one have it, else fp32, so that none is rounded to fewer bits than its parameter has."""
+    return operand.dtype if all(dtype == operand.dtype for dtype, need in params if need) else torch.float32
 
 
 class _LayerNorm(Function):
@@ -111,7 +113,6 @@ class _LinearAct(Function):
         y, pre = torch.ops.act_lib.linear_act_fwd(xc, wc, bias, residual, act, act != "none")
         ctx.save_for_backward(xc, wc, pre)
         ctx.act, ctx.x_dtype, ctx.param = act, x.dtype, (weight.dtype, None if bias is None else bias.dtype)
-        ctx.grad_dtype = _grad_dtype(weight, wc)
         return y
 
     @staticmethod
@@ -121,7 +122,7 @@ class _LinearAct(Function):
         x, weight, pre = ctx.saved_tensors
         need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
         dx, dw, db = torch.ops.act_lib.linear_act_bwd(dy.to(x.dtype), x, weight, pre, ctx.act, None, "none", need_x, need_w, need_b,
-                                                      ctx.grad_dtype)
+                                                      _grad_dtype(x, (ctx.param[0], need_w), (ctx.param[1], need_b)))
         return (_to(dx, ctx.x_dtype), _to(dw, ctx.param[0]), _to(db, ctx.param[1]) if need_b else None, dy if need_r else None, None)
 
 
@@ -142,7 +143,6 @@ class _Mlp(Function):
         ctx.save_for_backward(xc, w1c, w2c, h, pre)
         ctx.act, ctx.x_dtype = act, x.dtype
         ctx.param = tuple(None if t is None else t.dtype for t in (w1, b1, w2, b2))
-        ctx.grad_dtypes = _grad_dtype(w1, w1c), _grad_dtype(w2, w2c)
         return y
 
     @staticmethod
@@ -151,14 +151,14 @@ class _Mlp(Function):
     def backward(ctx, dy):
         x, w1, w2, h, pre = ctx.saved_tensors
         need_x, need_w1, need_b1, need_w2, need_b2, need_r, _ = ctx.needs_input_grad
+        t1, u1, t2, u2 = ctx.param
         first = need_x or need_w1 or need_b1
         dz, dw2, db2 = torch.ops.act_lib.linear_act_bwd(dy.to(x.dtype), h, w2, None, "none", pre, ctx.act, first, need_w2, need_b2,
-                                                        ctx.grad_dtypes[1])
+                                                        _grad_dtype(x, (t2, need_w2), (u2, need_b2)))
         dx = dw1 = db1 = None
         if first:
             dx, dw1, db1 = torch.ops.act_lib.linear_act_bwd(dz, x, w1, None, "none", None, "none", need_x, need_w1, need_b1,
-                                                            ctx.grad_dtypes[0])
-        t1, u1, t2, u2 = ctx.param
+                                                            _grad_dtype(x, (t1, need_w1), (u1, need_b1)))
         return (_to(dx, ctx.x_dtype), _to(dw1, t1), _to(db1, u1) if need_b1 else None, _to(dw2, t2), _to(db2, u2) if need_b2 else None,
                 dy if need_r else None, None)
 

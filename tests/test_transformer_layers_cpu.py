@@ -120,3 +120,22 @@ def test_forward_over_reverse_raises(i):
     y = f(t)
     with fw.dual_level(), pytest.raises((NotImplementedError, RuntimeError)):
         torch.autograd.grad(y, t, fw.make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+
+@pytest.mark.parametrize("act", ["none", "gelu"])
+def test_a_32_bit_bias_has_its_gradient_in_32_bits(act):
+    """Beside a 16-bit weight too: the column sums are not rounded to 16 bits on their way (the bound is one rounding to 32 bits)."""
+    x, w, dy = _rand(1, 40, 8), _rand(2, 6, 8).requires_grad_(), _rand(3, 40, 6)
+    b = _rand(4, 6, dtype=F32).requires_grad_()
+    T.linear_act(x, w, b, None, act).backward(dy)
+    pre = _linear_act_fwd(x, w.detach(), b.detach(), None, act, True)[1]
+    want = ref.linear_bwd(dy, x, w.detach(), pre, act, None, "none")
+    ref.close(b.grad, want[2], 0.0, "bias")
+    ref.close(w.grad, want[1], ref.U[F32] * want[1].abs(), "weight")
+    assert b.grad.dtype == F32 and w.grad.dtype == BF16
+    w1, b1, w2, b2 = _rand(5, 12, 8).requires_grad_(), _rand(6, 12, dtype=F32).requires_grad_(), _rand(7, 6, 12), _rand(8, 6, dtype=F32).requires_grad_()
+    T.mlp(x, w1, b1, w2, b2, None, act).backward(dy)
+    ref.close(b2.grad, dy.double().sum(0), 0.0, "second bias")
+    h, pre = _linear_act_fwd(x, w1.detach(), b1.detach(), None, act, True)
+    dz = _linear_act_bwd(dy, h, w2, None, "none", pre if act != "none" else None, act, True, False, False, F32)[0]
+    ref.close(b1.grad, dz.double().sum(0), 0.0, "first bias")
