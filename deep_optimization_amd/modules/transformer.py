@@ -192,6 +192,23 @@ def dropout_add(x: Tensor, residual: Optional[Tensor], p: float, seed: int, offs
     return _DropoutAdd.apply(x, residual, p, seed, offset, step)
 
 
+_HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
+
+
+def _bare(m: nn.Module, cls: type) -> bool:
+    """Whether calling m does what cls.forward does and nothing else, so that a fused call may read its parameters instead: a layer that
+    was replaced, has a forward of its own or hooks (pruning sets the weight in one) is called."""
+    return (isinstance(m, cls) and type(m).forward is cls.forward and "forward" not in vars(m) and not any(getattr(m, h) for h in _HOOKS)
+            and not nn.modules.module._has_any_global_hook())
+
+
+def norm_residual(norm: nn.Module, x: Tensor):
+    """(norm(x), x) for x + f(norm(x)): by layer_norm_residual where norm is a LayerNorm of this module."""
+    if _bare(norm, LayerNorm):
+        return layer_norm_residual(x, norm.weight, norm.bias, norm.eps)
+    return norm(x), x
+
+
 class LayerNorm(nn.LayerNorm):
     """torch.nn.LayerNorm over the last axis. ``residual(x)`` is (norm(x), x) for x + f(norm(x))."""
 
@@ -204,7 +221,7 @@ class LayerNorm(nn.LayerNorm):
         return layer_norm(x, self.weight, self.bias, self.eps)
 
     def residual(self, x):
-        return layer_norm_residual(x, self.weight, self.bias, self.eps)
+        return norm_residual(self, x)
 
 
 class LinearAct(nn.Module):
@@ -289,8 +306,10 @@ class Mlp(nn.Module):
     def forward(self, x, residual=None):
         if self.drop1 is not None and self.training:
             return self.drop2(self.fc2(self.drop1(self.fc1(x))), residual)
+        if not (_bare(self.fc1, LinearAct) and _bare(self.fc2, LinearAct) and self.fc2.act == "none"):
+            return self.fc2(self.fc1(x), residual)
         return mlp(x, self.fc1.weight, self.fc1.bias, self.fc2.weight, self.fc2.bias, residual, self.fc1.act)
 
 
-__all__ = ["layer_norm", "layer_norm_residual", "linear_act", "mlp", "dropout_add", "LayerNorm", "LinearAct", "DropoutRng", "DropoutAdd",
-           "Mlp"]
+__all__ = ["layer_norm", "layer_norm_residual", "linear_act", "mlp", "dropout_add", "norm_residual", "LayerNorm", "LinearAct", "DropoutRng",
+           "DropoutAdd", "Mlp"]

@@ -102,9 +102,9 @@ class FusedBlock(nn.Module):
         self.mlp = transformer.Mlp(dim, int(dim * mlp_ratio), "gelu", drop, rng)
 
     def forward(self, x):
-        h, x = self.norm1.residual(x)
+        h, x = transformer.norm_residual(self.norm1, x)
         x = self.attn(h, x)
-        h, x = self.norm2.residual(x)
+        h, x = transformer.norm_residual(self.norm2, x)
         return self.mlp(h, x)
 
 

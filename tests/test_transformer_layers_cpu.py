@@ -139,3 +139,91 @@ def test_a_32_bit_bias_has_its_gradient_in_32_bits(act):
     h, pre = _linear_act_fwd(x, w1.detach(), b1.detach(), None, act, True)
     dz = _linear_act_bwd(dy, h, w2, None, "none", pre if act != "none" else None, act, True, False, False, F32)[0]
     ref.close(b1.grad, dz.double().sum(0), 0.0, "first bias")
+
+
+def _block(drop=0.0):
+    from deep_optimization_amd.vit import FusedBlock
+
+    torch.manual_seed(0)
+    rng = T.DropoutRng(5) if drop else None
+    return FusedBlock(16, 2, drop=drop, rng=rng).to(BF16), rng
+
+
+@pytest.mark.parametrize("training", [True, False])
+@pytest.mark.parametrize("drop", [0.0, 0.5])
+def test_hooks_of_the_layers_inside_run(drop, training):
+    """Forward, forward-pre and backward hooks of every layer of a block, in each mode, and global ones; the results stay what they are."""
+    block, rng = _block(drop)
+    block.train(training)
+    x = _rand(1, 2, 3, 16)
+
+    def run():
+        if rng is not None:
+            rng.step.zero_()
+            rng.train(training)(x)
+        t = x.clone().requires_grad_()
+        y = block(t)
+        y.backward(torch.ones_like(y))
+        return y.detach(), t.grad
+
+    want = run()
+    layers = {n: m for n, m in block.named_modules() if isinstance(m, (T.LayerNorm, T.LinearAct))}
+    assert set(layers) == {"norm1", "norm2", "attn.qkv", "attn.proj", "mlp.fc1", "mlp.fc2"}
+    for register in ("register_forward_hook", "register_forward_pre_hook", "register_full_backward_hook", "register_full_backward_pre_hook"):
+        seen = []
+        handles = [getattr(m, register)(lambda m, *a, n=n: seen.append(n)) for n, m in layers.items()]
+        got = run()
+        assert sorted(seen) == sorted(layers), (register, seen)
+        for h in handles:
+            h.remove()
+        assert torch.equal(got[0], want[0])
+        ref.close(got[1], want[1], 2.0 ** -6 * want[1].abs().max(), register)  # (where the residual's gradient is added rounds once more)
+    seen = []
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda m, *a: seen.append(m))
+    run()
+    handle.remove()
+    assert all(m in seen for m in layers.values())
+    assert all(torch.equal(a, b) for a, b in zip(run(), want))
+
+
+def test_weights_that_a_pre_hook_computes_are_not_stale():
+    """torch.nn.utils.prune sets the weight in a forward-pre hook: an Mlp follows its optimizer's steps."""
+    from torch.nn.utils import prune
+
+    torch.manual_seed(0)
+    m, x = T.Mlp(8, 16).to(BF16), _rand(1, 5, 8)
+    for layer in (m.fc1, m.fc2):
+        prune.random_unstructured(layer, "weight", amount=0.25)
+    m(x)
+    with torch.no_grad():
+        m.fc1.weight_orig.mul_(2)
+        m.fc2.weight_orig.add_(1)
+    w1, w2 = ((layer.weight_orig * layer.weight_mask).detach() for layer in (m.fc1, m.fc2))
+    h = _linear_act_fwd(x, w1, m.fc1.bias, None, "gelu", False)[0]
+    assert torch.equal(m(x), _linear_act_fwd(h, w2, m.fc2.bias, None, "none", False)[0])
+    m(x).sum().backward()
+    assert m.fc1.weight_orig.grad.any() and m.fc2.weight_orig.grad.any()
+
+
+def test_layers_of_another_kind_inside():
+    """An Mlp's or a block's layers replaced, or with a forward of their own: those run."""
+    class Doubled(T.LinearAct):
+        def forward(self, x, residual=None):
+            return 2 * super().forward(x, residual)
+
+    torch.manual_seed(0)
+    m, x = T.Mlp(8, 16).to(BF16), _rand(1, 5, 8)
+    m.fc1 = Doubled(8, 16, act="gelu").to(BF16)
+    h = 2 * _linear_act_fwd(x, m.fc1.weight, m.fc1.bias, None, "gelu", False)[0]
+    want = _linear_act_fwd(h, m.fc2.weight, m.fc2.bias, None, "none", False)[0]
+    assert torch.equal(m(x), want)
+    patched = m.fc2.forward
+    m.fc2.forward = lambda *a, **k: -patched(*a, **k)
+    assert torch.equal(m(x), -want)
+    block, _ = _block()
+    x = _rand(1, 2, 3, 16)
+    want = block(x)
+    norm = torch.nn.LayerNorm(16, eps=1e-6).to(BF16)
+    norm.load_state_dict(block.norm1.state_dict())
+    block.norm1 = norm
+    ref.close(block(x), want, 2.0 ** -6 * want.abs().max(), "block")
