@@ -245,7 +245,8 @@ class DropoutRng(nn.Module):
     """The masks of a model's dropout layers: a seed, and a count of passes that lies on the device, so that a captured
     step draws new masks on every replay. Call it once at the start of a pass, on the input: it returns that and steps the
     count. Every layer has an offset of its own (``site``). ``step`` is part of the state dict; the seed is not: ranks that
-    train on different data each give their own (default: from torch's initial seed)."""
+    train on different data each give their own (default: from torch's initial seed). One process per GPU: the layers refuse to run
+    in nn.DataParallel's replicas."""
 
     def __init__(self, seed: Optional[int] = None):
         super().__init__()
@@ -281,6 +282,8 @@ class DropoutAdd(nn.Module):
         if not self.training or self.p == 0.0:
             return x if residual is None else residual + x.to(residual.dtype)
         rng = self._rng[0]
+        if getattr(self, "_is_replica", False):
+            raise RuntimeError("DropoutAdd does not run in nn.DataParallel replicas, whose DropoutRng it would not see: use one process per GPU")
         if rng.current is None:
             raise RuntimeError("DropoutAdd: call the model's DropoutRng at the start of the pass")
         return dropout_add(x, residual, self.p, rng.seed, self.offset, rng.current)

@@ -227,3 +227,17 @@ def test_layers_of_another_kind_inside():
     norm.load_state_dict(block.norm1.state_dict())
     block.norm1 = norm
     ref.close(block(x), want, 2.0 ** -6 * want.abs().max(), "block")
+
+
+def test_data_parallel_replicas_are_refused():
+    """A replica of a dropout layer holds the first device's count, which would give it the masks of an earlier pass (or another
+    device's memory to read): it raises, whatever that count is."""
+    rng = T.DropoutRng(5)
+    layer, x = T.DropoutAdd(0.5, rng), _rand(1, 4, 8)
+    rng(x)
+    assert layer(x).shape == x.shape
+    replica = layer._replicate_for_data_parallel()
+    with pytest.raises(RuntimeError, match="DataParallel"):
+        replica(x)
+    replica.eval()
+    assert replica(x) is x
