@@ -76,10 +76,17 @@ def _stream(t: Tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(dev)
 
 
-def _require_cuda(*ts: Tensor) -> None:
+def _require_cuda(*ts: Optional[Tensor]) -> None:
+    """Tensors that a kernel reads together: on the GPU, all on one."""
+    first = None
     for t in ts:
-        if t is not None and t.device.type != "cuda":
+        if t is None:
+            continue
+        if t.device.type != "cuda":
             raise RuntimeError("act_lib operators run on HIP (cuda) tensors only")
+        first = first or t.device
+        if t.device != first:
+            raise RuntimeError(f"act_lib operators take tensors of one device, got {first} and {t.device}")
 
 
 def _aligned(t: Tensor) -> Tensor:

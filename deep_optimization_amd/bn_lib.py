@@ -239,7 +239,7 @@ bn_relu_fwd_norm_fused_quant_pack = _op(
 
 # ------------------------------------------------------------------ backward
 def _bwd_common(mode, DY, M, HW, x_hat=None, packed=None, relu_packed=None, scale=None, xmin=None):
-    _require_cuda(DY)
+    _require_cuda(DY, x_hat, packed, relu_packed, scale, xmin)
     DY3, N, C = _geom(DY, M, HW)
     xh = None if x_hat is None else _geom(x_hat, M, HW)[0].to(torch.bfloat16).contiguous()
     c = lambda t: None if t is None else t.contiguous()  # noqa: E731

@@ -70,6 +70,20 @@ void require_cuda(const Tensor& t) {
     TORCH_CHECK(t.device().is_cuda(), "act_lib operators run on HIP (cuda) tensors only");
 }
 
+const Tensor* given(const Tensor& t) { return &t; }
+const Tensor* given(const std::optional<Tensor>& t) { return t ? &*t : nullptr; }
+
+// tensors (the rest may be optional) that a kernel reads together: on one device, as act_lib._require_cuda
+template <class... Rest>
+void require_cuda(const Tensor& first, const Rest&... rest) {
+    require_cuda(first);
+    for (const Tensor* t : {given(rest)...}) {
+        if (!t) continue;
+        require_cuda(*t);
+        TORCH_CHECK(t->device() == first.device(), "act_lib operators take tensors of one device, got ", first.device(), " and ", t->device());
+    }
+}
+
 // the C ABI launches on the calling thread's current device: where the Python implementation refuses tensors of
 // another device (act_lib._stream) instead of switching to it, so does the native one
 void require_current(const Tensor& t) {
@@ -102,8 +116,7 @@ std::tuple<Tensor, Tensor, Tensor> quant_pack_launch(const Tensor& x_in, int64_t
     const int xc = dtype_code(x_in.scalar_type(), "quant_pack");
     TORCH_CHECK(scale_dtype == ScalarType::Float || scale_dtype == ScalarType::BFloat16,
                 "quant_pack: scale dtype must be float32 or bfloat16, got ", scale_dtype);
-    require_cuda(x_in);
-    if (noise_in) require_cuda(*noise_in);
+    require_cuda(x_in, noise_in);
     const Tensor x = aligned(x_in);
     const auto opts = x.options();
     Tensor packed = at::empty({n_groups, nwords}, opts.dtype(at::kInt));
@@ -197,9 +210,7 @@ Tensor dequant_launch(const Tensor& packed_in, const Tensor& scale_in, const Ten
     TORCH_CHECK(packed_in.numel() * packed_in.element_size() == n_groups * nwords * 4, "dequant_unpack: packed holds ",
                 packed_in.numel() * packed_in.element_size(), " bytes, expected ", n_groups * nwords * 4, " (",
                 n_groups, " groups of ", nwords, " words)");
-    require_cuda(packed_in);
-    require_cuda(scale_in);
-    require_cuda(xmin_in);
+    require_cuda(packed_in, scale_in, xmin_in);
     const Tensor packed = aligned(packed_in), scale = scale_in.contiguous(), xmin = xmin_in.contiguous();
     check(dopt_dequant_unpack((const uint32_t*)packed.data_ptr(), scale.data_ptr(), xmin.data_ptr(),
                               meta_code(scale.scalar_type()), n_groups, (int)group_size, (int)bits, tile,
@@ -284,9 +295,7 @@ Tensor dequant_unpack_triton(const Tensor& packed, const Tensor& scale, const Te
                 "dequant_unpack_triton: avg_alam takes the bf16 scale and min its quantizer writes");
     TORCH_CHECK(packed.numel() == N * G * anw, "dequant_unpack_triton: packed holds ", packed.numel(),
                 " words, expected ", N * G * anw, " (", N * G, " groups of ", anw, ")");
-    require_cuda(packed);
-    require_cuda(scale);
-    require_cuda(xmin);
+    require_cuda(packed, scale, xmin);
     const Tensor p = packed.contiguous(), s = scale.contiguous(), m = xmin.contiguous();
     check(dopt_alam_dequant_unpack((const uint32_t*)p.data_ptr(), (const uint16_t*)s.data_ptr(),
                                    (const uint16_t*)m.data_ptr(), N * G, (int)group_size, (int)bits, (int)alam_bits,
@@ -332,8 +341,7 @@ Tensor relu_bwd_fused_unpack(const Tensor& packed_in, const Tensor& dy_in, int64
     TORCH_CHECK(packed_in.numel() * packed_in.element_size() * 8 >= dy_in.numel() * bits,
                 "relu_bwd_fused_unpack: packed holds ", packed_in.numel() * packed_in.element_size(),
                 " bytes, too few for ", dy_in.numel(), " ", bits, "-bit masks");
-    require_cuda(packed_in);
-    require_cuda(dy_in);
+    require_cuda(packed_in, dy_in);
     const c10::DeviceGuard guard(dy_in.device());
     const Tensor packed = aligned(packed_in), dy = aligned(dy_in);
     Tensor dx = at::empty(dy.sizes(), dy.options().dtype(at::kBFloat16));
@@ -420,10 +428,7 @@ Tensor act_dequant_mul(const Tensor& packed_in, const Tensor& dy_in, const Tenso
     TORCH_CHECK(scale_in.numel() == n_groups && xmin_in.numel() == n_groups &&
                     packed_in.numel() * packed_in.element_size() == n_groups * nwords * 4,
                 "fused activation backward: packed / scale / min do not hold ", n_groups, " groups");
-    require_cuda(packed_in);
-    require_cuda(dy_in);
-    require_cuda(scale_in);
-    require_cuda(xmin_in);
+    require_cuda(packed_in, dy_in, scale_in, xmin_in);
     require_current(dy_in);
     const Tensor packed = aligned(packed_in), dy = aligned(dy_in);
     const Tensor scale = scale_in.contiguous(), xmin = xmin_in.contiguous();
@@ -459,8 +464,7 @@ Tensor silu_bwd_fused_dequan_unpack(const Tensor& packed, const Tensor& dy, cons
 // ---------------------------------------------------------------------------- Linear weight gradient
 std::tuple<Tensor, std::optional<Tensor>> dw_gemm_any(const Tensor& dy_in, const Tensor& x_in, bool bias_grad,
                                                       ScalarType out_dtype) {
-    require_cuda(dy_in);
-    require_cuda(x_in);
+    require_cuda(dy_in, x_in);
     TORCH_CHECK(dy_in.dim() == 2 && x_in.dim() == 2 && dy_in.size(0) == x_in.size(0) &&
                     dy_in.scalar_type() == ScalarType::BFloat16 && x_in.scalar_type() == ScalarType::BFloat16,
                 "dw_gemm_any: dy and x_hat must be bf16 [K, M] and [K, N] matrices, got ", dy_in.sizes(), " ",
@@ -490,8 +494,7 @@ Tensor fp8_gemm_nt(const Tensor& a_in, const Tensor& b_in, double out_scale) {
                 "fp8_gemm_nt expects torch.float8_e4m3fn operands");
     TORCH_CHECK(a_in.dim() == 2 && b_in.dim() == 2 && a_in.size(1) == b_in.size(1), "fp8_gemm_nt: shapes ",
                 a_in.sizes(), " x ", b_in.sizes(), "^T do not contract");
-    require_cuda(a_in);
-    require_cuda(b_in);
+    require_cuda(a_in, b_in);
     require_current(a_in);
     const Tensor a = aligned(a_in), b = aligned(b_in);
     const int64_t M = a.size(0), K = a.size(1), N = b.size(0);
@@ -522,8 +525,7 @@ Tensor fp8_linear(const Tensor& a, const Tensor& b, double out_scale) {
                 "fp8_linear expects torch.float8_e4m3fn operands");
     TORCH_CHECK(a.dim() == 2 && b.dim() == 2 && a.size(1) == b.size(0), "fp8_linear: shapes ", a.sizes(), " x ",
                 b.sizes(), " do not contract");
-    require_cuda(a);
-    require_cuda(b);
+    require_cuda(a, b);
     require_current(a);
     const int64_t M = a.size(0), K = a.size(1), N = b.size(1);
     Tensor c = at::empty({M, N}, a.options().dtype(at::kBFloat16));
@@ -592,11 +594,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> bn_train_fwd(
     words_per_group(bits, g);
     const bool has_rm = running_mean_in.defined() && running_mean_in.numel() > 0;
     const bool has_rv = running_var_in.defined() && running_var_in.numel() > 0;
-    require_cuda(X);
-    require_cuda(weight);
-    require_cuda(bias);
-    if (has_rm) require_cuda(running_mean_in);
-    if (has_rv) require_cuda(running_var_in);
+    require_cuda(X, weight, bias);
+    if (has_rm) require_cuda(X, running_mean_in);
+    if (has_rv) require_cuda(X, running_var_in);
     TORCH_CHECK(X.dim() >= 2 && (X.scalar_type() == ScalarType::Float || X.scalar_type() == ScalarType::Half ||
                                  X.scalar_type() == ScalarType::BFloat16),
                 "bn_train_fwd: X must be an [N, C, ...] float tensor, got ", X.sizes(), " ", X.scalar_type());
@@ -668,7 +668,7 @@ std::tuple<Tensor, Tensor, Tensor> bn_train_bwd(const Tensor& packed_in, const s
     TORCH_CHECK(w.numel() == C && v.numel() == C, "BatchNorm backward: per-channel vectors must hold ", C,
                 " values, got ", w.numel(), " and ", v.numel());
     TORCH_CHECK(m != DOPT_BN_RELU_QUANT || rp.has_value(), "bn_train_bwd: the ReLU kinds need the saved ReLU mask");
-    for (const Tensor* t : {&p, &sc, &mn, &w, &v}) require_cuda(*t);
+    require_cuda(dy, p, sc, mn, w, v, rp);
     Tensor dx = at::empty({N, C, HW}, DY3.options().dtype(at::kBFloat16));
     Tensor dw = at::empty({C}, DY3.options().dtype(at::kFloat));
     Tensor db = at::empty_like(dw);
@@ -716,18 +716,12 @@ Tensor fresh(at::IntArrayRef sizes, ScalarType dtype, const Tensor& like) {
     return at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt);
 }
 
-void require_cuda(const std::optional<Tensor>& t) {
-    if (t) require_cuda(*t);
-}
-
 std::tuple<Tensor, Tensor, Tensor> layer_norm_fwd(const Tensor& x_in, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias,
                                                   double eps, ScalarType out_dtype) {
     const int64_t D = ln_dim("layer_norm_fwd", x_in);
     const int code = ln_params("layer_norm_fwd", D, weight, bias);
     TORCH_CHECK(is_float(out_dtype), "layer_norm_fwd: out_dtype must be float32, float16 or bfloat16, got ", out_dtype);
-    require_cuda(x_in);
-    require_cuda(weight);
-    require_cuda(bias);
+    require_cuda(x_in, weight, bias);
     require_current(x_in);
     const Tensor x = x_in.contiguous();
     const auto w = contiguous(weight), b = contiguous(bias);
@@ -755,9 +749,7 @@ std::tuple<Tensor, std::optional<Tensor>, std::optional<Tensor>> layer_norm_bwd(
                     " must hold ", rows, " float32 values, got ", t->sizes(), " ", t->scalar_type());
     TORCH_CHECK(!dresidual || (dresidual->sizes() == x_in.sizes() && dresidual->scalar_type() == x_in.scalar_type()),
                 "layer_norm_bwd: dresidual must have x's shape and type");
-    for (const Tensor* t : {&dy_in, &x_in, &mean_in, &rstd_in}) require_cuda(*t);
-    require_cuda(weight);
-    require_cuda(dresidual);
+    require_cuda(x_in, dy_in, mean_in, rstd_in, weight, dresidual);
     require_current(x_in);
     const Tensor dy = dy_in.contiguous(), x = x_in.contiguous(), mean = mean_in.contiguous(), rstd = rstd_in.contiguous();
     const auto w = contiguous(weight), dr = contiguous(dresidual);
@@ -782,9 +774,7 @@ Tensor dropout_launch(const char* what, const Tensor& x_in, const std::optional<
     TORCH_CHECK(p >= 0.0 && p <= 1.0, what, ": p must lie in [0, 1], got ", p);
     TORCH_CHECK(!residual || residual->sizes() == x_in.sizes(), what, ": residual must have x's shape ", x_in.sizes());
     TORCH_CHECK(!step || (step->scalar_type() == ScalarType::Long && step->numel() == 1), what, ": step must be a one-element int64 tensor");
-    require_cuda(x_in);
-    require_cuda(residual);
-    require_cuda(step);
+    require_cuda(x_in, residual, step);
     require_current(x_in);
     const Tensor x = x_in.contiguous();
     const auto r = contiguous(residual);
@@ -918,10 +908,7 @@ std::tuple<Tensor, std::optional<Tensor>> linear_act_fwd(const Tensor& x, const 
     const ScalarType dt = x.scalar_type();
     if (bias) lin_like(what, "bias", *bias, {N}, is_float(bias->scalar_type()));
     if (residual) lin_like(what, "residual", *residual, shape, residual->scalar_type() == dt || residual->scalar_type() == ScalarType::Float);
-    require_cuda(x);
-    require_cuda(weight);
-    require_cuda(bias);
-    require_cuda(residual);
+    require_cuda(x, weight, bias, residual);
     require_current(x);
     LinRows a(x, M, K), b(weight, N, K);
     if (M && N && K) {
@@ -956,9 +943,7 @@ std::tuple<std::optional<Tensor>, std::optional<Tensor>, std::optional<Tensor>> 
                 in_pre ? "given)" : "missing)");
     if (pre) lin_like(what, "pre", *pre, shape, pre->scalar_type() == dt);
     if (in_pre) lin_like(what, "in_pre", *in_pre, x.sizes(), in_pre->scalar_type() == dt);
-    for (const Tensor* t : {&dy, &x, &weight}) require_cuda(*t);
-    require_cuda(pre);
-    require_cuda(in_pre);
+    require_cuda(x, dy, weight, pre, in_pre);
     require_current(x);
     const int tc = dtype_code(dt, what);
     void* const stream = stream_of(x);

@@ -32,7 +32,7 @@ def _dw_gemm(dy: Tensor, x_hat: Optional[Tensor], packed: Optional[Tensor], scal
              min: Optional[Tensor], N: int, bits: int, group_size: int, bias_grad: bool, out_dtype: torch.dtype):
     """dy bf16 [K, M]; x_hat bf16 [K, N] or (packed, scale, min) codes of the flat [K*N] activation
     -> (dW [M, N] in out_dtype (float32 or bfloat16), db fp32 [M] or None)."""
-    _require_cuda(dy)
+    _require_cuda(dy, x_hat, packed, scale, min)
     if dy.dim() != 2 or dy.dtype != torch.bfloat16:
         raise RuntimeError(f"dw_gemm: dy must be a bf16 [K, M] matrix, got {tuple(dy.shape)} {dy.dtype}")
     if out_dtype not in (torch.float32, torch.bfloat16):
