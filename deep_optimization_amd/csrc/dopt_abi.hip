@@ -1170,6 +1170,15 @@ static int check_linear(int dtype, int64_t M, int64_t N, int64_t K, int64_t lda,
     return DOPT_OK;
 }
 
+// one product's launch and its status
+static int launch_product(const dopt::LinArgs& p, int kind, int dtype, void* stream, const char* what) {
+    (void)hipGetLastError();
+    if (dopt::launch_linear(p, kind, dtype == DOPT_F16, (hipStream_t)stream))
+        return fail(DOPT_EUNSUPPORTED, "linear: a result of %lld x %lld has more tiles than a launch takes (operands whose rows start at "
+                    "multiples of 16 bytes get larger ones)", (long long)p.M, (long long)p.N);
+    return hip_status(what);
+}
+
 // operands of a product's size (the kernels read whole rows): pointers and row strides
 static int check_linear_rows(const void* a, int64_t lda, int64_t a_cols, const void* b, int64_t ldb, int64_t b_cols) {
     if (!a || !b) return fail(DOPT_EINVAL, "linear: null operand pointer");
@@ -1256,9 +1265,7 @@ int dopt_linear_forward(const void* x, int64_t ldx, const void* weight, int64_t 
     p.y = y;
     p.y_f32 = y_dtype == DOPT_F32;
     p.pre = (uint16_t*)pre;
-    (void)hipGetLastError();
-    dopt::launch_linear(p, dopt::LIN_NT, dtype == DOPT_F16, (hipStream_t)stream);
-    return hip_status("linear_forward launch");
+    return launch_product(p, dopt::LIN_NT, dtype, stream, "linear_forward launch");
 }
 
 static int check_input_grad(const void* dz, int64_t ldz, const void* weight, int64_t ldw, int dtype, int64_t M, int64_t N, int64_t K,
@@ -1291,9 +1298,7 @@ int dopt_linear_input_grad(const void* dz, int64_t ldz, const void* weight, int6
     if (int rc = check_input_grad(dz, ldz, weight, ldw, dtype, M, N, K, in_pre, in_act, dx)) return rc;
     if (M == 0 || K == 0) return ok();
     const dopt::LinArgs p = input_grad_args(dz, ldz, weight, ldw, M, N, K, in_pre, in_act, dx);
-    (void)hipGetLastError();
-    dopt::launch_linear(p, dopt::LIN_KN, dtype == DOPT_F16, (hipStream_t)stream);
-    return hip_status("linear_input_grad launch");
+    return launch_product(p, dopt::LIN_KN, dtype, stream, "linear_input_grad launch");
 }
 
 int64_t dopt_linear_layout_workspace_floats(int64_t rows, int64_t cols) {
@@ -1340,7 +1345,8 @@ int dopt_linear_layout(const dopt_linear_rows* rows, int n, int dtype, void* str
     }
     if (items.n == 0 && !sums) return ok();
     (void)hipGetLastError();
-    dopt::launch_linear_rows(items, dtype == DOPT_F16, (hipStream_t)stream);
+    if (dopt::launch_linear_rows(items, dtype == DOPT_F16, (hipStream_t)stream))
+        return fail(DOPT_EUNSUPPORTED, "linear: sums of more columns than a launch takes");
     for (int k = 0; k < n; ++k) {
         const dopt_linear_rows& r = rows[k];
         const int groups = r.rows > 0 ? dopt::linear_sum_groups(r.rows, r.cols) : 0;
@@ -1404,8 +1410,7 @@ int dopt_linear_weight_grad(const void* dz, int64_t ldz, const void* x, int64_t 
         return hip_status("linear_weight_grad launch");
     }
     const dopt::LinArgs p = weight_grad_args(dz, ldz, x, ldx, M, N, K, dw_f32, dw_16, db, db_16);
-    dopt::launch_linear(p, dopt::LIN_TN, dtype == DOPT_F16, (hipStream_t)stream);
-    return hip_status("linear_weight_grad launch");
+    return launch_product(p, dopt::LIN_TN, dtype, stream, "linear_weight_grad launch");
 }
 
 int dopt_linear_backward(const void* dz, int64_t ldz, const void* x, int64_t ldx, const void* weight, int64_t ldw, int dtype, int64_t M,

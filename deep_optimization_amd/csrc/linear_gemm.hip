@@ -59,13 +59,18 @@ float estimate(const TileCost& c, int kind, int64_t M, int64_t N, int64_t K, int
     return c.start + nk * std::max(c.alone[kind] * rounds, c.shared[kind] * (float)per_cu) + c.epilogue * extras * (float)per_cu;
 }
 
+// Whether a grid of `blocks` workgroups has fewer than 2^32 work-items, which is what a launch takes.
+bool grid_fits(int64_t blocks, int threads) { return blocks < ((int64_t)1 << 32) / threads; }
+
 // the tile with the least estimate: of the REG ones where rows lie at any element, else of the others (the 256-wide ones
-// if `big`). extras: what an epilogue costs beside a plain one.
+// if `big`; their grid is one workgroup a CU). extras: what an epilogue costs beside a plain one. -2: none whose grid fits a launch.
 int plan(int kind, int64_t M, int64_t N, int64_t K, int n_cu, bool reg, bool big, float extras, float* us) {
-    int best = -1;
-    float least = 0.0f;
+    int best = -2;
+    float least = 1e30f;
     for (int t = reg ? T_REG32x64 : 0; t < (reg ? T_COUNT : big && kind != LIN_TN ? T_REG32x64 : T_BIG160); ++t) {
-        const float e = estimate(TILE_COST[t], kind, M, N, K, n_cu, extras);
+        const TileCost& c = TILE_COST[t];
+        if (t != T_BIG160 && t != T_BIG256 && !grid_fits(((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn), 256)) continue;
+        const float e = estimate(c, kind, M, N, K, n_cu, extras);
         if (best < 0 || e < least) {
             least = e;
             best = t;
@@ -81,14 +86,14 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 bool whole_rows(const void* p, int64_t ld, int64_t cols) { return aligned16(p) && ld % 8 == 0 && ld >= (cols + 7) / 8 * 8; }
 
 template <int KIND, bool F16>
-void launch(const LinArgs& p, hipStream_t s) {
+int launch(const LinArgs& p, hipStream_t s) {
     const int n_cu = device_cu_count();
     const bool reg = !whole_rows(p.A, p.lda, KIND == LIN_TN ? p.M : p.K) || !whole_rows(p.B, p.ldb, KIND == LIN_NT ? p.K : p.N);
     if constexpr (KIND == LIN_NT) {
         if (p.M <= 16) {
             if (reg) lin_small_launch<8, F16, true>(p, s);
             else lin_small_launch<8, F16, false>(p, s);
-            return;
+            return 0;
         }
     }
     // what the 256-wide tiles take: whole 16-byte chunks in the results' rows, 32-bit offsets in a tile of them
@@ -99,19 +104,22 @@ void launch(const LinArgs& p, hipStream_t s) {
     if constexpr (KIND != LIN_TN) {
         if (t == T_BIG160 || t == T_BIG256) {
             const int bm = TILE_COST[t].bm;
-            if constexpr (KIND == LIN_KN) return F16 ? lin_big_kn_f16(p, bm, n_cu, s) : lin_big_kn_bf16(p, bm, n_cu, s);
-            else return F16 ? lin_big_nt_f16(p, bm, n_cu, s) : lin_big_nt_bf16(p, bm, n_cu, s);
+            if constexpr (KIND == LIN_KN) F16 ? lin_big_kn_f16(p, bm, n_cu, s) : lin_big_kn_bf16(p, bm, n_cu, s);
+            else F16 ? lin_big_nt_f16(p, bm, n_cu, s) : lin_big_nt_bf16(p, bm, n_cu, s);
+            return 0;
         }
     }
     switch (t) {
-        case T_32x64: return lin_gemm_launch<32, 64, 4, 3, KIND, F16>(p, s);
-        case T_64x64: return lin_gemm_launch<64, 64, 4, 2, KIND, F16>(p, s);
-        case T_64x64_4: return lin_gemm_launch<64, 64, 2, 4, KIND, F16>(p, s);
-        case T_128x64: return lin_gemm_launch<128, 64, 3, 2, KIND, F16>(p, s);
-        case T_REG32x64: return lin_gemm_launch<32, 64, 2, 4, KIND, F16, true>(p, s);
-        case T_REG64x64: return lin_gemm_launch<64, 64, 2, 3, KIND, F16, true>(p, s);
-        default: return lin_gemm_launch<128, 128, 2, 2, KIND, F16>(p, s);
+        case T_32x64: lin_gemm_launch<32, 64, 4, 3, KIND, F16>(p, s); break;
+        case T_64x64: lin_gemm_launch<64, 64, 4, 2, KIND, F16>(p, s); break;
+        case T_64x64_4: lin_gemm_launch<64, 64, 2, 4, KIND, F16>(p, s); break;
+        case T_128x64: lin_gemm_launch<128, 64, 3, 2, KIND, F16>(p, s); break;
+        case T_128x128: lin_gemm_launch<128, 128, 2, 2, KIND, F16>(p, s); break;
+        case T_REG32x64: lin_gemm_launch<32, 64, 2, 4, KIND, F16, true>(p, s); break;
+        case T_REG64x64: lin_gemm_launch<64, 64, 2, 3, KIND, F16, true>(p, s); break;
+        default: return -1;
     }
+    return 0;
 }
 
 // Elements i .. i + 7 of rows at any element, those from `have` on as zeros; `total` elements exist from p on. One vector load,
@@ -222,22 +230,23 @@ __global__ __launch_bounds__(1024) void lin_sum_kernel(const float* partial, int
 
 }  // namespace
 
-// A's and B's offsets of one tile and slab stay within a buffer resource, a grid's work-items below 2^32
+// A's and B's offsets of one tile and slab stay within a buffer resource, the tiles' number within 32 bits (whether a tile's grid
+// fits a launch is its choice's to see: plan)
 bool lin_shape_fits(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb) {
     const int64_t ld = std::max(lda, ldb), most = (int64_t)1 << 24;
     return ld < ((int64_t)1 << 21) && K < ((int64_t)1 << 28) && M < ((int64_t)1 << 37) && N < ((int64_t)1 << 26) &&
            (M + 127) / 128 < most / ((N + 127) / 128 + 1);
 }
 
+// -1: no tile's grid fits a launch (nothing is launched)
 int launch_linear(const LinArgs& p, int kind, bool f16, hipStream_t s) {
     if (p.M == 0 || p.N == 0) return 0;
-    if (kind == LIN_KN) f16 ? launch<LIN_KN, true>(p, s) : launch<LIN_KN, false>(p, s);
-    else if (kind == LIN_TN) f16 ? launch<LIN_TN, true>(p, s) : launch<LIN_TN, false>(p, s);
-    else f16 ? launch<LIN_NT, true>(p, s) : launch<LIN_NT, false>(p, s);
-    return 0;
+    if (kind == LIN_KN) return f16 ? launch<LIN_KN, true>(p, s) : launch<LIN_KN, false>(p, s);
+    if (kind == LIN_TN) return f16 ? launch<LIN_TN, true>(p, s) : launch<LIN_TN, false>(p, s);
+    return f16 ? launch<LIN_NT, true>(p, s) : launch<LIN_NT, false>(p, s);
 }
 
-// The tile that a product gets (an index of TILE_COST; -1: the kernel of at most 16 rows) and its estimate. M, N, K as in
+// The tile that a product gets (an index of TILE_COST; -1: the kernel of at most 16 rows; -2: none takes it) and its estimate. M, N, K as in
 // LinArgs; reg: an operand's rows lie at any element.
 int linear_tile(int kind, int64_t M, int64_t N, int64_t K, bool reg, bool big, float* us) {
     const int n_cu = device_cu_count();
@@ -302,6 +311,7 @@ int launch_linear_pair(const LinArgs& dx, const LinArgs& dw, int tile, bool f16,
     return 0;
 }
 
+// -1: more columns to sum than a launch's grid takes (nothing is launched)
 int launch_linear_rows(LinRowItems items, bool f16, hipStream_t s) {
     uint32_t blocks = 0;
     for (int k = 0; k < items.n; ++k) {
@@ -312,11 +322,12 @@ int launch_linear_rows(LinRowItems items, bool f16, hipStream_t s) {
             p.lg = p.groups == 1 ? 2 : 5;
             p.blocks = (uint32_t)((cpr + (1 << p.lg) - 1) >> p.lg) * p.groups;
         } else {
-            p.blocks = (uint32_t)std::min<int64_t>((p.rows * cpr + ROWS_THREADS - 1) / ROWS_THREADS, 1 << 20);
+            p.blocks = (uint32_t)std::min<int64_t>((p.rows * cpr + ROWS_THREADS - 1) / ROWS_THREADS, 1 << 19);
         }
         blocks += p.blocks;
     }
     if (blocks == 0) return 0;
+    if (!grid_fits(blocks, ROWS_THREADS)) return -1;
     if (f16) hipLaunchKernelGGL(lin_rows_kernel<true>, dim3(blocks), dim3(ROWS_THREADS), 0, s, items);
     else hipLaunchKernelGGL(lin_rows_kernel<false>, dim3(blocks), dim3(ROWS_THREADS), 0, s, items);
     return 0;

@@ -516,7 +516,7 @@ int dopt_linear_backward(const void* dz, int64_t ldz, const void* x, int64_t ldx
                          int64_t N, int64_t K, const void* in_pre, int in_act, void* dx, float* workspace, float* dw_f32, void* dw_16,
                          float* db, void* db_16, void* stream);
 /* Which tile a product gets (an index of the launcher's table; -1: the kernel of at most 16 rows; 100: dopt_dw_gemm_any's
- * kernels; -2: bad arguments); any_rows: an operand's rows lie at any element. */
+ * kernels; -2: bad arguments, or more tiles than a launch takes); any_rows: an operand's rows lie at any element. */
 int dopt_linear_tile(int product, int64_t M, int64_t N, int64_t K, int any_rows);
 /* Whether a product is estimated to run faster on aligned rows than on operands that lie at any element, where laying those out
  * again takes `launches` more launches and `elements` elements of copying. */
