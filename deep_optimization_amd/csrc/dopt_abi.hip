@@ -1323,9 +1323,10 @@ int dopt_linear_layout(const dopt_linear_rows* rows, int n, int dtype, void* str
             sums |= r.cols > 0;
         }
         if (r.rows == 0 || r.cols == 0) continue;
-        if (!r.src || !r.dst || (r.act != DOPT_LIN_NONE && !r.pre) || (r.sum && !r.workspace && dopt_linear_layout_workspace_floats(r.rows, r.cols) > 0))
+        const bool sums_only = r.sum && !r.dst && r.ld_dst == 0;
+        if (!r.src || (!r.dst && !sums_only) || (r.act != DOPT_LIN_NONE && !r.pre) || (r.sum && !r.workspace && dopt_linear_layout_workspace_floats(r.rows, r.cols) > 0))
             return fail(DOPT_EINVAL, "linear: null src/pre/dst/workspace pointer");
-        if (r.ld_src < r.cols || r.ld_dst < r.cols || ((uintptr_t)r.src & 1u) || ((uintptr_t)r.pre & 1u) || ((uintptr_t)r.dst & 1u))
+        if (r.ld_src < r.cols || (r.ld_dst < r.cols && !sums_only) || ((uintptr_t)r.src & 1u) || ((uintptr_t)r.pre & 1u) || ((uintptr_t)r.dst & 1u))
             return fail(DOPT_EINVAL, "linear: src's and dst's rows must lie at whole elements, at least cols apart");
         if (r.ld_src >= ((int64_t)1 << 44) / r.rows || r.ld_dst >= ((int64_t)1 << 44) / r.rows)
             return fail(DOPT_EUNSUPPORTED, "linear: matrices below 2^44 elements");
@@ -1336,7 +1337,7 @@ int dopt_linear_layout(const dopt_linear_rows* rows, int n, int dtype, void* str
         item.rows = r.rows;
         item.cols = r.cols;
         item.dst = (uint16_t*)r.dst;
-        item.ld_dst = r.ld_dst;
+        item.ld_dst = sums_only ? r.cols : r.ld_dst;
         item.act = r.act;
         item.sum = r.sum;
         item.sum_dt = r.sum_dtype;

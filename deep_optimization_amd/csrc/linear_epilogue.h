@@ -28,8 +28,8 @@ struct LinArgs {
 };
 
 // Rows laid out for the products: dst[r][c] = src[r][c] act'(pre[r][c]) for c < cols, 0 for the columns up to ld_dst (act
-// LIN_NONE: a copy), and with `sum` the columns' sums of it before its rounding; partial: [groups][cols] where those are not 1. src rows ld_src and dst rows
-// ld_dst elements apart, pre [rows][cols] contiguous.
+// LIN_NONE: a copy), and with `sum` the columns' sums of it before its rounding; partial: [groups][cols] where those are not 1.
+// src rows ld_src and dst rows ld_dst elements apart, pre [rows][cols] contiguous. Without dst (ld_dst = cols) the sums alone.
 struct LinRowItem {
     const uint16_t* src;
     int64_t ld_src;

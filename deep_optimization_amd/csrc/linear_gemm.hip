@@ -144,7 +144,7 @@ __device__ __forceinline__ void lin_load_row8(const uint16_t* p, int64_t i, int6
 // its threads add their 8 columns in fp32 over the rows they take, and the threads of equal columns meet over the lanes of
 // a wave and then over the waves in LDS, in an order that the sizes fix. The sums are of the fp32 values: the bias gradient is then
 // as exact as its own rounding, where the sum of the rounded dz that the weight gradient's product makes on its way is off by up
-// to half a rounding more.
+// to half a rounding more. Without a dst it reads alone: 25216 x 2304 22 us a call (through the weight gradient's product 105).
 constexpr int ROWS_THREADS = 1024;
 template <bool F16>
 __global__ __launch_bounds__(ROWS_THREADS, 8) void lin_rows_kernel(LinRowItems items) {
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(ROWS_THREADS, 8) void lin_rows_kernel(LinRowItems i
             lin_load_row8<DT>(p.pre, r * p.cols + c, p.rows * p.cols, have, z);
             lin_act_grad8(p.act, z, v);
         }
-        lin_store8<DT>(p.dst, r * p.ld_dst + c, (int)min((int64_t)8, p.ld_dst - c), v);
+        if (p.dst) lin_store8<DT>(p.dst, r * p.ld_dst + c, (int)min((int64_t)8, p.ld_dst - c), v);
     };
     if (p.sum) {
         const int across = 1 << p.lg, x = threadIdx.x & (across - 1), y = threadIdx.x >> p.lg, tall = ROWS_THREADS >> p.lg;

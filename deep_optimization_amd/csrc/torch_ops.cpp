@@ -839,20 +839,22 @@ void lin_plan(int product, int64_t M, int64_t N, int64_t K, LinRows& a, LinRows&
         if (r->loose()) r->copy = true;
 }
 
-// one launch that lays out those operands that are marked; `pre`, `act`, `sum`: of the one that is written
-// (linear_lib._layout)
+// one launch that lays out those operands that are marked; `pre`, `act`, `sum`: the first one's, which may have nothing but its
+// columns summed (linear_lib._layout)
 void lin_layout(std::initializer_list<LinRows*> operands, const void* pre, int act, const std::optional<Tensor>& sum, ScalarType dt, void* stream) {
     dopt_linear_rows items[4];
     Tensor sources[4], space;
     int n = 0;
     for (LinRows* r : operands) {
-        if (!r->copy && !r->written) continue;
-        const int64_t width = r->copy ? pad8(r->cols) : r->cols;
-        Tensor out = fresh({r->rows, width}, dt, r->t);
+        const bool first = r == *operands.begin(), sums = first && sum;
+        if (!r->copy && !r->written && !sums) continue;
+        const int64_t width = r->copy ? pad8(r->cols) : r->written ? r->cols : 0;
+        Tensor out;
+        if (width) out = fresh({r->rows, width}, dt, r->t);
         dopt_linear_rows& d = items[n++];
-        d = {r->t.data_ptr(), r->ld, r->written ? pre : nullptr, r->rows, r->cols, out.data_ptr(), width, r->written ? act : DOPT_LIN_NONE,
-             0, nullptr, nullptr};
-        if (r->written && sum) {
+        d = {r->t.data_ptr(), r->ld, first ? pre : nullptr, r->rows, r->cols, width ? out.data_ptr() : nullptr, width,
+             first ? act : DOPT_LIN_NONE, 0, nullptr, nullptr};
+        if (sums) {
             const int64_t floats = dopt_linear_layout_workspace_floats(r->rows, r->cols);
             if (floats > 0) space = fresh({floats}, at::kFloat, r->t);
             d.sum = sum->data_ptr();
@@ -862,6 +864,7 @@ void lin_layout(std::initializer_list<LinRows*> operands, const void* pre, int a
             d.rows = 1;
             d.cols = d.ld_src = d.ld_dst = r->rows * r->cols;
         }
+        if (!width) continue;
         // (a source that was made contiguous lives until the launch: the next result could take its memory)
         sources[n - 1] = std::exchange(r->t, out);
         r->whole = width % 8 == 0;
@@ -948,16 +951,16 @@ std::tuple<std::optional<Tensor>, std::optional<Tensor>, std::optional<Tensor>> 
     const int tc = dtype_code(dt, what);
     void* const stream = stream_of(x);
     const bool empty = M == 0 || N == 0 || K == 0;
-    // dz is dy, or written by the launch that lays out the operands whose rows the products do better to read aligned
-    // (and, where no product sums it, or only once it is rounded, for its sums)
+    // dz is dy, or written by the launch that lays out the operands whose rows the products do better to read aligned;
+    // that launch makes its sums where no product does, or only once it is rounded
     std::optional<Tensor> db, sum;
     if (bias_grad) db = fresh({N}, grad_dtype, x);
-    if (db && (code != DOPT_LIN_NONE || K == 0 || M == 0)) sum = db;
-    const bool z = (code != DOPT_LIN_NONE && M && N) || sum;
+    if (db && (code != DOPT_LIN_NONE || !weight_grad || K == 0 || M == 0)) sum = db;
+    const bool z = code != DOPT_LIN_NONE && M && N && (input_grad || weight_grad);
     LinRows dz(dy, M, N, z), w(weight, N, K), xr(x, M, K);
     if (!empty) {
-        if (input_grad) lin_plan(DOPT_LIN_INPUT_GRAD, M, N, K, dz, w, z);
-        if (weight_grad || (db && !sum)) lin_plan(DOPT_LIN_WEIGHT_GRAD, M, N, K, dz, xr, z || dz.copy || w.copy);
+        if (input_grad) lin_plan(DOPT_LIN_INPUT_GRAD, M, N, K, dz, w, z || sum);
+        if (weight_grad) lin_plan(DOPT_LIN_WEIGHT_GRAD, M, N, K, dz, xr, z || sum || dz.copy || w.copy);
     }
     const auto p = contiguous(pre);
     lin_layout({&dz, &w, &xr}, ptr(p), code, sum, dt, stream);
@@ -969,7 +972,7 @@ std::tuple<std::optional<Tensor>, std::optional<Tensor>, std::optional<Tensor>> 
     }
     int64_t K8 = K;
     Tensor ws;
-    if (weight_grad || (db && !sum)) {
+    if (weight_grad) {
         // the kernels that split the sum write whole chunks of a row
         if (K % 8 && N && dz.whole && xr.whole && dopt_linear_tile(DOPT_LIN_WEIGHT_GRAD, M, N, pad8(K), 0) == 100) K8 = pad8(K);
         dw = fresh({N, K8}, grad_dtype, x);
@@ -992,7 +995,6 @@ std::tuple<std::optional<Tensor>, std::optional<Tensor>, std::optional<Tensor>> 
             check(dopt_linear_weight_grad(dz.t.data_ptr(), dz.ld, xr.t.data_ptr(), xr.ld, tc, M, N, K8, wsp, dw32, dw16, db32, db16, stream), what);
     }
     if (K8 != K) dw = dw->narrow(1, 0, K).contiguous();
-    if (!weight_grad) dw.reset();
     return {dx, dw, db};
 }
 

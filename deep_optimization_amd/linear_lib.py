@@ -17,8 +17,8 @@ Backward: dy and pre [..., N] in x's type. With ``in_act`` other than "none", x 
 activation that feeds the layer, and dx is the gradient of in_pre [..., K]: an MLP's second layer hands its first one the
 gradient of the pre-activation in one pass. dz is rounded to x's type for the products (both read it on matrix
 instructions of that type); dbias is the sum of dz before that rounding. dweight and dbias come in ``grad_dtype`` (float32 or
-x's type; both are summed in fp32); what is not asked for is None, and without an activation bias_grad alone still runs the weight
-gradient's product, which sums dy on its way.
+x's type; both are summed in fp32); what is not asked for is None. The weight gradient's product sums an activation-less dz on its
+way; without that product, or with an activation, the launch that writes dz (or one that writes nothing else) makes dbias.
 
 Rows may be strided (x[:, 0] of a [B, T, K] tensor) and lie at any element. Where they start at multiples of 16 bytes
 and hold whole 16-byte chunks the faster kernels read them; others are read through registers, or copied into
@@ -82,13 +82,14 @@ def _plan(product: int, M: int, N: int, K: int, a: _Rows, b: _Rows, launched: bo
 
 def _layout(items, dtype: torch.dtype, stream) -> None:
     """One launch that lays out [(operand, pre, act, sum)]; each then holds its new rows. With an activation the rows become dy act'(pre),
-    padded only where a copy is marked; ``sum`` (or None) receives their columns' sums."""
+    padded only where a copy is marked; ``sum`` (or None) receives their columns' sums, which is all that an operand gets that is neither
+    to be copied nor written."""
     if not items:
         return
     rows, kept = (_lib.LinearRows * len(items))(), []
     for d, (r, pre, act, total) in zip(rows, items):
-        width = _pad8(r.cols) if r.copy else r.cols
-        out = torch.empty((r.rows, width), dtype=dtype, device=r.t.device)
+        width = _pad8(r.cols) if r.copy else r.cols if r.written else 0
+        out = torch.empty((r.rows, width), dtype=dtype, device=r.t.device) if width else None
         n, cols, src, dst = r.rows, r.cols, r.ld, width
         space = None
         if total is not None:
@@ -100,8 +101,9 @@ def _layout(items, dtype: torch.dtype, stream) -> None:
         # (what the launch reads lives until then: the next result could take its memory)
         kept.append((r.t, space))
         d.src, d.ld_src, d.pre, d.rows, d.cols, d.dst, d.ld_dst, d.act = (r.t.data_ptr(), src, None if pre is None else pre.data_ptr(), n,
-                                                                          cols, out.data_ptr(), dst, act)
-        r.t, r.ld, r.whole, r.copy = out, width, width % 8 == 0, False
+                                                                          cols, None if out is None else out.data_ptr(), dst, act)
+        if out is not None:
+            r.t, r.ld, r.whole, r.copy = out, width, width % 8 == 0, False
     _lib.check(_lib.lib().dopt_linear_layout(rows, len(items), _DTYPE_CODE[dtype], stream), "linear_act")
 
 
@@ -176,20 +178,20 @@ def _linear_act_bwd(dy: Tensor, x: Tensor, weight: Tensor, pre: Optional[Tensor]
     _require_cuda(dy, x, weight, pre, in_pre)
     L, dt, stream = _lib.lib(), _DTYPE_CODE[x.dtype], _stream(x)
     empty = M == 0 or N == 0 or K == 0
-    # dz is dy, or written by the launch that lays out the operands whose rows the products do better to read aligned
-    # (and, where no product sums it, or only once it is rounded, for its sums)
+    # dz is dy, or written by the launch that lays out the operands whose rows the products do better to read aligned;
+    # that launch makes its sums where no product does, or only once it is rounded
     db = torch.empty(N, dtype=grad_dtype, device=x.device) if bias_grad else None
-    summed = db is not None and (code != 0 or K == 0 or M == 0)
-    z = (code != 0 and M > 0 and N > 0) or summed
+    summed = db is not None and (code != 0 or not weight_grad or K == 0 or M == 0)
+    z = code != 0 and M > 0 and N > 0 and (input_grad or weight_grad)
     dz, w, xr = _Rows(dy, M, N, z), _Rows(weight, N, K), _Rows(x, M, K)
     if not empty:
         if input_grad:
-            _plan(1, M, N, K, dz, w, z)
-        if weight_grad or (bias_grad and not summed):
-            _plan(2, M, N, K, dz, xr, z or dz.copy or w.copy)
+            _plan(1, M, N, K, dz, w, z or summed)
+        if weight_grad:
+            _plan(2, M, N, K, dz, xr, z or summed or dz.copy or w.copy)
     pre = None if pre is None else pre.contiguous()
     _layout([(r, p, a, s) for r, p, a, s in ((dz, pre, code, db if summed else None), (w, None, 0, None), (xr, None, 0, None))
-             if r.copy or r.written], x.dtype, stream)
+             if r.copy or r.written or s is not None], x.dtype, stream)
     dx = dw = None
     dx_args = dw_args = ()
     if input_grad:
@@ -197,7 +199,7 @@ def _linear_act_bwd(dy: Tensor, x: Tensor, weight: Tensor, pre: Optional[Tensor]
         in_pre = None if in_pre is None else in_pre.contiguous()
         dx_args = (None if in_pre is None else in_pre.data_ptr(), in_code, dx.data_ptr())
     K8 = K
-    if weight_grad or (bias_grad and not summed):
+    if weight_grad:
         # the kernels that split the sum write whole chunks of a row
         if K % 8 and N and dz.whole and xr.whole and L.dopt_linear_tile(2, M, N, _pad8(K), 0) == 100:
             K8 = _pad8(K)
@@ -217,7 +219,7 @@ def _linear_act_bwd(dy: Tensor, x: Tensor, weight: Tensor, pre: Optional[Tensor]
             _lib.check(L.dopt_linear_weight_grad(dz.t.data_ptr(), dz.ld, xr.t.data_ptr(), xr.ld, dt, M, N, K8, *dw_args, stream), what)
     if K8 != K:
         dw = dw[:, :K].contiguous()
-    return dx, dw if weight_grad else None, db
+    return dx, dw, db
 
 
 def _linear_act_bwd_fake(dy, x, weight, pre, act, in_pre, in_act, input_grad, weight_grad, bias_grad, grad_dtype):

@@ -490,7 +490,7 @@ int dopt_linear_input_grad(const void* dz, int64_t ldz, const void* weight, int6
 /* Rows laid out for the products, up to 4 matrices in one launch: dst[r][c] = src[r][c] * act'(pre[r][c]) for c < cols, 0 for the
  * columns up to ld_dst; with DOPT_LIN_NONE a copy (pre is not read). src's and dst's rows ld_src and ld_dst elements apart, at
  * any element; pre [rows, cols] contiguous. sum (or NULL): the columns' sums of the fp32 values before their rounding, [cols] of
- * sum_dtype (dtype or DOPT_F32), in an order that the sizes fix; workspace: dopt_linear_layout_workspace_floats floats (0: it may
+ * sum_dtype (dtype or DOPT_F32), in an order that the sizes fix, with dst NULL and ld_dst 0 nothing else; workspace: dopt_linear_layout_workspace_floats floats (0: it may
  * be NULL; else the sums take a second launch). */
 typedef struct {
     const void* src;
