@@ -75,6 +75,7 @@ EXPORTS = (
     "dopt_linear_weight_grad",
     "dopt_linear_backward",
     "dopt_linear_tile",
+    "dopt_linear_epilogue_tile",
     "dopt_linear_copy_preferred",
 )
 
@@ -232,6 +233,9 @@ def lib() -> ctypes.CDLL:
         L.dopt_linear_backward.restype = i32
         L.dopt_linear_tile.argtypes = [i32, i64, i64, i64, i32]
         L.dopt_linear_tile.restype = i32
+        # product, M, N, K, any_rows, act, side, pre, y_f32
+        L.dopt_linear_epilogue_tile.argtypes = [i32, i64, i64, i64, i32, i32, i32, i32, i32]
+        L.dopt_linear_epilogue_tile.restype = i32
         L.dopt_linear_copy_preferred.argtypes = [i32, i64, i64, i64, i64, i32]
         L.dopt_linear_copy_preferred.restype = i32
         _lib = L

@@ -42,6 +42,7 @@ int launch_dropout(const void* x, int x_dt, const void* residual, uint64_t n, ui
 bool lin_shape_fits(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb);
 int launch_linear(const LinArgs& p, int kind, bool f16, hipStream_t s);
 int linear_tile(int kind, int64_t M, int64_t N, int64_t K, bool reg, bool big, float* us);
+int linear_chosen(const LinArgs& p, int kind, bool reg);
 int linear_pair(int64_t M, int64_t N, int64_t K, bool reg, float* us);
 int launch_linear_pair(const LinArgs& dx, const LinArgs& dw, int tile, bool f16, hipStream_t s);
 int linear_sum_groups(int64_t rows, int64_t cols);
@@ -1222,6 +1223,25 @@ int dopt_linear_tile(int product, int64_t M, int64_t N, int64_t K, int any_rows)
     int64_t m, n, k;
     linear_sizes(product, M, N, K, &m, &n, &k);
     return dopt::linear_tile(product, m, n, k, any_rows != 0, true, nullptr);
+}
+
+int dopt_linear_epilogue_tile(int product, int64_t M, int64_t N, int64_t K, int any_rows, int act, int side, int pre, int y_f32) {
+    if (product < DOPT_LIN_FORWARD || product > DOPT_LIN_WEIGHT_GRAD || M < 0 || N < 0 || K < 0 || act < DOPT_LIN_NONE || act > DOPT_LIN_SILU)
+        return -2;
+    if (product == DOPT_LIN_WEIGHT_GRAD && !any_rows && linear_dw_split(M, N, K)) return 100;
+    dopt::LinArgs p{};
+    linear_sizes(product, M, N, K, &p.M, &p.N, &p.K);
+    uint16_t* const aligned = (uint16_t*)(uintptr_t)16;  // (looked at for its alignment only)
+    p.y = aligned;
+    p.y_f32 = y_f32 != 0 && product != DOPT_LIN_INPUT_GRAD;
+    if (product != DOPT_LIN_WEIGHT_GRAD) p.act = act;
+    if (product == DOPT_LIN_FORWARD) {
+        p.res = side ? aligned : nullptr;
+        p.pre = pre ? aligned : nullptr;
+    } else if (product == DOPT_LIN_INPUT_GRAD) {
+        p.aux = act != DOPT_LIN_NONE ? aligned : nullptr;
+    }
+    return dopt::linear_chosen(p, product, any_rows != 0);
 }
 
 int dopt_linear_copy_preferred(int product, int64_t M, int64_t N, int64_t K, int64_t elements, int launches) {

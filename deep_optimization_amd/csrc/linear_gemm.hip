@@ -85,22 +85,28 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 // rows that the loads to LDS take: 16-byte aligned, with whole chunks
 bool whole_rows(const void* p, int64_t ld, int64_t cols) { return aligned16(p) && ld % 8 == 0 && ld >= (cols + 7) / 8 * 8; }
 
+// the tile of a product with its epilogue (-1: the kernel of at most 16 rows); reg: an operand's rows lie at any element
+int choose(const LinArgs& p, int kind, bool reg, int n_cu) {
+    if (kind == LIN_NT && p.M <= 16) return -1;
+    // what the 256-wide tiles take: whole 16-byte chunks in the results' rows, 32-bit offsets in a tile of them
+    const bool big = p.N % 8 == 0 && p.N < ((int64_t)1 << 21) && p.K >= LIN_BK && !p.y_f32 && n_cu >= LIN_XCDS && aligned16(p.y) &&
+                     aligned16(p.pre) && aligned16(p.res) && aligned16(p.aux);
+    const float extras = 1.0f + (p.pre ? 0.6f : 0.0f) + (p.res || p.aux ? 0.6f : 0.0f) + (p.act != LIN_NONE ? 0.4f : 0.0f);
+    return plan(kind, p.M, p.N, p.K, n_cu, reg, big, extras, nullptr);
+}
+
 template <int KIND, bool F16>
 int launch(const LinArgs& p, hipStream_t s) {
     const int n_cu = device_cu_count();
     const bool reg = !whole_rows(p.A, p.lda, KIND == LIN_TN ? p.M : p.K) || !whole_rows(p.B, p.ldb, KIND == LIN_NT ? p.K : p.N);
+    const int t = choose(p, KIND, reg, n_cu);
     if constexpr (KIND == LIN_NT) {
-        if (p.M <= 16) {
+        if (t == -1) {
             if (reg) lin_small_launch<8, F16, true>(p, s);
             else lin_small_launch<8, F16, false>(p, s);
             return 0;
         }
     }
-    // what the 256-wide tiles take: whole 16-byte chunks in the results' rows, 32-bit offsets in a tile of them
-    const bool big = p.N % 8 == 0 && p.N < ((int64_t)1 << 21) && p.K >= LIN_BK && !p.y_f32 && n_cu >= LIN_XCDS && aligned16(p.y) &&
-                     aligned16(p.pre) && aligned16(p.res) && aligned16(p.aux);
-    const float extras = 1.0f + (p.pre ? 0.6f : 0.0f) + (p.res || p.aux ? 0.6f : 0.0f) + (p.act != LIN_NONE ? 0.4f : 0.0f);
-    const int t = plan(KIND, p.M, p.N, p.K, n_cu, reg, big, extras, nullptr);
     if constexpr (KIND != LIN_TN) {
         if (t == T_BIG160 || t == T_BIG256) {
             const int bm = TILE_COST[t].bm;
@@ -246,8 +252,10 @@ int launch_linear(const LinArgs& p, int kind, bool f16, hipStream_t s) {
     return f16 ? launch<LIN_NT, true>(p, s) : launch<LIN_NT, false>(p, s);
 }
 
-// The tile that a product gets (an index of TILE_COST; -1: the kernel of at most 16 rows; -2: none takes it) and its estimate. M, N, K as in
-// LinArgs; reg: an operand's rows lie at any element.
+int linear_chosen(const LinArgs& p, int kind, bool reg) { return choose(p, kind, reg, device_cu_count()); }
+
+// The tile that a product with a plain epilogue and a 16-bit result gets (an index of TILE_COST; -1: the kernel of at most 16 rows; -2:
+// none takes it) and its estimate. M, N, K as in LinArgs; reg: an operand's rows lie at any element.
 int linear_tile(int kind, int64_t M, int64_t N, int64_t K, bool reg, bool big, float* us) {
     const int n_cu = device_cu_count();
     if (kind == LIN_NT && M <= 16) {

@@ -515,11 +515,15 @@ int dopt_linear_weight_grad(const void* dz, int64_t ldz, const void* x, int64_t 
 int dopt_linear_backward(const void* dz, int64_t ldz, const void* x, int64_t ldx, const void* weight, int64_t ldw, int dtype, int64_t M,
                          int64_t N, int64_t K, const void* in_pre, int in_act, void* dx, float* workspace, float* dw_f32, void* dw_16,
                          float* db, void* db_16, void* stream);
-/* Which tile a product gets (an index of the launcher's table; -1: the kernel of at most 16 rows; 100: dopt_dw_gemm_any's
- * kernels; -2: bad arguments, or more tiles than a launch takes); any_rows: an operand's rows lie at any element. */
+/* Which tile a product with a plain epilogue (no activation, residual or pre) and an aligned 16-bit result gets: an index of the
+ * launcher's table; -1: the kernel of at most 16 rows; 100: dopt_dw_gemm_any's kernels; -2: bad arguments, or more tiles than a
+ * launch takes; any_rows: an operand's rows lie at any element. */
 int dopt_linear_tile(int product, int64_t M, int64_t N, int64_t K, int any_rows);
+/* The same for a call with an epilogue, which the choice weighs: act (of the forward product, in_act of the input gradient), side (a
+ * residual), pre, y_f32 (an fp32 result). Results and side at multiples of 16 bytes. The tile that the call runs. */
+int dopt_linear_epilogue_tile(int product, int64_t M, int64_t N, int64_t K, int any_rows, int act, int side, int pre, int y_f32);
 /* Whether a product is estimated to run faster on aligned rows than on operands that lie at any element, where laying those out
- * again takes `launches` more launches and `elements` elements of copying. */
+ * again takes `launches` more launches and `elements` elements of copying. By the estimates of a plain epilogue, whatever the call's. */
 int dopt_linear_copy_preferred(int product, int64_t M, int64_t N, int64_t K, int64_t elements, int launches);
 
 /*
