@@ -18,6 +18,7 @@ reference's (controller.py:127-177 and :364-390):
 """
 from __future__ import annotations
 
+import warnings
 from typing import Dict, Optional, Sequence, Tuple
 
 import torch
@@ -150,6 +151,8 @@ class Controller:
         applies it to BatchNorm2d only, controller.py:131-135, and gives SyncBatchNorm the
         per-sample one its kernels do not use) and keep their bias and running statistics (the
         reference copies the weight only, controller.py:291);
+      * the transformer block layers (``modules.transformer``, ``vit.FusedBlock``) are leaves too: they are never swapped, and a
+        warning names them;
       * compressed layers already in the model are traced as leaves and left as they are, and the
         swap is made in ``self.model`` as well as in ``traced_model`` (the reference's swap reaches
         ``self.model`` only below its root, through the submodules the trace shares), so
@@ -268,7 +271,22 @@ class Controller:
             if tm is None or compute_activation_size_in_bytes(tm.shape, tm.dtype) <= 10:
                 continue
             chosen[node.target] = {"mod": mod, "tensor_meta": _node_input_meta(node)}
+        self._say_what_is_left(traced, named)
         return traced, chosen
+
+    @staticmethod
+    def _say_what_is_left(traced, named):
+        """The transformer block layers save their activations as they are, whatever the configuration: said, so that a model
+        built from them (``VisionTransformer(fused=True)``) is not taken for a compressed one."""
+        from .modules import transformer
+        from .vit import FusedBlock
+
+        left = [n.target for n in traced.graph.nodes
+                if n.op == "call_module" and isinstance(named[n.target], (transformer.LinearAct, transformer.Mlp, FusedBlock))]
+        if left:
+            warnings.warn(f"Controller: {len(left)} transformer block layers ({', '.join(left[:3])}{', ...' if len(left) > 3 else ''}) are left as "
+                          "they are: their activations are not compressed. Build the model of torch's layers (fused=False) to "
+                          "have those selected", stacklevel=4)
     def _new_module(self, target, mod):
         from .layers import DOConv1d, DOConv2d, DOConv3d, DOLinear
         from .modules.activations import DOGELU, DOReLU_Variance, DOSiLU
