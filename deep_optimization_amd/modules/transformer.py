@@ -33,11 +33,16 @@ _U63 = (1 << 63) - 1
 
 def _differentiated(*tensors: Optional[Tensor]) -> bool:
     """Whether a call on these goes through its autograd Function: one that does not would lose the tangents of forward mode, which
-    ask for no gradient (the Functions refuse them, and functorch's transforms)."""
-    if torch._C._are_functorch_transforms_active():
+    ask for no gradient (the Functions refuse them, and functorch's transforms). Inside a level of dual numbers every call does: asking
+    each tensor would be half of what a call on one token takes here."""
+    if forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active():
         return True
-    grad = torch.is_grad_enabled()
-    return any(t is not None and (grad and t.requires_grad or forward_ad.unpack_dual(t).tangent is not None) for t in tensors)
+    if not torch.is_grad_enabled():
+        return False
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
 
 
 def _first_order(backward):
@@ -46,7 +51,7 @@ def _first_order(backward):
     search for some tensors' gradients would pass that by, and add nothing."""
     @functools.wraps(backward)
     def guarded(ctx, *grads):
-        if any(g is not None and forward_ad.unpack_dual(g).tangent is not None for g in grads):
+        if forward_ad._current_level >= 0 and any(g is not None and forward_ad.unpack_dual(g).tangent is not None for g in grads):
             raise NotImplementedError("the transformer layers' gradients have no forward-mode derivatives")
         if not torch.is_grad_enabled():
             return backward(ctx, *grads)
@@ -192,14 +197,14 @@ def dropout_add(x: Tensor, residual: Optional[Tensor], p: float, seed: int, offs
     return _DropoutAdd.apply(x, residual, p, seed, offset, step)
 
 
-_HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
-
-
 def _bare(m: nn.Module, cls: type) -> bool:
     """Whether calling m does what cls.forward does and nothing else, so that a fused call may read its parameters instead: a layer that
     was replaced, has a forward of its own or hooks (pruning sets the weight in one) is called."""
-    return (isinstance(m, cls) and type(m).forward is cls.forward and "forward" not in vars(m) and not any(getattr(m, h) for h in _HOOKS)
-            and not nn.modules.module._has_any_global_hook())
+    if not isinstance(m, cls) or type(m).forward is not cls.forward:
+        return False
+    d = m.__dict__
+    return not ("forward" in d or d["_forward_hooks"] or d["_forward_pre_hooks"] or d["_backward_hooks"] or d["_backward_pre_hooks"]
+                or nn.modules.module._has_any_global_hook())
 
 
 def norm_residual(norm: nn.Module, x: Tensor):
