@@ -11,7 +11,7 @@
 // Bound by memory: 25216 x 768 in bf16 with a residual 31.7 us, 4.9 TB/s, the rate of a large copy, and 4.7 in
 // ln_param_kernel (1.6 MB of partial rows; latency). 6304 x 591 in fp32 12.3 + 4.0 us, 3.6 TB/s: a wave takes one or two rows
 // there, one after the other; reading the next row ahead needs more than the 128 registers that 16 waves leave (41
-// spilled). 302592 x 64 in bf16 26.7 us (4.4 TB/s), with a whole wave
+// spilled; fewer waves with more registers each were not tried). 302592 x 64 in bf16 26.7 us (4.4 TB/s), with a whole wave
 // a row 67. A few hundred rows are bound by the two launches (10-11 us a call).
 #include <algorithm>
 

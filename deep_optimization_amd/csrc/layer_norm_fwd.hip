@@ -5,7 +5,8 @@
 // All in fp32. TPR lanes hold a row (16 and 32 up to 64 and 128 elements, one wave up to 1024, then 4 and 16 waves up to 4096 and 16384), ACC
 // accesses of 4 elements each; the lanes of a launch keep their columns' weight and bias in registers over all the
 // rows they take. Rows of other widths (under 4, over 16384) go through ln_fwd_any_kernel, which reads
-// x three times, the second and third time mostly from the caches.
+// x three times, the second and third time mostly from the caches, an element a lane and a workgroup a row: right for any width, and
+// no more (2000 x 20000 in bf16 95 us, 1.7 TB/s; 300000 x 3 916 us).
 //
 // Bound by memory: 25216 x 768 in bf16 13.8 us, 5.6 TB/s (part of it from the cache behind the L2s; a copy of 2 GiB runs
 // at 5.0). 302592 x 64 18.4 us, 4.2 TB/s, with a whole wave a row 56.5. One row is bound by its launch: 2.3 us in the kernel, 6.2

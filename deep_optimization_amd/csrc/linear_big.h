@@ -25,11 +25,12 @@
 // holds 8 consecutive columns of its row and 16 lanes' rows cover 64 contiguous bytes each; bias, activation and
 // residual in fp32, 16-byte stores. The residual's (aux's) loads run one fragment row ahead.
 //
-// Bound by the part's power at the MFMA rate: 8192^3 766 us, 1.44 PFLOP/s, 4096^3 96 us (a library product of 8192^3: 1.45).
-// 25216 rows of 3072 -> 768 with bias and residual 121 us, 0.98 PFLOP/s (160-high tiles; 256-high 134 against 104 in a loop on
-// the same buffers: 297 tiles are 2 rounds as 474 are). 768 -> 3072 with GELU and pre 156 us, 0.76 PFLOP/s: a tile is 12 slabs
-// there, and its 256 KB of results leave at about 4 TB/s before the next tile's third slab can be waited for (without pre
-// 142 us, without GELU too 112). Workgroups that start up to a tile's time apart, nontemporal stores and two
+// 8192^3 766 us, 1.44 PFLOP/s, 4096^3 96 us (a library product of 8192^3: 1.45): the part's power at the MFMA rate. At shorter
+// sums the matrix pipes wait. 25216 rows of 3072 -> 768 with bias and residual 121 us, 0.98 PFLOP/s, busy in 40% of the cycles:
+// 474 tiles are 2 rounds of 256 CUs, each with its fill, and one workgroup a CU has nothing to multiply during its epilogue
+// (160-high tiles; 256-high 134 against 104 in a loop on the same buffers, 297 tiles being 2 rounds too). 768 -> 3072 with GELU and
+// pre 158 us, 0.75 PFLOP/s, busy in 29%: a tile is 12 slabs there, and its 256 KB of results leave at about 4 TB/s before the next
+// tile's third slab can be waited for (without pre 149 us, without GELU too 112). Workgroups that start up to a tile's time apart, nontemporal stores and two
 // workgroups of 192 x 128 tiles a CU measured the same or slower (125 -> 126..131, 156 -> 163, 126 -> 135 us). The
 // input gradient of 768 -> 2304 91 us.
 #pragma once

@@ -15,9 +15,11 @@ y in residual's type (x's without one). pre [..., N] in x's type.
 
 Backward: dy and pre [..., N] in x's type. With ``in_act`` other than "none", x is in_act(in_pre), the output of the
 activation that feeds the layer, and dx is the gradient of in_pre [..., K]: an MLP's second layer hands its first one the
-gradient of the pre-activation in one pass. dz is rounded to x's type for the products (both read it on matrix
-instructions of that type); dbias is the sum of dz before that rounding. dweight and dbias come in ``grad_dtype`` (float32 or
-x's type; both are summed in fp32); what is not asked for is None. The weight gradient's product sums an activation-less dz on its
+gradient of the pre-activation in one pass. dz is rounded to x's type for the products, which read it on matrix instructions of
+that type: with an activation dx and dweight are then off by that rounding beside their own (0.0023 of their norm where the one
+rounding alone is 0.0017, 2001 rows of 333 -> 1001 in bf16). dz as a sum of two 16-bit terms would keep twice the bits and double the
+products: their measured times put 25216 x 768 -> 3072 with GELU at 560 us for 334. dbias is the sum of dz before that rounding.
+dweight and dbias come in ``grad_dtype`` (float32 or x's type; both are summed in fp32); what is not asked for is None. The weight gradient's product sums an activation-less dz on its
 way; without that product, or with an activation, the launch that writes dz (or one that writes nothing else) makes dbias.
 
 Rows may be strided (x[:, 0] of a [B, T, K] tensor) and lie at any element. Where they start at multiples of 16 bytes

@@ -13,6 +13,11 @@ Functional forms on the GPU, differentiable once in reverse mode (forward mode a
 
 and as modules with torch's parameter names: LayerNorm, LinearAct, Mlp, DropoutAdd (with DropoutRng, the count that gives
 every pass of a model its own masks). Products run in bf16 or fp16: of that type, or under autocast.
+
+Gradients between the operators are in the products' type, as torch's are under autocast: mlp hands its first layer dz in 16 bits, so
+b1's gradient sums rounded terms (linear_act's sums fp32 ones), and an fp32 gradient that comes in (of an fp32
+residual's sum) is rounded to 16 bits for the products and the bias, while the residual gets it as it is. Each term of such a sum is off by
+up to 2^-9 of itself in bf16, independently of the others. Parameters in fp32 get fp32 sums.
 """
 from __future__ import annotations
 
@@ -251,7 +256,8 @@ class DropoutRng(nn.Module):
     step draws new masks on every replay. Call it once at the start of a pass, on the input: it returns that and steps the
     count. Every layer has an offset of its own (``site``). ``step`` is part of the state dict; the seed is not: ranks that
     train on different data each give their own (default: from torch's initial seed). One process per GPU: the layers refuse to run
-    in nn.DataParallel's replicas."""
+    in nn.DataParallel's replicas. The layers take the count of the latest call: call it outside of what activation checkpointing
+    recomputes, and recompute a pass before the next one begins."""
 
     def __init__(self, seed: Optional[int] = None):
         super().__init__()
