@@ -1209,9 +1209,10 @@ static bool linear_dw_shape(int64_t M, int64_t N, int64_t K) {
     return M >= 0 && N > 0 && K > 0 && K % 8 == 0 && N < ((int64_t)1 << 20) && K < ((int64_t)1 << 20);
 }
 
-// whether the weight gradient of aligned operands takes dopt_dw_gemm_any's kernels (their splits of the sum)
+// whether the weight gradient of aligned operands takes dopt_dw_gemm_any's kernels (their splits of the sum). Not for one split of
+// 128-row tiles: a few slabs then, which the other tiles' estimates are below (fp16 has no instance that writes its result).
 static bool linear_dw_split(int64_t M, int64_t N, int64_t K) {
-    if (!linear_dw_shape(M, N, K)) return false;
+    if (!linear_dw_shape(M, N, K) || (dopt::dw_splits(N, K, M) == 1 && dopt::dw_tile_rows(N, K) == 128)) return false;
     float us;
     dopt::linear_tile(DOPT_LIN_WEIGHT_GRAD, N, K, M, false, false, &us);
     return linear_dw_split_us(M, N, K) < us;

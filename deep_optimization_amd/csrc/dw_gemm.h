@@ -30,6 +30,7 @@ struct DwArgs {
 };
 
 int dw_splits(int64_t M, int64_t N, int64_t K);
+int dw_tile_rows(int64_t M, int64_t N);
 int64_t dw_workspace_floats(int64_t M, int64_t N, int64_t K);
 int64_t dw_any_workspace_floats(int64_t M, int64_t N, int64_t K);
 // the bias gradient in fp32 (db) or in dy's type (db16, DW_B_BF16 only), at most one of them

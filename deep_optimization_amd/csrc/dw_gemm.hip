@@ -964,9 +964,8 @@ int launch_dw_gemm(DwArgs a, int mode, float* out32, uint16_t* out16, float* db,
     } while (0)
         if (a.f16) {
             if (o16) {
-                if (bmt == 256) DOPT_DW2H(256, 256, true);
-                else if (bnt == 256) DOPT_DW2H(128, 256, true);
-                else DOPT_DW2H(128, 128, true);
+                if (bmt != 256) return -1;  // (no caller: one split of 128-row tiles is slower than a product without splits)
+                DOPT_DW2H(256, 256, true);
             } else {
                 if (bmt == 256) DOPT_DW2H(256, 256, false);
                 else if (bnt == 256) DOPT_DW2H(128, 256, false);
