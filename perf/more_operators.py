@@ -11,7 +11,7 @@ Kinds (``case["kind"]``) and the calls they make where ``own`` is set (``torch.o
                    weight_grad) -> (dx, dweight)
   rms_fp8      rms_norm_fp8(x, residual, weight, eps) -> (q, scale, s), then fp8_linear_rows(q, scale, b, out_scale) -> y
   gated_train  gated_linear_fwd(x, weight, bias, act, save_pre) -> (h, pre) and linear_act_fwd for the block's output, then
-                   gated_linear_bwd(dy, out_weight, pre, act, hidden) -> (dpre, None) and linear_act_bwd for the weights and the input
+                   gated_linear_bwd(dy, out_weight, pre, act, hidden) -> (dpre, h) and linear_act_bwd for the weights and the input
   gated_token  gated_linear_fwd and linear_act_fwd of a few tokens
 
 Definitions (rows are tokens, everything between the inputs and the outputs in 32 bits or more):
@@ -325,7 +325,8 @@ def run(state):
     y, _ = ops.linear_act_fwd(h, s["out_weight"], s["out_bias"], None, "none", False)
     if not train:
         return {"y": y}
-    dpre, _ = ops.gated_linear_bwd(s["dy"], s["out_weight"], pre, s["act"], False)
+    del h  # (the backward pass makes it again)
+    dpre, h = ops.gated_linear_bwd(s["dy"], s["out_weight"], pre, s["act"], True)
     _, dw2, db2 = ops.linear_act_bwd(s["dy"], h, s["out_weight"], None, "none", None, "none", False, True, bias, dt)
     dx, dw, db = ops.linear_act_bwd(dpre, s["x"], s["weight"], None, "none", None, "none", True, True, bias, dt)
     r = {"y": y, "dx": dx, "dweight": dw, "dout_weight": dw2}
