@@ -583,6 +583,7 @@ __global__ __launch_bounds__(64 * BWD_NW, 2) void attn_bwd_short_kernel(AttnArgs
     };
     const auto store_keys = [&](const Block& x) __attribute__((always_inline)) {
         const bool live = key < p.Lk;
+        if (key >= attn_length(p, x.b)) clear();  // (zeros, also where a query's dout is not finite, of which a probability of 0 makes NaN)
         uint16_t* const dkr = const_cast<uint16_t*>(at(p.dk, x.b, x.g)) + (int64_t)key * p.dk.l;
         uint16_t* const dvr = const_cast<uint16_t*>(at(p.dv, x.b, x.g)) + (int64_t)key * p.dv.l;
 #pragma unroll
