@@ -12,7 +12,8 @@ as those ends) and, with ``causal``, j <= i + Lk - Lq: the last query sees every
     s = scale q k^T (scale from 2^-100 to 2^100),  out = softmax(s) v,  lse = log sum exp s   (a query that sees no key: out 0, lse -inf)
 
 out [B, Lq, H, D] contiguous in q's type, lse fp32 [B, H, Lq] (None unless save_lse). Scores, softmax and sums are fp32; the
-probabilities, and in the backward pass ds, are rounded to q's type for the products that read them on matrix instructions; delta is of out as it
+probabilities, and in the backward pass ds, are rounded to q's type for the products that read them on matrix instructions (in fp16 times powers of two that
+keep them in its range, whatever the size of dout); delta is of out as it
 was returned, rounded to q's type (felt where a query sees a few keys only: 0.0037 of dq's norm at two keys in bf16, 0.0024 at many). What lies in k and v
 past a sequence's length is never used (NaN and infinities included) and has zero gradients. attention_qkv_bwd is attention_bwd
 for q, k and v that are the parts of one tensor qkv [B, L, H + 2 G, D], ``heads`` = H: its gradient in one tensor.

@@ -7,7 +7,7 @@
 //
 // Seven products where one kernel that does all would need five: its dq would be summed over the key tiles in memory, in an order of
 // arrival, or in as many copies as there are key tiles. p and ds are rounded to the operands' type for the products that read them: each
-// gradient is then off by 1.4 times what its own rounding costs (0.0024 of its norm for 0.0017 in bf16). delta is of out as it is kept, rounded once: where a
+// gradient is then off by 1.4 times what its own rounding costs (0.0024 of its norm for 0.0017 in bf16, 0.0003 for 0.0002 in fp16, see P_BITS). delta is of out as it is kept, rounded once: where a
 // query sees few keys, dp - delta is a small difference and feels that (0.0037 at two keys, 0.0027 at six; with one key, whose ds is 0, what is left is
 // that rounding times dp). Summing p dp instead would take a second pass over the scores. As in the forward kernel the vector arithmetic between the
 // products bounds all of them.
@@ -28,6 +28,55 @@ __device__ __forceinline__ void attn_widen2(uint32_t w, float& a, float& b) {
     } else {
         a = __uint_as_float(w << 16);
         b = __uint_as_float(w & 0xffff0000u);
+    }
+}
+
+// What p and ds are multiplied by for their products in fp16, which holds 2^-24 to 65504 where bf16 has fp32's range. All are powers of two, so that nothing is
+// rounded by them, and are undone in the sums. p, at most 1, is taken times 2^14. ds may be of any size (a gradient of 1e-5 over 4096 keys makes 1e-9 of it):
+// it has a power of two for each of a sum's columns, t, which follows the largest |ds| of the column's terms. Where a block's passes 2^15 / t, t is
+// set anew so that it lies at 2^7 to 2^8, and the sums so far are scaled along; what is rounded below fp16's normal numbers is then less than 2^-21 of the
+// column's largest term. It starts at the most that an fp32 number takes. It costs fp16 a largest value and a product a score, on one box: dq of 1536 heads of
+// 64, 197 and 197 64 -> 65 us, of 96 heads of 80, 985 and 985 70 -> 77, of 64 causal heads of 128, 4096 and 4096 420 -> 445; dk and dv 75 -> 81, 91 -> 98 and
+// 690 -> 725.
+template <bool F16>
+constexpr float P_BITS = F16 ? 14.0f : 0.0f;
+template <bool F16>
+constexpr float P_UNDO = F16 ? 0x1p-14f : 1.0f;
+constexpr float DS_START = 0x1p126f;
+
+// the largest |ds| of a lane's column in a block
+__device__ __forceinline__ float attn_top(const attn_v16f_t& ds) {
+    float top = fabsf(ds[0]);
+#pragma unroll
+    for (int e = 1; e < 16; ++e) top = fmaxf(top, fabsf(ds[e]));
+    return attn_max_halves(top);
+}
+template <int JD>
+__device__ __forceinline__ void attn_follow(float top, attn_v16f_t* sums, float& t) {
+    const bool past = top * t > 32768.0f;
+    if (wave_any(past)) {
+        const float next = past ? fminf(t, ldexpf(1.0f, 8 - __builtin_amdgcn_frexp_expf(top))) : t;
+        const float a = ldexpf(next, 1 - __builtin_amdgcn_frexp_expf(t));  // next / t
+        t = next;
+#pragma unroll
+        for (int j = 0; j < JD; ++j) sums[j] *= a;
+    }
+}
+// a block's ds, times t in fp16
+template <bool F16, int JD>
+__device__ __forceinline__ void attn_fit(attn_v16f_t& ds, attn_v16f_t* sums, float& t) {
+    if constexpr (F16) {
+        attn_follow<JD>(attn_top(ds), sums, t);
+        ds *= t;
+    }
+}
+// the sums without it
+template <bool F16, int JD>
+__device__ __forceinline__ void attn_unfit(attn_v16f_t* sums, float t) {
+    if constexpr (F16) {
+        const float undo = ldexpf(1.0f, 1 - __builtin_amdgcn_frexp_expf(t));
+#pragma unroll
+        for (int j = 0; j < JD; ++j) sums[j] *= undo;
     }
 }
 
@@ -100,6 +149,7 @@ __global__ __launch_bounds__(64 * BWD_NW, 2) void attn_dq_kernel(AttnArgs p, int
 #pragma unroll
     for (int j = 0; j < JD; ++j) dq[j] = attn_zero();
     const float c = p.scale * LOG2E;
+    float t = DS_START;
     attn_v16f_t minus_delta;  // what the sums of dp start from
 #pragma unroll
     for (int v = 0; v < 16; ++v) minus_delta[v] = -delta;
@@ -125,6 +175,7 @@ __global__ __launch_bounds__(64 * BWD_NW, 2) void attn_dq_kernel(AttnArgs p, int
             }
 #pragma unroll
             for (int v = 0; v < 16; ++v) s[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], c, -lse)) * dp[v];
+            attn_fit<F16, JD>(s, dq, t);
 #pragma unroll
             for (int hs = 0; hs < 2; ++hs) {
                 const lin_v4i_t ds = attn_operand<F16>(s, hs);
@@ -140,6 +191,7 @@ __global__ __launch_bounds__(64 * BWD_NW, 2) void attn_dq_kernel(AttnArgs p, int
     }
     if (i < tiles) tile(sK0, sV0, sK1, sV1, i);
     __builtin_amdgcn_s_waitcnt(0x0070);  // the load past the last tile lands before the workgroup ends
+    attn_unfit<F16, JD>(dq, t);
     uint16_t* const out = const_cast<uint16_t*>(p.dq.p) + b * p.dq.b + (int64_t)row * p.dq.l + h * p.dq.h;
 #pragma unroll
     for (int j = 0; j < JD; ++j) attn_store_block<F16>(out, dq[j], p.scale, j, p.D, lane, live);
@@ -219,6 +271,7 @@ __global__ __launch_bounds__(64 * BWD_NW, 2) void attn_dkv_kernel(AttnArgs p, in
 #pragma unroll
     for (int j = 0; j < JD; ++j) dk[j] = dv[j] = attn_zero();
     const float c = p.scale * LOG2E;
+    float t = DS_START;
     int row = t0 * BQ;  // of the tile that is worked on
 
     auto tile = [&](uint8_t* sq, uint8_t* so, float* ss, uint8_t* nq, uint8_t* no, float* ns) __attribute__((always_inline)) {
@@ -254,9 +307,10 @@ __global__ __launch_bounds__(64 * BWD_NW, 2) void attn_dkv_kernel(AttnArgs p, in
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                s[e] = __builtin_amdgcn_exp2f(s[e] * c);
+                s[e] = __builtin_amdgcn_exp2f(F16 ? __builtin_fmaf(s[e], c, P_BITS<F16>) : s[e] * c);
                 dp[e] *= s[e];
             }
+            attn_fit<F16, JD>(dp, dk, t);
 #pragma unroll
             for (int hs = 0; hs < 2; ++hs) {
                 const lin_v4i_t pr = attn_operand<F16>(s, hs), ds = attn_operand<F16>(dp, hs);
@@ -276,21 +330,23 @@ __global__ __launch_bounds__(64 * BWD_NW, 2) void attn_dkv_kernel(AttnArgs p, in
 #pragma unroll
         for (int j = 0; j < JD; ++j) dk[j] = dv[j] = attn_zero();
     }
+    attn_unfit<F16, JD>(dk, t);
     const bool live = key < p.Lk;
     uint16_t* const dkr = const_cast<uint16_t*>(p.dk.p) + b * p.dk.b + (int64_t)key * p.dk.l + g * p.dk.h;
     uint16_t* const dvr = const_cast<uint16_t*>(p.dv.p) + b * p.dv.b + (int64_t)key * p.dv.l + g * p.dv.h;
 #pragma unroll
     for (int j = 0; j < JD; ++j) {
-        attn_store_block<F16>(dkr, dk[j], p.scale, j, p.D, lane, live);
-        attn_store_block<F16>(dvr, dv[j], 1.0f, j, p.D, lane, live);
+        attn_store_block<F16>(dkr, dk[j], p.scale * P_UNDO<F16>, j, p.D, lane, live);
+        attn_store_block<F16>(dvr, dv[j], P_UNDO<F16>, j, p.D, lane, live);
     }
 }
 
 // The same for heads of more than 96 elements, whose sums and fragments (128 and 64 registers a lane) leave one wave a SIMD: it has to have its own
 // next MFMAs to run while its vector arithmetic does. 64 causal heads of 128 that share 16, 4096 and 4096: 620 to 675 us, 0.81 to 0.89 PFLOP/s,
 // where attn_dkv_kernel took 900, and 1240 with two waves a SIMD, whose registers spill. For heads of 64 and 96 two waves a SIMD fit.
-template <int DP, bool F16>
+template <bool F16>
 __global__ __launch_bounds__(64 * BWD_NW, 1) void attn_dkv_wide_kernel(AttnArgs p, int k_tiles) {
+    constexpr int DP = 128;
     using Tile = AttnTile<DP>;
     constexpr int KS = DP / 16, JD = DP / 32, NW = BWD_NW, BQ = BWD_T;
     __shared__ __attribute__((aligned(1024))) uint8_t sQ0[BQ * Tile::ROWB];
@@ -342,6 +398,7 @@ __global__ __launch_bounds__(64 * BWD_NW, 1) void attn_dkv_wide_kernel(AttnArgs 
 #pragma unroll
     for (int j = 0; j < JD; ++j) dk[j] = dv[j] = attn_zero();
     const float c = p.scale * LOG2E;
+    float t = DS_START;
 
     // A tile's two blocks of 32 rows go through three steps: scores and dp (MFMAs), p and ds (vector arithmetic), dv and dk (MFMAs). The
     // arithmetic of one block runs between the MFMAs of the other, and fragments are read from LDS half a step (KS MFMAs) ahead of
@@ -371,18 +428,27 @@ __global__ __launch_bounds__(64 * BWD_NW, 1) void attn_dkv_wide_kernel(AttnArgs 
             dp = attn_mfma<F16>(f[2 * q + 1], v[half * (KS / 2) + q], dp);
         }
     };
-    auto middle = [&](int n, int least, attn_v16f_t& sc, attn_v16f_t& dp, lin_v4i_t* pr, lin_v4i_t* ds) __attribute__((always_inline)) {
+    // (in fp16 ds waits for its power of two: pack_ds, in the next step)
+    auto middle = [&](int n, int least, attn_v16f_t& sc, attn_v16f_t& dp, lin_v4i_t* pr, lin_v4i_t* ds, float& top) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             // (asked of every element of every tile: a second form of the loop without it cost more in registers than it saved)
             const float x = 32 * n + 8 * (e >> 2) + (e & 3) >= least ? sc[e] : -INFINITY;
-            sc[e] = __builtin_amdgcn_exp2f(x * c);
+            sc[e] = __builtin_amdgcn_exp2f(F16 ? __builtin_fmaf(x, c, P_BITS<F16>) : x * c);
             dp[e] *= sc[e];
         }
+        if constexpr (F16) top = attn_top(dp);
 #pragma unroll
         for (int hs = 0; hs < 2; ++hs) {
             pr[hs] = attn_operand<F16>(sc, hs);
-            ds[hs] = attn_operand<F16>(dp, hs);
+            if constexpr (!F16) ds[hs] = attn_operand<F16>(dp, hs);
+        }
+    };
+    auto pack_ds = [&](attn_v16f_t& dp, lin_v4i_t* ds) __attribute__((always_inline)) {
+        if constexpr (F16) {
+            dp *= t;
+#pragma unroll
+            for (int hs = 0; hs < 2; ++hs) ds[hs] = attn_operand<F16>(dp, hs);
         }
     };
     auto back = [&](const lin_v4i_t* f, const lin_v4i_t& pr, const lin_v4i_t& ds) __attribute__((always_inline)) {
@@ -407,12 +473,15 @@ __global__ __launch_bounds__(64 * BWD_NW, 1) void attn_dkv_wide_kernel(AttnArgs 
     using N3 = std::integral_constant<int, 3>;
     using M1 = std::integral_constant<int, KS>;
     using M2 = std::integral_constant<int, 2 * KS>;
-    using V = std::integral_constant<int, KS == 8 ? 7 : KS == 6 ? 9 : 14>;
+    using V = std::integral_constant<int, 7>;
+    using V1 = std::integral_constant<int, F16 ? 8 : 7>;
+    using V2 = std::integral_constant<int, F16 ? 3 : 0>;
     int row = t0 * BQ;  // of the tile that is worked on
     auto tile = [&](uint8_t* sq, uint8_t* so, float* ss, const uint8_t* nq, const uint8_t* no, const float* ns) __attribute__((always_inline)) {
         const int least = key - shift - row - 4 * (lane >> 5);  // (query i sees the keys up to i + shift)
         row = row + BQ >= p.Lq ? t0 * BQ : row + BQ;
         lin_v4i_t p0[2], g0[2], p1[2], g1[2];
+        float top0, top1;
         read_rows(sq, so, 0, 1, fb);
         front(fa, 0, s0, d0);
         read_rows(sq, so, 1, 0, fa);
@@ -423,17 +492,21 @@ __global__ __launch_bounds__(64 * BWD_NW, 1) void attn_dkv_wide_kernel(AttnArgs 
         front(fa, 0, s1, d1);
         read_cols(sq, so, 0, 0, fa);
         front(fb, 1, s1, d1);
-        middle(0, least, s0, d0, p0, g0);
+        middle(0, least, s0, d0, p0, g0, top0);
         mix(M2{}, N2{}, V{});
+        if constexpr (F16) attn_follow<JD>(top0, dk, t);
         read_cols(sq, so, 0, 1, fb);
+        pack_ds(d0, g0);
         back(fa, p0[0], g0[0]);
         read_cols(sq, so, 1, 0, fa);
         back(fb, p0[1], g0[1]);
-        middle(1, least, s1, d1, p1, g1);
-        mix(M2{}, N2{}, V{});
+        middle(1, least, s1, d1, p1, g1, top1);
+        mix(M2{}, N2{}, V1{});
+        if constexpr (F16) attn_follow<JD>(top1, dk, t);
         read_cols(sq, so, 1, 1, fb);
+        pack_ds(d1, g1);
         back(fa, p1[0], g1[0]);
-        mix(M1{}, N2{}, N0{});
+        mix(M1{}, N2{}, V2{});
         // every wave's reads of this tile are done and the next one is there: the one after it into this one's place
         __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0)
         asm volatile("s_barrier" ::: "memory");
@@ -459,13 +532,14 @@ __global__ __launch_bounds__(64 * BWD_NW, 1) void attn_dkv_wide_kernel(AttnArgs 
 #pragma unroll
         for (int j = 0; j < JD; ++j) dk[j] = dv[j] = attn_zero();
     }
+    attn_unfit<F16, JD>(dk, t);
     const bool live = key < p.Lk;
     uint16_t* const dkr = const_cast<uint16_t*>(p.dk.p) + b * p.dk.b + (int64_t)key * p.dk.l + g * p.dk.h;
     uint16_t* const dvr = const_cast<uint16_t*>(p.dv.p) + b * p.dv.b + (int64_t)key * p.dv.l + g * p.dv.h;
 #pragma unroll
     for (int j = 0; j < JD; ++j) {
-        attn_store_block<F16>(dkr, dk[j], p.scale, j, p.D, lane, live);
-        attn_store_block<F16>(dvr, dv[j], 1.0f, j, p.D, lane, live);
+        attn_store_block<F16>(dkr, dk[j], p.scale * P_UNDO<F16>, j, p.D, lane, live);
+        attn_store_block<F16>(dvr, dv[j], P_UNDO<F16>, j, p.D, lane, live);
     }
 }
 
@@ -479,8 +553,10 @@ __global__ __launch_bounds__(64 * BWD_NW, 1) void attn_dkv_wide_kernel(AttnArgs 
 // place of 32; 192 heads with 1024 and 77 53 in place of 61, with 128 and 128 13.2 in place of 16.1. With 8 waves and up to 256 keys
 // there is one workgroup a CU, whose barrier every turn left its waves idle 40 % of the time: 1536 heads with 197 and 197 134 to 139
 // in place of 139, 48 of them 22 in place of 20; not kept.
-template <bool F16>
+// Of bf16 alone: in fp16 the ds of a query's keys would need one power of two across the four waves, and those of a key's queries another (P_BITS); the two kernels
+// take 68 us there for 1536 heads with 128 and 128.
 __global__ __launch_bounds__(64 * BWD_NW, 2) void attn_bwd_short_kernel(AttnArgs p, int per_head) {
+    constexpr bool F16 = false;
     constexpr int NW = BWD_NW, DP = 64, KS = DP / 16, JD = DP / 32, BQ = 32, TPR = 2 * NW, EL = DP / TPR;  // delta: TPR threads a row, EL elements each
     using Tile = AttnTile<DP>;
     __shared__ __attribute__((aligned(1024))) uint8_t sQ0[BQ * Tile::ROWB];
@@ -783,17 +859,17 @@ template <int DP, bool F16>
 void launch(const AttnArgs& p, hipStream_t s) {
     constexpr int ROWS = 32 * BWD_NW;
     const int q_tiles = (p.Lq + ROWS - 1) / ROWS, k_tiles = (p.Lk + ROWS - 1) / ROWS;
-    if constexpr (DP == 64) {
+    if constexpr (DP == 64 && !F16) {
         if (attn_bwd_is_short(p)) {
             const uint32_t heads = (uint32_t)(p.B * p.G);
-            hipLaunchKernelGGL(attn_bwd_short_kernel<F16>, dim3(std::min(heads, 512u)), dim3(64 * BWD_NW), 0, s, p, (p.Lq + 31) / 32);
+            hipLaunchKernelGGL(attn_bwd_short_kernel, dim3(std::min(heads, 512u)), dim3(64 * BWD_NW), 0, s, p, (p.Lq + 31) / 32);
             return;
         }
     }
     if (q_tiles) hipLaunchKernelGGL((attn_dq_kernel<DP, F16>), dim3((uint32_t)q_tiles * (uint32_t)(p.B * p.H)), dim3(64 * BWD_NW), 0, s, p, q_tiles);
     if (!k_tiles) return;
     const dim3 grid((uint32_t)k_tiles * (uint32_t)(p.B * p.G));
-    if constexpr (DP == 128) hipLaunchKernelGGL((attn_dkv_wide_kernel<DP, F16>), grid, dim3(64 * BWD_NW), 0, s, p, k_tiles);
+    if constexpr (DP == 128) hipLaunchKernelGGL((attn_dkv_wide_kernel<F16>), grid, dim3(64 * BWD_NW), 0, s, p, k_tiles);
     else hipLaunchKernelGGL((attn_dkv_kernel<DP, F16>), grid, dim3(64 * BWD_NW), 0, s, p, k_tiles);
 }
 
