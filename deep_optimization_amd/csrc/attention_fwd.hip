@@ -89,7 +89,7 @@ __global__ __launch_bounds__(64 * FWD_NW, 2) void attn_fwd_kernel(AttnArgs p, in
         for (int v = 1; v < 16; ++v) top = vmax3(top, s[0][v], s[1][v]);
         top = attn_max_halves(top) * c;
         if (wave_any(top > m + 8.0f)) {
-            const float next = vmax(m, top);
+            const float next = F16 ? ceilf(vmax(m, top)) : vmax(m, top);  // (see attn_base)
             const float a = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - next);
             m = next;
             l *= a;
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(64 * FWD_NW, 2) void attn_fwd_kernel(AttnArgs p, in
 #pragma unroll
                 for (int v = 0; v < 16; ++v) o[j][v] *= a;
         }
-        const float base = m == -INFINITY ? 0.0f : -m;
+        const float base = attn_base<F16>(m);
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
 #pragma unroll
@@ -131,7 +131,7 @@ __global__ __launch_bounds__(64 * FWD_NW, 2) void attn_fwd_kernel(AttnArgs p, in
     uint16_t* const out = const_cast<uint16_t*>(p.out.p) + b * p.out.b + (int64_t)row * p.out.l + h * p.out.h;
 #pragma unroll
     for (int j = 0; j < JD; ++j) attn_store_block<F16>(out, o[j], inv, j, p.D, lane, live);
-    if (p.lse && live && lane < 32) p.lse[(int64_t)bh * p.Lq + row] = (m + __builtin_amdgcn_logf(l)) * LN2;
+    if (p.lse && live && lane < 32) p.lse[(int64_t)bh * p.Lq + row] = attn_lse<F16>(m, l);
 }
 
 template <int DP, bool F16>

@@ -93,7 +93,7 @@ __global__ __launch_bounds__(64 * NW) void attn_token_kernel(AttnArgs p, int row
         for (int v = 2; v < 16; ++v) top = fmaxf(top, s[v]);
         top = attn_max_halves(top) * c;
         if (wave_any(top > m + 8.0f)) {  // (see attn_fwd_kernel)
-            const float next = fmaxf(m, top);
+            const float next = F16 ? ceilf(fmaxf(m, top)) : fmaxf(m, top);
             const float a = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - next);
             m = next;
             l *= a;
@@ -102,7 +102,7 @@ __global__ __launch_bounds__(64 * NW) void attn_token_kernel(AttnArgs p, int row
 #pragma unroll
                 for (int v = 0; v < 16; ++v) o[j][v] *= a;
         }
-        const float base = m == -INFINITY ? 0.0f : -m;
+        const float base = attn_base<F16>(m);
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
             s[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], c, base));
@@ -176,7 +176,7 @@ __global__ __launch_bounds__(64 * NW) void attn_token_kernel(AttnArgs p, int row
             for (int e = 0; e < 8; ++e) v[e] *= inv;
             uint16_t* dst = const_cast<uint16_t*>(p.out.p) + b * p.out.b + (int64_t)qi * p.out.l + h * p.out.h + d;
             *(lin_v4u_t*)dst = lin_v4u_t{attn_pack<F16>(v[0], v[1]), attn_pack<F16>(v[2], v[3]), attn_pack<F16>(v[4], v[5]), attn_pack<F16>(v[6], v[7])};
-            if (p.lse && d == 0) p.lse[((int64_t)b * p.H + h) * p.Lq + qi] = (peak + __builtin_amdgcn_logf(total)) * LN2;
+            if (p.lse && d == 0) p.lse[((int64_t)b * p.H + h) * p.Lq + qi] = attn_lse<F16>(peak, total);
         }
     }
 }
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(64 * JOIN_NW) void attn_join_kernel(AttnArgs p) {
     }
     const float inv = total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : total;  // (NaN stays)
     if (in) *(uint32_t*)(const_cast<uint16_t*>(p.out.p) + b * p.out.b + (int64_t)qi * p.out.l + h * p.out.h + 2 * lane) = attn_pack<F16>(v0 * inv, v1 * inv);
-    if (p.lse && lane == 0) p.lse[((int64_t)b * p.H + h) * p.Lq + qi] = (peak + __builtin_amdgcn_logf(total)) * LN2;
+    if (p.lse && lane == 0) p.lse[((int64_t)b * p.H + h) * p.Lq + qi] = attn_lse<F16>(peak, total);
 }
 
 int row_tiles(const AttnArgs& p) { return (p.Lq * (p.H / p.G) + 31) / 32; }

@@ -9,6 +9,7 @@ import torch
 
 import deep_optimization_amd  # noqa: F401
 from tests import attention_reference as ref
+from tests.block_reference import close
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -72,3 +73,36 @@ def test_gradients_of_probabilities_below_the_smallest_normal_number(D):
     gen = torch.Generator(device=DEV).manual_seed(4)
     Lq, Lk = 70, 131072
     _gradients(_rand(gen, (1, Lq, 1, D)), _rand(gen, (1, Lk, 1, D)), _rand(gen, (1, Lk, 1, D)), _rand(gen, (1, Lq, 1, D)), D ** -0.5, False)
+
+
+@pytest.mark.parametrize("Lq", [1, 40])
+@pytest.mark.parametrize("D", [64, 80, 128])
+def test_many_small_probabilities_beside_a_large_one(Lq, D):
+    """One key has all but 0.3 % of the probability and no value, so that the output is the other keys' alone."""
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    Lk = 131072
+    q, k = torch.zeros((1, Lq, 1, D), device=DEV, dtype=F16), torch.zeros((1, Lk, 1, D), device=DEV, dtype=F16)
+    q[..., 0] = 1
+    k[:, 0, :, 0] = 17.7
+    k[:, 1:, :, 0] = _rand(gen, (1, Lk - 1, 1), 0.3)
+    v = (1 + 0.1 * torch.randn((1, Lk, 1, D), generator=gen, device=DEV)).to(F16)
+    v[:, 0] = 0
+    out, lse = ops.attention_fwd(q, k, v, None, 1.0, False, True)
+    torch.cuda.synchronize()
+    want, wlse, tol, tlse = ref.forward(q, k, v, None, 1.0, False)
+    assert 0.002 < float(want.max()) < 0.004
+    close(out, want, tol, "out")
+    close(lse, wlse, tlse, "lse")
+
+
+@pytest.mark.parametrize("shift", [0.0, 30.0, -200.0])
+@pytest.mark.parametrize("Lq", [2, 70])
+def test_scores_far_from_zero_and_growing_maxima(Lq, shift):
+    gen = torch.Generator(device=DEV).manual_seed(6)
+    q, k, v = _rand(gen, (1, Lq, 2, 64)), _rand(gen, (1, 1500, 2, 64)), _rand(gen, (1, 1500, 2, 64))
+    q[..., 0] = 8
+    k[..., 0] = (torch.linspace(0, 10, 1500, device=DEV) + shift).to(F16)[None, :, None]
+    out, lse = ops.attention_fwd(q, k, v, None, 1.0, False, True)
+    want, wlse, tol, tlse = ref.forward(q, k, v, None, 1.0, False)
+    close(out, want, tol, "out")
+    close(lse, wlse, tlse, "lse")
