@@ -43,7 +43,8 @@ typedef float attn_v16f_t __attribute__((ext_vector_type(16)));
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 // The forward pass' probabilities, relative to a running maximum that they pass by 2^8 at most, are 2^7 times that in fp16: up to 2^15 of its 65504, so that
-// those of 2^-31 of the largest still count (a long row may hold many). The maximum is a whole number there: what is added to an exponent, 7 - m, is exact.
+// those of 2^-31 of the largest still count (a long row may hold many). What is added to an exponent for that, 7 - m as it is rounded, is a factor of all
+// of a row's probabilities, which their sum takes out again; the largest is a power of two still, and one key's value its output.
 template <bool F16>
 constexpr float FWD_BITS = F16 ? 7.0f : 0.0f;
 template <bool F16>
@@ -53,7 +54,7 @@ __device__ __forceinline__ float attn_base(float m) {
 // log of a row's sum
 template <bool F16>
 __device__ __forceinline__ float attn_lse(float m, float sum) {
-    return (m + (__builtin_amdgcn_logf(sum) - FWD_BITS<F16>)) * LN2;
+    return (__builtin_amdgcn_logf(sum) - attn_base<F16>(m)) * LN2;
 }
 
 // v_mfma_f32_32x32x16: lane l holds row (column) l % 32 and the 8 elements from 8 (l / 32) of K on; of the result column

@@ -89,7 +89,7 @@ __global__ __launch_bounds__(64 * FWD_NW, 2) void attn_fwd_kernel(AttnArgs p, in
         for (int v = 1; v < 16; ++v) top = vmax3(top, s[0][v], s[1][v]);
         top = attn_max_halves(top) * c;
         if (wave_any(top > m + 8.0f)) {
-            const float next = F16 ? ceilf(vmax(m, top)) : vmax(m, top);  // (see attn_base)
+            const float next = vmax(m, top);
             const float a = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - next);
             m = next;
             l *= a;

@@ -93,7 +93,7 @@ __global__ __launch_bounds__(64 * NW) void attn_token_kernel(AttnArgs p, int row
         for (int v = 2; v < 16; ++v) top = fmaxf(top, s[v]);
         top = attn_max_halves(top) * c;
         if (wave_any(top > m + 8.0f)) {  // (see attn_fwd_kernel)
-            const float next = F16 ? ceilf(fmaxf(m, top)) : fmaxf(m, top);
+            const float next = fmaxf(m, top);
             const float a = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - next);
             m = next;
             l *= a;

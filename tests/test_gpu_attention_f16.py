@@ -106,3 +106,11 @@ def test_scores_far_from_zero_and_growing_maxima(Lq, shift):
     want, wlse, tol, tlse = ref.forward(q, k, v, None, 1.0, False)
     close(out, want, tol, "out")
     close(lse, wlse, tlse, "lse")
+
+
+@pytest.mark.parametrize("Lq,Lk", [(1, 1), (40, 1), (50, 50), (5, 700)])
+def test_a_query_of_one_key_returns_its_value(Lq, Lk):
+    gen = torch.Generator(device=DEV).manual_seed(7)
+    q, k, v = _rand(gen, (3, Lq, 2, 64), 3.0), _rand(gen, (3, Lk, 2, 64), 3.0), _rand(gen, (3, Lk, 2, 64))
+    n = torch.ones(3, dtype=torch.int32, device=DEV)
+    assert torch.equal(ops.attention_fwd(q, k, v, n, 0.5, False, False)[0], v[:, :1].expand(3, Lq, 2, 64))
