@@ -14,8 +14,9 @@ as those ends) and, with ``causal``, j <= i + Lk - Lq: the last query sees every
 out [B, Lq, H, D] contiguous in q's type, lse fp32 [B, H, Lq] (None unless save_lse). Scores, softmax and sums are fp32; the
 probabilities, and in the backward pass ds, are rounded to q's type for the products that read them on matrix instructions (in fp16 times powers of two that
 keep them in its range, whatever the size of dout); delta is of out as it
-was returned, rounded to q's type (felt where a query sees a few keys only: 0.0037 of dq's norm at two keys in bf16, 0.0024 at many). What lies in k and v
-past a sequence's length is never used (NaN and infinities included) and has zero gradients. attention_qkv_bwd is attention_bwd
+was returned, rounded to q's type (felt where a query sees a few keys only: 0.0039 of dq's norm at two keys in bf16, 0.0024 at many). What lies in k and v
+past a sequence's length is never used (NaN and infinities included) and has zero gradients. What ``causal`` hides is multiplied by probabilities of 0: a value
+or key that is not finite makes NaN of earlier queries of its tile too, and a query's q or dout of later keys' gradients. attention_qkv_bwd is attention_bwd
 for q, k and v that are the parts of one tensor qkv [B, L, H + 2 G, D], ``heads`` = H: its gradient in one tensor.
 
 Any strides whose last one is 1; the kernels read where tokens lie at multiples of 16 bytes, at least D and less than 2^23 elements apart,

@@ -73,12 +73,7 @@ __device__ __forceinline__ attn_v16f_t attn_zero() {
     return z;
 }
 
-// the same lane of the other half of the wave
-__device__ __forceinline__ float attn_other_half(float v) {
-    const uint32_t a = __float_as_uint(v);
-    const auto r = __builtin_amdgcn_permlane32_swap(a, a, false, false);
-    return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
-}
+// over a lane and the same one of the other half of the wave
 __device__ __forceinline__ float attn_max_halves(float v) {
     const uint32_t a = __float_as_uint(v);
     const auto r = __builtin_amdgcn_permlane32_swap(a, a, false, false);

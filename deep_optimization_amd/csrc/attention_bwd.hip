@@ -7,10 +7,10 @@
 //
 // Seven products where one kernel that does all would need five: its dq would be summed over the key tiles in memory, in an order of
 // arrival, or in as many copies as there are key tiles. p and ds are rounded to the operands' type for the products that read them: each
-// gradient is then off by 1.4 times what its own rounding costs (0.0024 of its norm for 0.0017 in bf16, 0.0003 for 0.0002 in fp16, see P_BITS). delta is of out as it is kept, rounded once: where a
-// query sees few keys, dp - delta is a small difference and feels that (0.0037 at two keys, 0.0027 at six; with one key, whose ds is 0, what is left is
-// that rounding times dp). Summing p dp instead would take a second pass over the scores. As in the forward kernel the vector arithmetic between the
-// products bounds all of them.
+// gradient is then off by 1.4 times what its own rounding costs (0.0024 of its norm for 0.0017 in bf16, 0.0003 for 0.0002 in fp16, see P_BITS). delta is of out as it is given, rounded: where a
+// query sees few keys, dp - delta is a small difference and feels that (0.0039 at two keys, 0.0028 at 2 to 16, 0.0005 and 0.00035 in fp16; one key's value is out
+// itself, and its ds 0 but for the order of two sums). Summing p dp instead would take a second pass over the scores of rows with more than a tile of keys, and
+// would make the gradient one of another out than the caller's. As in the forward kernel the vector arithmetic between the products bounds all of them.
 #include <algorithm>
 
 #include "attention.h"
@@ -35,9 +35,9 @@ __device__ __forceinline__ void attn_widen2(uint32_t w, float& a, float& b) {
 // rounded by them, and are undone in the sums. p, at most 1, is taken times 2^14. ds may be of any size (a gradient of 1e-5 over 4096 keys makes 1e-9 of it):
 // it has a power of two for each of a sum's columns, t, which follows the largest |ds| of the column's terms. Where a block's passes 2^15 / t, t is
 // set anew so that it lies at 2^7 to 2^8, and the sums so far are scaled along; what is rounded below fp16's normal numbers is then less than 2^-21 of the
-// column's largest term. It starts at the most that an fp32 number takes. It costs fp16 a largest value and a product a score, on one box: dq of 1536 heads of
-// 64, 197 and 197 64 -> 65 us, of 96 heads of 80, 985 and 985 70 -> 77, of 64 causal heads of 128, 4096 and 4096 420 -> 445; dk and dv 75 -> 81, 91 -> 98 and
-// 690 -> 725.
+// column's largest term. It starts at the most that an fp32 number takes. It costs fp16 a largest value and a product a score, both sides on one box: dq of 1536
+// heads of 64, 197 and 197 62 -> 66 us, of 96 heads of 80, 985 and 985 70 -> 78, of 64 causal heads of 128, 4096 and 4096 420 -> 447; dk and dv 74 -> 82, 91 -> 100
+// and 690 -> 728.
 template <bool F16>
 constexpr float P_BITS = F16 ? 14.0f : 0.0f;
 template <bool F16>

@@ -315,7 +315,7 @@ __global__ __launch_bounds__(256, 1) void lin_big_kernel(LinArgs p) {
     // columns come out of the exchange of blocks 4 q and 4 q + 2, 4 q + 1 and 4 q + 3.
     // The stores of pre and of the gradient's two results bound these forms, as the plain one's bound linear_act_fwd's: a workgroup has its CU to itself
     // and runs no MFMAs meanwhile. 25216 x 768 -> 2 x 2048 with silu, bf16: 190 to 205 us (its product alone takes 119 at the rate of a large one, the 348 MB
-    // of pre, h, x 69 at a large copy's); the gradient, 768 -> 2048, with h 150 to 165 (59 and 109).
+    // of pre, h, x 69 at a large copy's); the gradient, 768 -> 2048, with h 165 to 180, without 150 (59 and 109).
     auto gated_epilogue = [&](uint32_t i_tile) __attribute__((always_inline)) {
         uint32_t tm, tn;
         coords(i_tile, tm, tn);

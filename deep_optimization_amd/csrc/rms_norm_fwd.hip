@@ -5,8 +5,8 @@
 // rounded to x's type, so that it carries one rounding. The row's lanes, its accesses and the widths' classes are the layer norm's
 // (layer_norm_fwd.hip). The e4m3 form takes a second exchange over the row's lanes, for the largest |y|.
 //
-// Bound by memory: 25216 x 768 bf16 with a residual 27 to 29 us, 5.3 to 5.7 TB/s where a large copy reaches 5.0; 6304 x 591 fp32 7.0 (4.3 TB/s: scalar
-// accesses of odd rows); to e4m3, 4096 x 4096 bf16 with a residual 23 to 26 (117 MB, 4.6 to 5.1 TB/s), one row 3.3.
+// Bound by memory: 25216 x 768 bf16 with a residual 27 to 29 us, 5.3 to 5.7 TB/s where a large copy reaches 5.0; 6304 x 591 fp32 7.0 (4.3 TB/s;
+// ten times the rows 51, 5.8: 30 MB are few beside a launch's beginning and end. An odd width costs nothing, 592 takes the same); to e4m3, 4096 x 4096 bf16 with a residual 23 to 26 (117 MB, 4.6 to 5.1 TB/s), one row 3.3.
 #include <algorithm>
 
 #include "rms_norm.h"

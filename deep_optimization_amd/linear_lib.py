@@ -29,7 +29,7 @@ way; without that product, or with an activation, the launch that writes dz (or 
 
 The gated layer: weight [2 H, K], bias [2 H], h [..., H], pre and dpre [..., 2 H]; both projections, the activation and the product in one
 kernel. Its backward pass with the Linear layer behind it (out_weight [N, H], dy [..., N]) is one product too, which makes dpre from its sums, and
-h once more for out_weight's gradient, so that only x and pre are kept; x's and weight's gradients are linear_act_bwd(dpre, x, weight, None, "none", ..).
+h once more for out_weight's gradient, so that a caller who asks for it may keep x and pre only; x's and weight's gradients are linear_act_bwd(dpre, x, weight, None, "none", ..).
 h comes from the fp32 sums, rounded once; the backward pass reads g and u as pre holds them, in x's type, and rounds dpre to it: x's and
 weight's gradients are then off by 0.003 of their norm where their own rounding alone is 0.0017 (25216 rows of 768 -> 2 x 2048 with
 silu in bf16). pre in fp32 would double the 207 MB that are written and read there, some 80 us of 800, and leave dpre's rounding.

@@ -570,7 +570,8 @@ int dopt_gated_tile(int product, int64_t M, int64_t H, int64_t K, int any_rows, 
  *   s_ij = scale q_i . k_j for the keys j that query i sees: j < lengths[b] and, if causal, j <= i + k_len - q_len
  *   out_i = sum_j softmax(s_i)_j v_j,  lse_i = log sum_j exp(s_ij);  a query that sees no key: out 0, lse -infinity
  * Query head h reads key head h / (heads / kv_heads). lengths: int32 [batch] on the device, or NULL (k_len); a value outside 0..k_len
- * counts as the nearer end. Keys and values past a sequence's length are not used, whatever they hold. scale from 2^-100 to 2^100.
+ * counts as the nearer end. Keys and values past a sequence's length are not used, whatever they hold; those that `causal`
+ * hides are multiplied by probabilities of 0, and have to be finite. scale from 2^-100 to 2^100.
  * Tensors are [batch, tokens, heads, dim] with dim contiguous elements: 16-byte aligned, dim and the strides (in elements) multiples of 8,
  * dim at most 128, the tokens' stride at least dim and below 2^23 (strides of sizes of 1 are not looked at).
  * Forward: out and lse (fp32 [batch, heads, q_len] contiguous, may be NULL). workspace: dopt_attention_workspace_floats floats
